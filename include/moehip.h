@@ -365,6 +365,134 @@ moe_status moe_greedy_dev(const float* logits, int n, int32_t* next);
 moe_status moe_head_greedy_dev(const float* x, const float* W, int N, int K, float* logits,
                                int32_t* next);
 
+/* ---- many requests over a paged cache ------------------------------------
+ * Keys and values of many requests in pages of page_size positions that any
+ * request may hold, instead of moe_model's one contiguous cache.  A step:
+ *   moe_paged_plan_dev    pages for the new tokens, each token's place
+ *   moe_paged_heads_dev   (every layer) q/k norm, rotation, K and V to pages
+ *   moe_paged_attn_dev    (every layer) attention over the requests' pages
+ * All pointers are device memory unless said otherwise; the three allocate
+ * nothing, read no device value on the host and may be captured into a graph
+ * on the library's stream.  Arguments are checked before any GPU work
+ * (MOE_ERR_ARG / MOE_ERR_UNSUPPORTED with a message); what lies in device
+ * memory is bounds-checked by the kernels as said at each.  Sums are fp32
+ * and their order is the kernels' own: close to, not bit-identical to
+ * moe_model_forward's sequential chains.  No reference counterpart: the
+ * reference recomputes one sequence (test_model_trace.c:526-579). */
+
+/* element types of a paged cache */
+enum { MOE_PAGE_F32 = 0, MOE_PAGE_F16 = 1, MOE_PAGE_BF16 = 4, MOE_PAGE_E4M3 = 5 };
+
+/* One layer's cache.  Element (page, head, offset, dim) of K is
+ *   k[page * page_stride + head * head_stride + offset * slot_stride + dim]
+ * (strides in elements, the same for v), so pages may be slot-major or
+ * head-major, and K and V may share pages.  k, v and the strides' bytes are
+ * multiples of 16, head_dim a multiple of 16 up to 256, every stride at least
+ * head_dim, n_pages * page_size below 2^31.  MOE_PAGE_E4M3 holds
+ * value / scale (OCP 8-bit, rounded to nearest even, saturated at 448), with
+ * one fp32 scale a head in k_scale / v_scale (NULL: 1); both are NULL for the
+ * other types. */
+typedef struct {
+  void* k;
+  void* v;
+  int dtype;
+  int n_pages, page_size, n_kv, head_dim;
+  long long page_stride, head_stride, slot_stride;
+  const float* k_scale;
+  const float* v_scale;
+} moe_pages;
+
+/* The state of a server's cache and one step over it.  ring holds page
+ * numbers; the free ones are the ring_at[1] entries from ring[ring_at[0]] on,
+ * wrapping at n_pages.  tables[r][i] is the page of request r's positions
+ * i * page_size .. + page_size - 1. */
+typedef struct {
+  int n_req, max_pages;        /* requests, pages a table row holds */
+  int n_pages, page_size;
+  int max_tokens;              /* rows of req, pos and slot */
+  const int32_t* fresh;        /* [n_req] new tokens of this step, or -1: ended */
+  const int32_t* held;         /* [n_req] positions in the cache before it */
+  const int32_t* ring_at;      /* [2] */
+  int32_t* ring;               /* [n_pages] */
+  int32_t* tables;             /* [n_req][max_pages] */
+  int32_t* held_out;           /* [n_req], may be held */
+  int32_t* ring_at_out;        /* [2], may be ring_at */
+  int32_t* starts;             /* [n_req + 1] first token of each request */
+  int32_t* req;                /* [max_tokens] request of each token */
+  int32_t* pos;                /* [max_tokens] its position in the request */
+  int32_t* slot;               /* [max_tokens] its slot, page * page_size + offset */
+  int32_t* status;             /* [1] */
+} moe_paged_plan;
+/* Takes free pages, oldest first, for the requests in order, extends their
+ * tables, gives an ended request's pages back behind the free ones (for the
+ * next step; its held becomes 0), and places the tokens: request r's are rows
+ * starts[r] .. starts[r + 1] - 1.  Rows behind the last token get req = pos =
+ * slot = -1.  *status: 0 done; 1 too few free pages, 2 more than max_tokens
+ * tokens, 3 a request outgrows its table row, 4 the state is broken (a
+ * negative length, fresh under -1, a ring that cannot be): then every row is
+ * -1, starts are 0, held and ring_at are copied, and tables and ring keep
+ * their entries.  A table or ring entry that is no page yields a slot that
+ * moe_paged_heads_dev refuses. */
+moe_status moe_paged_plan_dev(const moe_paged_plan* plan);
+
+/* qkv [T x ld]: n_q query heads, n_kv key heads, n_kv value heads of head_dim
+ * a row.  Query and key heads: RMS norm over head_dim with weight q_norm /
+ * k_norm [head_dim] (NULL: no norm, eps unused), then the first rope_dim
+ * values turned by the row's position: (y_i, y_{i + rope_dim / 2}) by
+ * rope_cos / rope_sin [rope_len x rope_dim / 2] (test_model_trace.c:310-336;
+ * rope_dim even, 0: none, tables may be NULL).  Queries go to q_out [T x ldq]
+ * (may be qkv with the same stride), keys and values, converted, to slot[t].
+ * A row with slot[t] < 0 is left as it is, in q_out too.  A slot at or past
+ * n_pages * page_size or a position outside [0, rope_len) makes the row's
+ * queries NaN; nothing is written outside the cache (a bad position's key is
+ * NaN in it).  Two rows of one slot: either one's values stay. */
+typedef struct {
+  const float* qkv;
+  long long ld;
+  int T, n_q;
+  const int32_t* pos;     /* [T] */
+  const int32_t* slot;    /* [T] */
+  const float* q_norm;
+  const float* k_norm;
+  float eps;
+  const float* rope_cos;
+  const float* rope_sin;
+  int rope_len, rope_dim;
+  float* q_out;
+  long long ldq;
+} moe_paged_heads;
+moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* pages);
+
+/* Row t of q [T x ldq] (n_q heads of head_dim) attends positions 0 .. pos[t]
+ * of request req[t] (NULL: request t), each query head to key-value head
+ * h / (n_q / n_kv):  out[t] = softmax(scale q . k) v, out [T x ldo], not q.
+ * pos[t] < 0, or every score -inf: zeros.  req[t] < 0: the row of out is left
+ * as it is.  A request at or past n_req, a position at or past max_pages *
+ * page_size, or a table entry that is no page: NaN in the row, nothing read
+ * outside the cache or the tables.  A NaN or an infinity in an attended
+ * position's key or value, or in the query, may make the row NaN; what lies
+ * in the pages behind pos[t] never matters.  Several rows may belong to one request (a prompt's
+ * tokens, once moe_paged_heads_dev has written them all); each reads the
+ * cache for itself.  work: moe_paged_attn_work_bytes(T, n_q, n_kv, head_dim)
+ * bytes, 16-byte aligned, used from this call's launch to its end: calls or
+ * graphs that may run at the same time need their own. */
+typedef struct {
+  const float* q;
+  long long ldq;
+  int T, n_q;
+  const int32_t* req;
+  const int32_t* pos;      /* [T] */
+  const int32_t* tables;   /* [n_req][max_pages] */
+  int n_req, max_pages;
+  float scale;
+  float* out;
+  long long ldo;
+  void* work;
+  size_t work_bytes;
+} moe_paged_attn;
+size_t moe_paged_attn_work_bytes(int T, int n_q, int n_kv, int head_dim);
+moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* pages);
+
 /* Name of the kernel variant the GEMV entry points use for a shape. */
 const char* moe_gemv_variant(int dtype, int M, int N, int K);
 

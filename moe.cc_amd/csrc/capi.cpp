@@ -92,6 +92,7 @@ moe_status ensure_init() {
 }
 
 hipStream_t stream() { return g_stream; }
+int device() { return g_device; }
 
 namespace {
 

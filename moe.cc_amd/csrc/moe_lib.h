@@ -13,6 +13,8 @@ moe_status check_hip(hipError_t e, const char* what);
 moe_status ensure_init();
 // The library's stream.
 hipStream_t stream();
+// The device it belongs to (-1 before initialisation).
+int device();
 // Layers and models alive (moe_shutdown refuses while any is).
 void live_objects(int delta);
 // Free the library-owned device buffers of one translation unit (the

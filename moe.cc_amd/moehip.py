@@ -49,7 +49,45 @@ class QJob(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_LL = ctypes.c_longlong
+_F = ctypes.c_float
 _SZ = ctypes.c_size_t
+
+# element types of a paged cache (MOE_PAGE_*)
+PAGE_F32, PAGE_F16, PAGE_BF16, PAGE_E4M3 = 0, 1, 4, 5
+
+
+class Pages(ctypes.Structure):
+    """moe_pages: one layer's paged cache."""
+
+    _fields_ = [("k", _P), ("v", _P), ("dtype", _I), ("n_pages", _I), ("page_size", _I),
+                ("n_kv", _I), ("head_dim", _I), ("page_stride", _LL), ("head_stride", _LL),
+                ("slot_stride", _LL), ("k_scale", _P), ("v_scale", _P)]
+
+
+class PagedPlan(ctypes.Structure):
+    """moe_paged_plan: the state of a paged cache and one step over it."""
+
+    _fields_ = [(n, _I) for n in ("n_req", "max_pages", "n_pages", "page_size", "max_tokens")] + \
+               [(n, _P) for n in ("fresh", "held", "ring_at", "ring", "tables", "held_out",
+                                  "ring_at_out", "starts", "req", "pos", "slot", "status")]
+
+
+class PagedHeads(ctypes.Structure):
+    """moe_paged_heads: q/k norm, rotation, K and V into the pages."""
+
+    _fields_ = [("qkv", _P), ("ld", _LL), ("T", _I), ("n_q", _I), ("pos", _P), ("slot", _P),
+                ("q_norm", _P), ("k_norm", _P), ("eps", _F), ("rope_cos", _P), ("rope_sin", _P),
+                ("rope_len", _I), ("rope_dim", _I), ("q_out", _P), ("ldq", _LL)]
+
+
+class PagedAttn(ctypes.Structure):
+    """moe_paged_attn: attention of rows over their requests' pages."""
+
+    _fields_ = [("q", _P), ("ldq", _LL), ("T", _I), ("n_q", _I), ("req", _P), ("pos", _P),
+                ("tables", _P), ("n_req", _I), ("max_pages", _I), ("scale", _F), ("out", _P),
+                ("ldo", _LL), ("work", _P), ("work_bytes", _SZ)]
+
 
 _SIGS = {
     "matmul_adaptive": (None, [_P, _P, _P, _P, _I, _I, _I]),
@@ -99,6 +137,10 @@ _SIGS = {
     "moe_layer_forward_noalloc": (_I, [_P, _P, _P, _I, _P, _P, _P]),
     "moe_block_forward": (_I, [_P, _P, _I, _P, ctypes.c_float]),
     "moe_rmsnorm_dev": (_I, [_P, _P, _P, _I, _I, ctypes.c_float]),
+    "moe_paged_plan_dev": (_I, [_P]),
+    "moe_paged_heads_dev": (_I, [_P, _P]),
+    "moe_paged_attn_work_bytes": (_SZ, [_I, _I, _I, _I]),
+    "moe_paged_attn_dev": (_I, [_P, _P]),
     "moe_layer_debug_buffers": (_I, [_P, ctypes.POINTER(_P), ctypes.POINTER(_P),
                                      ctypes.POINTER(_P)]),
     "moe_model_create": (_I, [_P, _P, _I, ctypes.POINTER(_P)]),

@@ -1,0 +1,189 @@
+"""moe_paged_attn_dev against a 64-bit evaluation on the values that the pages hold; the bound on an fp32 evaluation
+is derived in paged_cases.attend.  Every slot that no position fills holds a NaN or an infinity."""
+import numpy as np
+import pytest
+
+import paged_cases as C
+
+pytestmark = pytest.mark.gpu
+
+ARG = 2
+
+
+class Batch:
+    """Requests of given lengths on pages in no order, queries, and the call."""
+
+    def __init__(self, M, dtype, lens, nq, nkv, hd, ps, order="slot", seed=0, ld_extra=0, spare=2, gain=1.0):
+        self.M, self.lens, self.nq, self.hd, self.ps = M, lens, nq, hd, ps
+        rng = np.random.default_rng(1000 + seed)
+        scales = [0.01 + 0.02 * rng.random(nkv) for _ in "kv"] if dtype == C.E4M3 else [None, None]
+        used = [-(-n // ps) for n in lens]
+        self.width = max(max(used), 1) + 1
+        n_pages = sum(used) + spare
+        self.pool = C.Pool(M, dtype, n_pages, ps, nkv, hd, order, *scales)
+        order_of = rng.permutation(n_pages)
+        self.tables = np.full((len(lens), self.width), -7, np.int32)
+        at = 0
+        for r, n in enumerate(lens):
+            self.tables[r, :used[r]] = order_of[at:at + used[r]]
+            at += used[r]
+            if n:
+                p = np.arange(n)
+                k, v = (rng.standard_normal((n, nkv, hd)).astype(np.float32) * g for g in (gain, 1.0))
+                slot = (self.tables[r][p // ps], p % ps)
+                for side, (pool, x) in enumerate(((self.pool.k, k), (self.pool.v, v))):
+                    pool[slot] = C.encode((x / self.pool.factor(side)).astype(np.float32), dtype)
+        self.pool.upload()
+        self.scale = float(np.float32(1 / np.sqrt(hd)))
+        self.rng, self.ld = rng, nq * hd + ld_extra
+
+    def run(self, req=None, pos=None, T=None, q=None, work_from=0xA5):
+        """-> (out [T, ld], q [T, nq, hd]); out starts as 7s"""
+        M = self.M
+        T = T or len(self.lens)
+        pos = np.asarray(self.lens, np.int32) - 1 if pos is None else np.asarray(pos, np.int32)
+        if q is None:
+            q = self.rng.standard_normal((T, self.ld)).astype(np.float32)
+        out = np.full((T, self.ld), 7.0, np.float32)
+        need = M.lib().moe_paged_attn_work_bytes(T, self.nq, self.pool.n_kv, self.hd)
+        bufs = [M.DeviceBuffer.from_array(x) for x in (q, pos, self.tables, out)]
+        rq = None if req is None else M.DeviceBuffer.from_array(np.asarray(req, np.int32))
+        work = M.DeviceBuffer.from_array(np.full(need, work_from, np.uint8))
+        a = M.PagedAttn(bufs[0].ptr, self.ld, T, self.nq, None if rq is None else rq.ptr, bufs[1].ptr, bufs[2].ptr, len(self.lens), self.width,
+                        self.scale, bufs[3].ptr, self.ld, work.ptr, need)
+        M.check(M.lib().moe_paged_attn_dev(C.ref(a), C.ref(self.pool.pages)), "paged_attn")
+        return bufs[3].download(out.shape, np.float32), q[:, :self.nq * self.hd].reshape(T, self.nq, self.hd)
+
+    def check(self, out, q, t, r, n):
+        k, v = self.pool.rows(self.tables[r], n)
+        want, tol = C.attend(q[t].astype(np.float64), k, v, self.scale)
+        got = out[t, :self.nq * self.hd].reshape(self.nq, self.hd)
+        assert np.isfinite(got).all(), f"row {t} of {n} positions: not finite"
+        off = np.abs(got - want) / np.maximum(tol, 1e-30)
+        if n == 0:
+            assert not got.any()
+        else:
+            assert off.max() <= 1, f"row {t} of {n} positions: {off.max():.2f} times the bound at {np.unravel_index(off.argmax(), off.shape)}"
+        assert (out[t, self.nq * self.hd:] == 7).all()
+
+
+def _all(b, out, q):
+    for t, n in enumerate(b.lens):
+        b.check(out, q, t, t, n)
+
+
+LENS = [1, 0, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129, 255, 257, 300]
+
+
+@pytest.mark.parametrize("kind", list(C.TYPES))
+@pytest.mark.parametrize("nq,nkv,hd,ps,order", [
+    (32, 4, 128, 16, "slot"), (8, 8, 64, 32, "head"), (6, 2, 80, 24, "slot"), (16, 1, 256, 64, "shared"), (40, 2, 128, 7, "head"),
+    (3, 3, 16, 1, "slot"), (5, 1, 48, 128, "shared"), (34, 2, 96, 16, "head"), (4, 4, 208, 100, "slot")])
+def test_shapes(moehip, kind, nq, nkv, hd, ps, order):
+    print("paged attention", kind, nq, nkv, hd, ps, order, flush=True)
+    b = Batch(moehip, C.TYPES[kind], LENS, nq, nkv, hd, ps, order, seed=hd + ps, ld_extra=3 if hd == 80 else 0)
+    out, q = b.run()
+    _all(b, out, q)
+
+
+@pytest.mark.parametrize("kind", list(C.TYPES))
+@pytest.mark.parametrize("lens", [[5000], [70000], [1] * 300, [3, 40000, 1, 9, 2000, 0, 12], list(range(0, 1100, 4))],
+                         ids=lambda v: f"{len(v)}x{max(v)}")
+def test_lengths(moehip, kind, lens):
+    print("paged attention lengths", kind, len(lens), max(lens), flush=True)
+    b = Batch(moehip, C.TYPES[kind], lens, 8, 2, 64, 32, seed=len(lens))
+    out, q = b.run()
+    for t in range(0, len(lens), max(1, len(lens) // 40)):
+        b.check(out, q, t, t, lens[t])
+
+
+def test_same_bits_every_time(moehip):
+    """The split and its join are fixed by the lengths: the same call gives the same bits."""
+    b = Batch(moehip, C.BF16, [9000, 1, 300, 2500], 32, 4, 128, 16, seed=3)
+    out, q = b.run()
+    for fill in (0, 0xFF):
+        again, _ = b.run(q=q.reshape(4, -1), work_from=fill)
+        np.testing.assert_array_equal(out.view(np.uint32), again.view(np.uint32))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_of_one_request_and_padding(moehip, kind):
+    """A prompt's rows (each sees one position more), rows of other requests between them, rows that no request fills."""
+    b = Batch(moehip, C.TYPES[kind], [90, 33], 8, 4, 64, 16, seed=5)
+    rows = [(0, p) for p in range(60, 90)] + [(-1, 5), (1, 32), (1, 0), (-1, -1), (0, 0), (0, -1), (-3, 1 << 30)]
+    req, pos = zip(*rows)
+    out, q = b.run(req=req, pos=pos, T=len(rows))
+    for t, (r, p) in enumerate(rows):
+        if r < 0:
+            assert (out[t] == 7).all(), f"row {t} of no request was written"
+        else:
+            b.check(out, q, t, r, p + 1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "e4m3"])
+@pytest.mark.parametrize("bad_page", [-1, 10 ** 9, -2 ** 31])
+def test_bad_pages_and_places(moehip, kind, bad_page):
+    """A table entry that is no page, a request or a position past the tables: that row is NaN, the others are right."""
+    lens = [100, 700, 40, 3000, 64]
+    b = Batch(moehip, C.TYPES[kind], lens, 8, 2, 64, 16, seed=9)
+    b.tables[1, 20] = bad_page
+    b.tables[3, 0] = b.pool.n_pages
+    b.tables[4, 4:] = bad_page           # behind the last position: never read
+    wide = b.width * 16
+    req = [0, 1, 2, 3, 4, 5, 2 ** 31 - 1, 0, 0]
+    pos = [99, 699, 39, 2999, 63, 3, 3, wide, 2 ** 31 - 1]
+    out, q = b.run(req=req, pos=pos, T=9)
+    for t in (0, 2, 4):
+        b.check(out, q, t, t, lens[t])
+    for t in (1, 3, 5, 6, 7, 8):
+        assert np.isnan(out[t]).all(), f"row {t}"
+
+
+@pytest.mark.parametrize("kind", list(C.TYPES))
+def test_far_scores(moehip, kind):
+    """Scores hundreds apart: the running maximum carries every earlier weight to zero and none overflows."""
+    b = Batch(moehip, C.TYPES[kind], [1, 50, 3000, 700], 8, 2, 64, 16, seed=11, gain=40.0 if kind != "e4m3" else 4.0)
+    out, q = b.run()
+    _all(b, out, q)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_nan_stays_in_its_heads(moehip, kind):
+    """NaN in an attended key or value makes its heads NaN and no others."""
+    b = Batch(moehip, C.TYPES[kind], [40, 2000, 40], 4, 2, 64, 16, seed=13)
+    k = b.pool.k
+    k[b.tables[1, 7], 3, 1, 5] = C.NAN_BITS[C.TYPES[kind]] if kind != "f32" else np.nan
+    b.pool.v[b.tables[2, 1], 2, 0, 9] = C.NAN_BITS[C.TYPES[kind]] if kind != "f32" else np.nan
+    b.pool.upload()
+    out, q = b.run()
+    o = out.reshape(3, 4, 64)
+    b.check(out, q, 0, 0, 40)
+    assert np.isnan(o[1, 2:]).all() and np.isfinite(o[1, :2]).all()
+    assert np.isnan(o[2, :2, 9]).all() and np.isfinite(o[2, 2:]).all()
+
+
+def test_offsets_past_32_bits(moehip):
+    """Pages 2^28 elements apart: the last lie past 2^32 bytes and elements."""
+    M = moehip
+    n_pages, ps, hd, nkv = 18, 16, 64, 2
+    stride = 1 << 28
+    pool = M.DeviceBuffer(n_pages * stride)
+    rng = np.random.default_rng(17)
+    table = np.array([[17, 0, 16, 9]], np.int32)
+    k, v = (rng.standard_normal((64, nkv, hd)).astype(np.float32) for _ in "kv")
+    gap = ps * nkv * hd   # V's rows behind K's in each page
+    for i, page in enumerate(table[0]):
+        for side, x in enumerate((k, v)):
+            pool.upload(C.encode(x[i * ps:(i + 1) * ps], C.E4M3), offset=int(page) * stride + side * gap)
+    pages = M.Pages(pool.ptr, pool.ptr + gap, C.E4M3, n_pages, ps, nkv, hd, stride, hd, nkv * hd, None, None)
+    q = rng.standard_normal((1, 4 * hd)).astype(np.float32)
+    bufs = [M.DeviceBuffer.from_array(x) for x in (q, np.array([59], np.int32), table, np.zeros_like(q))]
+    need = M.lib().moe_paged_attn_work_bytes(1, 4, nkv, hd)
+    work = M.DeviceBuffer(need)
+    a = M.PagedAttn(bufs[0].ptr, 4 * hd, 1, 4, None, bufs[1].ptr, bufs[2].ptr, 1, 4, 0.125, bufs[3].ptr, 4 * hd, work.ptr, need)
+    M.check(M.lib().moe_paged_attn_dev(C.ref(a), C.ref(pages)))
+    got = bufs[3].download((4, hd), np.float32)
+    kd, vd = (C.decode(C.encode(x[:60], C.E4M3), C.E4M3) for x in (k, v))
+    want, tol = C.attend(q.reshape(4, hd).astype(np.float64), kd, vd, 0.125)
+    assert (np.abs(got - want) <= tol).all()
+    pool.free()
