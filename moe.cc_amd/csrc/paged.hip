@@ -1,11 +1,11 @@
 // paged.hip - many requests over a paged key-value cache (include/moehip.h,
 // "many requests over a paged cache"): the step's plan, the new rows' heads
-// into their pages, and attention over the pages.
+// into their pages, and the entry points (attention: paged_attn.hip).
 #include <math.h>
 
 #include "moe_device.h"
 #include "moe_lib.h"
-#include "paged.h"
+#include "paged_attn.h"
 
 namespace moe {
 namespace {
@@ -57,17 +57,14 @@ moe_status check_pages(const moe_pages* g, const char* who, PageMap* m) {
 
 struct CacheF32 {
   using T = float;
-  static __device__ float load(const T* p) { return *p; }
   static __device__ T make(float x) { return x; }
 };
 struct CacheF16 {
   using T = _Float16;
-  static __device__ float load(const T* p) { return (float)*p; }
   static __device__ T make(float x) { return (_Float16)x; }
 };
 struct CacheBF16 {
   using T = uint16_t;
-  static __device__ float load(const T* p) { return __uint_as_float((uint32_t)*p << 16); }
   static __device__ T make(float x) {
     const uint32_t u = __float_as_uint(x);
     if ((u & 0x7fffffffu) > 0x7f800000u) return (T)(u >> 16 | 0x40);   // NaN stays one
@@ -76,7 +73,6 @@ struct CacheBF16 {
 };
 struct CacheE4M3 {
   using T = uint8_t;
-  static __device__ float load(const T* p) { return __builtin_amdgcn_cvt_f32_fp8((int)*p, 0); }
   // saturated here: the conversion itself turns what is past 448 into NaN
   static __device__ T make(float x) {
     const float c = x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x;   // NaN passes
@@ -287,87 +283,6 @@ __global__ __launch_bounds__(64) void heads_pages_kernel(HeadsArgs a) {
   }
 }
 
-// ------------------------------------------------------------ attention
-
-struct AttnPages {
-  moe_paged_attn a;
-  PageMap map;
-  const void* k;
-  const void* v;
-  const float* k_scale;
-  const float* v_scale;
-};
-
-constexpr int kAttnWaves = 4;
-
-// A block a (row, query head): its waves take every fourth position, each with
-// its own running maximum and sum, joined at the end.
-template <class C>
-__global__ __launch_bounds__(64 * kAttnWaves) void paged_attn_kernel(AttnPages g) {
-  const moe_paged_attn& a = g.a;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, hd = g.map.head_dim;
-  const int t = (int)blockIdx.x, head = (int)blockIdx.y, kv = head / (a.n_q / g.map.n_kv);
-  const int req = a.req ? a.req[t] : t, pos = a.pos[t];
-  if (req < 0) return;
-  __shared__ float part[kAttnWaves][256 + 2];
-  __shared__ int bad_s;
-  if (threadIdx.x == 0) bad_s = req >= a.n_req || (pos >= 0 && (long long)pos >= (long long)a.max_pages * g.map.page_size);
-  __syncthreads();
-  float q[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = lane + 64 * i < hd ? a.q[(size_t)t * a.ldq + (size_t)head * hd + lane + 64 * i] : 0.0f;
-  const float scale = a.scale * (g.k_scale ? g.k_scale[kv] : 1.0f);
-  bool bad = bad_s;
-  if (!bad) {
-    const int* table = a.tables + (size_t)req * a.max_pages;
-    for (int p = wave; p <= pos; p += kAttnWaves) {
-      const int pg = (int)divide((uint32_t)p, g.map.per), page = table[pg];
-      if (!page_ok(g.map, page)) {
-        bad = true;
-        break;
-      }
-      const long long at = page_row(g.map, page, kv, p - pg * g.map.page_size);
-      float s = 0.0f, vv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < hd) {
-          s = fmaf(q[i], C::load((const typename C::T*)g.k + at + lane + 64 * i), s);
-          vv[i] = C::load((const typename C::T*)g.v + at + lane + 64 * i);
-        } else {
-          vv[i] = 0.0f;
-        }
-      for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
-      s *= scale;
-      const float top = s > m || s != s ? s : m;   // NaN stays
-      if (top == -INFINITY) continue;              // nothing yet
-      const float keep = m == -INFINITY ? 0.0f : expf(m - top), e = expf(s - top);
-      m = top;
-      l = l * keep + e;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + e * vv[i];
-    }
-  }
-  if (bad) bad_s = 1;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = o[i];
-  if (lane == 0) part[wave][256] = m, part[wave][257] = l;
-  __syncthreads();
-  float top = -INFINITY;
-  for (int w = 0; w < kAttnWaves; ++w) top = part[w][256] > top || part[w][256] != part[w][256] ? part[w][256] : top;
-  const float vs = g.v_scale ? g.v_scale[kv] : 1.0f;
-  for (int d = threadIdx.x; d < hd; d += 64 * kAttnWaves) {
-    float sum = 0.0f, acc = 0.0f;
-    for (int w = 0; w < kAttnWaves; ++w) {
-      const float f = part[w][256] == -INFINITY ? 0.0f : expf(part[w][256] - top);
-      sum += part[w][257] * f;
-      acc += part[w][d] * f;
-    }
-    float r = top == -INFINITY ? 0.0f : acc / sum * vs;
-    if (bad_s) r = NAN;
-    a.out[(size_t)t * a.ldo + (size_t)head * hd + d] = r;
-  }
-}
-
 // Runs f with the cache's type.
 template <class F>
 void with_type(int dtype, F f) {
@@ -433,8 +348,8 @@ moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* g) {
 }
 
 size_t moe_paged_attn_work_bytes(int T, int n_q, int n_kv, int head_dim) {
-  if (T < 0 || n_q < 1 || n_kv < 1 || head_dim < 1) return 0;
-  return 16;
+  if (T < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv || head_dim < 1) return 0;
+  return paged_attn_work(T, n_q, n_kv, head_dim);
 }
 
 moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* g) {
@@ -458,12 +373,8 @@ moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* g) {
   if ((st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
-  const AttnPages p{*a, map, g->k, g->v, g->k_scale, g->v_scale};
-  with_type(g->dtype, [&](auto c) {
-    hipLaunchKernelGGL(paged_attn_kernel<decltype(c)>, dim3((unsigned)a->T, (unsigned)a->n_q), dim3(64 * kAttnWaves), 0,
-                       stream(), p);
-  });
-  return check_hip(hipGetLastError(), "paged_attn launch");
+  return check_hip(launch_paged_attn(AttnPages{*a, map, g->k, g->v, g->k_scale, g->v_scale}, g->dtype, stream()),
+                   "paged_attn launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,24 @@
+// paged_attn.h - launcher of the attention over a paged cache
+// (paged_attn.hip).  Internal; the public ABI is include/moehip.h.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "moe_lib.h"
+#include "paged.h"
+
+namespace moe {
+
+struct AttnPages {
+  moe_paged_attn a;
+  PageMap map;
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+};
+
+// Bytes of moe_paged_attn::work.
+size_t paged_attn_work(int T, int n_q, int n_kv, int head_dim);
+hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t stream);
+
+}  // namespace moe

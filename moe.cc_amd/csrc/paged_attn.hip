@@ -1,0 +1,638 @@
+// paged_attn.hip - attention of new tokens over a paged cache
+// (moe_paged_attn_dev, include/moehip.h).
+//
+// For a row (token) and one key-value head, with its G = n_q / n_kv query
+// heads q_h and the row's positions j:
+//   s_hj = scale q_h . k_j,  out_h = sum_j exp(s_hj - m_h) v_j / sum_j exp(s_hj - m_h)
+// in one pass over the pages with a running maximum m_h.  The bytes of K and V
+// bound it (4 G operations a cached element), so a K or V byte is loaded once,
+// 16 bytes a lane, straight into the registers that the matrix instructions
+// read, with no LDS and no barrier in the loop:
+//   scores   16 keys x 16 heads a tile: lane l holds 16-byte pieces of key l % 16, and the matching query values of
+//            head l % 16; any order of the dimensions will do as long as both sides share it
+//   weights  come out as keys 4 (l / 16) + i of head l % 16, and go back in as the second operand from the same lane:
+//            the instruction's sum runs over the keys in that order
+//   values   lane l holds the keys 4 (l / 16) + i of both tiles at its 1 / 16 of the dimensions; pairs of keys are put
+//            side by side by byte permutes; the sums come out as 16 dimensions x 16 heads, so a lane rescales its own head
+// Rounding: the products run on 16-bit operands with fp32 sums.  Keys and values enter as they are stored (8-bit ones are
+// exact in bf16); the fp32 queries and weights are split into three 16-bit parts that hold all their bits, so that
+// nothing is lost against an fp32 evaluation.  The matrix work this triples is a tenth of what the bytes' time allows.
+// fp32 pages use the fp32 instruction (16 x 16 x 4) on the same layouts.
+//
+// Work is split over the length too.  Every block finds its item in the rows' lengths by itself (paged_item): rows are
+// cut into chunks of one size, chosen so that the chunks of all rows come to about kBlocks blocks; parts of a cut row go
+// to `work` and are joined by a second kernel, launched only if the tables are long enough for a cut.
+#include <math.h>
+
+#include "moe_device.h"
+#include "paged_attn.h"
+
+namespace moe {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kBlocks = 1024;      // blocks that the chunks of all rows come to
+constexpr int kUnit = 128;         // chunks are multiples of this many positions
+constexpr int kSplitRows = 2048;   // more rows than this are not cut
+
+enum { F32 = MOE_PAGE_F32, F16 = MOE_PAGE_F16, BF16 = MOE_PAGE_BF16, E4M3 = MOE_PAGE_E4M3 };
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// ---------------------------------------------------------------- the items
+
+struct AttnLaunch {
+  AttnPages g;
+  int head_tiles;   // of 16 query heads, a key-value head
+  int chunks;       // chunks of all rows at most, besides one a row; 0: rows are not cut
+  int2* rows;       // [T] work: parts and first part of each row
+  float* part_ml;   // [parts][n_q][2] work: maximum and sum
+  float* part_o;    // [parts][n_q][head_dim] work
+};
+
+struct Item {
+  int row, first, end;   // positions first .. end - 1
+  int parts, part;       // of the row; part: this one's place in `work`
+  int bad;               // request or position outside the tables
+};
+
+// Positions that a row attends; -1: no row.  A row outside the tables has none.
+__device__ int row_length(const AttnPages& g, int t, int* bad) {
+  const moe_paged_attn& a = g.a;
+  const int r = a.req ? a.req[t] : t, p = a.pos[t];
+  if (r < 0) return -1;
+  *bad = r >= a.n_req || p >= a.max_pages * g.map.page_size;
+  return *bad || p < 0 ? 0 : p + 1;
+}
+
+// The block's item.  The chunk is a multiple of kUnit no smaller than total / chunks, so that the rows have no more than
+// T + chunks items, and the cut ones no more than 2 chunks parts (a cut row is longer than a chunk).
+__device__ bool paged_item(const AttnLaunch& L, int b, Item* out) {
+  const AttnPages& g = L.g;
+  const int T = g.a.T;
+  if (!L.chunks) {
+    if (b >= T) return false;
+    int bad = 0;
+    const int n = row_length(g, b, &bad);
+    *out = Item{b, 0, max(n, 0), 1, 0, bad};
+    return n >= 0;
+  }
+  constexpr int kPer = kSplitRows / kThreads;
+  __shared__ unsigned long long sum_s[kWaves];
+  __shared__ uint32_t scan_s[kWaves];
+  __shared__ Item item_s;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int per = (T + kThreads - 1) / kThreads, t0 = tid * per;
+  int len[kPer];
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    int bad = 0;
+    len[i] = i < per && t0 + i < T ? row_length(g, t0 + i, &bad) : -2;
+    sum += (unsigned long long)max(len[i], 0);
+  }
+#pragma unroll
+  for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+  if (lane == 0) sum_s[wave] = sum;
+  if (tid == 0) item_s.row = -1;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sum += sum_s[w];
+  // rounded up past every rounding of the division
+  const float units = (float)sum / ((float)L.chunks * kUnit);
+  const uint32_t chunk = kUnit * ((uint32_t)fminf(units * 1.000002f, 16777214.0f) + 1);
+  uint32_t mine = 0;   // items, and parts of cut rows in the upper half
+  int n[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    n[i] = len[i] == -2 ? 0 : len[i] <= 0 ? 1 : (int)(((uint32_t)len[i] + chunk - 1) / chunk);
+    mine += (uint32_t)n[i] + (n[i] > 1 ? (uint32_t)n[i] << 16 : 0);
+  }
+  uint32_t scan = mine;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const uint32_t x = __shfl_up(scan, d);
+    if (lane >= d) scan += x;
+  }
+  if (lane == kWave - 1) scan_s[wave] = scan;
+  __syncthreads();
+  uint32_t at = scan - mine;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    if (w < wave) at += scan_s[w];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int i0 = (int)(at & 0xffff), part0 = (int)(at >> 16);
+    if (b >= i0 && b < i0 + n[i]) {
+      int bad = 0, first = 0, end = max(row_length(g, t0 + i, &bad), 0);
+      if (n[i] > 1) {   // even chunks; the last is never empty, as they are no longer than `chunk`
+        const int even = (int)(((uint32_t)(end + n[i] - 1) / (uint32_t)n[i] + kUnit - 1) / kUnit * kUnit);
+        first = (b - i0) * even;
+        end = min(end, first + even);
+      }
+      item_s = Item{len[i] < 0 ? -1 : t0 + i, first, end, n[i], part0 + b - i0, bad};
+      if (b == i0 && blockIdx.y == 0) L.rows[t0 + i] = make_int2(len[i] < 0 ? 0 : n[i], part0);
+    }
+    at += (uint32_t)n[i] + (n[i] > 1 ? (uint32_t)n[i] << 16 : 0);
+  }
+  __syncthreads();
+  *out = item_s;
+  return out->row >= 0;
+}
+
+// ---------------------------------------------------------------- pieces
+
+// max over the four lanes of a head (l, l ^ 16, l ^ 32, l ^ 48)
+__device__ __forceinline__ float head_max(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float head_sum(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Two fp32 values into the same place of three operands whose sum they are: bf16 parts by truncation (8 + 8 + 8 bits),
+// f16 parts by the hardware's conversion toward zero (11 bits each).
+template <bool HALF>
+__device__ __forceinline__ void split2(float x, float y, uint32_t* a, uint32_t* b, uint32_t* c) {
+  if constexpr (HALF) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+    const float x1 = x - (float)h[0], y1 = y - (float)h[1];
+    const auto m = __builtin_amdgcn_cvt_pkrtz(x1, y1);
+    const auto l = __builtin_amdgcn_cvt_pkrtz(x1 - (float)m[0], y1 - (float)m[1]);
+    *a = __builtin_bit_cast(uint32_t, h);
+    *b = __builtin_bit_cast(uint32_t, m);
+    *c = __builtin_bit_cast(uint32_t, l);
+  } else {
+    const uint32_t xh = __float_as_uint(x), yh = __float_as_uint(y);
+    const float x1 = x - __uint_as_float(xh & 0xffff0000u), y1 = y - __uint_as_float(yh & 0xffff0000u);
+    const uint32_t xm = __float_as_uint(x1), ym = __float_as_uint(y1);
+    const float x2 = x1 - __uint_as_float(xm & 0xffff0000u), y2 = y1 - __uint_as_float(ym & 0xffff0000u);
+    *a = __builtin_amdgcn_perm(yh, xh, 0x07060302u);
+    *b = __builtin_amdgcn_perm(ym, xm, 0x07060302u);
+    *c = __builtin_amdgcn_perm(__float_as_uint(y2), __float_as_uint(x2), 0x07060302u);
+  }
+}
+
+template <bool HALF>
+__device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (HALF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// four 8-bit values -> two dwords of bf16 pairs (exact)
+__device__ __forceinline__ u32x2 widen(uint32_t x) {
+  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true))};
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_piece(const char* p, uint32_t* r) {
+  if constexpr (BYTES == 16) {
+    const u32x4 x = *(const u32x4*)p;
+    r[0] = x[0], r[1] = x[1], r[2] = x[2], r[3] = x[3];
+  } else if constexpr (BYTES == 8) {
+    const u32x2 x = *(const u32x2*)p;
+    r[0] = x[0], r[1] = x[1];
+  } else {
+    r[0] = *(const uint32_t*)p;
+  }
+}
+
+// ---------------------------------------------------------------- the kernel
+
+// CT: the pages' type.  HDP: head_dim, or the next of 64, 128, 256 (the pieces past head_dim repeat its last one against
+// zero queries, and their sums are not stored).  WHOLE: a tile of 16 positions lies in one page (page_size % 16 == 0), so
+// its address is one scalar lookup; otherwise each lane looks up one position and the lanes exchange addresses.
+template <int CT, int HDP, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
+  constexpr bool HALF = CT == F16;
+  constexpr int S = CT == F32 ? 4 : CT == E4M3 ? 1 : 2;
+  constexpr int E = 16 / S;                        // elements of a 16-byte piece
+  constexpr int NK = HDP / E / 4;                  // a lane's pieces of a key
+  constexpr int VE = HDP / 16;                     // a lane's dimensions of a value
+  constexpr int EV = VE < E ? VE : E, NV = VE / EV, VW = EV * S / 4;   // its pieces: elements, number, dwords
+  constexpr int KT = CT == F32 && HDP == 256 ? 1 : 2;                  // tiles of 16 positions a step
+  constexpr int NQ = CT == F32 ? 1 : HDP / 32;     // query operands of 8 values
+  constexpr int STEP = 16 * KT;
+  // weights are held times 2^14 where their parts are f16, far from its smallest numbers
+  constexpr float kLift = HALF ? 14.0f : 0.0f;
+
+  Item it;
+  if (!paged_item(L, (int)blockIdx.x, &it)) return;
+  const AttnPages& g = L.g;
+  const moe_paged_attn& a = g.a;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int col = lane % 16, quad = lane / 16, hd = g.map.head_dim;
+  const int G = a.n_q / g.map.n_kv, kv = (int)blockIdx.y / L.head_tiles, tile = (int)blockIdx.y % L.head_tiles;
+  const int head0 = kv * G + tile * 16, heads = min(16, G - tile * 16);   // this block's query heads
+
+  // ---- queries, times scale and log2(e): scores are powers of two
+  const float scale = a.scale * (g.k_scale ? g.k_scale[kv] : 1.0f) * 1.44269504088896340736f;
+  const float* q = a.q + (size_t)it.row * a.ldq + (size_t)(head0 + (col < heads ? col : 0)) * hd;
+  u32x4 qa[NQ], qb[NQ], qc[NQ];
+  f32x4 qf[CT == F32 ? NK : 1];
+  float unlift = 1.0f;
+  if constexpr (CT == F32) {
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      const int d = (4 * j + quad) * 4;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) qf[j][c] = d < hd && col < heads ? q[d + c] * scale : 0.0f;
+    }
+  } else {
+    float x[NQ][8];
+    float big = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NQ; ++s) {
+      const int d = CT == E4M3 ? (4 * (s / 2) + quad) * 16 + 8 * (s % 2) : (4 * s + quad) * 8;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        x[s][c] = d < hd && col < heads ? q[d + c] * scale : 0.0f;
+        big = fmaxf(big, fabsf(x[s][c]));
+      }
+    }
+    float lift = 1.0f;
+    if constexpr (HALF) {   // the head's largest value to 2^14 .. 2^15, so that f16 parts hold the others against it
+      big = head_max(big);
+      if (big > 0.0f && big < INFINITY) {
+        const int e = max((int)(__float_as_uint(big) >> 23) - 127, -100);
+        lift = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+        unlift = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < NQ; ++s)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t u, v, w;
+        split2<HALF>(x[s][2 * c] * lift, x[s][2 * c + 1] * lift, &u, &v, &w);
+        qa[s][c] = u, qb[s][c] = v, qc[s][c] = w;
+      }
+  }
+
+  // ---- addresses
+  const int* table = a.tables + (size_t)(it.bad ? 0 : a.req ? a.req[it.row] : it.row) * a.max_pages;
+  const long long head_at = (long long)kv * g.map.head_stride;
+  const char* kbase = (const char*)g.k + head_at * S;
+  const char* vbase = (const char*)g.v + head_at * S;
+  const int last_piece = hd * S - 16;                    // of a key's row, bytes
+  const int last_value = hd * S - EV * S;
+  const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: 16 of them fit 31 bits
+  int bad = it.bad;
+
+  const int end = it.end;
+  auto base_of = [&](int step) { return it.first + (step * kWaves + wave) * STEP; };
+  // page numbers of a step: WHOLE: of its tiles; else of the lane's position
+  struct Look { int p[WHOLE ? KT : 1]; };
+  auto look = [&](int step) {
+    Look r;
+    const int base = base_of(step);
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const int tb = min(base + 16 * t, (end - 1) & ~15);   // a tile past the end repeats the last one
+        r.p[t] = table[divide((uint32_t)tb, g.map.per)];
+      }
+    } else {
+      r.p[0] = table[divide((uint32_t)min(base + lane, end - 1), g.map.per)];
+    }
+    return r;
+  };
+  // row offsets (bytes) of a step's positions; positions past the end take the last one's, whose numbers are the row's own
+  struct At { long long tile[WHOLE ? KT : 1]; int lim[WHOLE ? KT : 1]; };
+  auto place = [&](int step, const Look& r) {
+    At o;
+    const int base = base_of(step);
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const int tb = min(base + 16 * t, (end - 1) & ~15);
+        int pg = r.p[t];
+        if (!page_ok(g.map, pg)) bad = 1, pg = 0;
+        const int off = tb - (int)divide((uint32_t)tb, g.map.per) * g.map.page_size;
+        o.tile[t] = ((long long)pg * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
+        o.lim[t] = min(end - 1 - tb, 15);
+      }
+    } else {
+      const int p = min(base + lane, end - 1);
+      int pg = r.p[0];
+      if (!page_ok(g.map, pg)) bad = 1, pg = 0;
+      const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
+      o.tile[0] = ((long long)pg * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
+      o.lim[0] = 15;
+    }
+    return o;
+  };
+  auto row_at = [&](const At& o, int t, int key) -> long long {   // of key `key` of tile t
+    if constexpr (WHOLE) return o.tile[t] + (uint32_t)min(key, o.lim[t]) * slot_bytes;
+    else return __shfl(o.tile[0], 16 * t + key);
+  };
+
+  uint32_t kr[KT][NK][4], vr[4 * KT][NV][VW];
+  auto load_k = [&](const At& o) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const char* p = kbase + row_at(o, t, col);
+#pragma unroll
+      for (int j = 0; j < NK; ++j) load_piece<16>(p + min((4 * j + quad) * 16, last_piece), kr[t][j]);
+    }
+  };
+  auto load_v = [&](const At& o) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const char* p = vbase + row_at(o, t, 4 * quad + i);
+#pragma unroll
+        for (int h = 0; h < NV; ++h) load_piece<EV * S>(p + min((16 * h + col) * EV * S, last_value), vr[4 * t + i][h]);
+      }
+  };
+
+  f32x4 o[VE];
+#pragma unroll
+  for (int c = 0; c < VE; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;
+
+  if (base_of(0) < end) {
+    At at = place(0, look(0));
+    load_k(at);
+    load_v(at);
+    Look next{};
+    if (base_of(1) < end) next = look(1);
+    for (int step = 0;; ++step) {
+      const int base = base_of(step);
+      const bool more = base_of(step + 1) < end;
+      // ---- scores
+      f32x4 s[KT];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          if constexpr (CT == F32) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][j][c]), qf[j][c], s[t], 0, 0, 0);
+          } else if constexpr (CT == E4M3) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const u32x2 x = widen(kr[t][j][2 * u]), y = widen(kr[t][j][2 * u + 1]);
+              const u32x4 k = {x[0], x[1], y[0], y[1]};
+              s[t] = mfma32<HALF>(k, qa[2 * j + u], s[t]);
+              s[t] = mfma32<HALF>(k, qb[2 * j + u], s[t]);
+              s[t] = mfma32<HALF>(k, qc[2 * j + u], s[t]);
+            }
+          } else {
+            const u32x4 k = {kr[t][j][0], kr[t][j][1], kr[t][j][2], kr[t][j][3]};
+            s[t] = mfma32<HALF>(k, qa[j], s[t]);
+            s[t] = mfma32<HALF>(k, qb[j], s[t]);
+            s[t] = mfma32<HALF>(k, qc[j], s[t]);
+          }
+        }
+      if (more) {
+        at = place(step + 1, next);
+        load_k(at);
+        if (base_of(step + 2) < end) next = look(step + 2);
+      }
+      // ---- weights
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (HALF) s[t][i] *= unlift;
+          if (base + STEP > end && base + 16 * t + 4 * quad + i >= end) s[t][i] = -INFINITY;
+          top = fmaxf(top, s[t][i]);
+        }
+      top = fmaxf(m, head_max(top));
+      if (__any(top > m)) {
+        const float keep = top == -INFINITY ? 1.0f : exp2_hw(m - top);
+        l *= keep;
+#pragma unroll
+        for (int c = 0; c < VE; ++c) o[c] *= keep;
+        m = top;
+      }
+      const float from = (m == -INFINITY ? 0.0f : m) - kLift;
+      float p[KT][4];
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[t][i] = exp2_hw(s[t][i] - from);
+          l += p[t][i];
+        }
+      // ---- values
+      if constexpr (CT == F32) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < VE; ++c)
+              o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * t + i][c / EV][c % EV]), p[t][i], o[c], 0, 0, 0);
+      } else {
+        u32x4 pa, pb, pc;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t u, v, w;
+          split2<HALF>(p[c / 2][2 * (c % 2)], p[c / 2][2 * (c % 2) + 1], &u, &v, &w);
+          pa[c] = u, pb[c] = v, pc[c] = w;
+        }
+#pragma unroll
+        for (int h = 0; h < NV; ++h) {
+          constexpr int W16 = EV / 2;   // dwords of 16-bit pairs of a piece
+          uint32_t w16[8][W16];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int d = 0; d < VW; ++d) {
+              if constexpr (CT == E4M3) {
+                const u32x2 x = widen(vr[k][h][d]);
+                w16[k][2 * d] = x[0], w16[k][2 * d + 1] = x[1];
+              } else {
+                w16[k][d] = vr[k][h][d];
+              }
+            }
+#pragma unroll
+          for (int e = 0; e < EV; ++e) {
+            u32x4 x;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              x[c] = __builtin_amdgcn_perm(w16[2 * c + 1][e / 2], w16[2 * c][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+            o[h * EV + e] = mfma32<HALF>(x, pa, o[h * EV + e]);
+            o[h * EV + e] = mfma32<HALF>(x, pb, o[h * EV + e]);
+            o[h * EV + e] = mfma32<HALF>(x, pc, o[h * EV + e]);
+          }
+        }
+      }
+      if (!more) break;
+      load_v(at);
+    }
+  }
+  l = head_sum(l);
+  if (__any(bad)) l = NAN;
+
+  // ---- the waves' sums joined, 128 dimensions at a time
+  constexpr int PASS = HDP > 128 ? 2 : 1, VP = VE / PASS;
+  __shared__ float o_s[kWaves][16 * VP][17], m_s[kWaves][16], l_s[kWaves][16];
+  if (quad == 0) m_s[wave][col] = m, l_s[wave][col] = l;
+  __syncthreads();
+  float top = m_s[0][col];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_s[w][col]);
+  const float from = top == -INFINITY ? 0.0f : top;
+  const float mine = exp2_hw(m - from);
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sum += l_s[w][col] * exp2_hw(m_s[w][col] - from);
+  const bool cut = it.parts > 1;
+  // what a sum is multiplied by: 1 / l and the values' scale, or nothing in a part
+  const float vs = g.v_scale ? g.v_scale[kv] : 1.0f;
+  __shared__ float div_s[16];
+  if (wave == 0 && quad == 0) {
+    div_s[col] = sum;
+    if (cut && col < heads) {
+      float* ml = L.part_ml + ((size_t)it.part * a.n_q + head0 + col) * 2;
+      ml[0] = top;
+      ml[1] = sum;
+    }
+  }
+#pragma unroll
+  for (int ps = 0; ps < PASS; ++ps) {
+#pragma unroll
+    for (int c = 0; c < VP; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o_s[wave][(4 * quad + i) * VP + c][col] = o[ps * VP + c][i] * mine;
+    __syncthreads();
+    for (int x = threadIdx.x; x < heads * 16 * VP; x += kThreads) {
+      const int h = x / (16 * VP), at = x % (16 * VP), c = ps * VP + at % VP;
+      const int d = c / EV * 16 * EV + at / VP * EV + c % EV;
+      if (d >= hd) continue;
+      float y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) y += o_s[w][at][h];
+      if (cut) {
+        L.part_o[((size_t)it.part * a.n_q + head0 + h) * hd + d] = y;
+      } else {
+        const float z = div_s[h];
+        a.out[(size_t)it.row * a.ldo + (size_t)(head0 + h) * hd + d] = z == 0.0f ? 0.0f : y / z * vs;
+      }
+    }
+    if (ps + 1 < PASS) __syncthreads();
+  }
+}
+
+// A block a (row, query head): the parts of a cut row joined.
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
+  const AttnPages& g = L.g;
+  const moe_paged_attn& a = g.a;
+  const int t = (int)blockIdx.x, head = (int)blockIdx.y, hd = g.map.head_dim;
+  const int2 r = L.rows[t];
+  if (r.x <= 1) return;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  __shared__ float acc_s[kWaves][256], red_s[kWaves], sum_s[kWaves];
+  const float* ml = L.part_ml + ((size_t)r.y * a.n_q + head) * 2;
+  const size_t step = (size_t)a.n_q * 2;
+  float top = -INFINITY;
+  for (int i = tid; i < r.x; i += kThreads) top = fmaxf(top, ml[i * step]);
+  for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) red_s[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red_s[0], red_s[1]), fmaxf(red_s[2], red_s[3]));
+  if (top == -INFINITY) top = 0.0f;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+  for (int i = wave; i < r.x; i += kWaves) {
+    const float f = exp2_hw(ml[i * step] - top);
+    sum += ml[i * step + 1] * f;
+    const float* o = L.part_o + ((size_t)(r.y + i) * a.n_q + head) * hd;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane + 64 * c < hd) acc[c] += o[lane + 64 * c] * f;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) acc_s[wave][lane + 64 * c] = acc[c];
+  if (lane == 0) sum_s[wave] = sum;
+  __syncthreads();
+  const float all = sum_s[0] + sum_s[1] + sum_s[2] + sum_s[3];
+  const float vs = g.v_scale ? g.v_scale[head / (a.n_q / g.map.n_kv)] : 1.0f;
+  for (int d = tid; d < hd; d += kThreads) {
+    const float y = acc_s[0][d] + acc_s[1][d] + acc_s[2][d] + acc_s[3][d];
+    a.out[(size_t)t * a.ldo + (size_t)head * hd + d] = all == 0.0f ? 0.0f : y / all * vs;
+  }
+}
+
+// Chunks besides one a row; 0: rows are not cut.
+int chunks_for(int T, int n_q, int n_kv) {
+  if (T > kSplitRows) return 0;
+  const int tiles = (n_q / n_kv + 15) / 16;
+  return kBlocks / (n_kv * tiles) > 0 ? kBlocks / (n_kv * tiles) : 1;
+}
+
+template <int CT, int HDP>
+hipError_t launch(const AttnLaunch& L, bool whole, dim3 grid, hipStream_t s) {
+  if (whole) hipLaunchKernelGGL((paged_attn_kernel<CT, HDP, true>), grid, dim3(kThreads), 0, s, L);
+  else hipLaunchKernelGGL((paged_attn_kernel<CT, HDP, false>), grid, dim3(kThreads), 0, s, L);
+  return hipGetLastError();
+}
+
+template <int CT>
+hipError_t launch(const AttnLaunch& L, bool whole, dim3 grid, hipStream_t s) {
+  const int hd = L.g.map.head_dim;
+  return hd <= 64 ? launch<CT, 64>(L, whole, grid, s) : hd <= 128 ? launch<CT, 128>(L, whole, grid, s)
+                                                                  : launch<CT, 256>(L, whole, grid, s);
+}
+
+}  // namespace
+
+size_t paged_attn_work(int T, int n_q, int n_kv, int head_dim) {
+  const size_t parts = 2 * (size_t)chunks_for(T, n_q, n_kv);
+  return ((size_t)T * sizeof(int2) + 15) / 16 * 16 + parts * n_q * (2 + (size_t)head_dim) * 4 + 16;
+}
+
+hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
+  const moe_paged_attn& a = p.a;
+  const PageMap& map = p.map;
+  AttnLaunch L;
+  L.g = p;
+  L.head_tiles = (a.n_q / map.n_kv + 15) / 16;
+  // rows that no chunk can cut need neither the search for items nor the join
+  const long long longest = (long long)a.max_pages * map.page_size;
+  int chunks = longest <= kUnit ? 0 : chunks_for(a.T, a.n_q, map.n_kv);
+  L.chunks = chunks;
+  char* w = (char*)a.work;
+  L.rows = (int2*)w;
+  w += ((size_t)a.T * sizeof(int2) + 15) / 16 * 16;
+  const size_t parts = 2 * (size_t)chunks_for(a.T, a.n_q, map.n_kv);
+  L.part_o = (float*)w;
+  L.part_ml = (float*)w + parts * a.n_q * map.head_dim;
+  // no more items than the longest rows' chunks
+  const long long most = (longest + kUnit - 1) / kUnit * a.T;
+  const unsigned items = (unsigned)(a.T + (most < chunks ? most : chunks));
+  const dim3 grid(items, (unsigned)(map.n_kv * L.head_tiles));
+  const bool whole = map.page_size % 16 == 0 && map.slot_stride <= (1 << 24);
+  const hipError_t e = dtype == F32 ? launch<F32>(L, whole, grid, s) : dtype == F16 ? launch<F16>(L, whole, grid, s)
+                       : dtype == BF16 ? launch<BF16>(L, whole, grid, s) : launch<E4M3>(L, whole, grid, s);
+  if (e != hipSuccess || !chunks) return e;
+  hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)a.T, (unsigned)a.n_q), dim3(kThreads), 0, s, L);
+  return hipGetLastError();
+}
+
+}  // namespace moe
