@@ -24,6 +24,8 @@
 // to `work` and are joined by a second kernel, launched only if the tables are long enough for a cut.
 #include <math.h>
 
+#include <type_traits>
+
 #include "moe_device.h"
 #include "paged_attn.h"
 
@@ -38,6 +40,7 @@ constexpr int kSplitRows = 2048;   // more rows than this are not cut
 enum { F32 = MOE_PAGE_F32, F16 = MOE_PAGE_F16, BF16 = MOE_PAGE_BF16, E4M3 = MOE_PAGE_E4M3 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // queries may start at any float
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -45,105 +48,143 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+// Memory that no one writes while the kernel runs, read at an address all lanes share: through the scalar cache, apart
+// from the vector loads in flight.
+template <class T>
+__device__ __forceinline__ T scalar_load(const T* p, long long i) {
+  return ((const __attribute__((address_space(4))) T*)(uintptr_t)p)[i];
+}
+
 // ---------------------------------------------------------------- the items
 
 struct AttnLaunch {
   AttnPages g;
   int head_tiles;   // of 16 query heads, a key-value head
   int chunks;       // chunks of all rows at most, besides one a row; 0: rows are not cut
+  float per_unit;   // 1 / (chunks kUnit), raised
   int2* rows;       // [T] work: parts and first part of each row
   float* part_ml;   // [parts][n_q][2] work: maximum and sum
   float* part_o;    // [parts][n_q][head_dim] work
 };
 
 struct Item {
-  int row, first, end;   // positions first .. end - 1
-  int parts, part;       // of the row; part: this one's place in `work`
-  int bad;               // request or position outside the tables
+  int row, req;          // req: its request, -1: outside the tables
+  int first, end;        // positions first .. end - 1
+  int parts, part;       // parts of the row, this one's place in `work`
 };
 
-// Positions that a row attends; -1: no row.  A row outside the tables has none.
-__device__ int row_length(const AttnPages& g, int t, int* bad) {
-  const moe_paged_attn& a = g.a;
-  const int r = a.req ? a.req[t] : t, p = a.pos[t];
-  if (r < 0) return -1;
-  *bad = r >= a.n_req || p >= a.max_pages * g.map.page_size;
-  return *bad || p < 0 ? 0 : p + 1;
+// Positions that a row attends; kPadding: no row; kOutside: a request or position outside the tables.
+constexpr int kPadding = -1, kOutside = -2, kNone = -3;
+__device__ __forceinline__ int length_of(const AttnPages& g, int req, int pos) {
+  return req < 0 ? kPadding : req >= g.a.n_req || pos >= g.a.max_pages * g.map.page_size ? kOutside : max(pos + 1, 0);
 }
 
-// The block's item.  The chunk is a multiple of kUnit no smaller than total / chunks, so that the rows have no more than
-// T + chunks items, and the cut ones no more than 2 chunks parts (a cut row is longer than a chunk).
-__device__ bool paged_item(const AttnLaunch& L, int b, Item* out) {
+// Sums over the lanes up to each one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+__device__ __forceinline__ float wave_total(float x) {
+  auto step = [&](auto ctrl, auto mask) {
+    x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, decltype(mask)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+
+struct ItemShared {
+  float sum[kWaves];
+  uint32_t scan[kWaves];
+  Item item;
+};
+
+// The block's item among cut rows; PER rows a thread.  The chunk is a multiple of kUnit no smaller than total / chunks
+// (the total in fp32, raised past every rounding of it), so that the rows have no more than T + chunks items, and the cut
+// ones no more than 2 chunks parts (a cut row is longer than a chunk).
+template <int PER>
+__device__ __forceinline__ void find_item(const AttnLaunch& L, int b, ItemShared& sh) {
   const AttnPages& g = L.g;
-  const int T = g.a.T;
-  if (!L.chunks) {
-    if (b >= T) return false;
-    int bad = 0;
-    const int n = row_length(g, b, &bad);
-    *out = Item{b, 0, max(n, 0), 1, 0, bad};
-    return n >= 0;
-  }
-  constexpr int kPer = kSplitRows / kThreads;
-  __shared__ unsigned long long sum_s[kWaves];
-  __shared__ uint32_t scan_s[kWaves];
-  __shared__ Item item_s;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int per = (T + kThreads - 1) / kThreads, t0 = tid * per;
-  int len[kPer];
-  unsigned long long sum = 0;
+  const int T = g.a.T, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int per = PER == 1 ? 1 : (T + kThreads - 1) / kThreads, t0 = tid * per;
+  int len[PER], req[PER];
+  float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    int bad = 0;
-    len[i] = i < per && t0 + i < T ? row_length(g, t0 + i, &bad) : -2;
-    sum += (unsigned long long)max(len[i], 0);
+  for (int i = 0; i < PER; ++i) {
+    const int t = min(t0 + i, T - 1);
+    req[i] = g.a.req ? g.a.req[t] : t;
+    len[i] = g.a.pos[t];
   }
 #pragma unroll
-  for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-  if (lane == 0) sum_s[wave] = sum;
-  if (tid == 0) item_s.row = -1;
+  for (int i = 0; i < PER; ++i) {
+    len[i] = i < per && t0 + i < T ? length_of(g, req[i], len[i]) : kNone;
+    sum += (float)max(len[i], 0);
+  }
+  sum = wave_total(sum);
+  if (lane == 0) sh.sum[wave] = sum;
+  if (tid == 0) sh.item.row = -1;
   __syncthreads();
-  sum = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) sum += sum_s[w];
-  // rounded up past every rounding of the division
-  const float units = (float)sum / ((float)L.chunks * kUnit);
-  const uint32_t chunk = kUnit * ((uint32_t)fminf(units * 1.000002f, 16777214.0f) + 1);
+  sum = (sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]);
+  const uint32_t units = (uint32_t)fminf(sum * L.per_unit, 16777214.0f) + 1, chunk = kUnit * units;
   uint32_t mine = 0;   // items, and parts of cut rows in the upper half
-  int n[kPer];
+  int n[PER];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    n[i] = len[i] == -2 ? 0 : len[i] <= 0 ? 1 : (int)(((uint32_t)len[i] + chunk - 1) / chunk);
+  for (int i = 0; i < PER; ++i) {
+    n[i] = len[i] == kNone ? 0 : len[i] <= 0 ? 1 : (int)(((uint32_t)len[i] + chunk - 1) / chunk);
     mine += (uint32_t)n[i] + (n[i] > 1 ? (uint32_t)n[i] << 16 : 0);
   }
-  uint32_t scan = mine;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint32_t x = __shfl_up(scan, d);
-    if (lane >= d) scan += x;
-  }
-  if (lane == kWave - 1) scan_s[wave] = scan;
+  const uint32_t scan = wave_scan(mine);
+  if (lane == kWave - 1) sh.scan[wave] = scan;
   __syncthreads();
   uint32_t at = scan - mine;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    if (w < wave) at += scan_s[w];
+  for (int w = 0; w < kWaves - 1; ++w)
+    if (w < wave) at += sh.scan[w];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int i0 = (int)(at & 0xffff), part0 = (int)(at >> 16);
     if (b >= i0 && b < i0 + n[i]) {
-      int bad = 0, first = 0, end = max(row_length(g, t0 + i, &bad), 0);
+      int first = 0, end = max(len[i], 0);
       if (n[i] > 1) {   // even chunks; the last is never empty, as they are no longer than `chunk`
         const int even = (int)(((uint32_t)(end + n[i] - 1) / (uint32_t)n[i] + kUnit - 1) / kUnit * kUnit);
         first = (b - i0) * even;
         end = min(end, first + even);
       }
-      item_s = Item{len[i] < 0 ? -1 : t0 + i, first, end, n[i], part0 + b - i0, bad};
-      if (b == i0 && blockIdx.y == 0) L.rows[t0 + i] = make_int2(len[i] < 0 ? 0 : n[i], part0);
+      sh.item = Item{len[i] == kPadding ? -1 : t0 + i, len[i] == kOutside ? -1 : req[i], first, end, n[i], part0 + b - i0};
+      if (b == i0 && blockIdx.y == 0) L.rows[t0 + i] = make_int2(len[i] == kPadding ? 0 : n[i], part0);
     }
     at += (uint32_t)n[i] + (n[i] > 1 ? (uint32_t)n[i] << 16 : 0);
   }
   __syncthreads();
-  *out = item_s;
+}
+
+// The block's item, in scalar registers; false: it has none.
+__device__ __forceinline__ bool paged_item(const AttnLaunch& L, int b, Item* out) {
+  const AttnPages& g = L.g;
+  const int T = g.a.T;
+  if (!L.chunks) {
+    if (b >= T) return false;
+    const moe_paged_attn& a = g.a;
+    const int req = a.req ? scalar_load(a.req, b) : b;
+    const int n = length_of(g, req, scalar_load(a.pos, b));
+    *out = Item{b, n == kOutside ? -1 : req, 0, max(n, 0), 1, 0};
+    return n != kPadding;
+  }
+  __shared__ ItemShared sh;
+  if (T <= kThreads) find_item<1>(L, b, sh);
+  else find_item<kSplitRows / kThreads>(L, b, sh);
+  auto get = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  *out = Item{get(sh.item.row), get(sh.item.req), get(sh.item.first), get(sh.item.end), get(sh.item.parts), get(sh.item.part)};
   return out->row >= 0;
 }
 
@@ -221,7 +262,7 @@ __device__ __forceinline__ void load_piece(const char* p, uint32_t* r) {
 // zero queries, and their sums are not stored).  WHOLE: a tile of 16 positions lies in one page (page_size % 16 == 0), so
 // its address is one scalar lookup; otherwise each lane looks up one position and the lanes exchange addresses.
 template <int CT, int HDP, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kernel(AttnLaunch L) {
   constexpr bool HALF = CT == F16;
   constexpr int S = CT == F32 ? 4 : CT == E4M3 ? 1 : 2;
   constexpr int E = 16 / S;                        // elements of a 16-byte piece
@@ -243,59 +284,23 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
   const int G = a.n_q / g.map.n_kv, kv = (int)blockIdx.y / L.head_tiles, tile = (int)blockIdx.y % L.head_tiles;
   const int head0 = kv * G + tile * 16, heads = min(16, G - tile * 16);   // this block's query heads
 
-  // ---- queries, times scale and log2(e): scores are powers of two
-  const float scale = a.scale * (g.k_scale ? g.k_scale[kv] : 1.0f) * 1.44269504088896340736f;
-  const float* q = a.q + (size_t)it.row * a.ldq + (size_t)(head0 + (col < heads ? col : 0)) * hd;
-  u32x4 qa[NQ], qb[NQ], qc[NQ];
-  f32x4 qf[CT == F32 ? NK : 1];
-  float unlift = 1.0f;
-  if constexpr (CT == F32) {
+  // ---- queries: requested first, used after the first keys are requested
+  const float* q = a.q + (size_t)it.row * a.ldq + (size_t)(head0 + min(col, heads - 1)) * hd;
+  f32x4 x[CT == F32 ? NK : 2 * NQ];
+  auto query_dim = [&](int s) {   // of x[s]
+    return CT == F32 ? (4 * s + quad) * 4 : CT == E4M3 ? (4 * (s / 4) + quad) * 16 + 4 * (s % 4) : (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
+  };
+  constexpr int NX = CT == F32 ? NK : 2 * NQ;
 #pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      const int d = (4 * j + quad) * 4;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) qf[j][c] = d < hd && col < heads ? q[d + c] * scale : 0.0f;
-    }
-  } else {
-    float x[NQ][8];
-    float big = 0.0f;
-#pragma unroll
-    for (int s = 0; s < NQ; ++s) {
-      const int d = CT == E4M3 ? (4 * (s / 2) + quad) * 16 + 8 * (s % 2) : (4 * s + quad) * 8;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        x[s][c] = d < hd && col < heads ? q[d + c] * scale : 0.0f;
-        big = fmaxf(big, fabsf(x[s][c]));
-      }
-    }
-    float lift = 1.0f;
-    if constexpr (HALF) {   // the head's largest value to 2^14 .. 2^15, so that f16 parts hold the others against it
-      big = head_max(big);
-      if (big > 0.0f && big < INFINITY) {
-        const int e = max((int)(__float_as_uint(big) >> 23) - 127, -100);
-        lift = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        unlift = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < NQ; ++s)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t u, v, w;
-        split2<HALF>(x[s][2 * c] * lift, x[s][2 * c + 1] * lift, &u, &v, &w);
-        qa[s][c] = u, qb[s][c] = v, qc[s][c] = w;
-      }
-  }
+  for (int s = 0; s < NX; ++s) x[s] = *(const f32x4u*)(q + min(query_dim(s), hd - 4));
 
   // ---- addresses
-  const int* table = a.tables + (size_t)(it.bad ? 0 : a.req ? a.req[it.row] : it.row) * a.max_pages;
+  const int* table = a.tables + (size_t)max(it.req, 0) * a.max_pages;
   const long long head_at = (long long)kv * g.map.head_stride;
   const char* kbase = (const char*)g.k + head_at * S;
   const char* vbase = (const char*)g.v + head_at * S;
-  const int last_piece = hd * S - 16;                    // of a key's row, bytes
-  const int last_value = hd * S - EV * S;
-  const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: 16 of them fit 31 bits
-  int bad = it.bad;
+  const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: below 2^24
+  int bad = it.req < 0;
 
   const int end = it.end;
   auto base_of = [&](int step) { return it.first + (step * kWaves + wave) * STEP; };
@@ -307,15 +312,16 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
     if constexpr (WHOLE) {
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        const int tb = min(base + 16 * t, (end - 1) & ~15);   // a tile past the end repeats the last one
-        r.p[t] = table[divide((uint32_t)tb, g.map.per)];
+        const int tb = min(base + 16 * t, (end - 1) & ~15);   // tiles past the end repeat the last one
+        r.p[t] = scalar_load(table, divide((uint32_t)tb, g.map.per));
       }
     } else {
       r.p[0] = table[divide((uint32_t)min(base + lane, end - 1), g.map.per)];
     }
     return r;
   };
-  // row offsets (bytes) of a step's positions; positions past the end take the last one's, whose numbers are the row's own
+  // byte offsets: WHOLE: of a step's tiles, and the last position of each that counts; else of the lane's position.
+  // Positions past the end take the last one's row, whose numbers are the request's own
   struct At { long long tile[WHOLE ? KT : 1]; int lim[WHOLE ? KT : 1]; };
   auto place = [&](int step, const Look& r) {
     At o;
@@ -340,18 +346,20 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
     }
     return o;
   };
-  auto row_at = [&](const At& o, int t, int key) -> long long {   // of key `key` of tile t
-    if constexpr (WHOLE) return o.tile[t] + (uint32_t)min(key, o.lim[t]) * slot_bytes;
-    else return __shfl(o.tile[0], 16 * t + key);
-  };
-
+  // WHOLE: a scalar base a tile and 32-bit lane offsets; else a 64-bit row address a lane
+  uint32_t kpiece[NK], vpiece[NV];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) kpiece[j] = (uint32_t)min((4 * j + quad) * 16, hd * S - 16);
+#pragma unroll
+  for (int h = 0; h < NV; ++h) vpiece[h] = (uint32_t)min((16 * h + col) * EV * S, hd * S - EV * S);
   uint32_t kr[KT][NK][4], vr[4 * KT][NV][VW];
   auto load_k = [&](const At& o) {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const char* p = kbase + row_at(o, t, col);
+      const char* base = WHOLE ? kbase + o.tile[t] : kbase + __shfl(o.tile[0], 16 * t + col);
+      const uint32_t off = WHOLE ? __umul24((uint32_t)min(col, o.lim[t]), slot_bytes) : 0;
 #pragma unroll
-      for (int j = 0; j < NK; ++j) load_piece<16>(p + min((4 * j + quad) * 16, last_piece), kr[t][j]);
+      for (int j = 0; j < NK; ++j) load_piece<16>(base + (off + kpiece[j]), kr[t][j]);
     }
   };
   auto load_v = [&](const At& o) {
@@ -359,9 +367,10 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const char* p = vbase + row_at(o, t, 4 * quad + i);
+        const char* base = WHOLE ? vbase + o.tile[t] : vbase + __shfl(o.tile[0], 16 * t + 4 * quad + i);
+        const uint32_t off = WHOLE ? __umul24((uint32_t)min(4 * quad + i, o.lim[t]), slot_bytes) : 0;
 #pragma unroll
-        for (int h = 0; h < NV; ++h) load_piece<EV * S>(p + min((16 * h + col) * EV * S, last_value), vr[4 * t + i][h]);
+        for (int h = 0; h < NV; ++h) load_piece<EV * S>(base + (off + vpiece[h]), vr[4 * t + i][h]);
       }
   };
 
@@ -370,122 +379,158 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
   for (int c = 0; c < VE; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
 
+  f32x4 s[KT];
+  u32x4 qa[NQ], qb[NQ], qc[NQ];
+  float unlift = 1.0f;
+  auto score = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        if constexpr (CT == F32) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][j][c]), x[j][c], s[t], 0, 0, 0);
+        } else if constexpr (CT == E4M3) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x2 x = widen(kr[t][j][2 * u]), y = widen(kr[t][j][2 * u + 1]);
+            const u32x4 k = {x[0], x[1], y[0], y[1]};
+            s[t] = mfma32<HALF>(k, qa[2 * j + u], s[t]);
+            s[t] = mfma32<HALF>(k, qb[2 * j + u], s[t]);
+            s[t] = mfma32<HALF>(k, qc[2 * j + u], s[t]);
+          }
+        } else {
+          const u32x4 k = {kr[t][j][0], kr[t][j][1], kr[t][j][2], kr[t][j][3]};
+          s[t] = mfma32<HALF>(k, qa[j], s[t]);
+          s[t] = mfma32<HALF>(k, qb[j], s[t]);
+          s[t] = mfma32<HALF>(k, qc[j], s[t]);
+        }
+      }
+  };
+  // the scores' weights and their sums over the values; base: the step's first position
+  auto gather = [&](int base) __attribute__((always_inline)) {
+    // ---- weights
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (HALF) s[t][i] *= unlift;
+        if (base + STEP > end && base + 16 * t + 4 * quad + i >= end) s[t][i] = -INFINITY;
+        top = fmaxf(top, s[t][i]);
+      }
+    top = fmaxf(m, head_max(top));
+    if (__any(top > m)) {
+      const float keep = top == -INFINITY ? 1.0f : exp2_hw(m - top);
+      l *= keep;
+#pragma unroll
+      for (int c = 0; c < VE; ++c) o[c] *= keep;
+      m = top;
+    }
+    const float from = (m == -INFINITY ? 0.0f : m) - kLift;
+    float p[KT][4];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[t][i] = exp2_hw(s[t][i] - from);
+        l += p[t][i];
+      }
+    // ---- values
+    if constexpr (CT == F32) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < VE; ++c)
+            o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * t + i][c / EV][c % EV]), p[t][i], o[c], 0, 0, 0);
+    } else {
+      u32x4 pa, pb, pc;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t u, v, w;
+        split2<HALF>(p[c / 2][2 * (c % 2)], p[c / 2][2 * (c % 2) + 1], &u, &v, &w);
+        pa[c] = u, pb[c] = v, pc[c] = w;
+      }
+#pragma unroll
+      for (int h = 0; h < NV; ++h) {
+        constexpr int W16 = EV / 2;   // dwords of 16-bit pairs of a piece
+        uint32_t w16[8][W16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int d = 0; d < VW; ++d) {
+            if constexpr (CT == E4M3) {
+              const u32x2 x = widen(vr[k][h][d]);
+              w16[k][2 * d] = x[0], w16[k][2 * d + 1] = x[1];
+            } else {
+              w16[k][d] = vr[k][h][d];
+            }
+          }
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          u32x4 x;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            x[c] = __builtin_amdgcn_perm(w16[2 * c + 1][e / 2], w16[2 * c][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+          o[h * EV + e] = mfma32<HALF>(x, pa, o[h * EV + e]);
+          o[h * EV + e] = mfma32<HALF>(x, pb, o[h * EV + e]);
+          o[h * EV + e] = mfma32<HALF>(x, pc, o[h * EV + e]);
+        }
+      }
+    }
+  };
+
   if (base_of(0) < end) {
     At at = place(0, look(0));
     load_k(at);
     load_v(at);
-    Look next{};
-    if (base_of(1) < end) next = look(1);
-    for (int step = 0;; ++step) {
-      const int base = base_of(step);
-      const bool more = base_of(step + 1) < end;
-      // ---- scores
-      f32x4 s[KT];
+    Look next = look(1);
+    // ---- queries times scale and log2(e): scores are powers of two
+    const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
+    float lift = 1.0f;
 #pragma unroll
-      for (int t = 0; t < KT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < NX; ++s) x[s] *= query_dim(s) < hd && col < heads ? scale : 0.0f;
+    if constexpr (HALF) {   // the head's largest value to 2^14 .. 2^15, so that f16 parts hold the others against it
+      float big = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NK; ++j)
+      for (int s = 0; s < NX; ++s)
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          if constexpr (CT == F32) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][j][c]), qf[j][c], s[t], 0, 0, 0);
-          } else if constexpr (CT == E4M3) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const u32x2 x = widen(kr[t][j][2 * u]), y = widen(kr[t][j][2 * u + 1]);
-              const u32x4 k = {x[0], x[1], y[0], y[1]};
-              s[t] = mfma32<HALF>(k, qa[2 * j + u], s[t]);
-              s[t] = mfma32<HALF>(k, qb[2 * j + u], s[t]);
-              s[t] = mfma32<HALF>(k, qc[2 * j + u], s[t]);
-            }
-          } else {
-            const u32x4 k = {kr[t][j][0], kr[t][j][1], kr[t][j][2], kr[t][j][3]};
-            s[t] = mfma32<HALF>(k, qa[j], s[t]);
-            s[t] = mfma32<HALF>(k, qb[j], s[t]);
-            s[t] = mfma32<HALF>(k, qc[j], s[t]);
-          }
-        }
-      if (more) {
-        at = place(step + 1, next);
-        load_k(at);
-        if (base_of(step + 2) < end) next = look(step + 2);
+        for (int c = 0; c < 4; ++c) big = fmaxf(big, fabsf(x[s][c]));
+      big = head_max(big);
+      if (big > 0.0f && big < INFINITY) {
+        const int e = max((int)(__float_as_uint(big) >> 23) - 127, -100);
+        lift = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+        unlift = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
       }
-      // ---- weights
-      float top = -INFINITY;
+    }
+    if constexpr (CT != F32)
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (HALF) s[t][i] *= unlift;
-          if (base + STEP > end && base + 16 * t + 4 * quad + i >= end) s[t][i] = -INFINITY;
-          top = fmaxf(top, s[t][i]);
-        }
-      top = fmaxf(m, head_max(top));
-      if (__any(top > m)) {
-        const float keep = top == -INFINITY ? 1.0f : exp2_hw(m - top);
-        l *= keep;
-#pragma unroll
-        for (int c = 0; c < VE; ++c) o[c] *= keep;
-        m = top;
-      }
-      const float from = (m == -INFINITY ? 0.0f : m) - kLift;
-      float p[KT][4];
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[t][i] = exp2_hw(s[t][i] - from);
-          l += p[t][i];
-        }
-      // ---- values
-      if constexpr (CT == F32) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int c = 0; c < VE; ++c)
-              o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * t + i][c / EV][c % EV]), p[t][i], o[c], 0, 0, 0);
-      } else {
-        u32x4 pa, pb, pc;
+      for (int s = 0; s < NQ; ++s)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          const f32x4 y = x[2 * s + c / 2];
           uint32_t u, v, w;
-          split2<HALF>(p[c / 2][2 * (c % 2)], p[c / 2][2 * (c % 2) + 1], &u, &v, &w);
-          pa[c] = u, pb[c] = v, pc[c] = w;
+          split2<HALF>(y[2 * (c % 2)] * lift, y[2 * (c % 2) + 1] * lift, &u, &v, &w);
+          qa[s][c] = u, qb[s][c] = v, qc[s][c] = w;
         }
-#pragma unroll
-        for (int h = 0; h < NV; ++h) {
-          constexpr int W16 = EV / 2;   // dwords of 16-bit pairs of a piece
-          uint32_t w16[8][W16];
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-#pragma unroll
-            for (int d = 0; d < VW; ++d) {
-              if constexpr (CT == E4M3) {
-                const u32x2 x = widen(vr[k][h][d]);
-                w16[k][2 * d] = x[0], w16[k][2 * d + 1] = x[1];
-              } else {
-                w16[k][d] = vr[k][h][d];
-              }
-            }
-#pragma unroll
-          for (int e = 0; e < EV; ++e) {
-            u32x4 x;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              x[c] = __builtin_amdgcn_perm(w16[2 * c + 1][e / 2], w16[2 * c][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
-            o[h * EV + e] = mfma32<HALF>(x, pa, o[h * EV + e]);
-            o[h * EV + e] = mfma32<HALF>(x, pb, o[h * EV + e]);
-            o[h * EV + e] = mfma32<HALF>(x, pc, o[h * EV + e]);
-          }
-        }
-      }
-      if (!more) break;
+
+    // keys are requested a step ahead while the weights and values are worked on, values while the scores are
+    int step = 0;
+    for (; base_of(step + 1) < end; ++step) {
+      score();
+      at = place(step + 1, next);
+      load_k(at);
+      next = look(step + 2);
+      gather(base_of(step));
       load_v(at);
     }
+    score();
+    gather(base_of(step));
   }
   l = head_sum(l);
   if (__any(bad)) l = NAN;
@@ -505,7 +550,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
   for (int w = 0; w < kWaves; ++w) sum += l_s[w][col] * exp2_hw(m_s[w][col] - from);
   const bool cut = it.parts > 1;
   // what a sum is multiplied by: 1 / l and the values' scale, or nothing in a part
-  const float vs = g.v_scale ? g.v_scale[kv] : 1.0f;
+  const float vs = g.v_scale ? scalar_load(g.v_scale, kv) : 1.0f;
   __shared__ float div_s[16];
   if (wave == 0 && quad == 0) {
     div_s[col] = sum;
@@ -540,7 +585,9 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(AttnLaunch L) {
   }
 }
 
-// A block a (row, query head): the parts of a cut row joined.
+// A block a (row, query head): the parts of a cut row joined, four dimensions a thread, so that kThreads / (head_dim / 4)
+// parts are read side by side.
+constexpr int kMaxParts = kBlocks + 1;   // of one row
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
@@ -548,34 +595,59 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
   const int2 r = L.rows[t];
   if (r.x <= 1) return;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  __shared__ float acc_s[kWaves][256], red_s[kWaves], sum_s[kWaves];
+  __shared__ float by_s[kMaxParts], red_s[kWaves], sum_s[kWaves];
+  __shared__ f32x4 acc_s[kThreads];
   const float* ml = L.part_ml + ((size_t)r.y * a.n_q + head) * 2;
   const size_t step = (size_t)a.n_q * 2;
-  float top = -INFINITY;
-  for (int i = tid; i < r.x; i += kThreads) top = fmaxf(top, ml[i * step]);
+  // what each part counts for
+  float m[(kMaxParts + kThreads - 1) / kThreads], l[(kMaxParts + kThreads - 1) / kThreads], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < (kMaxParts + kThreads - 1) / kThreads; ++c) {
+    const int i = tid + c * kThreads;
+    m[c] = i < r.x ? ml[i * step] : -INFINITY;
+    l[c] = i < r.x ? ml[i * step + 1] : 0.0f;
+    top = fmaxf(top, m[c]);
+  }
+#pragma unroll
   for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
   if (lane == 0) red_s[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red_s[0], red_s[1]), fmaxf(red_s[2], red_s[3]));
   if (top == -INFINITY) top = 0.0f;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-  for (int i = wave; i < r.x; i += kWaves) {
-    const float f = exp2_hw(ml[i * step] - top);
-    sum += ml[i * step + 1] * f;
-    const float* o = L.part_o + ((size_t)(r.y + i) * a.n_q + head) * hd;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (lane + 64 * c < hd) acc[c] += o[lane + 64 * c] * f;
+  for (int c = 0; c < (kMaxParts + kThreads - 1) / kThreads; ++c) {
+    const int i = tid + c * kThreads;
+    const float f = exp2_hw(m[c] - top);
+    if (i < r.x) by_s[i] = f;
+    sum += l[c] * f;
   }
-#pragma unroll
-  for (int c = 0; c < 4; ++c) acc_s[wave][lane + 64 * c] = acc[c];
+  sum = wave_total(sum);
   if (lane == 0) sum_s[wave] = sum;
   __syncthreads();
-  const float all = sum_s[0] + sum_s[1] + sum_s[2] + sum_s[3];
-  const float vs = g.v_scale ? g.v_scale[head / (a.n_q / g.map.n_kv)] : 1.0f;
-  for (int d = tid; d < hd; d += kThreads) {
-    const float y = acc_s[0][d] + acc_s[1][d] + acc_s[2][d] + acc_s[3][d];
-    a.out[(size_t)t * a.ldo + (size_t)head * hd + d] = all == 0.0f ? 0.0f : y / all * vs;
+  const int width = hd / 4, rows = kThreads / width, row = tid / width, d = tid % width * 4;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (row < rows) {
+    const float* o = L.part_o + ((size_t)r.y * a.n_q + head) * hd + d;
+    const size_t next = (size_t)a.n_q * hd;
+    int i = row;
+    for (; i + 3 * rows < r.x; i += 4 * rows) {   // four requests in flight
+      f32x4 y[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) y[c] = *(const f32x4*)(o + (size_t)(i + c * rows) * next);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc += y[c] * by_s[i + c * rows];
+    }
+    for (; i < r.x; i += rows) acc += *(const f32x4*)(o + (size_t)i * next) * by_s[i];
+  }
+  acc_s[tid] = acc;
+  __syncthreads();
+  if (row == 0) {
+    for (int i = 1; i < rows && i < r.x; ++i) acc += acc_s[i * width + tid];
+    const float all = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
+    const float vs = g.v_scale ? g.v_scale[head / (a.n_q / g.map.n_kv)] : 1.0f;
+    float* out = a.out + (size_t)t * a.ldo + (size_t)head * hd + d;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) out[c] = all == 0.0f ? 0.0f : acc[c] / all * vs;
   }
 }
 
@@ -617,6 +689,7 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   const long long longest = (long long)a.max_pages * map.page_size;
   int chunks = longest <= kUnit ? 0 : chunks_for(a.T, a.n_q, map.n_kv);
   L.chunks = chunks;
+  L.per_unit = chunks ? 1.00001f / ((float)chunks * kUnit) : 0.0f;
   char* w = (char*)a.work;
   L.rows = (int2*)w;
   w += ((size_t)a.T * sizeof(int2) + 15) / 16 * 16;
@@ -627,7 +700,7 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   const long long most = (longest + kUnit - 1) / kUnit * a.T;
   const unsigned items = (unsigned)(a.T + (most < chunks ? most : chunks));
   const dim3 grid(items, (unsigned)(map.n_kv * L.head_tiles));
-  const bool whole = map.page_size % 16 == 0 && map.slot_stride <= (1 << 24);
+  const bool whole = map.page_size % 16 == 0 && map.slot_stride < (1 << 22);
   const hipError_t e = dtype == F32 ? launch<F32>(L, whole, grid, s) : dtype == F16 ? launch<F16>(L, whole, grid, s)
                        : dtype == BF16 ? launch<BF16>(L, whole, grid, s) : launch<E4M3>(L, whole, grid, s);
   if (e != hipSuccess || !chunks) return e;
