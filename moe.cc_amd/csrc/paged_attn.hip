@@ -19,9 +19,9 @@
 // nothing is lost against an fp32 evaluation.  The matrix work this triples is a tenth of what the bytes' time allows.
 // fp32 pages use the fp32 instruction (16 x 16 x 4) on the same layouts.
 //
-// Work is split over the length too.  Every block finds its item in the rows' lengths by itself (paged_item): rows are
-// cut into chunks of one size, chosen so that the chunks of all rows come to about kBlocks blocks; parts of a cut row go
-// to `work` and are joined by a second kernel, launched only if the tables are long enough for a cut.
+// Work is split over the length too.  The rows' positions, in units of kUnit, are laid end to end and cut into as many
+// even pieces as the chip holds blocks at once; a block walks the rows of its piece, whose place it finds in the rows'
+// lengths by itself (find_first).  Parts of a row that pieces cut go to `work` and are joined by a second kernel.
 #include <math.h>
 
 #include <type_traits>
@@ -33,9 +33,10 @@ namespace moe {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kBlocks = 1024;      // blocks that the chunks of all rows come to
-constexpr int kUnit = 128;         // chunks are multiples of this many positions
-constexpr int kSplitRows = 2048;   // more rows than this are not cut
+constexpr int kUnit = 128;         // positions of a unit: a step of every wave
+constexpr int kSplitRows = 2048;   // more rows than this are not cut: a block a row
+constexpr int kCUs = 256;
+constexpr long long kStreamBytes = 64ll << 20;   // pages of K from which loads pass the caches
 
 enum { F32 = MOE_PAGE_F32, F16 = MOE_PAGE_F16, BF16 = MOE_PAGE_BF16, E4M3 = MOE_PAGE_E4M3 };
 
@@ -60,18 +61,17 @@ __device__ __forceinline__ T scalar_load(const T* p, long long i) {
 struct AttnLaunch {
   AttnPages g;
   int head_tiles;   // of 16 query heads, a key-value head
-  int chunks;       // chunks of all rows at most, besides one a row; 0: rows are not cut
-  float per_unit;   // 1 / (chunks kUnit), raised
-  int2* rows;       // [T] work: parts and first part of each row
-  float* part_ml;   // [parts][n_q][2] work: maximum and sum
-  float* part_o;    // [parts][n_q][head_dim] work
+  int pieces;       // 0: rows are not cut, a block a row
+  int2* rows;       // [T] work: parts of each row, and the piece its first lies in
+  float* part_ml;   // [2 pieces][n_q][2] work: maximum and sum of a part
+  float* part_o;    // [2 pieces][n_q][head_dim] work: its values' sums
 };
 
-struct Item {
-  int row, req;          // req: its request, -1: outside the tables
-  int first, end;        // positions first .. end - 1
-  int parts, part;       // parts of the row, this one's place in `work`
-};
+// A piece holds at most two parts of rows that go on in other pieces: part 0 of one (its start), in 2 piece + 1, and a
+// later part of another, in 2 piece.
+__device__ __forceinline__ int part_place(int first_piece, int i) {
+  return i == 0 ? 2 * first_piece + 1 : 2 * (first_piece + i);
+}
 
 // Positions that a row attends; kPadding: no row; kOutside: a request or position outside the tables.
 constexpr int kPadding = -1, kOutside = -2, kNone = -3;
@@ -103,22 +103,30 @@ __device__ __forceinline__ float wave_total(float x) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
 }
 
-struct ItemShared {
-  float sum[kWaves];
-  uint32_t scan[kWaves];
-  Item item;
+__device__ __forceinline__ uint32_t units_of(int len) {
+  return len == kPadding || len == kNone ? 0 : max(((uint32_t)max(len, 0) + kUnit - 1) / kUnit, 1u);
+}
+
+// Where a block's piece starts: units begin .. end - 1 of all, in row `row` of request `req`, whose first unit is `at`.
+struct Piece {
+  uint32_t begin, end, per;   // per: units of a piece
+  int row, req, len;          // len: as length_of
+  uint32_t at;
 };
 
-// The block's item among cut rows; PER rows a thread.  The chunk is a multiple of kUnit no smaller than total / chunks
-// (the total in fp32, raised past every rounding of it), so that the rows have no more than T + chunks items, and the cut
-// ones no more than 2 chunks parts (a cut row is longer than a chunk).
+struct PieceShared {
+  uint32_t scan[kWaves];
+  Piece piece;
+};
+
+// Finds piece b; PER rows a thread.  The host sees to it that the units' sum fits 32 bits.
 template <int PER>
-__device__ __forceinline__ void find_item(const AttnLaunch& L, int b, ItemShared& sh) {
+__device__ __forceinline__ void find_first(const AttnLaunch& L, uint32_t b, PieceShared& sh) {
   const AttnPages& g = L.g;
   const int T = g.a.T, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int per = PER == 1 ? 1 : (T + kThreads - 1) / kThreads, t0 = tid * per;
   int len[PER], req[PER];
-  float sum = 0.0f;
+  uint32_t mine = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int t = min(t0 + i, T - 1);
@@ -128,63 +136,44 @@ __device__ __forceinline__ void find_item(const AttnLaunch& L, int b, ItemShared
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     len[i] = i < per && t0 + i < T ? length_of(g, req[i], len[i]) : kNone;
-    sum += (float)max(len[i], 0);
-  }
-  sum = wave_total(sum);
-  if (lane == 0) sh.sum[wave] = sum;
-  if (tid == 0) sh.item.row = -1;
-  __syncthreads();
-  sum = (sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]);
-  const uint32_t units = (uint32_t)fminf(sum * L.per_unit, 16777214.0f) + 1, chunk = kUnit * units;
-  uint32_t mine = 0;   // items, and parts of cut rows in the upper half
-  int n[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    n[i] = len[i] == kNone ? 0 : len[i] <= 0 ? 1 : (int)(((uint32_t)len[i] + chunk - 1) / chunk);
-    mine += (uint32_t)n[i] + (n[i] > 1 ? (uint32_t)n[i] << 16 : 0);
+    mine += units_of(len[i]);
+    if (len[i] == kPadding && b == 0 && blockIdx.y == 0) L.rows[t0 + i] = make_int2(0, 0);
   }
   const uint32_t scan = wave_scan(mine);
   if (lane == kWave - 1) sh.scan[wave] = scan;
+  if (tid == 0) sh.piece.row = -1;
   __syncthreads();
-  uint32_t at = scan - mine;
+  uint32_t at = scan - mine, total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves - 1; ++w)
+  for (int w = 0; w < kWaves; ++w) {
     if (w < wave) at += sh.scan[w];
+    total += sh.scan[w];
+  }
+  const uint32_t each = (total + L.pieces - 1) / L.pieces, begin = b * each;   // (b < pieces: no overflow past total + pieces)
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int i0 = (int)(at & 0xffff), part0 = (int)(at >> 16);
-    if (b >= i0 && b < i0 + n[i]) {
-      int first = 0, end = max(len[i], 0);
-      if (n[i] > 1) {   // even chunks; the last is never empty, as they are no longer than `chunk`
-        const int even = (int)(((uint32_t)(end + n[i] - 1) / (uint32_t)n[i] + kUnit - 1) / kUnit * kUnit);
-        first = (b - i0) * even;
-        end = min(end, first + even);
-      }
-      sh.item = Item{len[i] == kPadding ? -1 : t0 + i, len[i] == kOutside ? -1 : req[i], first, end, n[i], part0 + b - i0};
-      if (b == i0 && blockIdx.y == 0) L.rows[t0 + i] = make_int2(len[i] == kPadding ? 0 : n[i], part0);
-    }
-    at += (uint32_t)n[i] + (n[i] > 1 ? (uint32_t)n[i] << 16 : 0);
+    const uint32_t n = units_of(len[i]);
+    if (begin >= at && begin - at < n) sh.piece = Piece{begin, min(begin + each, total), each, t0 + i, req[i], len[i], at};
+    at += n;
   }
   __syncthreads();
 }
 
-// The block's item, in scalar registers; false: it has none.
-__device__ __forceinline__ bool paged_item(const AttnLaunch& L, int b, Item* out) {
+__device__ __forceinline__ bool find_piece(const AttnLaunch& L, int b, Piece* out) {
   const AttnPages& g = L.g;
-  const int T = g.a.T;
-  if (!L.chunks) {
-    if (b >= T) return false;
-    const moe_paged_attn& a = g.a;
-    const int req = a.req ? scalar_load(a.req, b) : b;
-    const int n = length_of(g, req, scalar_load(a.pos, b));
-    *out = Item{b, n == kOutside ? -1 : req, 0, max(n, 0), 1, 0};
-    return n != kPadding;
+  const moe_paged_attn& a = g.a;
+  if (!L.pieces) {
+    const int req = a.req ? scalar_load(a.req, b) : b, len = length_of(g, req, scalar_load(a.pos, b));
+    const uint32_t n = units_of(len);
+    *out = Piece{0, n, n, b, req, len, 0};
+    return n > 0;
   }
-  __shared__ ItemShared sh;
-  if (T <= kThreads) find_item<1>(L, b, sh);
-  else find_item<kSplitRows / kThreads>(L, b, sh);
-  auto get = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  *out = Item{get(sh.item.row), get(sh.item.req), get(sh.item.first), get(sh.item.end), get(sh.item.parts), get(sh.item.part)};
+  __shared__ PieceShared sh;
+  if (a.T <= kThreads) find_first<1>(L, (uint32_t)b, sh);
+  else find_first<kSplitRows / kThreads>(L, (uint32_t)b, sh);
+  auto get = [](auto x) { return (decltype(x))__builtin_amdgcn_readfirstlane((int)x); };
+  *out = Piece{get(sh.piece.begin), get(sh.piece.end), get(sh.piece.per), get(sh.piece.row), get(sh.piece.req),
+               get(sh.piece.len), get(sh.piece.at)};
   return out->row >= 0;
 }
 
@@ -243,17 +232,17 @@ __device__ __forceinline__ u32x2 widen(uint32_t x) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true))};
 }
 
-template <int BYTES>
+// BYTES at p; STREAM: past the caches.
+template <int BYTES, bool STREAM>
 __device__ __forceinline__ void load_piece(const char* p, uint32_t* r) {
-  if constexpr (BYTES == 16) {
-    const u32x4 x = *(const u32x4*)p;
-    r[0] = x[0], r[1] = x[1], r[2] = x[2], r[3] = x[3];
-  } else if constexpr (BYTES == 8) {
-    const u32x2 x = *(const u32x2*)p;
-    r[0] = x[0], r[1] = x[1];
-  } else {
-    r[0] = *(const uint32_t*)p;
-  }
+  typedef uint32_t V __attribute__((ext_vector_type(BYTES / 4)));
+  V x;
+  if constexpr (STREAM) x = __builtin_nontemporal_load((const V*)p);
+  else x = *(const V*)p;
+  if constexpr (BYTES == 4) r[0] = x.x;
+  else
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) r[i] = x[i];
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -261,7 +250,7 @@ __device__ __forceinline__ void load_piece(const char* p, uint32_t* r) {
 // CT: the pages' type.  HDP: head_dim, or the next of 64, 128, 256 (the pieces past head_dim repeat its last one against
 // zero queries, and their sums are not stored).  WHOLE: a tile of 16 positions lies in one page (page_size % 16 == 0), so
 // its address is one scalar lookup; otherwise each lane looks up one position and the lanes exchange addresses.
-template <int CT, int HDP, bool WHOLE>
+template <int CT, int HDP, bool WHOLE, bool STREAM>
 __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kernel(AttnLaunch L) {
   constexpr bool HALF = CT == F16;
   constexpr int S = CT == F32 ? 4 : CT == E4M3 ? 1 : 2;
@@ -275,17 +264,38 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   // weights are held times 2^14 where their parts are f16, far from its smallest numbers
   constexpr float kLift = HALF ? 14.0f : 0.0f;
 
-  Item it;
-  if (!paged_item(L, (int)blockIdx.x, &it)) return;
+  Piece pc;
+  if (!find_piece(L, (int)blockIdx.x, &pc)) return;
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int col = lane % 16, quad = lane / 16, hd = g.map.head_dim;
+  const int hd = g.map.head_dim;
   const int G = a.n_q / g.map.n_kv, kv = (int)blockIdx.y / L.head_tiles, tile = (int)blockIdx.y % L.head_tiles;
   const int head0 = kv * G + tile * 16, heads = min(16, G - tile * 16);   // this block's query heads
+  const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
+  const float vs = g.v_scale ? scalar_load(g.v_scale, kv) : 1.0f;
+  const long long head_at = (long long)kv * g.map.head_stride;
+  const char* kbase = (const char*)g.k + head_at * S;
+  const char* vbase = (const char*)g.v + head_at * S;
+  const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: below 2^24
+  for (;;) {   // the rows of the piece
+  // (the lane's places anew for every row: addresses made from them once would fill the registers that the loop needs)
+  int col = lane % 16, quad = lane / 16;
+  asm volatile("" : "+v"(col), "+v"(quad));
+  const uint32_t units = units_of(pc.len), unit0 = max(pc.begin, pc.at) - pc.at, unit1 = min(pc.end - pc.at, units);
+  const int first = (int)unit0 * kUnit, end = (int)min((long long)max(pc.len, 0), (long long)unit1 * kUnit);
+  // the row after this one, asked for now
+  const int row2 = min(pc.row + 1, a.T - 1), req2 = a.req ? scalar_load(a.req, row2) : row2, pos2 = scalar_load(a.pos, row2);
+
+  // WHOLE: a scalar base a tile and 32-bit lane offsets; else a 64-bit row address a lane
+  uint32_t kpiece[NK], vpiece[NV];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) kpiece[j] = (uint32_t)min((4 * j + quad) * 16, hd * S - 16);
+#pragma unroll
+  for (int h = 0; h < NV; ++h) vpiece[h] = (uint32_t)min((16 * h + col) * EV * S, hd * S - EV * S);
 
   // ---- queries: requested first, used after the first keys are requested
-  const float* q = a.q + (size_t)it.row * a.ldq + (size_t)(head0 + min(col, heads - 1)) * hd;
+  const float* q = a.q + (size_t)pc.row * a.ldq + (size_t)(head0 + min(col, heads - 1)) * hd;
   f32x4 x[CT == F32 ? NK : 2 * NQ];
   auto query_dim = [&](int s) {   // of x[s]
     return CT == F32 ? (4 * s + quad) * 4 : CT == E4M3 ? (4 * (s / 4) + quad) * 16 + 4 * (s % 4) : (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
@@ -295,15 +305,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   for (int s = 0; s < NX; ++s) x[s] = *(const f32x4u*)(q + min(query_dim(s), hd - 4));
 
   // ---- addresses
-  const int* table = a.tables + (size_t)max(it.req, 0) * a.max_pages;
-  const long long head_at = (long long)kv * g.map.head_stride;
-  const char* kbase = (const char*)g.k + head_at * S;
-  const char* vbase = (const char*)g.v + head_at * S;
-  const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: below 2^24
-  int bad = it.req < 0;
-
-  const int end = it.end;
-  auto base_of = [&](int step) { return it.first + (step * kWaves + wave) * STEP; };
+  const int* table = a.tables + (size_t)(pc.len == kOutside ? 0 : pc.req) * a.max_pages;
+  int bad = pc.len == kOutside;
+  auto base_of = [&](int step) { return first + (step * kWaves + wave) * STEP; };
   // page numbers of a step: WHOLE: of its tiles; else of the lane's position
   struct Look { int p[WHOLE ? KT : 1]; };
   auto look = [&](int step) {
@@ -346,12 +350,6 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
     }
     return o;
   };
-  // WHOLE: a scalar base a tile and 32-bit lane offsets; else a 64-bit row address a lane
-  uint32_t kpiece[NK], vpiece[NV];
-#pragma unroll
-  for (int j = 0; j < NK; ++j) kpiece[j] = (uint32_t)min((4 * j + quad) * 16, hd * S - 16);
-#pragma unroll
-  for (int h = 0; h < NV; ++h) vpiece[h] = (uint32_t)min((16 * h + col) * EV * S, hd * S - EV * S);
   uint32_t kr[KT][NK][4], vr[4 * KT][NV][VW];
   auto load_k = [&](const At& o) {
 #pragma unroll
@@ -359,7 +357,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
       const char* base = WHOLE ? kbase + o.tile[t] : kbase + __shfl(o.tile[0], 16 * t + col);
       const uint32_t off = WHOLE ? __umul24((uint32_t)min(col, o.lim[t]), slot_bytes) : 0;
 #pragma unroll
-      for (int j = 0; j < NK; ++j) load_piece<16>(base + (off + kpiece[j]), kr[t][j]);
+      for (int j = 0; j < NK; ++j) load_piece<16, STREAM>(base + (off + kpiece[j]), kr[t][j]);
     }
   };
   auto load_v = [&](const At& o) {
@@ -370,7 +368,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
         const char* base = WHOLE ? vbase + o.tile[t] : vbase + __shfl(o.tile[0], 16 * t + 4 * quad + i);
         const uint32_t off = WHOLE ? __umul24((uint32_t)min(4 * quad + i, o.lim[t]), slot_bytes) : 0;
 #pragma unroll
-        for (int h = 0; h < NV; ++h) load_piece<EV * S>(base + (off + vpiece[h]), vr[4 * t + i][h]);
+        for (int h = 0; h < NV; ++h) load_piece<EV * S, STREAM>(base + (off + vpiece[h]), vr[4 * t + i][h]);
       }
   };
 
@@ -491,7 +489,6 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
     load_v(at);
     Look next = look(1);
     // ---- queries times scale and log2(e): scores are powers of two
-    const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
     float lift = 1.0f;
 #pragma unroll
     for (int s = 0; s < NX; ++s) x[s] *= query_dim(s) < hd && col < heads ? scale : 0.0f;
@@ -536,6 +533,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   if (__any(bad)) l = NAN;
 
   // ---- the waves' sums joined, 128 dimensions at a time
+  asm volatile("" : "+v"(col), "+v"(quad));
   constexpr int PASS = HDP > 128 ? 2 : 1, VP = VE / PASS;
   __shared__ float o_s[kWaves][16 * VP][17], m_s[kWaves][16], l_s[kWaves][16];
   if (quad == 0) m_s[wave][col] = m, l_s[wave][col] = l;
@@ -548,17 +546,19 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   float sum = 0.0f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) sum += l_s[w][col] * exp2_hw(m_s[w][col] - from);
-  const bool cut = it.parts > 1;
-  // what a sum is multiplied by: 1 / l and the values' scale, or nothing in a part
-  const float vs = g.v_scale ? scalar_load(g.v_scale, kv) : 1.0f;
+  // a row that goes on in other pieces leaves its part
+  const uint32_t piece0 = pc.at / pc.per, parts = units ? (pc.at + units - 1) / pc.per - piece0 + 1 : 0;
+  const bool cut = L.pieces && parts > 1;
+  const size_t part = (size_t)part_place((int)blockIdx.x - (unit0 != 0), unit0 != 0);
   __shared__ float div_s[16];
   if (wave == 0 && quad == 0) {
     div_s[col] = sum;
     if (cut && col < heads) {
-      float* ml = L.part_ml + ((size_t)it.part * a.n_q + head0 + col) * 2;
+      float* ml = L.part_ml + (part * a.n_q + head0 + col) * 2;
       ml[0] = top;
       ml[1] = sum;
     }
+    if (L.pieces && unit0 == 0 && blockIdx.y == 0 && lane == 0) L.rows[pc.row] = make_int2((int)parts, (int)piece0);
   }
 #pragma unroll
   for (int ps = 0; ps < PASS; ++ps) {
@@ -575,19 +575,29 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) y += o_s[w][at][h];
       if (cut) {
-        L.part_o[((size_t)it.part * a.n_q + head0 + h) * hd + d] = y;
+        L.part_o[(part * a.n_q + head0 + h) * hd + d] = y;
       } else {
         const float z = div_s[h];
-        a.out[(size_t)it.row * a.ldo + (size_t)(head0 + h) * hd + d] = z == 0.0f ? 0.0f : y / z * vs;
+        a.out[(size_t)pc.row * a.ldo + (size_t)(head0 + h) * hd + d] = z == 0.0f ? 0.0f : y / z * vs;
       }
     }
     if (ps + 1 < PASS) __syncthreads();
+  }
+
+  pc.at += units;
+  if (pc.at >= pc.end) return;
+  pc.row = row2, pc.req = req2, pc.len = length_of(g, req2, pos2);
+  while (units_of(pc.len) == 0) {   // rows of no request between
+    ++pc.row;
+    pc.req = a.req ? scalar_load(a.req, pc.row) : pc.row;
+    pc.len = length_of(g, pc.req, scalar_load(a.pos, pc.row));
+  }
   }
 }
 
 // A block a (row, query head): the parts of a cut row joined, four dimensions a thread, so that kThreads / (head_dim / 4)
 // parts are read side by side.
-constexpr int kMaxParts = kBlocks + 1;   // of one row
+constexpr int kMaxParts = 3 * kCUs;   // of one row: no more than pieces
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
@@ -597,15 +607,15 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   __shared__ float by_s[kMaxParts], red_s[kWaves], sum_s[kWaves];
   __shared__ f32x4 acc_s[kThreads];
-  const float* ml = L.part_ml + ((size_t)r.y * a.n_q + head) * 2;
+  const float* ml = L.part_ml + (size_t)head * 2;
   const size_t step = (size_t)a.n_q * 2;
   // what each part counts for
   float m[(kMaxParts + kThreads - 1) / kThreads], l[(kMaxParts + kThreads - 1) / kThreads], top = -INFINITY, sum = 0.0f;
 #pragma unroll
   for (int c = 0; c < (kMaxParts + kThreads - 1) / kThreads; ++c) {
     const int i = tid + c * kThreads;
-    m[c] = i < r.x ? ml[i * step] : -INFINITY;
-    l[c] = i < r.x ? ml[i * step + 1] : 0.0f;
+    m[c] = i < r.x ? ml[part_place(r.y, i) * step] : -INFINITY;
+    l[c] = i < r.x ? ml[part_place(r.y, i) * step + 1] : 0.0f;
     top = fmaxf(top, m[c]);
   }
 #pragma unroll
@@ -627,17 +637,17 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
   const int width = hd / 4, rows = kThreads / width, row = tid / width, d = tid % width * 4;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   if (row < rows) {
-    const float* o = L.part_o + ((size_t)r.y * a.n_q + head) * hd + d;
+    const float* o = L.part_o + (size_t)head * hd + d;
     const size_t next = (size_t)a.n_q * hd;
     int i = row;
     for (; i + 3 * rows < r.x; i += 4 * rows) {   // four requests in flight
       f32x4 y[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) y[c] = *(const f32x4*)(o + (size_t)(i + c * rows) * next);
+      for (int c = 0; c < 4; ++c) y[c] = *(const f32x4*)(o + part_place(r.y, i + c * rows) * next);
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc += y[c] * by_s[i + c * rows];
     }
-    for (; i < r.x; i += rows) acc += *(const f32x4*)(o + (size_t)i * next) * by_s[i];
+    for (; i < r.x; i += rows) acc += *(const f32x4*)(o + part_place(r.y, i) * next) * by_s[i];
   }
   acc_s[tid] = acc;
   __syncthreads();
@@ -651,32 +661,39 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
   }
 }
 
-// Chunks besides one a row; 0: rows are not cut.
-int chunks_for(int T, int n_q, int n_kv) {
-  if (T > kSplitRows) return 0;
-  const int tiles = (n_q / n_kv + 15) / 16;
-  return kBlocks / (n_kv * tiles) > 0 ? kBlocks / (n_kv * tiles) : 1;
+// Pieces that the rows are cut into: as many as blocks of all heads are resident at once.
+int pieces_for(int n_q, int n_kv, int head_dim) {
+  const int blocks = kCUs * (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1), per = n_kv * ((n_q / n_kv + 15) / 16);
+  return blocks > per ? blocks / per : 1;
 }
 
 template <int CT, int HDP>
-hipError_t launch(const AttnLaunch& L, bool whole, dim3 grid, hipStream_t s) {
-  if (whole) hipLaunchKernelGGL((paged_attn_kernel<CT, HDP, true>), grid, dim3(kThreads), 0, s, L);
-  else hipLaunchKernelGGL((paged_attn_kernel<CT, HDP, false>), grid, dim3(kThreads), 0, s, L);
+hipError_t launch(const AttnLaunch& L, bool whole, bool stream, dim3 grid, hipStream_t s) {
+  auto go = [&](auto w, auto n) {
+    hipLaunchKernelGGL((paged_attn_kernel<CT, HDP, decltype(w)::value, decltype(n)::value>), grid, dim3(kThreads), 0, s, L);
+  };
+  using std::false_type;
+  using std::true_type;
+  if (whole && stream) go(true_type{}, true_type{});
+  else if (whole) go(true_type{}, false_type{});
+  else if (stream) go(false_type{}, true_type{});
+  else go(false_type{}, false_type{});
   return hipGetLastError();
 }
 
 template <int CT>
-hipError_t launch(const AttnLaunch& L, bool whole, dim3 grid, hipStream_t s) {
+hipError_t launch(const AttnLaunch& L, bool whole, bool stream, dim3 grid, hipStream_t s) {
   const int hd = L.g.map.head_dim;
-  return hd <= 64 ? launch<CT, 64>(L, whole, grid, s) : hd <= 128 ? launch<CT, 128>(L, whole, grid, s)
-                                                                  : launch<CT, 256>(L, whole, grid, s);
+  return hd <= 64    ? launch<CT, 64>(L, whole, stream, grid, s)
+         : hd <= 128 ? launch<CT, 128>(L, whole, stream, grid, s)
+                     : launch<CT, 256>(L, whole, stream, grid, s);
 }
 
 }  // namespace
 
 size_t paged_attn_work(int T, int n_q, int n_kv, int head_dim) {
-  const size_t parts = 2 * (size_t)chunks_for(T, n_q, n_kv);
-  return ((size_t)T * sizeof(int2) + 15) / 16 * 16 + parts * n_q * (2 + (size_t)head_dim) * 4 + 16;
+  const size_t rows = ((size_t)T * sizeof(int2) + 15) / 16 * 16;
+  return rows + 2 * (size_t)pieces_for(n_q, n_kv, head_dim) * n_q * (2 + (size_t)head_dim) * 4;
 }
 
 hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
@@ -685,25 +702,22 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   AttnLaunch L;
   L.g = p;
   L.head_tiles = (a.n_q / map.n_kv + 15) / 16;
-  // rows that no chunk can cut need neither the search for items nor the join
-  const long long longest = (long long)a.max_pages * map.page_size;
-  int chunks = longest <= kUnit ? 0 : chunks_for(a.T, a.n_q, map.n_kv);
-  L.chunks = chunks;
-  L.per_unit = chunks ? 1.00001f / ((float)chunks * kUnit) : 0.0f;
-  char* w = (char*)a.work;
-  L.rows = (int2*)w;
-  w += ((size_t)a.T * sizeof(int2) + 15) / 16 * 16;
-  const size_t parts = 2 * (size_t)chunks_for(a.T, a.n_q, map.n_kv);
-  L.part_o = (float*)w;
-  L.part_ml = (float*)w + parts * a.n_q * map.head_dim;
-  // no more items than the longest rows' chunks
-  const long long most = (longest + kUnit - 1) / kUnit * a.T;
-  const unsigned items = (unsigned)(a.T + (most < chunks ? most : chunks));
-  const dim3 grid(items, (unsigned)(map.n_kv * L.head_tiles));
+  // rows that no piece can cut (a unit at most), and more than a block's search takes, get a block each
+  const long long units = ((long long)a.max_pages * map.page_size + kUnit - 1) / kUnit * a.T;   // at most
+  const int most = pieces_for(a.n_q, map.n_kv, map.head_dim);
+  L.pieces = units > a.T && units <= 0xffff0000ll && a.T <= kSplitRows ? most : 0;
+  L.rows = (int2*)a.work;
+  L.part_o = (float*)((char*)a.work + ((size_t)a.T * sizeof(int2) + 15) / 16 * 16);
+  L.part_ml = L.part_o + 2 * (size_t)most * a.n_q * map.head_dim;
+  const dim3 grid((unsigned)(L.pieces ? (units < most ? units : most) : a.T), (unsigned)(map.n_kv * L.head_tiles));
   const bool whole = map.page_size % 16 == 0 && map.slot_stride < (1 << 22);
-  const hipError_t e = dtype == F32 ? launch<F32>(L, whole, grid, s) : dtype == F16 ? launch<F16>(L, whole, grid, s)
-                       : dtype == BF16 ? launch<BF16>(L, whole, grid, s) : launch<E4M3>(L, whole, grid, s);
-  if (e != hipSuccess || !chunks) return e;
+  const int size = dtype == F32 ? 4 : dtype == E4M3 ? 1 : 2;
+  const bool stream = (long long)map.n_pages * map.page_stride * size >= kStreamBytes;
+  const hipError_t e = dtype == F32    ? launch<F32>(L, whole, stream, grid, s)
+                       : dtype == F16  ? launch<F16>(L, whole, stream, grid, s)
+                       : dtype == BF16 ? launch<BF16>(L, whole, stream, grid, s)
+                                       : launch<E4M3>(L, whole, stream, grid, s);
+  if (e != hipSuccess || !L.pieces) return e;
   hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)a.T, (unsigned)a.n_q), dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
