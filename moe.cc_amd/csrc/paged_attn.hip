@@ -62,7 +62,8 @@ struct AttnLaunch {
   AttnPages g;
   int head_tiles;   // of 16 query heads, a key-value head
   int pieces;       // 0: rows are not cut, a block a row
-  int2* rows;       // [T] work: parts of each row, and the piece its first lies in
+  int by_row;       // joins are listed a row (T <= pieces) or a piece
+  int4* joins;      // [min(T, pieces)] work: row, parts, the piece its first lies in; of a piece: of the row that ends there
   float* part_ml;   // [2 pieces][n_q][2] work: maximum and sum of a part
   float* part_o;    // [2 pieces][n_q][head_dim] work: its values' sums
 };
@@ -137,11 +138,14 @@ __device__ __forceinline__ void find_first(const AttnLaunch& L, uint32_t b, Piec
   for (int i = 0; i < PER; ++i) {
     len[i] = i < per && t0 + i < T ? length_of(g, req[i], len[i]) : kNone;
     mine += units_of(len[i]);
-    if (len[i] == kPadding && b == 0 && blockIdx.y == 0) L.rows[t0 + i] = make_int2(0, 0);
+    if (len[i] == kPadding && L.by_row && b == 0 && blockIdx.y == 0) L.joins[t0 + i] = int4{0, 0, 0, 0};
   }
   const uint32_t scan = wave_scan(mine);
   if (lane == kWave - 1) sh.scan[wave] = scan;
-  if (tid == 0) sh.piece.row = -1;
+  if (tid == 0) {
+    sh.piece.row = -1;
+    if (!L.by_row && blockIdx.y == 0) L.joins[b] = int4{0, 0, 0, 0};
+  }
   __syncthreads();
   uint32_t at = scan - mine, total = 0;
 #pragma unroll
@@ -558,7 +562,12 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
       ml[0] = top;
       ml[1] = sum;
     }
-    if (L.pieces && unit0 == 0 && blockIdx.y == 0 && lane == 0) L.rows[pc.row] = make_int2((int)parts, (int)piece0);
+    if (cut && blockIdx.y == 0 && lane == 0) {
+      const bool last = pc.end >= pc.at + units;
+      if (L.by_row ? unit0 == 0 : last) L.joins[L.by_row ? pc.row : blockIdx.x] = int4{pc.row, (int)parts, (int)piece0, 0};
+    } else if (L.by_row && unit0 == 0 && blockIdx.y == 0 && lane == 0) {
+      L.joins[pc.row] = int4{0, 0, 0, 0};
+    }
   }
 #pragma unroll
   for (int ps = 0; ps < PASS; ++ps) {
@@ -595,69 +604,66 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   }
 }
 
-// A block a (row, query head): the parts of a cut row joined, four dimensions a thread, so that kThreads / (head_dim / 4)
-// parts are read side by side.
+// A block a (cut row, query head): its parts joined, four dimensions a thread, so that WAVES 64 / (head_dim / 4) parts are
+// read side by side.  Latency: the parts' first rows are requested with their maxima.
 constexpr int kMaxParts = 3 * kCUs;   // of one row: no more than pieces
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnLaunch L) {
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L) {
+  constexpr int N = WAVES * kWave, U = 4;
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
-  const int t = (int)blockIdx.x, head = (int)blockIdx.y, hd = g.map.head_dim;
-  const int2 r = L.rows[t];
-  if (r.x <= 1) return;
+  const int head = (int)blockIdx.y, hd = g.map.head_dim;
+  const int4 r = L.joins[blockIdx.x];   // row, parts, first piece
+  const int parts = r.y;
+  if (parts <= 1) return;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  __shared__ float by_s[kMaxParts], red_s[kWaves], sum_s[kWaves];
-  __shared__ f32x4 acc_s[kThreads];
+  const int width = hd / 4, rows = N / width, row = tid / width, d = tid % width * 4;
+  __shared__ float by_s[WAVES][kMaxParts];
+  __shared__ f32x4 acc_s[N];
   const float* ml = L.part_ml + (size_t)head * 2;
-  const size_t step = (size_t)a.n_q * 2;
-  // what each part counts for
-  float m[(kMaxParts + kThreads - 1) / kThreads], l[(kMaxParts + kThreads - 1) / kThreads], top = -INFINITY, sum = 0.0f;
+  const float* o = L.part_o + (size_t)head * hd + d;
+  const size_t step = (size_t)a.n_q * 2, next = (size_t)a.n_q * hd;
+  f32x4 y[U];
 #pragma unroll
-  for (int c = 0; c < (kMaxParts + kThreads - 1) / kThreads; ++c) {
-    const int i = tid + c * kThreads;
-    m[c] = i < r.x ? ml[part_place(r.y, i) * step] : -INFINITY;
-    l[c] = i < r.x ? ml[part_place(r.y, i) * step + 1] : 0.0f;
-    top = fmaxf(top, m[c]);
+  for (int c = 0; c < U; ++c) {
+    const int i = row + c * rows;
+    y[c] = *(const f32x4*)(o + part_place(r.z, i < parts ? i : 0) * next);
   }
+  // what each part counts for; every wave for itself
+  float top = -INFINITY, sum = 0.0f;
+  for (int i = lane; i < parts; i += kWave) top = fmaxf(top, ml[part_place(r.z, i) * step]);
 #pragma unroll
-  for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
-  if (lane == 0) red_s[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red_s[0], red_s[1]), fmaxf(red_s[2], red_s[3]));
+  for (int c = 32; c; c /= 2) top = fmaxf(top, __shfl_xor(top, c));
   if (top == -INFINITY) top = 0.0f;
-#pragma unroll
-  for (int c = 0; c < (kMaxParts + kThreads - 1) / kThreads; ++c) {
-    const int i = tid + c * kThreads;
-    const float f = exp2_hw(m[c] - top);
-    if (i < r.x) by_s[i] = f;
-    sum += l[c] * f;
+  for (int i = lane; i < parts; i += kWave) {
+    const float* p = ml + part_place(r.z, i) * step;
+    const float f = exp2_hw(p[0] - top);
+    by_s[wave][i] = f;
+    sum += p[1] * f;
   }
   sum = wave_total(sum);
-  if (lane == 0) sum_s[wave] = sum;
-  __syncthreads();
-  const int width = hd / 4, rows = kThreads / width, row = tid / width, d = tid % width * 4;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   if (row < rows) {
-    const float* o = L.part_o + (size_t)head * hd + d;
-    const size_t next = (size_t)a.n_q * hd;
-    int i = row;
-    for (; i + 3 * rows < r.x; i += 4 * rows) {   // four requests in flight
-      f32x4 y[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) y[c] = *(const f32x4*)(o + part_place(r.y, i + c * rows) * next);
+    for (int c = 0; c < U; ++c)
+      if (row + c * rows < parts) acc += y[c] * by_s[wave][row + c * rows];
+    int i = row + U * rows;
+    for (; i + (U - 1) * rows < parts; i += U * rows) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc += y[c] * by_s[i + c * rows];
+      for (int c = 0; c < U; ++c) y[c] = *(const f32x4*)(o + part_place(r.z, i + c * rows) * next);
+#pragma unroll
+      for (int c = 0; c < U; ++c) acc += y[c] * by_s[wave][i + c * rows];
     }
-    for (; i < r.x; i += rows) acc += *(const f32x4*)(o + part_place(r.y, i) * next) * by_s[i];
+    for (; i < parts; i += rows) acc += *(const f32x4*)(o + part_place(r.z, i) * next) * by_s[wave][i];
   }
   acc_s[tid] = acc;
   __syncthreads();
   if (row == 0) {
-    for (int i = 1; i < rows && i < r.x; ++i) acc += acc_s[i * width + tid];
-    const float all = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
+    for (int i = 1; i < rows && i < parts; ++i) acc += acc_s[i * width + tid];
     const float vs = g.v_scale ? g.v_scale[head / (a.n_q / g.map.n_kv)] : 1.0f;
-    float* out = a.out + (size_t)t * a.ldo + (size_t)head * hd + d;
+    float* out = a.out + (size_t)r.x * a.ldo + (size_t)head * hd + d;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) out[c] = all == 0.0f ? 0.0f : acc[c] / all * vs;
+    for (int c = 0; c < 4; ++c) out[c] = sum == 0.0f ? 0.0f : acc[c] / sum * vs;
   }
 }
 
@@ -692,8 +698,8 @@ hipError_t launch(const AttnLaunch& L, bool whole, bool stream, dim3 grid, hipSt
 }  // namespace
 
 size_t paged_attn_work(int T, int n_q, int n_kv, int head_dim) {
-  const size_t rows = ((size_t)T * sizeof(int2) + 15) / 16 * 16;
-  return rows + 2 * (size_t)pieces_for(n_q, n_kv, head_dim) * n_q * (2 + (size_t)head_dim) * 4;
+  const size_t pieces = (size_t)pieces_for(n_q, n_kv, head_dim);
+  return ((size_t)T < pieces ? T : pieces) * sizeof(int4) + 2 * pieces * n_q * (2 + (size_t)head_dim) * 4 + 16;
 }
 
 hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
@@ -706,8 +712,9 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   const long long units = ((long long)a.max_pages * map.page_size + kUnit - 1) / kUnit * a.T;   // at most
   const int most = pieces_for(a.n_q, map.n_kv, map.head_dim);
   L.pieces = units > a.T && units <= 0xffff0000ll && a.T <= kSplitRows ? most : 0;
-  L.rows = (int2*)a.work;
-  L.part_o = (float*)((char*)a.work + ((size_t)a.T * sizeof(int2) + 15) / 16 * 16);
+  L.by_row = a.T <= most;
+  L.joins = (int4*)a.work;
+  L.part_o = (float*)(L.joins + (L.by_row ? a.T : most));
   L.part_ml = L.part_o + 2 * (size_t)most * a.n_q * map.head_dim;
   const dim3 grid((unsigned)(L.pieces ? (units < most ? units : most) : a.T), (unsigned)(map.n_kv * L.head_tiles));
   const bool whole = map.page_size % 16 == 0 && map.slot_stride < (1 << 22);
@@ -718,7 +725,10 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
                        : dtype == BF16 ? launch<BF16>(L, whole, stream, grid, s)
                                        : launch<E4M3>(L, whole, stream, grid, s);
   if (e != hipSuccess || !L.pieces) return e;
-  hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)a.T, (unsigned)a.n_q), dim3(kThreads), 0, s, L);
+  // few rows may have many parts each
+  const dim3 joins(L.by_row ? (unsigned)a.T : grid.x, (unsigned)a.n_q);
+  if (a.T <= 16) hipLaunchKernelGGL(paged_join_kernel<4>, joins, dim3(4 * kWave), 0, s, L);
+  else hipLaunchKernelGGL(paged_join_kernel<1>, joins, dim3(kWave), 0, s, L);
   return hipGetLastError();
 }
 
