@@ -63,8 +63,8 @@ MOE_BOTH int position_slot(int page, int p, int n_pages, int page_size, const Di
   return page * page_size + (p - (int)divide((uint32_t)p, per) * page_size);
 }
 
-// Pages that n positions fill.
-MOE_BOTH long long pages_for(long long n, int page_size) { return (n + page_size - 1) / page_size; }
+// Pages that n >= 0 positions fill.
+MOE_BOTH int pages_for(int n, const Divider& per) { return n ? (int)divide((uint32_t)n - 1, per) + 1 : 0; }
 
 // What a step's plan comes to, from its totals.
 enum PlanStatus { kPlanOk = 0, kPlanNoPages = 1, kPlanTokens = 2, kPlanLong = 3, kPlanBad = 4 };
@@ -78,7 +78,10 @@ MOE_BOTH int plan_status(bool bad, bool too_long, long long tokens, long long ne
   return kPlanOk;
 }
 
-// Place `i` entries past `from` in a ring of n (from < n, i <= 2 n).
-MOE_BOTH int ring_place(int from, long long i, int n) { return (int)((from + i) % n); }
+// Place `i` entries past `from` in a ring of n (0 <= from < n, 0 <= i <= n).
+MOE_BOTH int ring_place(int from, int i, int n) {
+  const uint32_t at = (uint32_t)from + (uint32_t)i;
+  return (int)(at >= (uint32_t)n ? at - (uint32_t)n : at);
+}
 
 }  // namespace moe

@@ -3,6 +3,8 @@
 // into their pages, and the entry points (attention: paged_attn.hip).
 #include <math.h>
 
+#include <type_traits>
+
 #include "moe_device.h"
 #include "moe_lib.h"
 #include "paged_attn.h"
@@ -53,166 +55,199 @@ moe_status check_pages(const moe_pages* g, const char* who, PageMap* m) {
   return MOE_OK;
 }
 
-// ------------------------------------------------------------ cache types
-
-struct CacheF32 {
-  using T = float;
-  static __device__ T make(float x) { return x; }
-};
-struct CacheF16 {
-  using T = _Float16;
-  static __device__ T make(float x) { return (_Float16)x; }
-};
-struct CacheBF16 {
-  using T = uint16_t;
-  static __device__ T make(float x) {
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (T)(u >> 16 | 0x40);   // NaN stays one
-    return (T)((u + 0x7fffu + (u >> 16 & 1)) >> 16);
-  }
-};
-struct CacheE4M3 {
-  using T = uint8_t;
-  // saturated here: the conversion itself turns what is past 448 into NaN
-  static __device__ T make(float x) {
-    const float c = x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x;   // NaN passes
-    return (T)(__builtin_amdgcn_cvt_pk_fp8_f32(c, c, 0, false) & 0xff);
-  }
-};
-
 // ------------------------------------------------------------ plan
-
-constexpr int kPlanThreads = 1024;
-
-// Exclusive sums over the block's threads of three numbers at once, and their
-// totals; ends with the block in step.
-__device__ int3 block_scan3(int3 v, int3* wave_sum, int3* total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  int3 s = v;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int x = __shfl_up(s.x, d), y = __shfl_up(s.y, d), z = __shfl_up(s.z, d);
-    if (lane >= d) s.x += x, s.y += y, s.z += z;
-  }
-  __syncthreads();
-  if (lane == kWave - 1) wave_sum[wave] = s;
-  __syncthreads();
-  int3 base = {0, 0, 0}, all = {0, 0, 0};
-  for (int w = 0; w < kPlanThreads / kWave; ++w) {
-    const int3 q = wave_sum[w];
-    if (w < wave) base.x += q.x, base.y += q.y, base.z += q.z;
-    all.x += q.x, all.y += q.y, all.z += q.z;
-  }
-  *total = all;
-  return {base.x + s.x - v.x, base.y + s.y - v.y, base.z + s.z - v.z};
-}
-
-// Largest i < n with first[i] <= x (first ascending from first[0] <= x).
-__device__ int last_at_most(const int* first, int n, int x) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (first[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
 
 struct PlanArgs {
   moe_paged_plan p;
   Divider per;
 };
 
-// One block: requests in pieces of one a thread.  First the totals, which say
-// whether the step can be done at all; then, piece by piece, sums over the
-// piece's requests place its tokens and page moves, which all threads then
-// share (an item finds its request by bisection of the piece's sums).
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
-  const moe_paged_plan& p = a.p;
-  __shared__ int3 wave_sum[kPlanThreads / kWave];
-  __shared__ int tok0[kPlanThreads], take0[kPlanThreads], back0[kPlanThreads], old_s[kPlanThreads], held_s[kPlanThreads];
-  __shared__ unsigned long long sums[3];
-  __shared__ int bad_s, long_s;
-  const int tid = threadIdx.x;
-  const int head = p.ring_at[0], count = p.ring_at[1];
-  if (tid < 3) sums[tid] = 0;
-  if (tid == 0) bad_s = long_s = 0;
+// Sums over the lanes up to each one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+struct Request {
+  int held, add, old, need, back;   // positions, new ones; pages it has, needs, gives back
+};
+
+// Tokens, pages taken and pages given back that lie before a request in its piece, and of the piece.
+struct Before {
+  int tok, take, back;
+};
+
+template <int N>
+struct PlanShared {
+  long long sum[N / kWave][3];
+  int odd[N / kWave];
+  Before wave[N / kWave];
+  int tok0[N], take0[N], back0[N], old[N], held[N];
+};
+
+template <int N>
+__device__ __forceinline__ Before place_piece(const Request& r, bool in, PlanShared<N>& sh, Before* all) {
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const Before s = {wave_scan(r.add), wave_scan(r.need), wave_scan(r.back)};
+  if (lane == kWave - 1) sh.wave[wave] = s;
   __syncthreads();
-  unsigned long long nt = 0, nn = 0, nb = 0;
-  for (int r = tid; r < p.n_req; r += kPlanThreads) {
-    const int held = p.held[r], fresh = p.fresh[r];
-    if (held < 0 || fresh < -1) {
-      bad_s = 1;
-      continue;
-    }
-    const long long old = pages_for(held, p.page_size);
-    if (old > p.max_pages) long_s = 1;
-    if (fresh < 0) {
-      nb += old;
-    } else {
-      const long long now = pages_for((long long)held + fresh, p.page_size);
-      if (now > p.max_pages) long_s = 1;
-      nt += fresh;
-      nn += now - old;
-    }
+  Before at = {s.tok - r.add, s.take - r.need, s.back - r.back};
+  *all = {0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < N / kWave; ++w) {
+    const Before q = sh.wave[w];
+    if (w < wave) at = {at.tok + q.tok, at.take + q.take, at.back + q.back};
+    *all = {all->tok + q.tok, all->take + q.take, all->back + q.back};
   }
-  atomicAdd(&sums[0], nt);
-  atomicAdd(&sums[1], nn);
-  atomicAdd(&sums[2], nb);
+  constexpr int kPast = 0x7fffffff;   // behind every item
+  sh.tok0[tid] = in ? at.tok : kPast;
+  sh.take0[tid] = in ? at.take : kPast;
+  sh.back0[tid] = in ? at.back : kPast;
+  sh.old[tid] = r.old;
+  sh.held[tid] = r.held;
   __syncthreads();
-  const int status = plan_status(bad_s, long_s, (long long)sums[0], (long long)sums[1], (long long)sums[2], head, count,
-                                 p.n_pages, p.max_tokens);
+  return at;
+}
+
+// U items at once: the last request that starts at or before each (first ascending, its first entry 0).
+template <int N, int U>
+__device__ __forceinline__ void owners(const int* first, const int (&item)[U], int (&q)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) q[u] = 0;
+#pragma unroll
+  for (int s = N / 2; s; s /= 2)
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first[q[u] + s] <= item[u]) q[u] += s;
+}
+
+// One block, as the step is done in place: requests in pieces of one a thread.  First the totals, which say whether the
+// step can be done at all; then, piece by piece, sums over the piece's requests place its tokens and page moves, which
+// all threads then share, four at a time (an item finds its request by bisection of the piece's sums).  Latency: two
+// levels of loads and the sums; 64 requests, 64 tokens: see DESIGN
+template <int N>
+__global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
+  constexpr int U = 4;
+  const moe_paged_plan& p = a.p;
+  __shared__ PlanShared<N> sh;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const long long most = (long long)p.max_pages * p.page_size;
+  int held0 = 0, fresh0 = 0;   // of the first piece
+  if (tid < p.n_req) held0 = p.held[tid], fresh0 = p.fresh[tid];
+  const int head = p.ring_at[0], count = p.ring_at[1];
+  auto request = [&](int held, int fresh, int* odd) {
+    Request r = {held, max(fresh, 0), 0, 0, 0};
+    if (held < 0 || fresh < -1) *odd |= 1;
+    else if (held + (long long)r.add > most) *odd |= 2;
+    else {
+      r.old = pages_for(held, a.per);
+      r.need = pages_for(held + r.add, a.per) - r.old;
+      r.back = fresh < 0 ? r.old : 0;
+    }
+    return r;
+  };
+  int odd = 0;
+  Request first = request(held0, fresh0, &odd);
+  long long sum[3] = {first.add, first.need, first.back};
+  for (int r = tid + N; r < p.n_req; r += N) {
+    const Request x = request(p.held[r], p.fresh[r], &odd);
+    sum[0] += x.add, sum[1] += x.need, sum[2] += x.back;
+  }
+#pragma unroll
+  for (int d = kWave / 2; d; d /= 2) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sum[i] += __shfl_xor(sum[i], d);
+    odd |= __shfl_xor(odd, d);
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sh.sum[wave][i] = sum[i];
+    sh.odd[wave] = odd;
+  }
+  __syncthreads();
+  sum[0] = sum[1] = sum[2] = odd = 0;
+#pragma unroll
+  for (int w = 0; w < N / kWave; ++w) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sum[i] += sh.sum[w][i];
+    odd |= sh.odd[w];
+  }
+  const int status = plan_status(odd & 1, odd & 2, sum[0], sum[1], sum[2], head, count, p.n_pages, p.max_tokens);
   const bool ok = status == kPlanOk;
   int done_t = 0, done_n = 0, done_b = 0;   // tokens and pages of the pieces before
-  for (int r0 = 0; r0 < p.n_req; r0 += kPlanThreads) {
-    const int r = r0 + tid, n = min(kPlanThreads, p.n_req - r0);
+  for (int r0 = 0; r0 < p.n_req; r0 += N) {
+    const int r = r0 + tid;
     const bool in = r < p.n_req;
-    const int held = in ? p.held[r] : 0;
+    if (r0) held0 = in ? p.held[r] : 0, fresh0 = in ? p.fresh[r] : 0;
     if (!ok) {
-      if (in) p.starts[r] = 0, p.held_out[r] = held;
+      if (in) p.starts[r] = 0, p.held_out[r] = held0;
       continue;
     }
-    const int fresh = in ? p.fresh[r] : 0, add = max(fresh, 0);
-    const int old = (int)pages_for(held, p.page_size);
-    const int need = (int)pages_for((long long)held + add, p.page_size) - old, back = fresh < 0 ? old : 0;
-    int3 all;
-    const int3 at = block_scan3({add, need, back}, wave_sum, &all);
-    tok0[tid] = at.x;
-    take0[tid] = at.y;
-    back0[tid] = at.z;
-    old_s[tid] = old;
-    held_s[tid] = held;
+    const Request x = r0 ? request(held0, fresh0, &odd) : first;
+    Before all;
+    const Before at = place_piece<N>(x, in, sh, &all);
     if (in) {
-      p.starts[r] = done_t + at.x;
-      p.held_out[r] = fresh < 0 ? 0 : held + add;
+      p.starts[r] = done_t + at.tok;
+      p.held_out[r] = fresh0 < 0 ? 0 : held0 + x.add;
     }
-    __syncthreads();
-    for (int i = tid; i < all.y; i += kPlanThreads) {   // pages taken
-      const int q = last_at_most(take0, n, i);
-      p.tables[(size_t)(r0 + q) * p.max_pages + old_s[q] + i - take0[q]] =
-          p.ring[ring_place(head, done_n + i, p.n_pages)];
+    const int tail = ring_place(head, count, p.n_pages);
+    for (int i0 = tid; i0 < all.tok; i0 += U * N) {   // tokens
+      int i[U], q[U], page[U], pos[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) i[u] = min(i0 + u * N, all.tok - 1);
+      owners<N>(sh.tok0, i, q);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        pos[u] = sh.held[q[u]] + i[u] - sh.tok0[q[u]];
+        const int pg = (int)divide((uint32_t)pos[u], a.per), old = sh.old[q[u]];
+        // a page of this step is read from the ring: its table entry may not be there yet
+        page[u] = *(pg < old ? p.tables + (size_t)(r0 + q[u]) * p.max_pages + pg
+                             : p.ring + ring_place(head, done_n + sh.take0[q[u]] + pg - old, p.n_pages));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * N >= all.tok) break;
+        const int t = done_t + i[u];
+        p.req[t] = r0 + q[u];
+        p.pos[t] = pos[u];
+        p.slot[t] = position_slot(page[u], pos[u], p.n_pages, p.page_size, a.per);
+      }
     }
-    for (int i = tid; i < all.z; i += kPlanThreads) {   // pages given back
-      const int q = last_at_most(back0, n, i);
-      p.ring[ring_place(head, (long long)count + done_b + i, p.n_pages)] =
-          p.tables[(size_t)(r0 + q) * p.max_pages + i - back0[q]];
+    for (int i0 = tid; i0 < all.take; i0 += U * N) {   // pages taken
+      int i[U], q[U], page[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        i[u] = min(i0 + u * N, all.take - 1);
+        page[u] = p.ring[ring_place(head, done_n + i[u], p.n_pages)];
+      }
+      owners<N>(sh.take0, i, q);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * N < all.take)
+          p.tables[(size_t)(r0 + q[u]) * p.max_pages + sh.old[q[u]] + i[u] - sh.take0[q[u]]] = page[u];
     }
-    for (int i = tid; i < all.x; i += kPlanThreads) {   // tokens
-      const int q = last_at_most(tok0, n, i);
-      const int pos = held_s[q] + i - tok0[q], pg = (int)divide((uint32_t)pos, a.per);
-      // a page of this step is read from the ring: its table entry may not be there yet
-      const int page = pg < old_s[q] ? p.tables[(size_t)(r0 + q) * p.max_pages + pg]
-                                     : p.ring[ring_place(head, (long long)done_n + take0[q] + pg - old_s[q], p.n_pages)];
-      p.req[done_t + i] = r0 + q;
-      p.pos[done_t + i] = pos;
-      p.slot[done_t + i] = position_slot(page, pos, p.n_pages, p.page_size, a.per);
+    for (int i0 = tid; i0 < all.back; i0 += U * N) {   // pages given back
+      int i[U], q[U], page[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) i[u] = min(i0 + u * N, all.back - 1);
+      owners<N>(sh.back0, i, q);
+#pragma unroll
+      for (int u = 0; u < U; ++u) page[u] = p.tables[(size_t)(r0 + q[u]) * p.max_pages + i[u] - sh.back0[q[u]]];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * N < all.back) p.ring[ring_place(tail, done_b + i[u], p.n_pages)] = page[u];
     }
-    done_t += all.x;
-    done_n += all.y;
-    done_b += all.z;
+    done_t += all.tok;
+    done_n += all.take;
+    done_b += all.back;
     __syncthreads();
   }
-  for (int i = done_t + tid; i < p.max_tokens; i += kPlanThreads) p.req[i] = p.pos[i] = p.slot[i] = -1;
+  for (int i = done_t + tid; i < p.max_tokens; i += N) p.req[i] = p.pos[i] = p.slot[i] = -1;
   if (tid == 0) {
     p.starts[p.n_req] = done_t;
     p.ring_at_out[0] = ok ? ring_place(head, done_n, p.n_pages) : head;
@@ -223,6 +258,39 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
 
 // ------------------------------------------------------------ heads
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// V values of a cache type, stored at once.
+template <int CT, int V>
+__device__ __forceinline__ void store_values(void* base, long long at, const float (&x)[V]) {
+  if constexpr (CT == MOE_PAGE_F32) {
+    float* p = (float*)base + at;
+    if constexpr (V == 4) *(f32x4*)p = f32x4{x[0], x[1], x[2], x[3]};
+    else *p = x[0];
+  } else if constexpr (CT == MOE_PAGE_E4M3) {
+    // saturated here: the conversion turns what is past 448 into NaN; NaN stays one
+    float c[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = x[i] > 448.0f ? 448.0f : x[i] < -448.0f ? -448.0f : x[i];
+    uint8_t* p = (uint8_t*)base + at;
+    if constexpr (V == 4) {
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+      *(int*)p = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
+    } else {
+      *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[0], 0, false);
+    }
+  } else {
+    uint16_t h[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      h[i] = CT == MOE_PAGE_F16 ? __builtin_bit_cast(uint16_t, (_Float16)x[i]) : __builtin_bit_cast(uint16_t, (__bf16)x[i]);
+    uint16_t* p = (uint16_t*)base + at;
+    if constexpr (V == 4) *(u32x2*)p = u32x2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+    else *p = h[0];
+  }
+}
+
 struct HeadsArgs {
   moe_paged_heads h;
   PageMap map;
@@ -230,14 +298,30 @@ struct HeadsArgs {
   void* v;
   const float* k_scale;
   const float* v_scale;
+  Divider per;   // by the heads of a token
 };
 
-// A block a (token, head) row: norm, rotation, store.
-template <class C>
-__global__ __launch_bounds__(64) void heads_pages_kernel(HeadsArgs a) {
+// Sum over the 16 lanes of a row of lanes.
+__device__ __forceinline__ float row_sum(float x) {
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf, false));   // row_ror 8, 4, 2, 1
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 0xf, 0xf, false));
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x122, 0xf, 0xf, false));
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x121, 0xf, 0xf, false));
+  return x;
+}
+
+// (token, head) rows, 16 lanes each, 16 a block.  A lane holds V neighbouring pairs at a time: pair i is (i, i + half) of
+// the turned values, then two of the rest; so norm, rotation and conversion stay in its registers, and the only sum over
+// lanes is the squares', in fp32.  Bound by the bytes: with V = 4 every access is 16 bytes (8 or 4 into 16- or 8-bit
+// pages); V = 1 where a pointer, a stride or the rotation's width is not a multiple of four.
+template <int CT, int V>
+__global__ __launch_bounds__(256) void heads_pages_kernel(HeadsArgs a) {
+  constexpr int K = 128 / (16 * V);   // a lane's groups of pairs at most (head_dim 256)
   const moe_paged_heads& h = a.h;
-  const int lane = threadIdx.x, hd = a.map.head_dim, H = h.n_q + 2 * a.map.n_kv;
-  const int t = (int)(blockIdx.x / H), head = (int)(blockIdx.x % H);
+  const int hd = a.map.head_dim, H = h.n_q + 2 * a.map.n_kv, lane = threadIdx.x % 16;
+  const uint32_t row = blockIdx.x * 16u + threadIdx.x / 16;
+  const int t = (int)divide(row, a.per), head = (int)row - t * H;
+  if (t >= h.T) return;
   const int slot = h.slot[t], pos = h.pos[t];
   if (slot < 0) return;
   const bool is_q = head < h.n_q, is_v = head >= h.n_q + a.map.n_kv;
@@ -247,49 +331,81 @@ __global__ __launch_bounds__(64) void heads_pages_kernel(HeadsArgs a) {
   if (!is_q && !in) return;
   const float* x = h.qkv + (size_t)t * h.ld + (size_t)head * hd;
   const float* w = is_q ? h.q_norm : is_v ? nullptr : h.k_norm;
-  float inv = 1.0f;
-  if (w) {
-    float s = 0.0f;
-    for (int d = lane; d < hd; d += 64) s = fmaf(x[d], x[d], s);
-    for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
-    inv = 1.0f / sqrtf(s / (float)hd + h.eps);
-  }
   const int half = is_v ? 0 : h.rope_dim / 2, rest = hd / 2 - half;
-  const bool turned = !is_v && (half == 0 || (pos >= 0 && pos < h.rope_len));
-  const float* scale = is_v ? a.v_scale : a.k_scale;
-  const float sc = scale && !is_q ? scale[kv] : 1.0f;
-  for (int i = lane; i < hd / 2; i += 64) {
-    // pair i: turned (i, i + half) of the first rope_dim, else two of the rest
-    const bool rot = i < half;
-    const int e0 = rot ? i : half + i, e1 = rot ? i + half : e0 + rest;
-    float y0 = x[e0], y1 = x[e1];
-    if (w) y0 = y0 * inv * w[e0], y1 = y1 * inv * w[e1];
-    if (rot && turned) {
-      const float c = h.rope_cos[(size_t)pos * half + i], s = h.rope_sin[(size_t)pos * half + i];
-      const float r0 = y0 * c - y1 * s, r1 = y1 * c + y0 * s;
-      y0 = r0, y1 = r1;
-    }
-    if ((!is_v && !turned) || (is_q && !in)) y0 = y1 = NAN;
-    if (is_q) {
-      float* o = h.q_out + (size_t)t * h.ldq + (size_t)head * hd;
-      o[e0] = y0;
-      o[e1] = y1;
+  const bool turned = half == 0 || (pos >= 0 && pos < h.rope_len);
+  auto get = [](const float* p, float (&y)[V]) {
+    if constexpr (V == 4) {
+      const f32x4 v = *(const f32x4*)p;
+      y[0] = v[0], y[1] = v[1], y[2] = v[2], y[3] = v[3];
     } else {
-      typename C::T* o = (typename C::T*)(is_v ? a.v : a.k) + at;
-      if (scale) y0 /= sc, y1 /= sc;
-      o[e0] = C::make(y0);
-      o[e1] = C::make(y1);
+      y[0] = *p;
+    }
+  };
+  float y0[K][V], y1[K][V], ss = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = (lane + 16 * k) * V;
+    if (i >= hd / 2) break;
+    const int e0 = i < half ? i : half + i, e1 = e0 + (i < half ? half : rest);
+    get(x + e0, y0[k]);
+    get(x + e1, y1[k]);
+#pragma unroll
+    for (int c = 0; c < V; ++c) ss = fmaf(y1[k][c], y1[k][c], fmaf(y0[k][c], y0[k][c], ss));
+  }
+  const float inv = w ? 1.0f / sqrtf(row_sum(ss) / (float)hd + h.eps) : 1.0f;
+  const float* scale = is_q ? nullptr : is_v ? a.v_scale : a.k_scale;
+  const float by = scale ? scale[kv] : 1.0f;
+  const bool lost = !turned || (is_q && !in);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = (lane + 16 * k) * V;
+    if (i >= hd / 2) break;
+    const bool turn = i < half;
+    const int e0 = turn ? i : half + i, e1 = e0 + (turn ? half : rest);
+    if (w) {
+      float w0[V], w1[V];
+      get(w + e0, w0);
+      get(w + e1, w1);
+#pragma unroll
+      for (int c = 0; c < V; ++c) y0[k][c] = y0[k][c] * inv * w0[c], y1[k][c] = y1[k][c] * inv * w1[c];
+    }
+    if (turn && turned) {
+      float cs[V], sn[V];
+      get(h.rope_cos + (size_t)pos * half + i, cs);
+      get(h.rope_sin + (size_t)pos * half + i, sn);
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        const float r0 = y0[k][c] * cs[c] - y1[k][c] * sn[c], r1 = y1[k][c] * cs[c] + y0[k][c] * sn[c];
+        y0[k][c] = r0, y1[k][c] = r1;
+      }
+    }
+    if (lost) {
+#pragma unroll
+      for (int c = 0; c < V; ++c) y0[k][c] = y1[k][c] = NAN;
+    }
+    if (is_q) {
+      const long long o = (long long)t * h.ldq + (long long)head * hd;
+      store_values<MOE_PAGE_F32>(h.q_out, o + e0, y0[k]);
+      store_values<MOE_PAGE_F32>(h.q_out, o + e1, y1[k]);
+    } else {
+      if (CT == MOE_PAGE_E4M3 && scale) {
+#pragma unroll
+        for (int c = 0; c < V; ++c) y0[k][c] /= by, y1[k][c] /= by;
+      }
+      void* pool = is_v ? a.v : a.k;
+      store_values<CT>(pool, at + e0, y0[k]);
+      store_values<CT>(pool, at + e1, y1[k]);
     }
   }
 }
 
-// Runs f with the cache's type.
+// Runs f with the cache's type as a constant.
 template <class F>
 void with_type(int dtype, F f) {
-  if (dtype == MOE_PAGE_F32) f(CacheF32{});
-  else if (dtype == MOE_PAGE_F16) f(CacheF16{});
-  else if (dtype == MOE_PAGE_BF16) f(CacheBF16{});
-  else f(CacheE4M3{});
+  if (dtype == MOE_PAGE_F32) f(std::integral_constant<int, MOE_PAGE_F32>{});
+  else if (dtype == MOE_PAGE_F16) f(std::integral_constant<int, MOE_PAGE_F16>{});
+  else if (dtype == MOE_PAGE_BF16) f(std::integral_constant<int, MOE_PAGE_BF16>{});
+  else f(std::integral_constant<int, MOE_PAGE_E4M3>{});
 }
 
 }  // namespace
@@ -316,7 +432,10 @@ moe_status moe_paged_plan_dev(const moe_paged_plan* p) {
   if (st) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream(), PlanArgs{*p, make_divider((uint32_t)p->page_size)});
+  const PlanArgs args{*p, make_divider((uint32_t)p->page_size)};
+  // few requests and tokens: four waves, whose sums and barriers are the shorter
+  if (p->n_req <= 256 && p->max_tokens <= 2048) hipLaunchKernelGGL(plan_kernel<256>, dim3(1), dim3(256), 0, stream(), args);
+  else hipLaunchKernelGGL(plan_kernel<1024>, dim3(1), dim3(1024), 0, stream(), args);
   return check_hip(hipGetLastError(), "paged_plan launch");
 }
 
@@ -333,16 +452,22 @@ moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* g) {
   if (h->rope_dim < 0 || h->rope_dim % 2 || h->rope_dim > map.head_dim || h->rope_len < 0)
     return set_error(MOE_ERR_ARG, "paged_heads: rope_dim %d, rope_len %d", h->rope_dim, h->rope_len);
   if (h->T == 0) return MOE_OK;
-  if (H * h->T > 0x7fffffffll) return set_error(MOE_ERR_ARG, "paged_heads: %d rows of %lld heads", h->T, H);
+  if (H * h->T > 0x7ffffff0ll) return set_error(MOE_ERR_ARG, "paged_heads: %d rows of %lld heads", h->T, H);
   if (!h->qkv || !h->pos || !h->slot || !h->q_out || (h->rope_dim && (!h->rope_cos || !h->rope_sin)))
     return set_error(MOE_ERR_ARG, "paged_heads: null pointer");
   if (h->q_out == h->qkv && h->ldq != h->ld) return set_error(MOE_ERR_ARG, "paged_heads: q_out is qkv with another stride");
   if ((st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
-  const HeadsArgs a{*h, map, g->k, g->v, g->k_scale, g->v_scale};
+  const HeadsArgs a{*h, map, g->k, g->v, g->k_scale, g->v_scale, make_divider((uint32_t)H)};
+  const dim3 grid((unsigned)((H * h->T + 15) / 16));
+  bool four = h->ld % 4 == 0 && h->ldq % 4 == 0 && h->rope_dim % 8 == 0;
+  for (const void* p : {(const void*)h->qkv, (const void*)h->q_out, (const void*)h->q_norm, (const void*)h->k_norm,
+                        (const void*)(h->rope_dim ? h->rope_cos : nullptr), (const void*)(h->rope_dim ? h->rope_sin : nullptr)})
+    four = four && aligned(p, 16);
   with_type(g->dtype, [&](auto c) {
-    hipLaunchKernelGGL(heads_pages_kernel<decltype(c)>, dim3((unsigned)(H * h->T)), dim3(64), 0, stream(), a);
+    if (four) hipLaunchKernelGGL((heads_pages_kernel<decltype(c)::value, 4>), grid, dim3(256), 0, stream(), a);
+    else hipLaunchKernelGGL((heads_pages_kernel<decltype(c)::value, 1>), grid, dim3(256), 0, stream(), a);
   });
   return check_hip(hipGetLastError(), "paged_heads launch");
 }

@@ -60,7 +60,7 @@ static void rows() {
       if (position_slot(3, p, 10, ps, per) != 3 * ps + p % ps) fail("position_slot", p, ps, 0);
       for (int page : {-1, 10, 11, (int)0x80000000})   // no page: the first slot behind the cache
         if (position_slot(page, p, 10, ps, per) != 10 * ps) fail("position_slot", p, page, 0);
-      if (pages_for(p, ps) != p / ps + (p % ps != 0)) fail("pages_for", p, ps, 0);
+      if (pages_for(p, per) != p / ps + (p % ps != 0)) fail("pages_for", p, ps, 0);
     }
   }
 }
@@ -81,8 +81,9 @@ static void plans() {
   }
   for (int n : {1, 2, 7, 100})
     for (int from = 0; from < n; ++from)
-      for (int i = 0; i <= 2 * n; ++i)
+      for (int i = 0; i <= n; ++i)
         if (ring_place(from, i, n) != (from + i) % n) fail("ring_place", from, i, n);
+  if (pages_for(0x7fffffff, make_divider(1)) != 0x7fffffff) fail("pages_for", 0, 0, 0);
   if (ring_place(0x7ffffffe, 0x7fffffff, 0x7fffffff) != 0x7ffffffe) fail("ring_place", 0, 0, 0);
 }
 
