@@ -84,7 +84,7 @@ struct Before {
 
 template <int N>
 struct PlanShared {
-  long long sum[N / kWave][3];
+  double sum[N / kWave][3];
   int odd[N / kWave];
   Before wave[N / kWave];
   int tok0[N], take0[N], back0[N], old[N], held[N];
@@ -114,16 +114,41 @@ __device__ __forceinline__ Before place_piece(const Request& r, bool in, PlanSha
   return at;
 }
 
-// U items at once: the last request that starts at or before each (first ascending, its first entry 0).
-template <int N, int U>
-__device__ __forceinline__ void owners(const int* first, const int (&item)[U], int (&q)[U]) {
+// Four neighbouring items: for each the last request that starts at or before it (first ascending, its first entry 0).
+// N = 1024, where the LDS reads of sixteen waves bound it: the inner two are sought only where the outer two differ;
+// else all side by side.
+constexpr int U = 4;
+template <int N>
+__device__ __forceinline__ void owners(const int* first, int item, int last, int (&i)[U], int (&q)[U]) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) q[u] = 0;
+  for (int u = 0; u < U; ++u) i[u] = min(item + u, last), q[u] = 0;
 #pragma unroll
-  for (int s = N / 2; s; s /= 2)
+  for (int s = N / 2; s; s /= 2) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (first[q[u] + s] <= item[u]) q[u] += s;
+    for (int u = 0; u < U; u += N < 1024 ? 1 : U - 1)
+      if (first[q[u] + s] <= i[u]) q[u] += s;
+  }
+  if (N < 1024) return;
+  q[1] = q[2] = q[0];
+  if (q[0] != q[3]) {
+    q[1] = q[2] = 0;
+#pragma unroll
+    for (int s = N / 2; s; s /= 2) {
+      if (first[q[1] + s] <= i[1]) q[1] += s;
+      if (first[q[2] + s] <= i[2]) q[2] += s;
+    }
+  }
+}
+
+typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// x to p[0 .. 3], the first n of them.
+__device__ __forceinline__ void store4(int32_t* p, const int (&x)[U], int n) {
+  if (n >= U) *(i32x4u*)p = i32x4u{x[0], x[1], x[2], x[3]};
+  else
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (u < n) p[u] = x[u];
 }
 
 // One block, as the step is done in place: requests in pieces of one a thread.  First the totals, which say whether the
@@ -132,7 +157,6 @@ __device__ __forceinline__ void owners(const int* first, const int (&item)[U], i
 // levels of loads and the sums; 64 requests, 64 tokens: see DESIGN
 template <int N>
 __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
-  constexpr int U = 4;
   const moe_paged_plan& p = a.p;
   __shared__ PlanShared<N> sh;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -153,21 +177,18 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
   };
   int odd = 0;
   Request first = request(held0, fresh0, &odd);
-  long long sum[3] = {first.add, first.need, first.back};
+  double sum[3] = {(double)first.add, (double)first.need, (double)first.back};
   for (int r = tid + N; r < p.n_req; r += N) {
     const Request x = request(p.held[r], p.fresh[r], &odd);
     sum[0] += x.add, sum[1] += x.need, sum[2] += x.back;
   }
+  const int odds = (__any(odd & 1) ? 1 : 0) | (__any(odd & 2) ? 2 : 0);
 #pragma unroll
-  for (int d = kWave / 2; d; d /= 2) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) sum[i] += __shfl_xor(sum[i], d);
-    odd |= __shfl_xor(odd, d);
-  }
+  for (int i = 0; i < 3; ++i) sum[i] = group_sum_f64<kWave>(sum[i]);   // (whole numbers below 2^53: exact)
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) sh.sum[wave][i] = sum[i];
-    sh.odd[wave] = odd;
+    sh.odd[wave] = odds;
   }
   __syncthreads();
   sum[0] = sum[1] = sum[2] = odd = 0;
@@ -177,7 +198,7 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
     for (int i = 0; i < 3; ++i) sum[i] += sh.sum[w][i];
     odd |= sh.odd[w];
   }
-  const int status = plan_status(odd & 1, odd & 2, sum[0], sum[1], sum[2], head, count, p.n_pages, p.max_tokens);
+  const int status = plan_status(odd & 1, odd & 2, (long long)sum[0], (long long)sum[1], (long long)sum[2], head, count, p.n_pages, p.max_tokens);
   const bool ok = status == kPlanOk;
   int done_t = 0, done_n = 0, done_b = 0;   // tokens and pages of the pieces before
   for (int r0 = 0; r0 < p.n_req; r0 += N) {
@@ -196,11 +217,9 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
       p.held_out[r] = fresh0 < 0 ? 0 : held0 + x.add;
     }
     const int tail = ring_place(head, count, p.n_pages);
-    for (int i0 = tid; i0 < all.tok; i0 += U * N) {   // tokens
+    for (int i0 = tid * U; i0 < all.tok; i0 += U * N) {   // tokens
       int i[U], q[U], page[U], pos[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) i[u] = min(i0 + u * N, all.tok - 1);
-      owners<N>(sh.tok0, i, q);
+      owners<N>(sh.tok0, i0, all.tok - 1, i, q);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         pos[u] = sh.held[q[u]] + i[u] - sh.tok0[q[u]];
@@ -211,43 +230,40 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (i0 + u * N >= all.tok) break;
-        const int t = done_t + i[u];
-        p.req[t] = r0 + q[u];
-        p.pos[t] = pos[u];
-        p.slot[t] = position_slot(page[u], pos[u], p.n_pages, p.page_size, a.per);
+        page[u] = position_slot(page[u], pos[u], p.n_pages, p.page_size, a.per);
+        q[u] += r0;
       }
+      store4(p.req + done_t + i0, q, all.tok - i0);
+      store4(p.pos + done_t + i0, pos, all.tok - i0);
+      store4(p.slot + done_t + i0, page, all.tok - i0);
     }
-    for (int i0 = tid; i0 < all.take; i0 += U * N) {   // pages taken
+    for (int i0 = tid * U; i0 < all.take; i0 += U * N) {   // pages taken
       int i[U], q[U], page[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        i[u] = min(i0 + u * N, all.take - 1);
-        page[u] = p.ring[ring_place(head, done_n + i[u], p.n_pages)];
-      }
-      owners<N>(sh.take0, i, q);
+      for (int u = 0; u < U; ++u) page[u] = p.ring[ring_place(head, done_n + min(i0 + u, all.take - 1), p.n_pages)];
+      owners<N>(sh.take0, i0, all.take - 1, i, q);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (i0 + u * N < all.take)
+        if (i0 + u < all.take)
           p.tables[(size_t)(r0 + q[u]) * p.max_pages + sh.old[q[u]] + i[u] - sh.take0[q[u]]] = page[u];
     }
-    for (int i0 = tid; i0 < all.back; i0 += U * N) {   // pages given back
+    for (int i0 = tid * U; i0 < all.back; i0 += U * N) {   // pages given back
       int i[U], q[U], page[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) i[u] = min(i0 + u * N, all.back - 1);
-      owners<N>(sh.back0, i, q);
+      owners<N>(sh.back0, i0, all.back - 1, i, q);
 #pragma unroll
       for (int u = 0; u < U; ++u) page[u] = p.tables[(size_t)(r0 + q[u]) * p.max_pages + i[u] - sh.back0[q[u]]];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (i0 + u * N < all.back) p.ring[ring_place(tail, done_b + i[u], p.n_pages)] = page[u];
+        if (i0 + u < all.back) p.ring[ring_place(tail, done_b + i[u], p.n_pages)] = page[u];
     }
     done_t += all.tok;
     done_n += all.take;
     done_b += all.back;
     __syncthreads();
   }
-  for (int i = done_t + tid; i < p.max_tokens; i += N) p.req[i] = p.pos[i] = p.slot[i] = -1;
+  const int none[U] = {-1, -1, -1, -1};
+  for (int i = done_t + tid * U; i < p.max_tokens; i += U * N)
+    for (int32_t* to : {p.req, p.pos, p.slot}) store4(to + i, none, p.max_tokens - i);
   if (tid == 0) {
     p.starts[p.n_req] = done_t;
     p.ring_at_out[0] = ok ? ring_place(head, done_n, p.n_pages) : head;
