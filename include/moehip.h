@@ -493,6 +493,23 @@ typedef struct {
 size_t moe_paged_attn_work_bytes(int T, int n_q, int n_kv, int head_dim);
 moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* pages);
 
+/* One step of a model over many requests, instead of moe_model_forward's one
+ * sequence: moe_paged_plan_dev(plan), then every layer with the tokens' keys
+ * and values in layers[0 .. n_layers - 1] (a host array; each n_pages pages of
+ * page_size positions, the model's heads; head_dim a multiple of 16), then
+ * the head.  ids [max_tokens] (device): request r's new tokens at the rows
+ * the plan gives it, in order of the requests; ids outside [0, vocab) are
+ * clamped, rows behind the last token may hold anything.  logits [n_req x
+ * vocab]: of each request's last new token (a request without new tokens: of
+ * a zero row); next [n_req]: moe_greedy_dev's choice on them (without new
+ * tokens: -1).  Either may be NULL.  A position at or past the model's
+ * max_seq makes its logits NaN.  Prompts and single tokens may share a step;
+ * every one of the max_tokens rows is computed, so a step is as dear as it.
+ * The model's own position and cache are not touched.  Scratch grows on the
+ * first call of a size, outside of any capture. */
+moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
+                                const int32_t* ids, float* logits, int32_t* next);
+
 /* Name of the kernel variant the GEMV entry points use for a shape. */
 const char* moe_gemv_variant(int dtype, int M, int N, int K);
 

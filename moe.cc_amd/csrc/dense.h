@@ -132,6 +132,10 @@ moe_status attention_rows(const AttnArgs& a, hipStream_t s);
 moe_status greedy_vec(const float* v, int n, const float* part, int rows, int32_t* out,
                       int32_t* out_hist, int32_t* hist_pos, hipStream_t s);
 
+// The same choice for each row of v [rows][n]; -1 for a row r of a request
+// without tokens (starts[r] == starts[r + 1], device memory).
+moe_status greedy_rows(const float* v, int n, int rows, const int32_t* starts, int32_t* out, hipStream_t s);
+
 // softmax_rows (test_model_trace.c:260-272) of one row of n values in place.
 moe_status softmax_vec(float* v, int n, hipStream_t s);
 

@@ -1681,6 +1681,41 @@ __global__ __launch_bounds__(kGreedyThreads) void greedy_kernel(const float* __r
   }
 }
 
+// greedy_kernel's choice for row blockIdx.x of v [rows][n]; a request without
+// tokens (starts[r] == starts[r + 1]) gets -1.
+__global__ __launch_bounds__(kGreedyThreads) void greedy_rows_kernel(const float* __restrict__ v, int n,
+                                                                    const int32_t* __restrict__ starts,
+                                                                    int32_t* __restrict__ out) {
+  __shared__ float fred[kGreedyThreads / kWave];
+  __shared__ int ired[kGreedyThreads / kWave];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const size_t r = blockIdx.x;
+  if (starts[r] == starts[r + 1]) {
+    if (tid == 0) out[r] = -1;
+    return;
+  }
+  v += r * n;
+  float mx = -__builtin_inff();
+#pragma unroll 8
+  for (int i = tid; i < n; i += kGreedyThreads) mx = nan_max(mx, v[i]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = nan_max(mx, __shfl_xor(mx, off, kWave));
+  if (lane == 0) fred[wave] = mx;
+  __syncthreads();
+  float m = fred[0];
+  for (int w = 1; w < kGreedyThreads / kWave; ++w) m = nan_max(m, fred[w]);
+  int first = INT_MAX;
+  if (m == m && m != __builtin_inff() && m != -__builtin_inff()) {
+#pragma unroll 8
+    for (int i = tid; i < n; i += kGreedyThreads) {
+      const float d = v[i] - m;
+      if (!(d < -1e-6f) && i < first && expf_glibc(d) == 1.0f) first = i;
+    }
+  }
+  first = block_min(first, ired);
+  if (tid == 0) out[r] = first == INT_MAX ? 0 : first;
+}
+
 constexpr int kSmThreads = 1024;
 constexpr int kSmChunk = 8192;
 
@@ -2090,6 +2125,11 @@ moe_status greedy_vec(const float* v, int n, const float* part, int rows, int32_
   hipLaunchKernelGGL(greedy_kernel, dim3(1), dim3(kGreedyThreads), 0, s, v, n, part, rows, out,
                      out_hist, hist_pos);
   return check_hip(hipGetLastError(), "greedy launch");
+}
+
+moe_status greedy_rows(const float* v, int n, int rows, const int32_t* starts, int32_t* out, hipStream_t s) {
+  hipLaunchKernelGGL(greedy_rows_kernel, dim3((unsigned)rows), dim3(kGreedyThreads), 0, s, v, n, starts, out);
+  return check_hip(hipGetLastError(), "greedy rows launch");
 }
 
 moe_status softmax_vec(float* v, int n, hipStream_t s) {

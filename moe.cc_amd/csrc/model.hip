@@ -28,6 +28,7 @@
 
 #include "dense.h"
 #include "moe_lib.h"
+#include "paged_attn.h"
 
 using namespace moe;
 
@@ -67,6 +68,7 @@ struct moe_model {
   float* rope_sin = nullptr;
   // per-forward scratch, grown on demand
   Buf x, xa, xn, qkv, H, S, ids;
+  Buf last, last_logits, attn_work;   // of steps over a paged cache
   float* xf = nullptr;
   float* logits = nullptr;
   float* head_part = nullptr;   // block maxima of the head's product
@@ -126,7 +128,8 @@ void free_model(moe_model* m) {
   dfree(m->tok_emb); dfree(m->final_norm); dfree(m->kc); dfree(m->vc);
   dfree(m->rope_cos); dfree(m->rope_sin); dfree(m->xf); dfree(m->logits);
   dfree(m->head_part); dfree(m->next); dfree(m->hist_pos);
-  for (Buf* b : {&m->x, &m->xa, &m->xn, &m->qkv, &m->H, &m->S, &m->ids, &m->hist})
+  for (Buf* b : {&m->x, &m->xa, &m->xn, &m->qkv, &m->H, &m->S, &m->ids, &m->hist, &m->last,
+                 &m->last_logits, &m->attn_work})
     if (b->p) (void)hipFree(b->p);
   delete m;
 }
@@ -285,6 +288,61 @@ moe_status forward_checked(moe_model* m, const int32_t* ids, int T, int ids_on_d
     ids_d = (const int32_t*)m->ids.p;
   }
   return forward_dev(m, ids_d, T, logits_out, next_out, false);
+}
+
+// One step over a paged cache: forward_dev's layers with each token at its
+// own request's position, K and V in the requests' pages.
+moe_status step_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* layers, const int32_t* ids,
+                      float* logits, int32_t* next) {
+  const QwenConfig& c = m->cfg;
+  hipStream_t s = stream();
+  const int D = c.d_model, T = p->max_tokens, R = p->n_req;
+  const float eps = c.rms_eps;
+  const size_t td = (size_t)T * D * 4, rd = (size_t)R * D * 4;
+  const size_t work = moe_paged_attn_work_bytes(T, c.n_q, c.n_kv, c.head_dim);
+  moe_status st;
+  if ((st = grow(m->x, td)) || (st = grow(m->xa, td)) || (st = grow(m->xn, td)) ||
+      (st = grow(m->qkv, (size_t)T * m->nqkv * 4)) || (st = grow(m->H, (size_t)T * m->Dq * 4)) ||
+      (st = grow(m->last, 2 * rd)) || (st = grow(m->attn_work, work)) ||
+      (!logits && (st = grow(m->last_logits, (size_t)R * c.vocab_size * 4))))
+    return st;
+  if ((st = moe_paged_plan_dev(p))) return st;
+  float* x = (float*)m->x.p;
+  float* xa = (float*)m->xa.p;
+  float* xn = (float*)m->xn.p;
+  float* qkv = (float*)m->qkv.p;
+  float* H = (float*)m->H.p;
+  if ((st = embed_rows(ids, T, m->tok_emb, c.vocab_size, D, x, s))) return st;
+  for (int l = 0; l < c.n_layers; ++l) {
+    DevLayer& L = m->layers[l];
+    DenseArgs qa{xn, D, L.wqkv, D, L.bqkv, nullptr, 0, qkv, m->nqkv, T, m->nqkv, D};
+    if (dense_norm_ok(T, D)) {
+      qa.A = x;
+      qa.norm = 1; qa.norm_w = L.rms1; qa.eps = eps;
+    } else if ((st = moe_rmsnorm_dev(x, L.rms1, xn, T, D, eps))) {
+      return st;
+    }
+    if ((st = dense_matmul(qa, s))) return st;
+    const moe_paged_heads ha{qkv, m->nqkv, T, c.n_q, p->pos, p->slot, L.q_norm, L.k_norm, eps, m->rope_cos, m->rope_sin,
+                             m->max_seq, c.head_dim, qkv, m->nqkv};
+    if ((st = moe_paged_heads_dev(&ha, &layers[l]))) return st;
+    const moe_paged_attn aa{qkv, m->nqkv, T, c.n_q, p->req, p->pos, p->tables, R, p->max_pages, m->scale, H, m->Dq,
+                            m->attn_work.p, work};
+    if ((st = moe_paged_attn_dev(&aa, &layers[l]))) return st;
+    DenseArgs oa{H, m->Dq, L.wo, m->Dq, L.bo, x, D, xa, D, T, D, m->Dq};
+    if ((st = dense_matmul(oa, s))) return st;
+    if ((st = moe_block_forward(L.moe, xa, T, x, eps))) return st;
+  }
+  // the last row of each request through the final norm and the head
+  float* xl = (float*)m->last.p;
+  float* xf = xl + (size_t)R * D;
+  float* lg = logits ? logits : (float*)m->last_logits.p;
+  if ((st = check_hip(launch_last_rows(x, p->starts, R, D, xl, s), "last rows launch")) ||
+      (st = moe_rmsnorm_dev(xl, m->final_norm, xf, R, D, eps)))
+    return st;
+  DenseArgs ha{xf, D, m->lm_head, D, nullptr, nullptr, 0, lg, c.vocab_size, R, c.vocab_size, D};
+  if ((st = dense_matmul(ha, s))) return st;
+  return next ? greedy_rows(lg, c.vocab_size, R, p->starts, next, s) : MOE_OK;
 }
 
 // ---- QW3W file (io.c:193-285) ----
@@ -776,6 +834,22 @@ moe_status moe_model_forward(moe_model* m, const int32_t* ids, int T, int ids_on
   if (!m || !ids) return set_error(MOE_ERR_ARG, "model_forward: null argument");
   std::lock_guard<std::mutex> lk(m->mu);
   return forward_checked(m, ids, T, ids_on_device, logits_dev, next_dev);
+}
+
+moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
+                                const int32_t* ids, float* logits, int32_t* next) {
+  if (!m || !plan || !layers || !ids || (!logits && !next)) return set_error(MOE_ERR_ARG, "step_paged: null argument");
+  if (plan->n_req < 1 || plan->max_tokens < 1)
+    return set_error(MOE_ERR_ARG, "step_paged: %d requests, %d tokens", plan->n_req, plan->max_tokens);
+  for (int l = 0; l < m->cfg.n_layers; ++l)
+    if (layers[l].n_kv != m->cfg.n_kv || layers[l].head_dim != m->cfg.head_dim || layers[l].n_pages != plan->n_pages ||
+        layers[l].page_size != plan->page_size)
+      return set_error(MOE_ERR_ARG, "step_paged: layer %d has %d pages of %d positions, %d heads of %d", l, layers[l].n_pages,
+                       layers[l].page_size, layers[l].n_kv, layers[l].head_dim);
+  moe_status st = ensure_init();
+  if (st) return st;
+  std::lock_guard<std::mutex> lk(m->mu);
+  return step_paged(m, plan, layers, ids, logits, next);
 }
 
 moe_status moe_model_forward_full(moe_model* m, const int32_t* ids, int T, int apply_softmax,

@@ -415,6 +415,14 @@ __global__ __launch_bounds__(256) void heads_pages_kernel(HeadsArgs a) {
   }
 }
 
+__global__ __launch_bounds__(256) void last_rows_kernel(const float* __restrict__ x, const int32_t* __restrict__ starts,
+                                                       int D, float* __restrict__ out) {
+  const size_t r = blockIdx.x;
+  const int first = starts[r], next = starts[r + 1];
+  const float* src = x + (size_t)max(next - 1, 0) * D;
+  for (int i = threadIdx.x; i < D; i += 256) out[r * D + i] = next > first ? src[i] : 0.0f;
+}
+
 // Runs f with the cache's type as a constant.
 template <class F>
 void with_type(int dtype, F f) {
@@ -425,6 +433,12 @@ void with_type(int dtype, F f) {
 }
 
 }  // namespace
+
+hipError_t launch_last_rows(const float* x, const int32_t* starts, int n_req, int D, float* out, hipStream_t s) {
+  hipLaunchKernelGGL(last_rows_kernel, dim3((unsigned)n_req), dim3(256), 0, s, x, starts, D, out);
+  return hipGetLastError();
+}
+
 }  // namespace moe
 
 using namespace moe;

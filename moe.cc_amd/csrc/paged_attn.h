@@ -21,4 +21,8 @@ struct AttnPages {
 size_t paged_attn_work(int T, int n_q, int n_kv, int head_dim);
 hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t stream);
 
+// x row of each request's last token (zeros for one without tokens): out
+// [n_req][D] from x [.][D] at starts[r + 1] - 1.
+hipError_t launch_last_rows(const float* x, const int32_t* starts, int n_req, int D, float* out, hipStream_t stream);
+
 }  // namespace moe

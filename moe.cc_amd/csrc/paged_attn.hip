@@ -604,11 +604,11 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   }
 }
 
-// A block a (cut row, query head): its parts joined, four dimensions a thread, so that WAVES 64 / (head_dim / 4) parts are
-// read side by side.  Latency: the parts' first rows are requested with their maxima.
+// A block a (cut row, query head, `slice` dimensions): its parts joined, four dimensions a thread, so that WAVES 64 /
+// (slice / 4) parts are read side by side.  Latency: the parts' first rows are requested with their maxima.
 constexpr int kMaxParts = 3 * kCUs;   // of one row: no more than pieces
 template <int WAVES>
-__global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L) {
+__global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L, int slice) {
   constexpr int N = WAVES * kWave, U = 4;
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
@@ -617,7 +617,7 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L)
   const int parts = r.y;
   if (parts <= 1) return;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int width = hd / 4, rows = N / width, row = tid / width, d = tid % width * 4;
+  const int width = slice / 4, rows = N / width, row = tid / width, d = (int)blockIdx.z * slice + tid % width * 4;
   __shared__ float by_s[WAVES][kMaxParts];
   __shared__ f32x4 acc_s[N];
   const float* ml = L.part_ml + (size_t)head * 2;
@@ -726,9 +726,10 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
                                        : launch<E4M3>(L, whole, stream, grid, s);
   if (e != hipSuccess || !L.pieces) return e;
   // few rows may have many parts each
-  const dim3 joins(L.by_row ? (unsigned)a.T : grid.x, (unsigned)a.n_q);
-  if (a.T <= 16) hipLaunchKernelGGL(paged_join_kernel<4>, joins, dim3(4 * kWave), 0, s, L);
-  else hipLaunchKernelGGL(paged_join_kernel<1>, joins, dim3(kWave), 0, s, L);
+  const int slice = a.T > 4 ? map.head_dim : map.head_dim % 32 ? 16 : 32;
+  const dim3 joins(L.by_row ? (unsigned)a.T : grid.x, (unsigned)a.n_q, (unsigned)(map.head_dim / slice));
+  if (a.T <= 16) hipLaunchKernelGGL(paged_join_kernel<4>, joins, dim3(4 * kWave), 0, s, L, slice);
+  else hipLaunchKernelGGL(paged_join_kernel<1>, joins, dim3(kWave), 0, s, L, slice);
   return hipGetLastError();
 }
 

@@ -154,6 +154,7 @@ _SIGS = {
     "moe_model_position": (_I, [_P]),
     "moe_model_forward": (_I, [_P, _P, _I, _I, _P, _P]),
     "moe_model_forward_full": (_I, [_P, _P, _I, _I, _P]),
+    "moe_model_step_paged": (_I, [_P] * 6),
     "moe_model_generate": (_I, [_P, _P, _I, _I, _P, ctypes.POINTER(ctypes.c_float),
                                 ctypes.POINTER(ctypes.c_float)]),
 }
@@ -382,6 +383,57 @@ class MoeLayer:
             pass
 
 
+# ---------------- many requests over a paged cache ----------------
+
+class PagedCache:
+    """Pages of every layer and the book-keeping of `n_req` requests on the
+    device: what moe_paged_plan_dev and moe_model_step_paged work on.
+
+    ``layers`` is an array of Pages (slot-major, one K and one V pool a
+    layer), ``plan`` the PagedPlan whose state is updated in place; the free
+    pages are 0 .. n_pages - 1 in order at the start."""
+
+    def __init__(self, n_layers, n_kv, head_dim, n_pages, page_size, n_req, max_pages, max_tokens,
+                 dtype=PAGE_F32, k_scale=None, v_scale=None):
+        self.n_req, self.max_tokens = n_req, max_tokens
+        side = n_pages * page_size * n_kv * head_dim * {PAGE_F32: 4, PAGE_E4M3: 1}.get(dtype, 2)
+        self._pools = [DeviceBuffer(2 * side) for _ in range(n_layers)]
+        self._scales = [None if s is None else DeviceBuffer.from_array(_f32(s))
+                        for s in (k_scale, v_scale)]
+        self.layers = (Pages * n_layers)(*[
+            Pages(b.ptr, b.ptr + side, dtype, n_pages, page_size, n_kv, head_dim,
+                  page_size * n_kv * head_dim, head_dim, n_kv * head_dim,
+                  *[None if s is None else s.ptr for s in self._scales]) for b in self._pools])
+        i32 = np.int32
+        self._b = {"ring": np.arange(n_pages, dtype=i32), "ring_at": np.array([0, n_pages], i32),
+                   "tables": np.full((n_req, max_pages), -1, i32), "held": np.zeros(n_req, i32),
+                   "fresh": np.zeros(n_req, i32), "starts": np.zeros(n_req + 1, i32),
+                   "req": np.zeros(max_tokens, i32), "pos": np.zeros(max_tokens, i32),
+                   "slot": np.zeros(max_tokens, i32), "status": np.zeros(1, i32),
+                   "ids": np.zeros(max_tokens, i32)}
+        self._b = {n: DeviceBuffer.from_array(a) for n, a in self._b.items()}
+        p = {n: b.ptr for n, b in self._b.items()}
+        self.plan = PagedPlan(n_req, max_pages, n_pages, page_size, max_tokens, p["fresh"], p["held"],
+                              p["ring_at"], p["ring"], p["tables"], p["held"], p["ring_at"],
+                              p["starts"], p["req"], p["pos"], p["slot"], p["status"])
+
+    def set_step(self, fresh, ids):
+        """New tokens of each request (-1: it ended) and their ids, request after request."""
+        fresh, ids = np.asarray(fresh, np.int32), np.asarray(ids, np.int32)
+        if fresh.shape != (self.n_req,) or ids.size > self.max_tokens:
+            raise MoeError(f"a step of {fresh.size} requests and {ids.size} tokens")
+        self._b["fresh"].upload(fresh)
+        self._b["ids"].upload(ids)
+
+    def array(self, name, *shape) -> np.ndarray:
+        """A copy of one of the plan's arrays."""
+        return self._b[name].download(shape, np.int32)
+
+    @property
+    def status(self) -> int:
+        return int(self.array("status", 1)[0])
+
+
 # ---------------- the whole model (test_model_trace.c:526-579) ----------------
 
 class QwenConfig(ctypes.Structure):
@@ -499,6 +551,15 @@ class Model:
         check(lib().moe_model_forward_full(self.h, ids.ctypes.data, ids.size, int(apply_softmax),
                                            out.ctypes.data), "moe_model_forward_full")
         return out
+
+    def step_paged(self, cache: PagedCache, fresh, ids):
+        """One step over many requests -> (logits [n_req, V], next ids [n_req])."""
+        cache.set_step(fresh, ids)
+        lg = DeviceBuffer(cache.n_req * self.V * 4)
+        nx = DeviceBuffer(cache.n_req * 4)
+        check(lib().moe_model_step_paged(self.h, ctypes.byref(cache.plan), cache.layers,
+                                         cache._b["ids"].ptr, lg.ptr, nx.ptr), "moe_model_step_paged")
+        return lg.download((cache.n_req, self.V), np.float32), nx.download((cache.n_req,), np.int32)
 
     def generate(self, prompt, n_new):
         """-> (ids [n_new], ms_prompt, ms_decode)"""
