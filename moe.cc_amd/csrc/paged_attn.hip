@@ -62,6 +62,7 @@ struct AttnLaunch {
   AttnPages g;
   int head_tiles;   // of 16 query heads, a key-value head
   int pieces;       // 0: rows are not cut, a block a row
+  Divider each;     // by the pieces
   int by_row;       // joins are listed a row (T <= pieces) or a piece
   int4* joins;      // [min(T, pieces)] work: row, parts, the piece its first lies in; of a piece: of the row that ends there
   float* part_ml;   // [2 pieces][n_q][2] work: maximum and sum of a part
@@ -120,7 +121,7 @@ struct PieceShared {
   Piece piece;
 };
 
-// Finds piece b; PER rows a thread.  The host sees to it that the units' sum fits 32 bits.
+// Finds piece b; PER rows a thread.  The host sees to it that the units' sum and the pieces fit 31 bits.
 template <int PER>
 __device__ __forceinline__ void find_first(const AttnLaunch& L, uint32_t b, PieceShared& sh) {
   const AttnPages& g = L.g;
@@ -153,7 +154,7 @@ __device__ __forceinline__ void find_first(const AttnLaunch& L, uint32_t b, Piec
     if (w < wave) at += sh.scan[w];
     total += sh.scan[w];
   }
-  const uint32_t each = (total + L.pieces - 1) / L.pieces, begin = b * each;   // (b < pieces: no overflow past total + pieces)
+  const uint32_t each = divide(total + L.pieces - 1, L.each), begin = b * each;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const uint32_t n = units_of(len[i]);
@@ -171,6 +172,21 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch& L, int b, Piece* ou
     const uint32_t n = units_of(len);
     *out = Piece{0, n, n, b, req, len, 0};
     return n > 0;
+  }
+  if (a.T <= kWave) {   // every wave by itself, a row a lane
+    const int lane = threadIdx.x % kWave, t = min(lane, a.T - 1);
+    const int req = a.req ? a.req[t] : t, len = lane < a.T ? length_of(g, req, a.pos[t]) : kNone;
+    const uint32_t n = units_of(len), scan = wave_scan(n), at = scan - n;
+    const uint32_t total = __builtin_amdgcn_readlane(scan, kWave - 1);
+    if (len == kPadding && L.by_row && b == 0 && blockIdx.y == 0 && threadIdx.x < kWave) L.joins[lane] = int4{0, 0, 0, 0};
+    if (!L.by_row && blockIdx.y == 0 && threadIdx.x == 0) L.joins[b] = int4{0, 0, 0, 0};
+    const uint32_t each = divide(total + L.pieces - 1, L.each), begin = (uint32_t)b * each;
+    const uint64_t mine = __ballot(begin >= at && begin - at < n);
+    if (!mine) return false;
+    const int row = __builtin_ctzll(mine);
+    *out = Piece{begin, min(begin + each, total), each, row, __builtin_amdgcn_readlane(req, row),
+                 __builtin_amdgcn_readlane(len, row), (uint32_t)__builtin_amdgcn_readlane(at, row)};
+    return true;
   }
   __shared__ PieceShared sh;
   if (a.T <= kThreads) find_first<1>(L, (uint32_t)b, sh);
@@ -556,7 +572,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   const size_t part = (size_t)part_place((int)blockIdx.x - (unit0 != 0), unit0 != 0);
   __shared__ float div_s[16];
   if (wave == 0 && quad == 0) {
-    div_s[col] = sum;
+    div_s[col] = sum == 0.0f ? 0.0f : vs / sum;
     if (cut && col < heads) {
       float* ml = L.part_ml + (part * a.n_q + head0 + col) * 2;
       ml[0] = top;
@@ -586,8 +602,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
       if (cut) {
         L.part_o[(part * a.n_q + head0 + h) * hd + d] = y;
       } else {
-        const float z = div_s[h];
-        a.out[(size_t)pc.row * a.ldo + (size_t)(head0 + h) * hd + d] = z == 0.0f ? 0.0f : y / z * vs;
+        a.out[(size_t)pc.row * a.ldo + (size_t)(head0 + h) * hd + d] = y * div_s[h];
       }
     }
     if (ps + 1 < PASS) __syncthreads();
@@ -629,13 +644,19 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L,
     const int i = row + c * rows;
     y[c] = *(const f32x4*)(o + part_place(r.z, i < parts ? i : 0) * next);
   }
-  // what each part counts for; every wave for itself
-  float top = -INFINITY, sum = 0.0f;
-  for (int i = lane; i < parts; i += kWave) top = fmaxf(top, ml[part_place(r.z, i) * step]);
+  // what each part counts for; every wave for itself, the first 64 parts' numbers kept between the two passes
+  const float* mine = ml + part_place(r.z, min(lane, parts - 1)) * step;
+  const float m0 = mine[0], l0 = mine[1];
+  float top = m0, sum = 0.0f;
+  for (int i = lane + kWave; i < parts; i += kWave) top = fmaxf(top, ml[part_place(r.z, i) * step]);
 #pragma unroll
   for (int c = 32; c; c /= 2) top = fmaxf(top, __shfl_xor(top, c));
   if (top == -INFINITY) top = 0.0f;
-  for (int i = lane; i < parts; i += kWave) {
+  if (lane < parts) {
+    by_s[wave][lane] = exp2_hw(m0 - top);
+    sum = l0 * exp2_hw(m0 - top);
+  }
+  for (int i = lane + kWave; i < parts; i += kWave) {
     const float* p = ml + part_place(r.z, i) * step;
     const float f = exp2_hw(p[0] - top);
     by_s[wave][i] = f;
@@ -711,7 +732,8 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   // rows that no piece can cut (a unit at most), and more than a block's search takes, get a block each
   const long long units = ((long long)a.max_pages * map.page_size + kUnit - 1) / kUnit * a.T;   // at most
   const int most = pieces_for(a.n_q, map.n_kv, map.head_dim);
-  L.pieces = units > a.T && units <= 0xffff0000ll && a.T <= kSplitRows ? most : 0;
+  L.pieces = units > a.T && units <= 0x7fff0000ll && a.T <= kSplitRows ? most : 0;
+  L.each = make_divider((uint32_t)most);
   L.by_row = a.T <= most;
   L.joins = (int4*)a.work;
   L.part_o = (float*)(L.joins + (L.by_row ? a.T : most));
