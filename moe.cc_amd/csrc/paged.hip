@@ -114,11 +114,10 @@ __device__ __forceinline__ Before place_piece(const Request& r, bool in, PlanSha
   return at;
 }
 
-// Four neighbouring items: for each the last request that starts at or before it (first ascending, its first entry 0).
-// N = 1024, where the LDS reads of sixteen waves bound it: the inner two are sought only where the outer two differ;
+// U neighbouring items: for each the last request that starts at or before it (first ascending, its first entry 0).
+// N = 1024, where the LDS reads of sixteen waves bound it: the inner ones are sought only where the outer two differ;
 // else all side by side.
-constexpr int U = 4;
-template <int N>
+template <int N, int U>
 __device__ __forceinline__ void owners(const int* first, int item, int last, int (&i)[U], int (&q)[U]) {
 #pragma unroll
   for (int u = 0; u < U; ++u) i[u] = min(item + u, last), q[u] = 0;
@@ -129,34 +128,40 @@ __device__ __forceinline__ void owners(const int* first, int item, int last, int
       if (first[q[u] + s] <= i[u]) q[u] += s;
   }
   if (N < 1024) return;
-  q[1] = q[2] = q[0];
-  if (q[0] != q[3]) {
-    q[1] = q[2] = 0;
+  if (q[0] == q[U - 1]) {
 #pragma unroll
-    for (int s = N / 2; s; s /= 2) {
-      if (first[q[1] + s] <= i[1]) q[1] += s;
-      if (first[q[2] + s] <= i[2]) q[2] += s;
-    }
+    for (int u = 1; u < U - 1; ++u) q[u] = q[0];
+  } else {
+#pragma unroll
+    for (int s = N / 2; s; s /= 2)
+#pragma unroll
+      for (int u = 1; u < U - 1; ++u)
+        if (first[q[u] + s] <= i[u]) q[u] += s;
   }
 }
 
 typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// x to p[0 .. 3], the first n of them.
-__device__ __forceinline__ void store4(int32_t* p, const int (&x)[U], int n) {
-  if (n >= U) *(i32x4u*)p = i32x4u{x[0], x[1], x[2], x[3]};
-  else
+// The first n of x to p.
+template <int U>
+__device__ __forceinline__ void store_items(int32_t* p, const int (&x)[U], int n) {
+  if (n >= U) {
+#pragma unroll
+    for (int u = 0; u < U; u += 4) *(i32x4u*)(p + u) = i32x4u{x[u], x[u + 1], x[u + 2], x[u + 3]};
+  } else {
 #pragma unroll
     for (int u = 0; u < U - 1; ++u)
       if (u < n) p[u] = x[u];
+  }
 }
 
 // One block, as the step is done in place: requests in pieces of one a thread.  First the totals, which say whether the
 // step can be done at all; then, piece by piece, sums over the piece's requests place its tokens and page moves, which
-// all threads then share, four at a time (an item finds its request by bisection of the piece's sums).  Latency: two
+// all threads then share, some at a time (an item finds its request by bisection of the piece's sums).  Latency: two
 // levels of loads and the sums; 64 requests, 64 tokens: see DESIGN
 template <int N>
 __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
+  constexpr int U = 4;   // items of a thread at once (8: 15.6 us for 1024 requests with 16k tokens, 4: 14.3)
   const moe_paged_plan& p = a.p;
   __shared__ PlanShared<N> sh;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
     const int tail = ring_place(head, count, p.n_pages);
     for (int i0 = tid * U; i0 < all.tok; i0 += U * N) {   // tokens
       int i[U], q[U], page[U], pos[U];
-      owners<N>(sh.tok0, i0, all.tok - 1, i, q);
+      owners<N, U>(sh.tok0, i0, all.tok - 1, i, q);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         pos[u] = sh.held[q[u]] + i[u] - sh.tok0[q[u]];
@@ -233,15 +238,15 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
         page[u] = position_slot(page[u], pos[u], p.n_pages, p.page_size, a.per);
         q[u] += r0;
       }
-      store4(p.req + done_t + i0, q, all.tok - i0);
-      store4(p.pos + done_t + i0, pos, all.tok - i0);
-      store4(p.slot + done_t + i0, page, all.tok - i0);
+      store_items(p.req + done_t + i0, q, all.tok - i0);
+      store_items(p.pos + done_t + i0, pos, all.tok - i0);
+      store_items(p.slot + done_t + i0, page, all.tok - i0);
     }
     for (int i0 = tid * U; i0 < all.take; i0 += U * N) {   // pages taken
       int i[U], q[U], page[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) page[u] = p.ring[ring_place(head, done_n + min(i0 + u, all.take - 1), p.n_pages)];
-      owners<N>(sh.take0, i0, all.take - 1, i, q);
+      owners<N, U>(sh.take0, i0, all.take - 1, i, q);
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i0 + u < all.take)
@@ -249,7 +254,7 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
     }
     for (int i0 = tid * U; i0 < all.back; i0 += U * N) {   // pages given back
       int i[U], q[U], page[U];
-      owners<N>(sh.back0, i0, all.back - 1, i, q);
+      owners<N, U>(sh.back0, i0, all.back - 1, i, q);
 #pragma unroll
       for (int u = 0; u < U; ++u) page[u] = p.tables[(size_t)(r0 + q[u]) * p.max_pages + i[u] - sh.back0[q[u]]];
 #pragma unroll
@@ -261,9 +266,11 @@ __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
     done_b += all.back;
     __syncthreads();
   }
-  const int none[U] = {-1, -1, -1, -1};
+  int none[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) none[u] = -1;
   for (int i = done_t + tid * U; i < p.max_tokens; i += U * N)
-    for (int32_t* to : {p.req, p.pos, p.slot}) store4(to + i, none, p.max_tokens - i);
+    for (int32_t* to : {p.req, p.pos, p.slot}) store_items(to + i, none, p.max_tokens - i);
   if (tid == 0) {
     p.starts[p.n_req] = done_t;
     p.ring_at_out[0] = ok ? ring_place(head, done_n, p.n_pages) : head;
@@ -357,14 +364,22 @@ __global__ __launch_bounds__(256) void heads_pages_kernel(HeadsArgs a) {
       y[0] = *p;
     }
   };
+  auto getx = [](const float* p, float (&y)[V]) {   // read once: past the caches (4096 tokens: 33.7 us, 37.5 through them)
+    if constexpr (V == 4) {
+      const f32x4 v = __builtin_nontemporal_load((const f32x4*)p);
+      y[0] = v[0], y[1] = v[1], y[2] = v[2], y[3] = v[3];
+    } else {
+      y[0] = *p;
+    }
+  };
   float y0[K][V], y1[K][V], ss = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int i = (lane + 16 * k) * V;
     if (i >= hd / 2) break;
     const int e0 = i < half ? i : half + i, e1 = e0 + (i < half ? half : rest);
-    get(x + e0, y0[k]);
-    get(x + e1, y1[k]);
+    getx(x + e0, y0[k]);
+    getx(x + e1, y1[k]);
 #pragma unroll
     for (int c = 0; c < V; ++c) ss = fmaf(y1[k][c], y1[k][c], fmaf(y0[k][c], y0[k][c], ss));
   }
