@@ -301,8 +301,11 @@ moe_status step_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* la
   const size_t td = (size_t)T * D * 4, rd = (size_t)R * D * 4;
   const size_t work = moe_paged_attn_work_bytes(T, c.n_q, c.n_kv, c.head_dim);
   moe_status st;
+  const size_t had = m->H.bytes;
   if ((st = grow(m->x, td)) || (st = grow(m->xa, td)) || (st = grow(m->xn, td)) ||
       (st = grow(m->qkv, (size_t)T * m->nqkv * 4)) || (st = grow(m->H, (size_t)T * m->Dq * 4)) ||
+      // (rows of no request keep what is there: numbers from the start)
+      (m->H.bytes > had && (st = check_hip(hipMemsetAsync(m->H.p, 0, m->H.bytes, s), "model scratch clear"))) ||
       (st = grow(m->last, 2 * rd)) || (st = grow(m->attn_work, work)) ||
       (!logits && (st = grow(m->last_logits, (size_t)R * c.vocab_size * 4))))
     return st;

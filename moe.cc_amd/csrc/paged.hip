@@ -3,6 +3,7 @@
 // into their pages, and the entry points (attention: paged_attn.hip).
 #include <math.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "moe_device.h"
@@ -32,6 +33,9 @@ struct OnDevice {
 
 int type_bytes(int dtype) { return dtype == MOE_PAGE_F32 ? 4 : dtype == MOE_PAGE_E4M3 ? 1 : 2; }
 
+// Rows of a call at most: a launch holds fewer than 2^32 threads.
+constexpr int kMostRows = (1 << 24) - 1;
+
 bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 
 // Checks a cache's description and fills its map.
@@ -47,6 +51,8 @@ moe_status check_pages(const moe_pages* g, const char* who, PageMap* m) {
   for (long long s : {g->page_stride, g->head_stride, g->slot_stride})
     if (s < g->head_dim || s % per16 || s > (1ll << 40))
       return set_error(MOE_ERR_ARG, "%s: stride %lld (at least head_dim, a multiple of %lld)", who, s, per16);
+  if (g->page_stride > (1ll << 48) / g->n_pages)
+    return set_error(MOE_ERR_ARG, "%s: %d pages of %lld elements", who, g->n_pages, g->page_stride);
   if (!aligned(g->k, 16) || !aligned(g->v, 16)) return set_error(MOE_ERR_ARG, "%s: pages not 16-byte aligned", who);
   if (g->dtype != MOE_PAGE_E4M3 && (g->k_scale || g->v_scale))
     return set_error(MOE_ERR_ARG, "%s: scales belong to 8-bit pages", who);
@@ -157,8 +163,9 @@ __device__ __forceinline__ void store_items(int32_t* p, const int (&x)[U], int n
 
 // One block, as the step is done in place: requests in pieces of one a thread.  First the totals, which say whether the
 // step can be done at all; then, piece by piece, sums over the piece's requests place its tokens and page moves, which
-// all threads then share, some at a time (an item finds its request by bisection of the piece's sums).  Latency: two
-// levels of loads and the sums; 64 requests, 64 tokens: see DESIGN
+// all threads then share, four at a time (an item finds its request by bisection of the piece's sums).  Latency bounds it:
+// launch, two levels of loads, the sums and the search; 64 requests with a token each 5.6 us, 1024 requests with 16k tokens
+// 14.3 us, of which the tokens' searches (the LDS reads of sixteen waves) are half.
 template <int N>
 __global__ __launch_bounds__(N) void plan_kernel(PlanArgs a) {
   constexpr int U = 4;   // items of a thread at once (8: 15.6 us for 1024 requests with 16k tokens, 4: 14.3)
@@ -335,8 +342,9 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // (token, head) rows, 16 lanes each, 16 a block.  A lane holds V neighbouring pairs at a time: pair i is (i, i + half) of
 // the turned values, then two of the rest; so norm, rotation and conversion stay in its registers, and the only sum over
-// lanes is the squares', in fp32.  Bound by the bytes: with V = 4 every access is 16 bytes (8 or 4 into 16- or 8-bit
-// pages); V = 1 where a pointer, a stride or the rotation's width is not a multiple of four.
+// lanes is the squares', in fp32.  Bound by the bytes: 4096 tokens of 32 / 4 heads of 128 into bf16 pages 33.7 us, 4.8 TB/s.
+// V = 4: every access is 16 bytes (8 or 4 into 16- or 8-bit pages); V = 1 (49.7 us) where a pointer, a stride or the
+// rotation's width does not allow it.
 template <int CT, int V>
 __global__ __launch_bounds__(256) void heads_pages_kernel(HeadsArgs a) {
   constexpr int K = 128 / (16 * V);   // a lane's groups of pairs at most (head_dim 256)
@@ -468,6 +476,8 @@ moe_status moe_paged_plan_dev(const moe_paged_plan* p) {
   if ((long long)p->n_pages * p->page_size > 0x7fffffffll || (long long)p->max_pages * p->page_size > 0x7fffffffll)
     return set_error(MOE_ERR_ARG, "paged_plan: %d pages of %d, %d a request: past 2^31 positions", p->n_pages, p->page_size,
                      p->max_pages);
+  if (p->n_req > kMostRows || p->max_tokens > kMostRows)
+    return set_error(MOE_ERR_ARG, "paged_plan: %d requests, %d tokens (%d at most)", p->n_req, p->max_tokens, kMostRows);
   for (const void* q : {(const void*)p->ring_at, (const void*)p->ring, (const void*)p->ring_at_out, (const void*)p->starts,
                         (const void*)p->status})
     if (!q) return set_error(MOE_ERR_ARG, "paged_plan: null pointer");
@@ -478,7 +488,8 @@ moe_status moe_paged_plan_dev(const moe_paged_plan* p) {
   OnDevice on;
   if ((st = on.enter())) return st;
   const PlanArgs args{*p, make_divider((uint32_t)p->page_size)};
-  // few requests and tokens: four waves, whose sums and barriers are the shorter
+  // few requests and tokens: four waves, whose sums and barriers are the shorter (64 requests 5.6 us, with sixteen 8.5);
+  // past them sixteen share the tokens
   if (p->n_req <= 256 && p->max_tokens <= 2048) hipLaunchKernelGGL(plan_kernel<256>, dim3(1), dim3(256), 0, stream(), args);
   else hipLaunchKernelGGL(plan_kernel<1024>, dim3(1), dim3(1024), 0, stream(), args);
   return check_hip(hipGetLastError(), "paged_plan launch");
@@ -497,7 +508,7 @@ moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* g) {
   if (h->rope_dim < 0 || h->rope_dim % 2 || h->rope_dim > map.head_dim || h->rope_len < 0)
     return set_error(MOE_ERR_ARG, "paged_heads: rope_dim %d, rope_len %d", h->rope_dim, h->rope_len);
   if (h->T == 0) return MOE_OK;
-  if (H * h->T > 0x7ffffff0ll) return set_error(MOE_ERR_ARG, "paged_heads: %d rows of %lld heads", h->T, H);
+  if (H * h->T > 16ll * kMostRows) return set_error(MOE_ERR_ARG, "paged_heads: %d rows of %lld heads", h->T, H);
   if (!h->qkv || !h->pos || !h->slot || !h->q_out || (h->rope_dim && (!h->rope_cos || !h->rope_sin)))
     return set_error(MOE_ERR_ARG, "paged_heads: null pointer");
   if (h->q_out == h->qkv && h->ldq != h->ld) return set_error(MOE_ERR_ARG, "paged_heads: q_out is qkv with another stride");
@@ -527,7 +538,7 @@ moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* g) {
   PageMap map;
   moe_status st = check_pages(g, "paged_attn", &map);
   if (st) return st;
-  if (a->T < 0 || a->n_q < 1 || a->n_q % map.n_kv || a->n_q > 65535)
+  if (a->T < 0 || a->T > kMostRows || a->n_q < 1 || a->n_q % map.n_kv || a->n_q > 65535)
     return set_error(MOE_ERR_ARG, "paged_attn: %d rows, %d query heads over %d", a->T, a->n_q, map.n_kv);
   if (a->ldq < (long long)a->n_q * map.head_dim || a->ldo < (long long)a->n_q * map.head_dim)
     return set_error(MOE_ERR_ARG, "paged_attn: rows of %lld and %lld floats", a->ldq, a->ldo);

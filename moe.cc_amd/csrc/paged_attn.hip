@@ -21,7 +21,14 @@
 //
 // Work is split over the length too.  The rows' positions, in units of kUnit, are laid end to end and cut into as many
 // even pieces as the chip holds blocks at once; a block walks the rows of its piece, whose place it finds in the rows'
-// lengths by itself (find_first).  Parts of a row that pieces cut go to `work` and are joined by a second kernel.
+// lengths by itself (find_piece).  Parts of a row that pieces cut go to `work` and are joined by a second kernel.  (Joined
+// in the same launch they would need a device-scope release a block, an L2 write-back here: 24 rows 18 -> 29 us, where the
+// second launch costs 4.)
+//
+// 32 / 4 heads of 128: 256 bf16 rows of 1..8192 positions 386 us (5.6 TB/s), one of 131072 52 us (5.2), 64 e4m3 rows of
+// 512..8192 55 us (5.2), 24 bf16 rows of 64..2048 18 us (2.9), a row of 40 in fp32 6.9 us.  The long ones are bound by the
+// bytes (the GEMVs of this library read 6.5 TB/s), the short ones by what comes one after another: launch, lengths, page
+// numbers, keys, the join.
 #include <math.h>
 
 #include <type_traits>
@@ -36,7 +43,10 @@ constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kUnit = 128;         // positions of a unit: a step of every wave
 constexpr int kSplitRows = 2048;   // more rows than this are not cut: a block a row
 constexpr int kCUs = 256;
-constexpr long long kStreamBytes = 64ll << 20;   // pages of K from which loads pass the caches
+// Bytes of K's pages from which loads pass the caches, since nothing of them is there at the next step: 64 e4m3 rows
+// (142 MB) 56 us against 63 through them, 256 bf16 rows 393 against 417; below, 8 bf16 rows of 1000..7000 (33 MB) 21 us
+// through the caches, 24 past them.
+constexpr long long kStreamBytes = 64ll << 20;
 
 enum { F32 = MOE_PAGE_F32, F16 = MOE_PAGE_F16, BF16 = MOE_PAGE_BF16, E4M3 = MOE_PAGE_E4M3 };
 
@@ -173,7 +183,7 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch& L, int b, Piece* ou
     *out = Piece{0, n, n, b, req, len, 0};
     return n > 0;
   }
-  if (a.T <= kWave) {   // every wave by itself, a row a lane
+  if (a.T <= kWave) {   // every wave by itself, a row a lane: no barrier (24 rows 17.9 us, 18.4 with the block's sums)
     const int lane = threadIdx.x % kWave, t = min(lane, a.T - 1);
     const int req = a.req ? a.req[t] : t, len = lane < a.T ? length_of(g, req, a.pos[t]) : kNone;
     const uint32_t n = units_of(len), scan = wave_scan(n), at = scan - n;
@@ -269,7 +279,9 @@ __device__ __forceinline__ void load_piece(const char* p, uint32_t* r) {
 
 // CT: the pages' type.  HDP: head_dim, or the next of 64, 128, 256 (the pieces past head_dim repeat its last one against
 // zero queries, and their sums are not stored).  WHOLE: a tile of 16 positions lies in one page (page_size % 16 == 0), so
-// its address is one scalar lookup; otherwise each lane looks up one position and the lanes exchange addresses.
+// its address is one scalar lookup; otherwise each lane looks up one position and the lanes exchange addresses (on pages
+// of 16 and more that takes 57.9 us for the e4m3 batch where WHOLE takes 54.9, 7.3 / 6.9 for one short row, 36.2 / 34.6
+// for heads of 64, 17.5 / 18.0 for 24 bf16 rows).  STREAM: loads past the caches.
 template <int CT, int HDP, bool WHOLE, bool STREAM>
 __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kernel(AttnLaunch L) {
   constexpr bool HALF = CT == F16;
@@ -688,7 +700,8 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L,
   }
 }
 
-// Pieces that the rows are cut into: as many as blocks of all heads are resident at once.
+// Pieces that the rows are cut into: as many as blocks of all heads are resident at once, by the kernels' registers.
+// (Twice as many, heads of 128: 24 rows 19.0 -> 21.5 us, one long row 52.8 -> 56.3, the e4m3 batch 56 -> 64.)
 int pieces_for(int n_q, int n_kv, int head_dim) {
   const int blocks = kCUs * (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1), per = n_kv * ((n_q / n_kv + 15) / 16);
   return blocks > per ? blocks / per : 1;
@@ -747,7 +760,8 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
                        : dtype == BF16 ? launch<BF16>(L, whole, stream, grid, s)
                                        : launch<E4M3>(L, whole, stream, grid, s);
   if (e != hipSuccess || !L.pieces) return e;
-  // few rows may have many parts each
+  // few rows may have many parts each: four waves to 16 rows (one row of 16000 15.2 us, 16.7 with one wave; 64 rows 34.7
+  // with four, 33.6 with one), and slices of the dimensions to 4 rows (15.7 against 17.3 whole)
   const int slice = a.T > 4 ? map.head_dim : map.head_dim % 32 ? 16 : 32;
   const dim3 joins(L.by_row ? (unsigned)a.T : grid.x, (unsigned)a.n_q, (unsigned)(map.head_dim / slice));
   if (a.T <= 16) hipLaunchKernelGGL(paged_join_kernel<4>, joins, dim3(4 * kWave), 0, s, L, slice);
