@@ -386,7 +386,8 @@ enum { MOE_PAGE_F32 = 0, MOE_PAGE_F16 = 1, MOE_PAGE_BF16 = 4, MOE_PAGE_E4M3 = 5 
 /* One layer's cache.  Element (page, head, offset, dim) of K is
  *   k[page * page_stride + head * head_stride + offset * slot_stride + dim]
  * (strides in elements, the same for v), so pages may be slot-major or
- * head-major, and K and V may share pages.  k, v and the strides' bytes are
+ * head-major, and K and V may share pages.  A request holds at most 2^30
+ * positions (max_pages * page_size), a call at most 2^24 - 1 rows.  k, v and the strides' bytes are
  * multiples of 16, head_dim a multiple of 16 up to 256, every stride at least
  * head_dim, n_pages * page_size below 2^31.  MOE_PAGE_E4M3 holds
  * value / scale (OCP 8-bit, rounded to nearest even, saturated at 448), with

@@ -33,8 +33,10 @@ struct OnDevice {
 
 int type_bytes(int dtype) { return dtype == MOE_PAGE_F32 ? 4 : dtype == MOE_PAGE_E4M3 ? 1 : 2; }
 
-// Rows of a call at most: a launch holds fewer than 2^32 threads.
+// Rows of a call at most: a launch holds fewer than 2^32 threads.  Positions of a request at most: what a step of the
+// kernels adds to one stays far inside an int.
 constexpr int kMostRows = (1 << 24) - 1;
+constexpr long long kMostPositions = 1ll << 30;
 
 bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 
@@ -473,9 +475,9 @@ moe_status moe_paged_plan_dev(const moe_paged_plan* p) {
   if (p->n_req < 0 || p->max_pages < 1 || p->n_pages < 1 || p->page_size < 1 || p->max_tokens < 0)
     return set_error(MOE_ERR_ARG, "paged_plan: %d requests of %d pages, %d pages of %d, %d tokens", p->n_req, p->max_pages,
                      p->n_pages, p->page_size, p->max_tokens);
-  if ((long long)p->n_pages * p->page_size > 0x7fffffffll || (long long)p->max_pages * p->page_size > 0x7fffffffll)
-    return set_error(MOE_ERR_ARG, "paged_plan: %d pages of %d, %d a request: past 2^31 positions", p->n_pages, p->page_size,
-                     p->max_pages);
+  if ((long long)p->n_pages * p->page_size > 0x7fffffffll || (long long)p->max_pages * p->page_size > kMostPositions)
+    return set_error(MOE_ERR_ARG, "paged_plan: %d pages of %d, %d a request: past 2^31 slots or 2^30 positions", p->n_pages,
+                     p->page_size, p->max_pages);
   if (p->n_req > kMostRows || p->max_tokens > kMostRows)
     return set_error(MOE_ERR_ARG, "paged_plan: %d requests, %d tokens (%d at most)", p->n_req, p->max_tokens, kMostRows);
   for (const void* q : {(const void*)p->ring_at, (const void*)p->ring, (const void*)p->ring_at_out, (const void*)p->starts,
@@ -542,7 +544,7 @@ moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* g) {
     return set_error(MOE_ERR_ARG, "paged_attn: %d rows, %d query heads over %d", a->T, a->n_q, map.n_kv);
   if (a->ldq < (long long)a->n_q * map.head_dim || a->ldo < (long long)a->n_q * map.head_dim)
     return set_error(MOE_ERR_ARG, "paged_attn: rows of %lld and %lld floats", a->ldq, a->ldo);
-  if (a->n_req < 0 || a->max_pages < 1 || (long long)a->max_pages * map.page_size > 0x7fffffffll)
+  if (a->n_req < 0 || a->max_pages < 1 || (long long)a->max_pages * map.page_size > kMostPositions)
     return set_error(MOE_ERR_ARG, "paged_attn: %d requests of %d pages", a->n_req, a->max_pages);
   if (!a->req && a->T > a->n_req) return set_error(MOE_ERR_ARG, "paged_attn: %d rows for %d requests", a->T, a->n_req);
   if (a->T == 0) return MOE_OK;

@@ -147,7 +147,7 @@ def test_far_scores(moehip, kind):
     _all(b, out, q)
 
 
-@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kind", list(C.TYPES))
 def test_nan_stays_in_its_heads(moehip, kind):
     """NaN in an attended key or value makes its heads NaN and no others."""
     b = Batch(moehip, C.TYPES[kind], [40, 2000, 40], 4, 2, 64, 16, seed=13)
@@ -187,3 +187,62 @@ def test_offsets_past_32_bits(moehip):
     want, tol = C.attend(q.reshape(4, hd).astype(np.float64), kd, vd, 0.125)
     assert (np.abs(got - want) <= tol).all()
     pool.free()
+
+
+@pytest.mark.parametrize("kind,T,nq,nkv,hd,long", [
+    ("bf16", 100, 16, 8, 128, 3000), ("f16", 200, 8, 8, 64, 1500), ("e4m3", 256, 4, 4, 128, 2000), ("bf16", 700, 8, 8, 64, 900), ("f32", 300, 4, 2, 256, 600),
+    ("bf16", 2048, 4, 4, 64, 400), ("f16", 2049, 4, 2, 64, 300), ("f32", 65, 32, 16, 128, 5000)])
+def test_many_rows(moehip, kind, T, nq, nkv, hd, long):
+    """More rows than a wave, a block's threads, the pieces, the rows that are cut; few of them long, some empty, some of
+    no request, several of one request."""
+    print("paged attention rows", kind, T, nq, nkv, hd, flush=True)
+    rng = np.random.default_rng(T)
+    lens = [int(n) for n in rng.integers(0, 200, 24)] + [long, 0, long // 2, 1]
+    b = Batch(moehip, C.TYPES[kind], lens, nq, nkv, hd, 16, "head", seed=T)
+    req = rng.integers(0, len(lens), T)
+    pos = np.array([rng.integers(-1, lens[r]) if lens[r] else -1 for r in req])
+    full = rng.random(T) < 0.2
+    pos[full] = np.array(lens)[req[full]] - 1
+    req[rng.random(T) < 0.15] = -1
+    req[[0, T - 1]] = -1, len(lens) - 4
+    pos[T - 1] = long - 1
+    out, q = b.run(req=req, pos=pos, T=T)
+    again, _ = b.run(req=req, pos=pos, T=T, q=q.reshape(T, -1), work_from=0x3C)
+    np.testing.assert_array_equal(out.view(np.uint32), again.view(np.uint32))
+    for t in list(range(0, T, max(1, T // 60))) + [T - 1]:
+        if req[t] < 0:
+            assert (out[t] == 7).all()
+        else:
+            b.check(out, q, t, int(req[t]), int(pos[t]) + 1)
+
+
+def test_no_row_of_any_request(moehip):
+    b = Batch(moehip, C.BF16, [300, 20], 8, 2, 64, 16, seed=21)
+    for T in (1, 40, 100, 400):
+        out, _ = b.run(req=[-1] * T, pos=[299] * T, T=T)
+        assert (out == 7).all()
+
+
+def test_two_calls_with_work_of_their_own_and_one_shared_in_turn(moehip):
+    """Calls one after another on the library's stream may share their work buffer, of any content, whatever their sizes."""
+    M = moehip
+    a, b = Batch(M, C.BF16, [5000, 1, 700], 8, 2, 64, 16, seed=31), Batch(M, C.F32, [900, 3000], 16, 4, 128, 32, seed=32)
+    need = max(M.lib().moe_paged_attn_work_bytes(len(x.lens), x.nq, x.pool.n_kv, x.hd) for x in (a, b))
+    work = M.DeviceBuffer.from_array(np.full(need, 0x7F, np.uint8))
+    calls, keep = [], []
+    for x in (a, b):
+        T = len(x.lens)
+        q, out = x.rng.standard_normal((T, x.ld)).astype(np.float32), np.zeros((T, x.ld), np.float32)
+        bufs = [M.DeviceBuffer.from_array(v) for v in (q, np.array(x.lens, np.int32) - 1, x.tables, out)]
+        keep.append(bufs)
+        calls.append((x, q, bufs, M.PagedAttn(bufs[0].ptr, x.ld, T, x.nq, None, bufs[1].ptr, bufs[2].ptr, T, x.width, x.scale, bufs[3].ptr, x.ld,
+                                              work.ptr, need)))
+    for _ in range(3):
+        for x, q, bufs, args in calls:
+            M.check(M.lib().moe_paged_attn_dev(C.ref(args), C.ref(x.pool.pages)))
+    for x, q, bufs, args in calls:
+        out = bufs[3].download((len(x.lens), x.ld), np.float32)
+        for t, n in enumerate(x.lens):
+            k, v = x.pool.rows(x.tables[t], n)
+            want, tol = C.attend(q[t].reshape(x.nq, x.hd).astype(np.float64), k, v, x.scale)
+            assert (np.abs(out[t].reshape(x.nq, x.hd) - want) <= tol).all()

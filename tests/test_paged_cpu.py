@@ -58,7 +58,7 @@ def _attn(**kw):
 PAGES = [(dict(k=None), ARG), (dict(v=None), ARG), (dict(dtype=2), ARG), (dict(dtype=-1), ARG), (dict(n_pages=0), ARG), (dict(page_size=0), ARG),
          (dict(n_kv=0), ARG), (dict(n_pages=1 << 20, page_size=1 << 11), ARG), (dict(head_dim=0), UNSUPPORTED), (dict(head_dim=72), UNSUPPORTED),
          (dict(head_dim=272), UNSUPPORTED), (dict(slot_stride=63), ARG), (dict(slot_stride=132), ARG), (dict(head_stride=-64), ARG),
-         (dict(page_stride=0), ARG), (dict(k=A + 8), ARG), (dict(v=A + 4), ARG), (dict(k_scale=A), ARG), (dict(v_scale=A), ARG)]
+         (dict(page_stride=0), ARG), (dict(n_pages=1 << 20, page_stride=1 << 30), ARG), (dict(k=A + 8), ARG), (dict(v=A + 4), ARG), (dict(k_scale=A), ARG), (dict(v_scale=A), ARG)]
 
 
 def _refused(st, want):
@@ -78,7 +78,7 @@ def test_pages_refused(bad, want):
 
 @needs_lib
 @pytest.mark.parametrize("bad", [dict(n_req=-1), dict(max_pages=0), dict(n_pages=0), dict(page_size=0), dict(max_tokens=-1),
-                                 dict(n_pages=1 << 28, page_size=8), dict(max_pages=1 << 30, page_size=2)]
+                                 dict(n_req=1 << 24), dict(max_tokens=1 << 24), dict(n_pages=1 << 28, page_size=8), dict(max_pages=(1 << 29) + 1, page_size=2)]
                          + [{n: None} for n in ("fresh", "held", "ring_at", "ring", "tables", "held_out", "ring_at_out", "starts", "req", "pos",
                                                 "slot", "status")], ids=str)
 def test_plan_refused(bad):
@@ -101,8 +101,8 @@ def test_heads_refused(bad):
 
 @needs_lib
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(n_q=0), dict(n_q=5), dict(ldq=255), dict(ldo=255), dict(n_req=-1), dict(max_pages=0),
-                                 dict(max_pages=1 << 28), dict(req=None, n_req=2), dict(q=None), dict(pos=None), dict(tables=None),
-                                 dict(out=None), dict(out=A), dict(work=None), dict(work=A + 8), dict(work_bytes=0)], ids=str)
+                                 dict(max_pages=(1 << 26) + 1), dict(req=None, n_req=2), dict(q=None), dict(pos=None), dict(tables=None),
+                                 dict(T=1 << 24, n_req=1 << 25), dict(out=None), dict(out=A), dict(work=None), dict(work=A + 8), dict(work_bytes=0)], ids=str)
 def test_attn_refused(bad):
     import moehip as M
     L, g = M.lib(), _pages()
