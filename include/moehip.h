@@ -387,12 +387,12 @@ enum { MOE_PAGE_F32 = 0, MOE_PAGE_F16 = 1, MOE_PAGE_BF16 = 4, MOE_PAGE_E4M3 = 5 
  *   k[page * page_stride + head * head_stride + offset * slot_stride + dim]
  * (strides in elements, the same for v), so pages may be slot-major or
  * head-major, and K and V may share pages.  A request holds at most 2^30
- * positions (max_pages * page_size), a call at most 2^24 - 1 rows.  k, v and the strides' bytes are
- * multiples of 16, head_dim a multiple of 16 up to 256, every stride at least
- * head_dim, n_pages * page_size below 2^31.  MOE_PAGE_E4M3 holds
- * value / scale (OCP 8-bit, rounded to nearest even, saturated at 448), with
- * one fp32 scale a head in k_scale / v_scale (NULL: 1); both are NULL for the
- * other types. */
+ * positions (max_pages * page_size), a call at most 2^24 - 1 rows.  k, v and
+ * the strides' bytes are multiples of 16, head_dim a multiple of 16 up to
+ * 256, every stride at least head_dim, n_pages * page_size below 2^31.
+ * MOE_PAGE_E4M3 holds value / scale (OCP 8-bit, rounded to nearest even,
+ * saturated at 448), with one fp32 scale a head in k_scale / v_scale (NULL:
+ * 1); both are NULL for the other types. */
 typedef struct {
   void* k;
   void* v;
@@ -472,9 +472,9 @@ moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* pages)
  * page_size, or a table entry that is no page: NaN in the row, nothing read
  * outside the cache or the tables.  A NaN or an infinity in an attended
  * position's key or value, or in the query, may make the row NaN; what lies
- * in the pages behind pos[t] never matters.  Several rows may belong to one request (a prompt's
- * tokens, once moe_paged_heads_dev has written them all); each reads the
- * cache for itself.  work: moe_paged_attn_work_bytes(T, n_q, n_kv, head_dim)
+ * in the pages behind pos[t] never matters.  Several rows may belong to one
+ * request (a prompt's tokens, once moe_paged_heads_dev has written them all);
+ * each reads the cache for itself.  work: moe_paged_attn_work_bytes(T, n_q, n_kv, head_dim)
  * bytes, 16-byte aligned, used from this call's launch to its end: calls or
  * graphs that may run at the same time need their own. */
 typedef struct {
@@ -506,8 +506,11 @@ moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* pages);
  * tokens: -1).  Either may be NULL.  A position at or past the model's
  * max_seq makes its logits NaN.  Prompts and single tokens may share a step;
  * every one of the max_tokens rows is computed, so a step is as dear as it.
- * The model's own position and cache are not touched.  Scratch grows on the
- * first call of a size, outside of any capture. */
+ * The model's own position and cache are not touched.  All arguments, every
+ * layer's pages among them, are checked before anything is queued.  The
+ * scratch is the model's and grows on the first call of a size, so a step is
+ * refused (MOE_ERR_ARG) while the library's stream is being captured; the
+ * three calls above may be. */
 moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
                                 const int32_t* ids, float* logits, int32_t* next);
 

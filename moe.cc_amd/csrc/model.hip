@@ -849,9 +849,14 @@ moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const 
         layers[l].page_size != plan->page_size)
       return set_error(MOE_ERR_ARG, "step_paged: layer %d has %d pages of %d positions, %d heads of %d", l, layers[l].n_pages,
                        layers[l].page_size, layers[l].n_kv, layers[l].head_dim);
-  moe_status st = ensure_init();
-  if (st) return st;
+  moe_status st = check_paged_step(plan, layers, m->cfg.n_layers, m->cfg.n_q, m->cfg.n_kv);
+  if (st || (st = ensure_init())) return st;
+  OnDevice on;
+  if ((st = on.enter())) return st;
   std::lock_guard<std::mutex> lk(m->mu);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if ((st = check_hip(hipStreamIsCapturing(stream(), &capture), "step_paged capture"))) return st;
+  if (capture != hipStreamCaptureStatusNone) return set_error(MOE_ERR_ARG, "step_paged: the stream is being captured");
   return step_paged(m, plan, layers, ids, logits, next);
 }
 

@@ -15,6 +15,21 @@ moe_status ensure_init();
 hipStream_t stream();
 // The device it belongs to (-1 before initialisation).
 int device();
+// Work is queued on the library's stream whatever device the calling thread
+// has current.
+struct OnDevice {
+  int was = -1;
+  moe_status enter() {
+    int d = -1;
+    moe_status st = check_hip(hipGetDevice(&d), "hipGetDevice");
+    if (st || d == device()) return st;
+    was = d;
+    return check_hip(hipSetDevice(device()), "hipSetDevice");
+  }
+  ~OnDevice() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
 // Layers and models alive (moe_shutdown refuses while any is).
 void live_objects(int delta);
 // Free the library-owned device buffers of one translation unit (the

@@ -15,22 +15,6 @@ namespace {
 
 // ------------------------------------------------------------ arguments
 
-// Work is queued on the library's stream whatever device the calling thread
-// has current.
-struct OnDevice {
-  int was = -1;
-  moe_status enter() {
-    int d = -1;
-    moe_status st = check_hip(hipGetDevice(&d), "hipGetDevice");
-    if (st || d == device()) return st;
-    was = d;
-    return check_hip(hipSetDevice(device()), "hipSetDevice");
-  }
-  ~OnDevice() {
-    if (was >= 0) (void)hipSetDevice(was);
-  }
-};
-
 int type_bytes(int dtype) { return dtype == MOE_PAGE_F32 ? 4 : dtype == MOE_PAGE_E4M3 ? 1 : 2; }
 
 // Rows of a call at most: a launch holds fewer than 2^32 threads.  Positions of a request at most: what a step of the
@@ -62,6 +46,26 @@ moe_status check_pages(const moe_pages* g, const char* who, PageMap* m) {
                make_divider((uint32_t)g->page_size)};
   return MOE_OK;
 }
+
+moe_status check_plan(const moe_paged_plan* p) {
+  if (!p) return set_error(MOE_ERR_ARG, "paged_plan: null argument");
+  if (p->n_req < 0 || p->max_pages < 1 || p->n_pages < 1 || p->page_size < 1 || p->max_tokens < 0)
+    return set_error(MOE_ERR_ARG, "paged_plan: %d requests of %d pages, %d pages of %d, %d tokens", p->n_req, p->max_pages,
+                     p->n_pages, p->page_size, p->max_tokens);
+  if ((long long)p->n_pages * p->page_size > 0x7fffffffll || (long long)p->max_pages * p->page_size > kMostPositions)
+    return set_error(MOE_ERR_ARG, "paged_plan: %d pages of %d, %d a request: past 2^31 slots or 2^30 positions", p->n_pages,
+                     p->page_size, p->max_pages);
+  if (p->n_req > kMostRows || p->max_tokens > kMostRows)
+    return set_error(MOE_ERR_ARG, "paged_plan: %d requests, %d tokens (%d at most)", p->n_req, p->max_tokens, kMostRows);
+  for (const void* q : {(const void*)p->ring_at, (const void*)p->ring, (const void*)p->ring_at_out, (const void*)p->starts,
+                        (const void*)p->status})
+    if (!q) return set_error(MOE_ERR_ARG, "paged_plan: null pointer");
+  if (p->n_req && (!p->fresh || !p->held || !p->tables || !p->held_out)) return set_error(MOE_ERR_ARG, "paged_plan: null pointer");
+  if (p->max_tokens && (!p->req || !p->pos || !p->slot)) return set_error(MOE_ERR_ARG, "paged_plan: null pointer");
+  return MOE_OK;
+}
+
+bool heads_fit(long long T, int n_q, int n_kv) { return (n_q + 2ll * n_kv) * T <= 16ll * kMostRows; }
 
 // ------------------------------------------------------------ plan
 
@@ -464,6 +468,17 @@ hipError_t launch_last_rows(const float* x, const int32_t* starts, int n_req, in
   return hipGetLastError();
 }
 
+moe_status check_paged_step(const moe_paged_plan* plan, const moe_pages* layers, int n_layers, int n_q, int n_kv) {
+  moe_status st = check_plan(plan);
+  for (int l = 0; !st && l < n_layers; ++l) {
+    PageMap map;
+    st = check_pages(&layers[l], "step_paged", &map);
+  }
+  if (!st && !heads_fit(plan->max_tokens, n_q, n_kv))
+    return set_error(MOE_ERR_ARG, "step_paged: %d rows of %d heads", plan->max_tokens, n_q);
+  return st;
+}
+
 }  // namespace moe
 
 using namespace moe;
@@ -471,22 +486,8 @@ using namespace moe;
 extern "C" {
 
 moe_status moe_paged_plan_dev(const moe_paged_plan* p) {
-  if (!p) return set_error(MOE_ERR_ARG, "paged_plan: null argument");
-  if (p->n_req < 0 || p->max_pages < 1 || p->n_pages < 1 || p->page_size < 1 || p->max_tokens < 0)
-    return set_error(MOE_ERR_ARG, "paged_plan: %d requests of %d pages, %d pages of %d, %d tokens", p->n_req, p->max_pages,
-                     p->n_pages, p->page_size, p->max_tokens);
-  if ((long long)p->n_pages * p->page_size > 0x7fffffffll || (long long)p->max_pages * p->page_size > kMostPositions)
-    return set_error(MOE_ERR_ARG, "paged_plan: %d pages of %d, %d a request: past 2^31 slots or 2^30 positions", p->n_pages,
-                     p->page_size, p->max_pages);
-  if (p->n_req > kMostRows || p->max_tokens > kMostRows)
-    return set_error(MOE_ERR_ARG, "paged_plan: %d requests, %d tokens (%d at most)", p->n_req, p->max_tokens, kMostRows);
-  for (const void* q : {(const void*)p->ring_at, (const void*)p->ring, (const void*)p->ring_at_out, (const void*)p->starts,
-                        (const void*)p->status})
-    if (!q) return set_error(MOE_ERR_ARG, "paged_plan: null pointer");
-  if (p->n_req && (!p->fresh || !p->held || !p->tables || !p->held_out)) return set_error(MOE_ERR_ARG, "paged_plan: null pointer");
-  if (p->max_tokens && (!p->req || !p->pos || !p->slot)) return set_error(MOE_ERR_ARG, "paged_plan: null pointer");
-  moe_status st = ensure_init();
-  if (st) return st;
+  moe_status st = check_plan(p);
+  if (st || (st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
   const PlanArgs args{*p, make_divider((uint32_t)p->page_size)};
@@ -510,7 +511,7 @@ moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* g) {
   if (h->rope_dim < 0 || h->rope_dim % 2 || h->rope_dim > map.head_dim || h->rope_len < 0)
     return set_error(MOE_ERR_ARG, "paged_heads: rope_dim %d, rope_len %d", h->rope_dim, h->rope_len);
   if (h->T == 0) return MOE_OK;
-  if (H * h->T > 16ll * kMostRows) return set_error(MOE_ERR_ARG, "paged_heads: %d rows of %lld heads", h->T, H);
+  if (!heads_fit(h->T, h->n_q, map.n_kv)) return set_error(MOE_ERR_ARG, "paged_heads: %d rows of %lld heads", h->T, H);
   if (!h->qkv || !h->pos || !h->slot || !h->q_out || (h->rope_dim && (!h->rope_cos || !h->rope_sin)))
     return set_error(MOE_ERR_ARG, "paged_heads: null pointer");
   if (h->q_out == h->qkv && h->ldq != h->ld) return set_error(MOE_ERR_ARG, "paged_heads: q_out is qkv with another stride");

@@ -421,7 +421,8 @@ class PagedCache:
     def set_step(self, fresh, ids):
         """New tokens of each request (-1: it ended) and their ids, request after request."""
         fresh, ids = np.asarray(fresh, np.int32), np.asarray(ids, np.int32)
-        if fresh.shape != (self.n_req,) or ids.size > self.max_tokens:
+        fits = fresh.shape == (self.n_req,) and ids.size <= self.max_tokens
+        if not fits or ids.size < min(int(np.maximum(fresh, 0).sum()), self.max_tokens):
             raise MoeError(f"a step of {fresh.size} requests and {ids.size} tokens")
         self._b["fresh"].upload(fresh)
         self._b["ids"].upload(ids)

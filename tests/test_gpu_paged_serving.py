@@ -280,3 +280,58 @@ def test_model_refusals(moehip):
     small = _caches(M, tm, C.F32, 2, 4, width=5)
     assert f(m.h, C.ref(ok.plan), small.layers, *args[3:]) == 2
     m.close()
+
+
+def test_model_refuses_before_any_work(moehip):
+    """Pages of the last layer that no call takes, a plan that none takes, a capture: refused with the state as it was."""
+    M, hip = moehip, Hip(moehip)
+    tm = O.TinyModel(seed=4)
+    m = M.model_from_tiny(tm)
+    c = _caches(M, tm, C.F32, 2, 4)
+    lg, nx = M.DeviceBuffer(2 * tm.V * 4), M.DeviceBuffer(8)
+    c.set_step([2, 1], [1, 2, 3])
+    names = (("held", 2), ("ring_at", 2), ("tables", 12), ("status", 1))
+    before = [c.array(*n) for n in names]
+
+    def step():
+        return M.lib().moe_model_step_paged(m.h, C.ref(c.plan), c.layers, c._b["ids"].ptr, lg.ptr, nx.ptr)
+
+    last = c.layers[tm.L - 1]
+    for name, bad in (("slot_stride", tm.hd - 1), ("head_stride", tm.hd + 1), ("dtype", 2), ("k", last.k + 4), ("v", None), ("k_scale", lg.ptr)):
+        good = getattr(last, name)
+        setattr(last, name, bad)
+        assert step() == 2, name
+        setattr(last, name, good)
+    good, c.plan.ring = c.plan.ring, None
+    assert step() == 2
+    c.plan.ring = good
+    hip.ok(hip.L.hipStreamBeginCapture(hip.stream, 1))
+    refused, graph = step(), ctypes.c_void_p()
+    hip.ok(hip.L.hipStreamEndCapture(hip.stream, ctypes.byref(graph)))
+    hip.ok(hip.L.hipGraphDestroy(graph))
+    assert refused == 2 and b"capture" in M.lib().moe_last_error()
+    for n, want in zip(names, before):
+        np.testing.assert_array_equal(c.array(*n), want, err_msg=n[0])
+    assert step() == 0 and c.status == 0
+    np.testing.assert_array_equal(c.array("held", 2), [2, 1])
+    with pytest.raises(M.MoeError):
+        c.set_step([2, 1], [1, 2])
+    with pytest.raises(M.MoeError):
+        c.set_step([1], [1])
+    m.close()
+
+
+def test_model_past_its_positions(moehip):
+    """A request that outgrows the model's rotation tables has NaN logits; the other request's stay numbers."""
+    M = moehip
+    tm = O.TinyModel(D=64, L=2, hd=16, nq=4, nkv=2, dff=32, E=16, V=97, seed=9, random_norms=True)
+    m = M.model_from_tiny(tm)
+    c = _caches(M, tm, C.F32, 2, 72, width=12)
+    ids = np.arange(72) % tm.V
+    lg, _ = m.step_paged(c, [64, 3], ids)
+    assert c.status == 0 and np.isfinite(lg).all()
+    lg, _ = m.step_paged(c, [1, 1], ids)
+    assert c.status == 0 and np.isnan(lg[0]).all() and np.isfinite(lg[1]).all()
+    lg, _ = m.step_paged(c, [-1, 1], ids)
+    assert c.status == 0 and not lg[0].any() and np.isfinite(lg[1]).all()
+    m.close()
