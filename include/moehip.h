@@ -474,7 +474,7 @@ moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* pages)
  * position's key or value, or in the query, may make the row NaN; what lies
  * in the pages behind pos[t] never matters.  Several rows may belong to one
  * request (a prompt's tokens, once moe_paged_heads_dev has written them all);
- * each reads the cache for itself.  work: moe_paged_attn_work_bytes(T, n_q, n_kv, head_dim)
+ * where T > n_req, neighbouring ones share their reads.  work: moe_paged_attn_work_bytes(T, n_q, n_kv, head_dim)
  * bytes, 16-byte aligned, used from this call's launch to its end: calls or
  * graphs that may run at the same time need their own. */
 typedef struct {

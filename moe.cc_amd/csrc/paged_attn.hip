@@ -73,12 +73,14 @@ __device__ __forceinline__ T scalar_load(const T* p, long long i) {
 struct AttnLaunch {
   AttnPages g;
   int head_tiles;   // of 16 query heads, a key-value head
-  int pieces;       // 0: rows are not cut, a block a row
+  int pieces;       // 0: rows are not cut, a block a row (SHARE: `share` rows)
   Divider each;     // by the pieces
-  int by_row;       // joins are listed a row (T <= pieces) or a piece
-  int4* joins;      // [min(T, pieces)] work: row, parts, the piece its first lies in; of a piece: of the row that ends there
-  float* part_ml;   // [2 pieces][n_q][2] work: maximum and sum of a part
-  float* part_o;    // [2 pieces][n_q][head_dim] work: its values' sums
+  int share;        // SHARE: rows that the 16 columns of a tile hold; else 1
+  Divider by_share, by_group;   // by share, by n_q / n_kv
+  int by_row;       // joins are listed a row (T <= pieces) or a piece (`share` of each)
+  int4* joins;      // work: row, parts, the piece its first lies in, its place in a run; of a piece: of the rows that end there
+  float* part_ml;   // [2 pieces][share][n_q][2] work: maximum and sum of a part
+  float* part_o;    // [2 pieces][share][n_q][head_dim] work: its values' sums
 };
 
 // A piece holds at most two parts of rows that go on in other pieces: part 0 of one (its start), in 2 piece + 1, and a
@@ -133,6 +135,94 @@ struct PieceShared {
   Piece piece;
 };
 
+// SHARE: rows of one request that follow one another and lie among the same `share` rows (counted from 0) are a run: one
+// item, whose columns are the heads of its rows, as long as the longest of them.  A prompt of 2048 bf16 positions, 8
+// heads to a key-value head, 2 rows a run: 211 us, each row for itself 538; 300 rows at position 8000 194 and 447; 1000
+// rows with a key-value head for each of 32 heads, 16 a run: 75 and 1052.
+
+// What a run counts for among the pieces: its units, and kRunUnits for what each takes besides (its first loads, the join
+// of the waves); the piece that starts among these has nothing to do for it.  512 / 2048 rows from position 0: none 41.6 /
+// 367 us, 2 37.3 / 211, 8 38.0 / 239; a block a run, which leaves a long row to one block, 27.8 / 192.
+constexpr uint32_t kRunUnits = 2;
+__device__ __forceinline__ uint32_t weight_of(int len) {
+  const uint32_t n = units_of(len);
+  return n ? n + kRunUnits : 0;
+}
+
+// The run that starts at `row`; a lane holds the length of row + lane.
+struct Run {
+  int n, req, longest, shortest;   // rows; longest: as length_of
+  int len;
+};
+__device__ __forceinline__ Run run_at(const AttnLaunch& L, int row, int req, int pos) {
+  const int lane = threadIdx.x % kWave;
+  const int past = min(((int)divide((uint32_t)row, L.by_share) + 1) * L.share, L.g.a.T) - row;
+  Run r;
+  r.len = lane < past ? length_of(L.g, req, pos) : kNone;
+  r.req = __builtin_amdgcn_readfirstlane(req);
+  const int len0 = __builtin_amdgcn_readfirstlane(r.len);
+  const uint64_t same = __ballot(r.len >= 0 && len0 >= 0 && req == r.req);
+  r.n = len0 >= 0 ? __builtin_ctzll(~same) : 1;   // (lanes past the run's 16 rows at most hold kNone)
+  int hi = lane < r.n ? r.len : kNone, lo = lane < r.n ? r.len : 0x7fffffff;
+#pragma unroll
+  for (int c = 8; c; c /= 2) hi = max(hi, __shfl_xor(hi, c)), lo = min(lo, __shfl_xor(lo, c));
+  r.longest = __builtin_amdgcn_readfirstlane(hi);
+  r.shortest = __builtin_amdgcn_readfirstlane(lo);
+  return r;
+}
+
+// Finds piece b of the runs' units, whole groups of `share` rows a thread.
+__device__ __forceinline__ void find_runs(const AttnLaunch& L, uint32_t b, bool lists, PieceShared& sh) {
+  constexpr int PER = 16;   // rows a thread at most: kSplitRows are 8 each, in groups of up to 16
+  const AttnPages& g = L.g;
+  const int T = g.a.T, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, share = L.share;
+  const int groups = (int)divide((uint32_t)(T + share - 1), L.by_share), per = (groups + kThreads - 1) / kThreads * share, t0 = tid * per;
+  int len[PER], req[PER];
+  uint32_t units[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = min(t0 + min(i, per - 1), T - 1);
+    req[i] = g.a.req[t];
+    len[i] = g.a.pos[t];
+  }
+  uint32_t follows = 0;   // bit i: row i belongs to the run of the row before it
+  int at_share = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    len[i] = i < per && t0 + i < T ? length_of(g, req[i], len[i]) : kNone;
+    if (i && at_share && len[i] >= 0 && len[i - 1] >= 0 && req[i] == req[i - 1]) follows |= 1u << i;
+    at_share = at_share + 1 == share ? 0 : at_share + 1;
+    if (len[i] == kPadding && L.by_row && b == 0 && lists) L.joins[t0 + i] = int4{0, 0, 0, 0};
+  }
+  uint32_t mine = 0;
+  int longest = kNone;
+#pragma unroll
+  for (int i = PER - 1; i >= 0; --i) {
+    longest = max(len[i], longest);
+    units[i] = follows >> i & 1 ? 0 : weight_of(longest);
+    if (!(follows >> i & 1)) longest = kNone;
+    mine += units[i];
+  }
+  const uint32_t scan = wave_scan(mine);
+  if (lane == kWave - 1) sh.scan[wave] = scan;
+  if (tid == 0) sh.piece.row = -1;
+  if (tid < share && !L.by_row && lists) L.joins[b * share + tid] = int4{0, 0, 0, 0};
+  __syncthreads();
+  uint32_t at = scan - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) at += sh.scan[w];
+    total += sh.scan[w];
+  }
+  const uint32_t each = divide(total + L.pieces - 1, L.each), begin = b * each;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (begin >= at && begin - at < units[i]) sh.piece = Piece{begin, min(begin + each, total), each, t0 + i, 0, 0, at};
+    at += units[i];
+  }
+  __syncthreads();
+}
+
 // Finds piece b; PER rows a thread.  The host sees to it that the units' sum and the pieces fit 31 bits.
 template <int PER>
 __device__ __forceinline__ void find_first(const AttnLaunch& L, uint32_t b, PieceShared& sh) {
@@ -176,16 +266,21 @@ __device__ __forceinline__ void find_first(const AttnLaunch& L, uint32_t b, Piec
   __syncthreads();
 }
 
-__device__ __forceinline__ bool find_piece(const AttnLaunch& L, int b, Piece* out) {
+template <bool SHARE>
+__device__ __forceinline__ bool find_piece(const AttnLaunch& L, int b, bool lists, Piece* out) {
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
+  if (SHARE && !L.pieces) {
+    *out = Piece{0, 1u << 30, 1u << 30, b * L.share, 0, 0, 0};
+    return true;
+  }
   if (!L.pieces) {
     const int req = a.req ? scalar_load(a.req, b) : b, len = length_of(g, req, scalar_load(a.pos, b));
     const uint32_t n = units_of(len);
     *out = Piece{0, n, n, b, req, len, 0};
     return n > 0;
   }
-  if (a.T <= kWave) {   // every wave by itself, a row a lane: no barrier (24 rows 17.9 us, 18.4 with the block's sums)
+  if (!SHARE && a.T <= kWave) {   // every wave by itself, a row a lane: no barrier (24 rows 17.9 us, 18.4 with the block's sums)
     const int lane = threadIdx.x % kWave, t = min(lane, a.T - 1);
     const int req = a.req ? a.req[t] : t, len = lane < a.T ? length_of(g, req, a.pos[t]) : kNone;
     const uint32_t n = units_of(len), scan = wave_scan(n), at = scan - n;
@@ -201,7 +296,8 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch& L, int b, Piece* ou
     return true;
   }
   __shared__ PieceShared sh;
-  if (a.T <= kThreads) find_first<1>(L, (uint32_t)b, sh);
+  if constexpr (SHARE) find_runs(L, (uint32_t)b, lists, sh);
+  else if (a.T <= kThreads) find_first<1>(L, (uint32_t)b, sh);
   else find_first<kSplitRows / kThreads>(L, (uint32_t)b, sh);
   auto get = [](auto x) { return (decltype(x))__builtin_amdgcn_readfirstlane((int)x); };
   *out = Piece{get(sh.piece.begin), get(sh.piece.end), get(sh.piece.per), get(sh.piece.row), get(sh.piece.req),
@@ -264,6 +360,15 @@ __device__ __forceinline__ u32x2 widen(uint32_t x) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true))};
 }
 
+// Not zero where one of the dword's values is an infinity or a NaN.
+template <int CT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+  constexpr uint32_t exps = CT == F32 ? 0x7f800000u : CT == BF16 ? 0x7f807f80u : CT == F16 ? 0x7c007c00u : 0x7f7f7f7fu;
+  constexpr uint32_t ones = CT == F32 ? 0x00800000u : CT == BF16 ? 0x00800080u : CT == F16 ? 0x04000400u : 0x01010101u;
+  constexpr uint32_t tops = CT == F32 ? 0x80000000u : CT == E4M3 ? 0x80808080u : 0x80008000u;
+  return ((x & exps) + ones) & tops;
+}
+
 // BYTES at p; STREAM: past the caches.
 template <int BYTES, bool STREAM>
 __device__ __forceinline__ void load_piece(const char* p, uint32_t* r) {
@@ -283,8 +388,9 @@ __device__ __forceinline__ void load_piece(const char* p, uint32_t* r) {
 // zero queries, and their sums are not stored).  WHOLE: a tile of 16 positions lies in one page (page_size % 16 == 0), so
 // its address is one scalar lookup; otherwise each lane looks up one position and the lanes exchange addresses (on pages
 // of 16 and more that takes 57.9 us for the e4m3 batch where WHOLE takes 54.9, 7.3 / 6.9 for one short row, 36.2 / 34.6
-// for heads of 64, 17.5 / 18.0 for 24 bf16 rows).  STREAM: loads past the caches.
-template <int CT, int HDP, bool WHOLE, bool STREAM>
+// for heads of 64, 17.5 / 18.0 for 24 bf16 rows).  STREAM: loads past the caches.  SHARE: a run of rows of one request
+// fills the tile's columns, so that a prompt's rows read the cache together.
+template <int CT, int HDP, bool WHOLE, bool STREAM, bool SHARE>
 __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kernel(AttnLaunch L) {
   constexpr bool HALF = CT == F16;
   constexpr int S = CT == F32 ? 4 : CT == E4M3 ? 1 : 2;
@@ -298,28 +404,62 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   // weights are held times 2^14 where their parts are f16, far from its smallest numbers
   constexpr float kLift = HALF ? 14.0f : 0.0f;
 
+  // SHARE: blocks of one L2 (every eighth) take neighbouring pieces of the same heads (512 rows at position 8000 312 us,
+  // in the grid's order 379)
+  int block = (int)blockIdx.x, heads_at = (int)blockIdx.y;
+  if (const uint32_t n = gridDim.x * gridDim.y; SHARE && L.pieces && n % 8 == 0) {
+    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, at = id % 8 * (n / 8) + id / 8;
+    heads_at = (int)(at / gridDim.x), block = (int)(at % gridDim.x);
+  }
   Piece pc;
-  if (!find_piece(L, (int)blockIdx.x, &pc)) return;
+  if (!find_piece<SHARE>(L, block, heads_at == 0, &pc)) return;
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int hd = g.map.head_dim;
-  const int G = a.n_q / g.map.n_kv, kv = (int)blockIdx.y / L.head_tiles, tile = (int)blockIdx.y % L.head_tiles;
-  const int head0 = kv * G + tile * 16, heads = min(16, G - tile * 16);   // this block's query heads
+  const int G = a.n_q / g.map.n_kv, kv = heads_at / L.head_tiles, tile = heads_at % L.head_tiles;
+  const int head0 = kv * G + tile * 16;   // this block's query heads
   const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
   const float vs = g.v_scale ? scalar_load(g.v_scale, kv) : 1.0f;
   const long long head_at = (long long)kv * g.map.head_stride;
   const char* kbase = (const char*)g.k + head_at * S;
   const char* vbase = (const char*)g.v + head_at * S;
   const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: below 2^24
+  // SHARE: the rows from the next one on, a lane each, and the first that is none of the block's
+  const int row_end = L.pieces ? a.T : min(pc.row + L.share, a.T);
+  int next_req = 0, next_pos = 0;
+  auto ask = [&](int row) {
+    const int t = min(row + (int)(threadIdx.x % kWave), a.T - 1);
+    next_req = a.req[t], next_pos = a.pos[t];
+  };
+  if constexpr (SHARE) ask(pc.row);
   for (;;) {   // the rows of the piece
+  Run run = {1, 0, 0, 0, 0};
+  if constexpr (SHARE) {
+    run = run_at(L, pc.row, next_req, next_pos);
+    pc.len = run.longest, pc.req = run.req;
+    ask(pc.row + run.n);
+    if (units_of(pc.len) == 0) {   // a row of no request
+      if (++pc.row >= row_end) return;
+      continue;
+    }
+  }
+  const int heads = SHARE ? run.n * G : min(16, G - tile * 16);   // columns
   // (the lane's places anew for every row: addresses made from them once would fill the registers that the loop needs)
   int col = lane % 16, quad = lane / 16;
   asm volatile("" : "+v"(col), "+v"(quad));
   const uint32_t units = units_of(pc.len), unit0 = max(pc.begin, pc.at) - pc.at, unit1 = min(pc.end - pc.at, units);
+  if (SHARE && unit0 >= units) {
+    pc.at += units + kRunUnits;
+    if (pc.at >= pc.end || (pc.row += run.n) >= row_end) return;
+    continue;
+  }
   const int first = (int)unit0 * kUnit, end = (int)min((long long)max(pc.len, 0), (long long)unit1 * kUnit);
   // the row after this one, asked for now
-  const int row2 = min(pc.row + 1, a.T - 1), req2 = a.req ? scalar_load(a.req, row2) : row2, pos2 = scalar_load(a.pos, row2);
+  const int row2 = min(pc.row + 1, a.T - 1), req2 = SHARE ? 0 : a.req ? scalar_load(a.req, row2) : row2, pos2 = SHARE ? 0 : scalar_load(a.pos, row2);
+  // SHARE: the column's row of the run, its positions; all columns have those before `lo`
+  const int run_row = SHARE ? min((int)divide((uint32_t)col, L.by_group), run.n - 1) : 0;
+  const int my_len = SHARE ? max(__shfl(run.len, run_row), 0) : 0, my_end = min(my_len, end), lo = min(run.shortest, end);
 
   // WHOLE: a scalar base a tile and 32-bit lane offsets; else a 64-bit row address a lane
   uint32_t kpiece[NK], vpiece[NV];
@@ -329,7 +469,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   for (int h = 0; h < NV; ++h) vpiece[h] = (uint32_t)min((16 * h + col) * EV * S, hd * S - EV * S);
 
   // ---- queries: requested first, used after the first keys are requested
-  const float* q = a.q + (size_t)pc.row * a.ldq + (size_t)(head0 + min(col, heads - 1)) * hd;
+  const float* q = a.q + (size_t)(pc.row + run_row) * a.ldq + (size_t)(head0 + min(col, heads - 1) - run_row * G) * hd;
   f32x4 x[CT == F32 ? NK : 2 * NQ];
   auto query_dim = [&](int s) {   // of x[s]
     return CT == F32 ? (4 * s + quad) * 4 : CT == E4M3 ? (4 * (s / 4) + quad) * 16 + 4 * (s % 4) : (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
@@ -340,7 +480,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
 
   // ---- addresses
   const int* table = a.tables + (size_t)(pc.len == kOutside ? 0 : pc.req) * a.max_pages;
-  int bad = pc.len == kOutside;
+  // something wrong; SHARE: from this position on
+  constexpr int kGood = SHARE ? 0x7fffffff : 0;
+  int bad = pc.len == kOutside ? SHARE ? -1 : 1 : kGood;
   auto base_of = [&](int step) { return first + (step * kWaves + wave) * STEP; };
   // page numbers of a step: WHOLE: of its tiles; else of the lane's position
   struct Look { int p[WHOLE ? KT : 1]; };
@@ -369,7 +511,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
       for (int t = 0; t < KT; ++t) {
         const int tb = min(base + 16 * t, (end - 1) & ~15);
         int pg = r.p[t];
-        if (!page_ok(g.map, pg)) bad = 1, pg = 0;
+        if (!page_ok(g.map, pg)) bad = SHARE ? min(bad, tb) : 1, pg = 0;
         const int off = tb - (int)divide((uint32_t)tb, g.map.per) * g.map.page_size;
         o.tile[t] = ((long long)pg * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
         o.lim[t] = min(end - 1 - tb, 15);
@@ -377,7 +519,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
     } else {
       const int p = min(base + lane, end - 1);
       int pg = r.p[0];
-      if (!page_ok(g.map, pg)) bad = 1, pg = 0;
+      if (!page_ok(g.map, pg)) bad = SHARE ? min(bad, p) : 1, pg = 0;
       const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
       o.tile[0] = ((long long)pg * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
       o.lim[0] = 15;
@@ -451,7 +593,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (HALF) s[t][i] *= unlift;
-        if (base + STEP > end && base + 16 * t + 4 * quad + i >= end) s[t][i] = -INFINITY;
+        if (base + STEP > (SHARE ? lo : end) && base + 16 * t + 4 * quad + i >= (SHARE ? my_end : end)) s[t][i] = -INFINITY;
         top = fmaxf(top, s[t][i]);
       }
     top = fmaxf(m, head_max(top));
@@ -471,6 +613,27 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
         p[t][i] = exp2_hw(s[t][i] - from);
         l += p[t][i];
       }
+    // SHARE: a value that is no number, at a position that some columns do not have, counts as zero (their weight for it,
+    // zero, would not make it one), and those that have it lose their sum
+    if (SHARE && base + STEP > lo) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t odd = 0;
+#pragma unroll
+          for (int h = 0; h < NV; ++h)
+#pragma unroll
+            for (int d = 0; d < VW; ++d) odd |= not_finite<CT>(vr[4 * t + i][h][d]);
+          if (__ballot(odd) >> (16 * quad) & 0xffff) {
+            if (base + 16 * t + 4 * quad + i < my_end) l = p[t][i] = NAN;
+#pragma unroll
+            for (int h = 0; h < NV; ++h)
+#pragma unroll
+              for (int d = 0; d < VW; ++d) vr[4 * t + i][h][d] = 0;
+          }
+        }
+    }
     // ---- values
     if constexpr (CT == F32) {
 #pragma unroll
@@ -564,7 +727,13 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
     gather(base_of(step));
   }
   l = head_sum(l);
-  if (__any(bad)) l = NAN;
+  if (__any(bad != kGood)) {
+    if constexpr (SHARE) {
+#pragma unroll
+      for (int c = 32; c; c /= 2) bad = min(bad, __shfl_xor(bad, c));
+    }
+    if (!SHARE || bad < my_len) l = NAN;
+  }
 
   // ---- the waves' sums joined, 128 dimensions at a time
   asm volatile("" : "+v"(col), "+v"(quad));
@@ -583,20 +752,23 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   // a row that goes on in other pieces leaves its part
   const uint32_t piece0 = pc.at / pc.per, parts = units ? (pc.at + units - 1) / pc.per - piece0 + 1 : 0;
   const bool cut = L.pieces && parts > 1;
-  const size_t part = (size_t)part_place((int)blockIdx.x - (unit0 != 0), unit0 != 0);
+  const size_t part = (size_t)part_place(block - (unit0 != 0), unit0 != 0);
   __shared__ float div_s[16];
   if (wave == 0 && quad == 0) {
     div_s[col] = sum == 0.0f ? 0.0f : vs / sum;
     if (cut && col < heads) {
-      float* ml = L.part_ml + (part * a.n_q + head0 + col) * 2;
+      float* ml = L.part_ml + ((SHARE ? part * L.share + run_row : part) * a.n_q + head0 + col - run_row * G) * 2;
       ml[0] = top;
       ml[1] = sum;
     }
-    if (cut && blockIdx.y == 0 && lane == 0) {
+    if (heads_at == 0 && col < run.n) {
+      const int row = pc.row + col;
       const bool last = pc.end >= pc.at + units;
-      if (L.by_row ? unit0 == 0 : last) L.joins[L.by_row ? pc.row : blockIdx.x] = int4{pc.row, (int)parts, (int)piece0, 0};
-    } else if (L.by_row && unit0 == 0 && blockIdx.y == 0 && lane == 0) {
-      L.joins[pc.row] = int4{0, 0, 0, 0};
+      if (cut) {
+        if (L.by_row ? unit0 == 0 : last) L.joins[L.by_row ? row : block * L.share + col] = int4{row, (int)parts, (int)piece0, col};
+      } else if (L.by_row && unit0 == 0) {
+        L.joins[row] = int4{0, 0, 0, 0};
+      }
     }
   }
 #pragma unroll
@@ -613,17 +785,22 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
       float y = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) y += o_s[w][at][h];
+      const int of = SHARE ? (int)divide((uint32_t)h, L.by_group) : 0, head = head0 + h - of * G;
       if (cut) {
-        L.part_o[(part * a.n_q + head0 + h) * hd + d] = y;
+        L.part_o[((SHARE ? part * L.share + of : part) * a.n_q + head) * hd + d] = y;
       } else {
-        a.out[(size_t)pc.row * a.ldo + (size_t)(head0 + h) * hd + d] = y * div_s[h];
+        a.out[(size_t)(pc.row + of) * a.ldo + (size_t)head * hd + d] = y * div_s[h];
       }
     }
     if (ps + 1 < PASS) __syncthreads();
   }
 
-  pc.at += units;
+  pc.at += SHARE ? units + kRunUnits : units;
   if (pc.at >= pc.end) return;
+  if constexpr (SHARE) {
+    if ((pc.row += run.n) >= row_end) return;
+    continue;
+  }
   pc.row = row2, pc.req = req2, pc.len = length_of(g, req2, pos2);
   while (units_of(pc.len) == 0) {   // rows of no request between
     ++pc.row;
@@ -642,16 +819,16 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L,
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
   const int head = (int)blockIdx.y, hd = g.map.head_dim;
-  const int4 r = L.joins[blockIdx.x];   // row, parts, first piece
+  const int4 r = L.joins[blockIdx.x];   // row, parts, first piece, place in its run
   const int parts = r.y;
   if (parts <= 1) return;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int width = slice / 4, rows = N / width, row = tid / width, d = (int)blockIdx.z * slice + tid % width * 4;
   __shared__ float by_s[WAVES][kMaxParts];
   __shared__ f32x4 acc_s[N];
-  const float* ml = L.part_ml + (size_t)head * 2;
-  const float* o = L.part_o + (size_t)head * hd + d;
-  const size_t step = (size_t)a.n_q * 2, next = (size_t)a.n_q * hd;
+  const float* ml = L.part_ml + ((size_t)r.w * a.n_q + head) * 2;
+  const float* o = L.part_o + ((size_t)r.w * a.n_q + head) * hd + d;
+  const size_t step = (size_t)L.share * a.n_q * 2, next = (size_t)L.share * a.n_q * hd;
   f32x4 y[U];
 #pragma unroll
   for (int c = 0; c < U; ++c) {
@@ -709,17 +886,22 @@ int pieces_for(int n_q, int n_kv, int head_dim) {
   return blocks > per ? blocks / per : 1;
 }
 
+// Rows of one request that a tile's columns hold.
+int rows_shared(int n_q, int n_kv) { return n_q / n_kv <= 8 ? 16 / (n_q / n_kv) : 1; }
+
 template <int CT, int HDP>
 hipError_t launch(const AttnLaunch& L, bool whole, bool stream, dim3 grid, hipStream_t s) {
-  auto go = [&](auto w, auto n) {
-    hipLaunchKernelGGL((paged_attn_kernel<CT, HDP, decltype(w)::value, decltype(n)::value>), grid, dim3(kThreads), 0, s, L);
-  };
   using std::false_type;
   using std::true_type;
-  if (whole && stream) go(true_type{}, true_type{});
-  else if (whole) go(true_type{}, false_type{});
-  else if (stream) go(false_type{}, true_type{});
-  else go(false_type{}, false_type{});
+  auto go = [&](auto w, auto n, auto r) {
+    hipLaunchKernelGGL((paged_attn_kernel<CT, HDP, decltype(w)::value, decltype(n)::value, decltype(r)::value>), grid, dim3(kThreads), 0, s, L);
+  };
+  if (L.share > 1 && whole) go(true_type{}, false_type{}, true_type{});
+  else if (L.share > 1) go(false_type{}, false_type{}, true_type{});
+  else if (whole && stream) go(true_type{}, true_type{}, false_type{});
+  else if (whole) go(true_type{}, false_type{}, false_type{});
+  else if (stream) go(false_type{}, true_type{}, false_type{});
+  else go(false_type{}, false_type{}, false_type{});
   return hipGetLastError();
 }
 
@@ -734,8 +916,8 @@ hipError_t launch(const AttnLaunch& L, bool whole, bool stream, dim3 grid, hipSt
 }  // namespace
 
 size_t paged_attn_work(int T, int n_q, int n_kv, int head_dim) {
-  const size_t pieces = (size_t)pieces_for(n_q, n_kv, head_dim);
-  return ((size_t)T < pieces ? T : pieces) * sizeof(int4) + 2 * pieces * n_q * (2 + (size_t)head_dim) * 4 + 16;
+  const size_t pieces = (size_t)pieces_for(n_q, n_kv, head_dim), rows = (size_t)rows_shared(n_q, n_kv);
+  return ((size_t)T <= pieces ? T : pieces * rows) * sizeof(int4) + 2 * pieces * rows * n_q * (2 + (size_t)head_dim) * 4 + 16;
 }
 
 hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
@@ -747,13 +929,18 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   // rows that no piece can cut (a unit at most), and more than a block's search takes, get a block each
   const long long units = ((long long)a.max_pages * map.page_size + kUnit - 1) / kUnit * a.T;   // at most
   const int most = pieces_for(a.n_q, map.n_kv, map.head_dim);
+  // rows outnumber the requests: some are of one request (or of none), so runs are looked for (where there are none the
+  // search costs: 24 rows with 6 of no request 22.3 us, 18.5 without it)
+  L.share = a.req && a.T > a.n_req ? rows_shared(a.n_q, map.n_kv) : 1;
+  L.by_share = make_divider((uint32_t)L.share);
+  L.by_group = make_divider((uint32_t)(a.n_q / map.n_kv));
   L.pieces = units > a.T && units <= 0x7fff0000ll && a.T <= kSplitRows ? most : 0;
   L.each = make_divider((uint32_t)most);
   L.by_row = a.T <= most;
   L.joins = (int4*)a.work;
-  L.part_o = (float*)(L.joins + (L.by_row ? a.T : most));
-  L.part_ml = L.part_o + 2 * (size_t)most * a.n_q * map.head_dim;
-  const dim3 grid((unsigned)(L.pieces ? (units < most ? units : most) : a.T), (unsigned)(map.n_kv * L.head_tiles));
+  L.part_o = (float*)(L.joins + (L.by_row ? a.T : (size_t)most * L.share));
+  L.part_ml = L.part_o + 2 * (size_t)most * L.share * a.n_q * map.head_dim;
+  const dim3 grid((unsigned)(L.pieces ? (units < most ? units : most) : (a.T + L.share - 1) / L.share), (unsigned)(map.n_kv * L.head_tiles));
   const bool whole = map.page_size % 16 == 0 && map.slot_stride < (1 << 22);
   const int size = dtype == F32 ? 4 : dtype == E4M3 ? 1 : 2;
   const bool stream = (long long)map.n_pages * map.page_stride * size >= kStreamBytes;
@@ -765,7 +952,7 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   // few rows may have many parts each: four waves to 16 rows (one row of 16000 15.2 us, 16.7 with one wave; 64 rows 34.7
   // with four, 33.6 with one), and slices of the dimensions to 4 rows (15.7 against 17.3 whole)
   const int slice = a.T > 4 ? map.head_dim : map.head_dim % 32 ? 16 : 32;
-  const dim3 joins(L.by_row ? (unsigned)a.T : grid.x, (unsigned)a.n_q, (unsigned)(map.head_dim / slice));
+  const dim3 joins(L.by_row ? (unsigned)a.T : grid.x * L.share, (unsigned)a.n_q, (unsigned)(map.head_dim / slice));
   if (a.T <= 16) hipLaunchKernelGGL(paged_join_kernel<4>, joins, dim3(4 * kWave), 0, s, L, slice);
   else hipLaunchKernelGGL(paged_join_kernel<1>, joins, dim3(kWave), 0, s, L, slice);
   return hipGetLastError();

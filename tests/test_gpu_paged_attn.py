@@ -246,3 +246,85 @@ def test_two_calls_with_work_of_their_own_and_one_shared_in_turn(moehip):
             k, v = x.pool.rows(x.tables[t], n)
             want, tol = C.attend(q[t].reshape(x.nq, x.hd).astype(np.float64), k, v, x.scale)
             assert (np.abs(out[t].reshape(x.nq, x.hd) - want) <= tol).all()
+
+
+# ---- rows of one request that share a tile's columns (more rows than requests)
+
+
+def _prompts(rng, lens, T):
+    """T rows: stretches of one request, mostly upwards, some down, repeated or empty, with rows of no request between"""
+    rows = []
+    while len(rows) < T:
+        r = int(rng.integers(0, len(lens)))
+        n, at = int(rng.integers(1, 40)), int(rng.integers(-1, max(lens[r], 1)))
+        step = int(rng.choice([1, 1, 1, 0, -1, 50]))
+        rows += [(r, min(max(at + i * step, -1), lens[r] - 1)) for i in range(n)]
+        if rng.random() < 0.3:
+            rows += [(-1, 3)] * int(rng.integers(1, 20))
+    return rows[:T]
+
+
+@pytest.mark.parametrize("kind", list(C.TYPES))
+@pytest.mark.parametrize("T,nq,nkv,hd,ps", [
+    (40, 4, 4, 64, 16), (70, 8, 4, 128, 7), (130, 6, 2, 80, 32), (300, 10, 2, 48, 16), (600, 8, 1, 256, 16), (2048, 4, 4, 32, 16), (2050, 9, 3, 64, 5)])
+def test_prompts_share_tiles(moehip, kind, T, nq, nkv, hd, ps):
+    """1, 2, 3, 5 and 8 query heads a key-value head: 16, 8, 5, 3 and 2 rows a tile; runs that cross a tile's rows, that
+    are cut into pieces, of one length and of many."""
+    print("paged attention prompts", kind, T, nq, nkv, hd, ps, flush=True)
+    rng = np.random.default_rng(T + hd)
+    lens = [700, 1, 90, 0, 3000 if T < 1000 else 400, 33, 250]
+    b = Batch(moehip, C.TYPES[kind], lens, nq, nkv, hd, ps, seed=T)
+    rows = _prompts(rng, lens, T)
+    req, pos = zip(*rows)
+    out, q = b.run(req=req, pos=pos, T=T)
+    again, _ = b.run(req=req, pos=pos, T=T, q=q.reshape(T, -1), work_from=0x3C)
+    np.testing.assert_array_equal(out.view(np.uint32), again.view(np.uint32))
+    for t in range(0, T, 1 + T // 150):
+        if req[t] < 0:
+            assert (out[t] == 7).all(), f"row {t} of no request was written"
+        else:
+            b.check(out, q, t, req[t], pos[t] + 1)
+
+
+@pytest.mark.parametrize("kind", list(C.TYPES))
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("ps,nq,hd", [(16, 4, 64), (7, 2, 128), (32, 16, 256)])
+def test_what_lies_behind_a_row_is_not_its_own(moehip, kind, side, ps, nq, hd):
+    """A NaN or an infinity at a position that only some rows of a run attend: those before it are right."""
+    b = Batch(moehip, C.TYPES[kind], [600, 40], nq, 2, hd, ps, seed=41)
+    for at, bits in ((300, C.NAN_BITS), (20, C.INF_BITS)):
+        pool = getattr(b.pool, side)
+        raw = np.array([bits[b.pool.dtype]], np.uint32).view(np.float32)[0] if kind == "f32" else bits[b.pool.dtype]
+        pool[b.tables[0 if at == 300 else 1, at // ps], at % ps, 0, 11] = raw
+    b.pool.upload()
+    rows = [(0, p) for p in range(290, 310)] + [(1, p) for p in (40 - 1, 19, 20, 5, 21, 0)] + [(0, 599), (0, 299), (0, 300)]
+    req, pos = zip(*rows)
+    out, q = b.run(req=req, pos=pos, T=len(rows))
+    half = nq // 2
+    for t, (r, p) in enumerate(rows):
+        hit = p >= (300 if r == 0 else 20)
+        o = out[t].reshape(nq, hd)
+        k, v = b.pool.rows(b.tables[r], p + 1)
+        first = half if hit else 0   # the heads of the other key-value head stay right
+        with np.errstate(invalid="ignore", over="ignore"):
+            want, tol = C.attend(q[t].astype(np.float64), k, v, b.scale)
+        assert (np.abs(o[first:] - want[first:]) <= tol[first:]).all(), f"row {t}"
+        if hit and (side == "v" or r == 0):
+            assert not np.isfinite(o[:half]).all(), f"row {t}"
+
+
+@pytest.mark.parametrize("kind,ps", [("f32", 16), ("bf16", 7), ("e4m3", 32)])
+def test_bad_pages_in_a_run(moehip, kind, ps):
+    """A table entry that is no page: the run's rows behind it are NaN, those before it right; a request or a position
+    outside the tables ends the run."""
+    b = Batch(moehip, C.TYPES[kind], [500, 200], 8, 2, 64, ps, seed=43)
+    page = 300 // ps
+    b.tables[0, page] = -5
+    rows = [(0, p) for p in range(page * ps - 9, page * ps + 9)] + [(1, 5), (1, b.width * ps), (1, 6), (7, 6), (1, 199), (0, 499), (0, 3)]
+    req, pos = zip(*rows)
+    out, q = b.run(req=req, pos=pos, T=len(rows))
+    for t, (r, p) in enumerate(rows):
+        if r == 7 or p >= b.width * ps or (r == 0 and p >= page * ps):
+            assert np.isnan(out[t]).all(), f"row {t}"
+        else:
+            b.check(out, q, t, r, p + 1)
