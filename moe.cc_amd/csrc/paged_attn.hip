@@ -16,7 +16,7 @@
 //            side by side by byte permutes; the sums come out as 16 dimensions x 16 heads, so a lane rescales its own head
 // Rounding: the products run on 16-bit operands with fp32 sums.  Keys and values enter as they are stored (8-bit ones are
 // exact in bf16); the fp32 queries and weights are split into three 16-bit parts that hold all their bits, so that
-// nothing is lost against an fp32 evaluation.  The matrix work this triples is a tenth of what the bytes' time allows.
+// nothing is lost against an fp32 evaluation.  The matrix units this triples the work of are busy a seventh of the long batches' time.
 // fp32 pages use the fp32 instruction (16 x 16 x 4) on the same layouts.
 //
 // Work is split over the length too.  The rows' positions, in units of kUnit, are laid end to end and cut into as many
@@ -25,8 +25,8 @@
 // in the same launch they would need a device-scope release a block, an L2 write-back here: 24 rows 18 -> 29 us, where the
 // second launch costs 4.)
 //
-// 32 / 4 heads of 128: 256 bf16 rows of 1..8192 positions 386 us (5.6 TB/s), one of 131072 52 us (5.2), 64 e4m3 rows of
-// 512..8192 55 us (5.2), 24 bf16 rows of 64..2048 18 us (2.9), a row of 40 in fp32 6.9 us.  The long ones are bound by the
+// 32 / 4 heads of 128: 256 bf16 rows of 1..8192 positions 354-386 us (5.6-6.1 TB/s), one of 131072 49 us (5.5), 64 e4m3
+// rows of 512..8192 55-61 us (4.7-5.2), 24 bf16 rows of 64..2048 17 us (3.0), a row of 40 in fp32 6.7 us.  The long ones are bound by the
 // bytes (the GEMVs of this library read 6.5 TB/s), the short ones by what comes one after another: launch, lengths, page
 // numbers, keys, the join.  128 rows of 4096 bf16 positions in head-major pages 172 us (6.2 TB/s), slot-major, where a
 // head's rows lie 256 bytes in every 1024, 180-185.  (Blocks with the heads side by side instead of one after another:
