@@ -42,9 +42,6 @@ namespace moe {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kUnit = 128;         // positions of a unit: a step of every wave
-constexpr int kSplitRows = 2048;   // more rows than this are not cut: a block a row
-constexpr int kCUs = 256;
 // Bytes of K's pages from which loads pass the caches, since nothing of them is there at the next step: 64 e4m3 rows
 // (142 MB) 56 us against 63 through them, 256 bf16 rows 393 against 417; below, 8 bf16 rows of 1000..7000 (33 MB) 21 us
 // through the caches, 24 past them.
@@ -83,16 +80,8 @@ struct AttnLaunch {
   float* part_o;    // [2 pieces][share][n_q][head_dim] work: its values' sums
 };
 
-// A piece holds at most two parts of rows that go on in other pieces: part 0 of one (its start), in 2 piece + 1, and a
-// later part of another, in 2 piece.
-__device__ __forceinline__ int part_place(int first_piece, int i) {
-  return i == 0 ? 2 * first_piece + 1 : 2 * (first_piece + i);
-}
-
-// Positions that a row attends; kPadding: no row; kOutside: a request or position outside the tables.
-constexpr int kPadding = -1, kOutside = -2, kNone = -3;
 __device__ __forceinline__ int length_of(const AttnPages& g, int req, int pos) {
-  return req < 0 ? kPadding : req >= g.a.n_req || pos >= g.a.max_pages * g.map.page_size ? kOutside : max(pos + 1, 0);
+  return row_length(req, pos, g.a.n_req, g.a.max_pages * g.map.page_size);
 }
 
 // Sums over the lanes up to each one.
@@ -119,10 +108,6 @@ __device__ __forceinline__ float wave_total(float x) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
 }
 
-__device__ __forceinline__ uint32_t units_of(int len) {
-  return len == kPadding || len == kNone ? 0 : max(((uint32_t)max(len, 0) + kUnit - 1) / kUnit, 1u);
-}
-
 // Where a block's piece starts: units begin .. end - 1 of all, in row `row` of request `req`, whose first unit is `at`.
 struct Piece {
   uint32_t begin, end, per;   // per: units of a piece
@@ -139,15 +124,6 @@ struct PieceShared {
 // item, whose columns are the heads of its rows, as long as the longest of them.  A prompt of 2048 bf16 positions, 8
 // heads to a key-value head, 2 rows a run: 211 us, each row for itself 538; 300 rows at position 8000 194 and 447; 1000
 // rows with a key-value head for each of 32 heads, 16 a run: 75 and 1052.
-
-// What a run counts for among the pieces: its units, and kRunUnits for what each takes besides (its first loads, the join
-// of the waves); the piece that starts among these has nothing to do for it.  512 / 2048 rows from position 0: none 41.6 /
-// 367 us, 2 37.3 / 211, 8 38.0 / 239; a block a run, which leaves a long row to one block, 27.8 / 192.
-constexpr uint32_t kRunUnits = 2;
-__device__ __forceinline__ uint32_t weight_of(int len) {
-  const uint32_t n = units_of(len);
-  return n ? n + kRunUnits : 0;
-}
 
 // The run that starts at `row`; a lane holds the length of row + lane.
 struct Run {
@@ -214,7 +190,7 @@ __device__ __forceinline__ void find_runs(const AttnLaunch& L, uint32_t b, bool 
     if (w < wave) at += sh.scan[w];
     total += sh.scan[w];
   }
-  const uint32_t each = divide(total + L.pieces - 1, L.each), begin = b * each;
+  const uint32_t each = piece_units(total, L.each), begin = b * each;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (begin >= at && begin - at < units[i]) sh.piece = Piece{begin, min(begin + each, total), each, t0 + i, 0, 0, at};
@@ -256,7 +232,7 @@ __device__ __forceinline__ void find_first(const AttnLaunch& L, uint32_t b, Piec
     if (w < wave) at += sh.scan[w];
     total += sh.scan[w];
   }
-  const uint32_t each = divide(total + L.pieces - 1, L.each), begin = b * each;
+  const uint32_t each = piece_units(total, L.each), begin = b * each;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const uint32_t n = units_of(len[i]);
@@ -287,7 +263,7 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch& L, int b, bool list
     const uint32_t total = __builtin_amdgcn_readlane(scan, kWave - 1);
     if (len == kPadding && L.by_row && b == 0 && blockIdx.y == 0 && threadIdx.x < kWave) L.joins[lane] = int4{0, 0, 0, 0};
     if (!L.by_row && blockIdx.y == 0 && threadIdx.x == 0) L.joins[b] = int4{0, 0, 0, 0};
-    const uint32_t each = divide(total + L.pieces - 1, L.each), begin = (uint32_t)b * each;
+    const uint32_t each = piece_units(total, L.each), begin = (uint32_t)b * each;
     const uint64_t mine = __ballot(begin >= at && begin - at < n);
     if (!mine) return false;
     const int row = __builtin_ctzll(mine);
@@ -448,7 +424,8 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
   // (the lane's places anew for every row: addresses made from them once would fill the registers that the loop needs)
   int col = lane % 16, quad = lane / 16;
   asm volatile("" : "+v"(col), "+v"(quad));
-  const uint32_t units = units_of(pc.len), unit0 = max(pc.begin, pc.at) - pc.at, unit1 = min(pc.end - pc.at, units);
+  const uint32_t units = units_of(pc.len);
+  const auto [unit0, unit1] = units_in(pc.begin, pc.end, pc.at, units);
   if (SHARE && unit0 >= units) {
     pc.at += units + kRunUnits;
     if (pc.at >= pc.end || (pc.row += run.n) >= row_end) return;
@@ -750,8 +727,8 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) sum += l_s[w][col] * exp2_hw(m_s[w][col] - from);
   // a row that goes on in other pieces leaves its part
-  const uint32_t piece0 = pc.at / pc.per, parts = units ? (pc.at + units - 1) / pc.per - piece0 + 1 : 0;
-  const bool cut = L.pieces && parts > 1;
+  const RowParts parts = parts_of(pc.at, units, pc.per);
+  const bool cut = L.pieces && parts.count > 1;
   const size_t part = (size_t)part_place(block - (unit0 != 0), unit0 != 0);
   __shared__ float div_s[16];
   if (wave == 0 && quad == 0) {
@@ -765,7 +742,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
       const int row = pc.row + col;
       const bool last = pc.end >= pc.at + units;
       if (cut) {
-        if (L.by_row ? unit0 == 0 : last) L.joins[L.by_row ? row : block * L.share + col] = int4{row, (int)parts, (int)piece0, col};
+        if (L.by_row ? unit0 == 0 : last) L.joins[L.by_row ? row : block * L.share + col] = int4{row, parts.count, parts.first, col};
       } else if (L.by_row && unit0 == 0) {
         L.joins[row] = int4{0, 0, 0, 0};
       }
@@ -812,7 +789,6 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void paged_attn_kerne
 
 // A block a (cut row, query head, `slice` dimensions): its parts joined, four dimensions a thread, so that WAVES 64 /
 // (slice / 4) parts are read side by side.  Latency: the parts' first rows are requested with their maxima.
-constexpr int kMaxParts = 3 * kCUs;   // of one row: no more than pieces
 template <int WAVES>
 __global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L, int slice) {
   constexpr int N = WAVES * kWave, U = 4;
@@ -879,16 +855,6 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L,
   }
 }
 
-// Pieces that the rows are cut into: as many as blocks of all heads are resident at once, by the kernels' registers.
-// (Twice as many, heads of 128: 24 rows 19.0 -> 21.5 us, one long row 52.8 -> 56.3, the e4m3 batch 56 -> 64.)
-int pieces_for(int n_q, int n_kv, int head_dim) {
-  const int blocks = kCUs * (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1), per = n_kv * ((n_q / n_kv + 15) / 16);
-  return blocks > per ? blocks / per : 1;
-}
-
-// Rows of one request that a tile's columns hold.
-int rows_shared(int n_q, int n_kv) { return n_q / n_kv <= 8 ? 16 / (n_q / n_kv) : 1; }
-
 template <int CT, int HDP>
 hipError_t launch(const AttnLaunch& L, bool whole, bool stream, dim3 grid, hipStream_t s) {
   using std::false_type;
@@ -926,21 +892,17 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t s) {
   AttnLaunch L;
   L.g = p;
   L.head_tiles = (a.n_q / map.n_kv + 15) / 16;
-  // rows that no piece can cut (a unit at most), and more than a block's search takes, get a block each
-  const long long units = ((long long)a.max_pages * map.page_size + kUnit - 1) / kUnit * a.T;   // at most
-  const int most = pieces_for(a.n_q, map.n_kv, map.head_dim);
-  // rows outnumber the requests: some are of one request (or of none), so runs are looked for (where there are none the
-  // search costs: 24 rows with 6 of no request 22.3 us, 18.5 without it)
-  L.share = a.req && a.T > a.n_req ? rows_shared(a.n_q, map.n_kv) : 1;
+  const AttnCut cut = cut_rows(a.T, a.n_req, a.req, (long long)a.max_pages * map.page_size, a.n_q, map.n_kv, map.head_dim);
+  L.share = cut.share;
   L.by_share = make_divider((uint32_t)L.share);
   L.by_group = make_divider((uint32_t)(a.n_q / map.n_kv));
-  L.pieces = units > a.T && units <= 0x7fff0000ll && a.T <= kSplitRows ? most : 0;
-  L.each = make_divider((uint32_t)most);
-  L.by_row = a.T <= most;
+  L.pieces = cut.pieces;
+  L.each = make_divider((uint32_t)cut.most);
+  L.by_row = cut.by_row;
   L.joins = (int4*)a.work;
-  L.part_o = (float*)(L.joins + (L.by_row ? a.T : (size_t)most * L.share));
-  L.part_ml = L.part_o + 2 * (size_t)most * L.share * a.n_q * map.head_dim;
-  const dim3 grid((unsigned)(L.pieces ? (units < most ? units : most) : (a.T + L.share - 1) / L.share), (unsigned)(map.n_kv * L.head_tiles));
+  L.part_o = (float*)(L.joins + (L.by_row ? a.T : (size_t)cut.most * L.share));
+  L.part_ml = L.part_o + 2 * (size_t)cut.most * L.share * a.n_q * map.head_dim;
+  const dim3 grid((unsigned)cut.blocks, (unsigned)(map.n_kv * L.head_tiles));
   const bool whole = map.page_size % 16 == 0 && map.slot_stride < (1 << 22);
   const int size = dtype == F32 ? 4 : dtype == E4M3 ? 1 : 2;
   const bool stream = (long long)map.n_pages * map.page_stride * size >= kStreamBytes;
