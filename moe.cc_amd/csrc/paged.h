@@ -168,4 +168,12 @@ MOE_BOTH RowParts parts_of(uint32_t at, uint32_t units, uint32_t per) {
 // later part of another, in 2 piece.
 MOE_BOTH int part_place(int first_piece, int i) { return i == 0 ? 2 * first_piece + 1 : 2 * (first_piece + i); }
 
+// Whether an entry of the join's list names parts to join: a row of the call, more than one part, all of them in its
+// pieces.  What the rows' kernel leaves does; the join takes nothing else, so that no content of `work` leads it outside
+// the call's buffers.
+MOE_BOTH bool join_ok(int row, int parts, int first_piece, int place, int T, int pieces, int share) {
+  return parts > 1 && row >= 0 && row < T && first_piece >= 0 && first_piece < pieces && parts <= pieces - first_piece && place >= 0 &&
+         place < share;
+}
+
 }  // namespace moe

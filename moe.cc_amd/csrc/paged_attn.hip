@@ -797,7 +797,7 @@ __global__ __launch_bounds__(WAVES * kWave) void paged_join_kernel(AttnLaunch L,
   const int head = (int)blockIdx.y, hd = g.map.head_dim;
   const int4 r = L.joins[blockIdx.x];   // row, parts, first piece, place in its run
   const int parts = r.y;
-  if (parts <= 1) return;
+  if (!join_ok(r.x, r.y, r.z, r.w, a.T, L.pieces, L.share)) return;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int width = slice / 4, rows = N / width, row = tid / width, d = (int)blockIdx.z * slice + tid % width * 4;
   __shared__ float by_s[WAVES][kMaxParts];

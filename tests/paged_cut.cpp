@@ -123,6 +123,7 @@ static void check(const Call& c) {
   for (int e = 0; e < (cut.by_row ? c.T : cut.blocks * cut.share); ++e) {
     const Join j = joins[e];
     if (j.parts < 0) fail(c, "an entry that no one wrote", e, 0);
+    if (join_ok(j.row, j.parts, j.first, j.place, c.T, cut.pieces, cut.share) != (j.parts > 1)) fail(c, "join_ok", j.row, j.parts);
     if (j.parts <= 1) continue;
     if (j.row < 0 || j.row >= c.T || row_joined[j.row]++) fail(c, "joined twice", e, j.row);
     for (int i = 0; i < j.parts; ++i) {
@@ -198,7 +199,21 @@ static void drawn() {
   }
 }
 
+// entries that name anything outside a call's rows, pieces or columns
+static void entries() {
+  const int junk[] = {-0x7fffffff - 1, -0x5a5a5a5b, -1, 0, 1, 2, 3, 7, 8, 9, 127, 128, 129, 768, 0x3c3c3c3c, 0x7f7f7f7f, 0x7fffffff};
+  for (int row : junk)
+    for (int parts : junk)
+      for (int first : junk)
+        for (int place : junk) {
+          const bool in = row >= 0 && row < 8 && parts >= 2 && first >= 0 && (long long)first + parts <= 128 && place >= 0 && place < 2;
+          if (join_ok(row, parts, first, place, 8, 128, 2) != in) std::printf("join_ok: %d %d %d %d\n", row, parts, first, place), std::exit(1);
+          if (in && part_place(first, parts - 1) >= 256) std::printf("part_place: %d %d\n", first, parts), std::exit(1);
+        }
+}
+
 int main() {
+  entries();
   chosen();
   drawn();
   std::printf("ok\n");
