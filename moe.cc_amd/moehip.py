@@ -556,6 +556,8 @@ class Model:
 
     def step_paged(self, cache: PagedCache, fresh, ids):
         """One step over many requests -> (logits [n_req, V], next ids [n_req])."""
+        if len(cache.layers) != self.cfg.n_layers:
+            raise MoeError(f"a cache of {len(cache.layers)} layers, a model of {self.cfg.n_layers}")
         cache.set_step(fresh, ids)
         lg = DeviceBuffer(cache.n_req * self.V * 4)
         nx = DeviceBuffer(cache.n_req * 4)
