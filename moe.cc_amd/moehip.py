@@ -396,6 +396,9 @@ class PagedCache:
 
     def __init__(self, n_layers, n_kv, head_dim, n_pages, page_size, n_req, max_pages, max_tokens,
                  dtype=PAGE_F32, k_scale=None, v_scale=None):
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if s is not None and np.shape(s) != (n_kv,):
+                raise MoeError(f"{name}: shape {np.shape(s)}, one scale a head is ({n_kv},)")
         self.n_req, self.max_tokens = n_req, max_tokens
         side = n_pages * page_size * n_kv * head_dim * {PAGE_F32: 4, PAGE_E4M3: 1}.get(dtype, 2)
         self._pools = [DeviceBuffer(2 * side) for _ in range(n_layers)]

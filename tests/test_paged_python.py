@@ -18,3 +18,15 @@ def test_cache_of_another_number_of_layers():
         with pytest.raises(M.MoeError, match="layers"):
             m.step_paged(cache, [1], np.zeros(1, np.int32))
     assert not moved
+
+
+@pytest.mark.parametrize("side", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("shape", [(), (1,), (3,), (5,), (4, 1)])
+def test_scales_of_another_number_of_heads(side, shape, monkeypatch):
+    """The kernels read one scale for each key-value head."""
+    def none(*a):
+        raise AssertionError("device memory was made")
+
+    monkeypatch.setattr(M.DeviceBuffer, "__init__", none)
+    with pytest.raises(M.MoeError, match=side):
+        M.PagedCache(2, 4, 64, 10, 16, 2, 4, 8, M.PAGE_E4M3, **{side: np.ones(shape, np.float32)})
