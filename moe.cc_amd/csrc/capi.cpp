@@ -83,6 +83,7 @@ void live_objects(int delta) { g_live.fetch_add(delta); }
 
 moe_status check_hip(hipError_t e, const char* what) {
   if (e == hipSuccess) return MOE_OK;
+  (void)hipGetLastError();   // the runtime keeps it; the next launch check must not see it
   return set_error(MOE_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
