@@ -309,6 +309,9 @@ moe_status step_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* la
       (st = grow(m->last, 2 * rd)) || (st = grow(m->attn_work, work)) ||
       (!logits && (st = grow(m->last_logits, (size_t)R * c.vocab_size * 4))))
     return st;
+  // everything the step allocates is there before its plan moves the requests on
+  for (DevLayer& L : m->layers)
+    if ((st = reserve_layer(L.moe, T))) return st;
   if ((st = moe_paged_plan_dev(p))) return st;
   float* x = (float*)m->x.p;
   float* xa = (float*)m->xa.p;

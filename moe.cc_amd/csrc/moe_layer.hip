@@ -1146,6 +1146,13 @@ void free_layer(LayerDev& L) {
 
 }  // namespace
 
+namespace moe {
+moe_status reserve_layer(moe_layer* layer, int T) {
+  std::lock_guard<std::mutex> lk(g_layer_mu);
+  return ensure_scratch(&layer->L, T);
+}
+}  // namespace moe
+
 extern "C" {
 
 moe_status moe_layer_create_raw(int dtype, int D, int d_ff, int E, int top_k,

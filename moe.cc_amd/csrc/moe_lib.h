@@ -32,6 +32,8 @@ struct OnDevice {
 };
 // Layers and models alive (moe_shutdown refuses while any is).
 void live_objects(int delta);
+// The scratch of a layer's forward over T rows, so that the forward allocates none.
+moe_status reserve_layer(moe_layer* layer, int T);
 // Free the library-owned device buffers of one translation unit (the
 // stream has drained; called by moe_shutdown only).
 void release_gemv_workspace();
