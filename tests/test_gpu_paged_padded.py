@@ -53,3 +53,26 @@ def test_short_prompt_beside_decode(moehip, kind, tokens):
     req = [r for r, k in enumerate(tokens) for _ in range(k)]
     pos = [b.lens[r] - k + i for r, k in enumerate(tokens) for i in range(k)]
     _check(b, req, pos)
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_drawn(moehip, seed):
+    """Batches of any make: rows of one request in stretches or apart, lengths to the table's end, rows of no request."""
+    rng = np.random.default_rng(900 + seed)
+    kind = list(C.TYPES)[seed % 4]
+    nq, nkv, hd = [(8, 1, 64), (4, 4, 32), (32, 4, 128), (6, 2, 80), (10, 2, 48), (3, 1, 256), (9, 3, 64), (24, 2, 64)][rng.integers(8)]
+    ps, n = int(rng.choice([1, 7, 16, 24, 64])), int(rng.integers(1, 40))
+    positions = max(1, int(rng.integers(20, 1500)) // ps) * ps
+    lens = [positions if rng.random() < 0.5 else int(rng.integers(0, positions + 1)) for _ in range(n)]
+    req, pos = [], []
+    T = n + int(rng.integers(0, 30))
+    while len(req) < T:
+        r = int(rng.integers(-1, n))
+        k = int(rng.integers(1, 12)) if rng.random() < 0.4 else 1
+        at = int(rng.integers(-1, lens[r])) if r >= 0 and lens[r] and rng.random() < 0.5 else (lens[r] if r >= 0 else 0) - 1
+        req += [r] * k
+        pos += [max(at - i, -1) for i in range(k)][::-1]
+    print("paged attention drawn", seed, kind, nq, nkv, hd, ps, n, positions, T, flush=True)
+    b = A.Batch(moehip, C.TYPES[kind], lens, nq, nkv, hd, ps, ["slot", "head"][seed % 2], seed=seed)
+    _widen(b, positions)
+    _check(b, req[:T], pos[:T])
