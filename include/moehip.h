@@ -446,7 +446,8 @@ moe_status moe_paged_plan_dev(const moe_paged_plan* plan);
  * A row with slot[t] < 0 is left as it is, in q_out too.  A slot at or past
  * n_pages * page_size or a position outside [0, rope_len) makes the row's
  * queries NaN; nothing is written outside the cache (a bad position's key is
- * NaN in it).  Two rows of one slot: either one's values stay. */
+ * NaN in it).  Two rows of one slot: each of its values is one of theirs, and
+ * which may differ from value to value. */
 typedef struct {
   const float* qkv;
   long long ld;
@@ -474,8 +475,11 @@ moe_status moe_paged_heads_dev(const moe_paged_heads* h, const moe_pages* pages)
  * position's key or value, or in the query, may make the row NaN; what lies
  * in the pages behind pos[t] never matters.  Several rows may belong to one
  * request (a prompt's tokens, once moe_paged_heads_dev has written them all);
- * where T > n_req, neighbouring ones share their reads.  work: moe_paged_attn_work_bytes(T, n_q, n_kv, head_dim)
- * bytes, 16-byte aligned, used from this call's launch to its end: calls or
+ * where T > n_req, neighbouring ones share their reads.  To 2048 rows a call
+ * spreads long ones over the whole card; in a larger one each is one block's a
+ * head, so give long decoding rows and thousands of a prompt's a call each.
+ * work: moe_paged_attn_work_bytes(T, n_q, n_kv, head_dim) bytes of any
+ * content, 16-byte aligned, used from this call's launch to its end: calls or
  * graphs that may run at the same time need their own. */
 typedef struct {
   const float* q;
@@ -507,10 +511,12 @@ moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* pages);
  * max_seq makes its logits NaN.  Prompts and single tokens may share a step;
  * every one of the max_tokens rows is computed, so a step is as dear as it.
  * The model's own position and cache are not touched.  All arguments, every
- * layer's pages among them, are checked before anything is queued.  The
- * scratch is the model's and grows on the first call of a size, so a step is
- * refused (MOE_ERR_ARG) while the library's stream is being captured; the
- * three calls above may be. */
+ * layer's pages among them, are checked before anything is queued, and memory
+ * that is not there fails the step with the requests as they were.  (A launch
+ * that fails later, MOE_ERR_HIP, leaves them moved on: end them.)  The scratch
+ * is the model's and grows on the first call of a size, so a step is refused
+ * (MOE_ERR_ARG) while the library's stream is being captured; the three calls
+ * above may be. */
 moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
                                 const int32_t* ids, float* logits, int32_t* next);
 

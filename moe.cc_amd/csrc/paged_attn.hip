@@ -16,7 +16,8 @@
 //            side by side by byte permutes; the sums come out as 16 dimensions x 16 heads, so a lane rescales its own head
 // Rounding: the products run on 16-bit operands with fp32 sums.  Keys and values enter as they are stored (8-bit ones are
 // exact in bf16); the fp32 queries and weights are split into three 16-bit parts that hold all their bits, so that
-// nothing is lost against an fp32 evaluation.  The matrix units this triples the work of are busy a seventh of the long batches' time.
+// nothing is lost against an fp32 evaluation.  (f16 parts hold what lies above 2^-38 of a head's largest query value or
+// weight; below it bits drop out of the products, of a weight those with its value, while its sum counts it.)  The matrix units this triples the work of are busy a seventh of the long batches' time.
 // fp32 pages use the fp32 instruction (16 x 16 x 4) on the same layouts.
 //
 // Work is split over the length too.  The rows' positions, in units of kUnit, are laid end to end and cut into as many
@@ -42,7 +43,8 @@ namespace moe {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-// Bytes of K's pages from which loads pass the caches, since nothing of them is there at the next step: 64 e4m3 rows
+// Bytes of K's pages, attended or not (the lengths are on the device), from which loads pass the caches, since nothing of
+// them is there at the next step: 64 e4m3 rows
 // (142 MB) 56 us against 63 through them, 256 bf16 rows 393 against 417; below, 8 bf16 rows of 1000..7000 (33 MB) 21 us
 // through the caches, 24 past them.
 constexpr long long kStreamBytes = 64ll << 20;
