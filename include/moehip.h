@@ -498,6 +498,136 @@ typedef struct {
 size_t moe_paged_attn_work_bytes(int T, int n_q, int n_kv, int head_dim);
 moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* pages);
 
+/* ---- several continuations of one prompt ----------------------------------
+ * A beam search, or several answers to one prompt, over a paged cache: requests
+ * that begin alike hold the same pages.  Between two steps
+ *   moe_beam_select_dev        the beams' next tokens, and which beam each continues
+ *   moe_paged_fork_dev         the tables after that: pages shared, taken, given back
+ *   moe_paged_copy_dev         the pages that can no longer be shared, in all layers
+ * and in a step, after its plan,
+ *   moe_paged_share_dev        which positions neighbouring rows have in common
+ *   moe_paged_attn_shared_dev  (every layer) attention that reads those once
+ * Pointers, streams, checks and captures as above. */
+
+/* Rows in n_groups groups of n_beam, one after another: row r is request r.
+ * logits [rows x ld], of the token after each row's last; score [rows]: the
+ * row's log probability so far; done [rows] (NULL: none): rows that have ended.
+ * A row's candidates: of a row that goes on, every token, with the value
+ * score + logit - log sum exp(logits); of one that has ended, itself, with the
+ * value score.  The n_beam candidates of a group with the largest value *
+ * weight[r] (NULL: 1; a length penalty is the caller's), largest first, become
+ * its rows.  Candidates of one row are ordered by logit, then the lower token;
+ * of several by value * weight in 64 bits, then the lower row.  A -inf logit is
+ * no candidate; a row with a NaN or +inf logit, a score that is not finite or a
+ * weight that is not finite and above 0 has none.
+ * New row r continues row parent[r] with token[r] (`pad` if that had ended);
+ * score_out its value, done_out 1 if it ended before or its token is `eos` (-1:
+ * no token ends a row); fresh 1 if it goes on, else 0.  Where a group has fewer
+ * candidates the rows left over get parent = token = -1, score -inf, done 0,
+ * fresh 0.  parent and fresh are what moe_paged_fork_dev and
+ * moe_paged_plan_dev take.  score_out may be score, done_out done.  A first
+ * step, of one row a group, is one whose other rows have the score -inf.
+ * n_beam at most 64, rows at most 65535.  work: moe_beam_select_work_bytes of
+ * any content, 16-byte aligned, in use from the call's launch to its end. */
+typedef struct {
+  int n_groups, n_beam, vocab;
+  const float* logits;
+  long long ld;
+  const float* score;
+  const int32_t* done;
+  const float* weight;
+  int eos, pad;
+  int32_t* parent;
+  int32_t* token;
+  float* score_out;
+  int32_t* done_out;
+  int32_t* fresh;
+  void* work;
+  size_t work_bytes;
+} moe_beam_select;
+size_t moe_beam_select_work_bytes(int n_groups, int n_beam, int vocab);
+moe_status moe_beam_select_dev(const moe_beam_select* s);
+
+/* Request r goes on as a copy of what request parent[r] was before the call;
+ * its own number: it stays, -1: it ends (it then holds 0 positions).  Copies
+ * share the full pages of what they copy.  A last page that is not full stays
+ * with the request itself, if it goes on, else with its first copy; every other
+ * copy takes a free page, oldest first, in order of the requests, and an entry
+ * {page, free page, positions} of copies, which moe_paged_copy_dev carries out.
+ * Pages that no request holds any more go behind the free ones, in order of
+ * their place in the tables, then of the lowest request that held them.
+ * tables_out may be tables; entries behind a request's pages stay as they are
+ * in tables.  held, ring_at, ring as in moe_paged_plan.  Requests that share
+ * pages are ended here, not by moe_paged_plan_dev, which gives a page back
+ * whoever else holds it; a page that several requests hold lies at one place of
+ * all their tables (as it does after calls of this function), and no request
+ * holds one twice.
+ * *status: 0 done; 1 too few free pages, 2 more than max_copies copies, 4 the
+ * state is broken (a parent that is no request, a length outside the table, a
+ * ring that cannot be): then nothing but the outputs that are separate from
+ * their inputs is written, as copies of these, and every entry of copies is -1
+ * (entries behind the last copy are, too).  A table entry that is no page is
+ * handed on and never given back.  n_req at most 4096.
+ * work: moe_paged_fork_work_bytes of any content, 16-byte aligned. */
+typedef struct {
+  int n_req, max_pages;        /* requests, pages a table row holds */
+  int n_pages, page_size;
+  int max_copies;              /* entries of copies; n_req is always enough */
+  const int32_t* parent;       /* [n_req] */
+  const int32_t* held;         /* [n_req] */
+  const int32_t* ring_at;      /* [2] */
+  int32_t* ring;               /* [n_pages] */
+  const int32_t* tables;       /* [n_req][max_pages] */
+  int32_t* held_out;           /* [n_req], may be held */
+  int32_t* ring_at_out;        /* [2], may be ring_at */
+  int32_t* tables_out;         /* [n_req][max_pages], may be tables */
+  int32_t* copies;             /* [max_copies][3] */
+  int32_t* status;             /* [1] */
+  void* work;
+  size_t work_bytes;
+} moe_paged_fork;
+size_t moe_paged_fork_work_bytes(int n_req, int max_pages, int n_pages);
+moe_status moe_paged_fork_dev(const moe_paged_fork* f);
+
+/* For each of n entries {from, to, positions} of copies [n][3] (device) the
+ * first `positions` positions of page `from`, keys and values of every head,
+ * to page `to`, in each of layers[0 .. n_layers - 1] (a host array; all of one
+ * type, size and strides).  An entry whose pages are none of the cache's is left
+ * out.  No page may be written twice, or written and read. */
+moe_status moe_paged_copy_dev(const int32_t* copies, int n, const moe_pages* layers, int n_layers);
+
+/* Rows as moe_paged_attn's (req NULL: request t), in groups of neighbours:
+ * group i is rows first[i] .. first[i + 1] - 1.  prefix[i]: how many leading
+ * positions all its rows hold in the same pages, whole pages only: page_size
+ * times the least, over its rows with a position to attend, of the leading
+ * table entries equal to the group's first such row's and of the pages that the
+ * row's own positions fill; 0 without such a row.  A `first` that falls, or
+ * leaves 0 .. T, makes every prefix 0.  plan: moe_paged_share_plan_bytes,
+ * 16-byte aligned: what moe_paged_attn_shared_dev reads of it, in every layer of
+ * the step; req, pos and tables stay as they are until then.  T and n_groups
+ * at most 65536. */
+typedef struct {
+  int T, n_req, max_pages, page_size;
+  int n_q, n_kv, head_dim;
+  const int32_t* req;
+  const int32_t* pos;      /* [T] */
+  const int32_t* tables;   /* [n_req][max_pages] */
+  int n_groups;
+  const int32_t* first;    /* [n_groups + 1] */
+  int32_t* prefix;         /* [n_groups] */
+  void* plan;
+  size_t plan_bytes;
+} moe_paged_share;
+size_t moe_paged_share_plan_bytes(int T, int n_groups, int n_q, int n_kv, int head_dim);
+moe_status moe_paged_share_dev(const moe_paged_share* s);
+
+/* moe_paged_attn_dev's results (a, pages: its arguments), with each group's
+ * prefix read once for all its rows instead of once a row.  s: as
+ * moe_paged_share_dev was given it for the same rows, tables and heads.
+ * work: moe_paged_attn_shared_work_bytes, else as moe_paged_attn's. */
+size_t moe_paged_attn_shared_work_bytes(int T, int n_groups, int n_q, int n_kv, int head_dim);
+moe_status moe_paged_attn_shared_dev(const moe_paged_attn* a, const moe_pages* pages, const moe_paged_share* s);
+
 /* One step of a model over many requests, instead of moe_model_forward's one
  * sequence: moe_paged_plan_dev(plan), then every layer with the tokens' keys
  * and values in layers[0 .. n_layers - 1] (a host array; each n_pages pages of

@@ -79,6 +79,9 @@ MOE_BOTH int plan_status(bool bad, bool too_long, long long tokens, long long ne
   return kPlanOk;
 }
 
+// What a call of moe_paged_fork_dev comes to.
+enum ForkStatus { kForkOk = 0, kForkNoPages = 1, kForkCopies = 2, kForkBad = 4 };
+
 // Place `i` entries past `from` in a ring of n (0 <= from < n, 0 <= i <= n).
 MOE_BOTH int ring_place(int from, int i, int n) {
   const uint32_t at = (uint32_t)from + (uint32_t)i;

@@ -11,20 +11,9 @@
 #include "paged_attn.h"
 
 namespace moe {
-namespace {
 
 // ------------------------------------------------------------ arguments
 
-int type_bytes(int dtype) { return dtype == MOE_PAGE_F32 ? 4 : dtype == MOE_PAGE_E4M3 ? 1 : 2; }
-
-// Rows of a call at most: a launch holds fewer than 2^32 threads.  Positions of a request at most: what a step of the
-// kernels adds to one stays far inside an int.
-constexpr int kMostRows = (1 << 24) - 1;
-constexpr long long kMostPositions = 1ll << 30;
-
-bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
-
-// Checks a cache's description and fills its map.
 moe_status check_pages(const moe_pages* g, const char* who, PageMap* m) {
   if (!g || !g->k || !g->v) return set_error(MOE_ERR_ARG, "%s: no pages", who);
   if (g->dtype != MOE_PAGE_F32 && g->dtype != MOE_PAGE_F16 && g->dtype != MOE_PAGE_BF16 && g->dtype != MOE_PAGE_E4M3)
@@ -39,13 +28,34 @@ moe_status check_pages(const moe_pages* g, const char* who, PageMap* m) {
       return set_error(MOE_ERR_ARG, "%s: stride %lld (at least head_dim, a multiple of %lld)", who, s, per16);
   if (g->page_stride > (1ll << 48) / g->n_pages)
     return set_error(MOE_ERR_ARG, "%s: %d pages of %lld elements", who, g->n_pages, g->page_stride);
-  if (!aligned(g->k, 16) || !aligned(g->v, 16)) return set_error(MOE_ERR_ARG, "%s: pages not 16-byte aligned", who);
+  if ((uintptr_t)g->k % 16 || (uintptr_t)g->v % 16) return set_error(MOE_ERR_ARG, "%s: pages not 16-byte aligned", who);
   if (g->dtype != MOE_PAGE_E4M3 && (g->k_scale || g->v_scale))
     return set_error(MOE_ERR_ARG, "%s: scales belong to 8-bit pages", who);
   *m = PageMap{g->n_pages, g->page_size, g->n_kv, g->head_dim, g->page_stride, g->head_stride, g->slot_stride,
                make_divider((uint32_t)g->page_size)};
   return MOE_OK;
 }
+
+moe_status check_attn(const moe_paged_attn* a, const moe_pages* g, const char* who, PageMap* m) {
+  if (!a) return set_error(MOE_ERR_ARG, "%s: null argument", who);
+  moe_status st = check_pages(g, who, m);
+  if (st) return st;
+  if (a->T < 0 || a->T > kMostRows || a->n_q < 1 || a->n_q % m->n_kv || a->n_q > 65535)
+    return set_error(MOE_ERR_ARG, "%s: %d rows, %d query heads over %d", who, a->T, a->n_q, m->n_kv);
+  if (a->ldq < (long long)a->n_q * m->head_dim || a->ldo < (long long)a->n_q * m->head_dim)
+    return set_error(MOE_ERR_ARG, "%s: rows of %lld and %lld floats", who, a->ldq, a->ldo);
+  if (a->n_req < 0 || a->max_pages < 1 || (long long)a->max_pages * m->page_size > kMostPositions)
+    return set_error(MOE_ERR_ARG, "%s: %d requests of %d pages", who, a->n_req, a->max_pages);
+  if (!a->req && a->T > a->n_req) return set_error(MOE_ERR_ARG, "%s: %d rows for %d requests", who, a->T, a->n_req);
+  if (a->T == 0) return MOE_OK;
+  if (!a->q || !a->pos || !a->tables || !a->out) return set_error(MOE_ERR_ARG, "%s: null pointer", who);
+  if (a->out == a->q) return set_error(MOE_ERR_ARG, "%s: out is q", who);
+  return MOE_OK;
+}
+
+namespace {
+
+bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 
 moe_status check_plan(const moe_paged_plan* p) {
   if (!p) return set_error(MOE_ERR_ARG, "paged_plan: null argument");
@@ -537,20 +547,10 @@ size_t moe_paged_attn_work_bytes(int T, int n_q, int n_kv, int head_dim) {
 }
 
 moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* g) {
-  if (!a) return set_error(MOE_ERR_ARG, "paged_attn: null argument");
   PageMap map;
-  moe_status st = check_pages(g, "paged_attn", &map);
-  if (st) return st;
-  if (a->T < 0 || a->T > kMostRows || a->n_q < 1 || a->n_q % map.n_kv || a->n_q > 65535)
-    return set_error(MOE_ERR_ARG, "paged_attn: %d rows, %d query heads over %d", a->T, a->n_q, map.n_kv);
-  if (a->ldq < (long long)a->n_q * map.head_dim || a->ldo < (long long)a->n_q * map.head_dim)
-    return set_error(MOE_ERR_ARG, "paged_attn: rows of %lld and %lld floats", a->ldq, a->ldo);
-  if (a->n_req < 0 || a->max_pages < 1 || (long long)a->max_pages * map.page_size > kMostPositions)
-    return set_error(MOE_ERR_ARG, "paged_attn: %d requests of %d pages", a->n_req, a->max_pages);
-  if (!a->req && a->T > a->n_req) return set_error(MOE_ERR_ARG, "paged_attn: %d rows for %d requests", a->T, a->n_req);
-  if (a->T == 0) return MOE_OK;
-  if (!a->q || !a->pos || !a->tables || !a->out || !a->work) return set_error(MOE_ERR_ARG, "paged_attn: null pointer");
-  if (a->out == a->q) return set_error(MOE_ERR_ARG, "paged_attn: out is q");
+  moe_status st = check_attn(a, g, "paged_attn", &map);
+  if (st || a->T == 0) return st;
+  if (!a->work) return set_error(MOE_ERR_ARG, "paged_attn: null pointer");
   const size_t need = moe_paged_attn_work_bytes(a->T, a->n_q, map.n_kv, map.head_dim);
   if (a->work_bytes < need || !aligned(a->work, 16))
     return set_error(MOE_ERR_ARG, "paged_attn: %zu bytes of work at %p, %zu needed, 16-byte aligned", a->work_bytes, a->work, need);

@@ -8,6 +8,18 @@
 
 namespace moe {
 
+inline int type_bytes(int dtype) { return dtype == MOE_PAGE_F32 ? 4 : dtype == MOE_PAGE_E4M3 ? 1 : 2; }
+
+// Rows of a call at most: a launch holds fewer than 2^32 threads.  Positions of a request at most: what a step of the
+// kernels adds to one stays far inside an int.
+constexpr int kMostRows = (1 << 24) - 1;
+constexpr long long kMostPositions = 1ll << 30;
+
+// Checks a cache's description and fills its map.
+moe_status check_pages(const moe_pages* g, const char* who, PageMap* m);
+// Checks moe_paged_attn_dev's arguments, without its work.
+moe_status check_attn(const moe_paged_attn* a, const moe_pages* g, const char* who, PageMap* m);
+
 struct AttnPages {
   moe_paged_attn a;
   PageMap map;

@@ -1,0 +1,384 @@
+// paged_fork.hip - requests of a paged cache that go on as copies of others:
+// the block tables (moe_paged_fork_dev) and the pages that are copied
+// (moe_paged_copy_dev).  include/moehip.h.
+//
+// Requests share pages only by being forked, so a shared page lies at the same
+// place of all its holders' tables.  Everything about a page is therefore
+// found in one column of the tables, and columns are independent of each
+// other: a block takes some columns of all requests and finds which of their
+// pages no request holds any more by marks in `work`, a number a page:
+//   0  every page of the old tables      1  every page of the new ones
+//   2 + n - 1 - r  of the rest, by the largest: the lowest request r that held it gives it back
+// Nothing is kept from one call for the next.
+#include <initializer_list>
+
+#include "moe_device.h"
+#include "moe_lib.h"
+#include "paged_attn.h"
+
+namespace moe {
+namespace {
+
+constexpr int kN = 1024;             // threads of a block
+constexpr int kMostRequests = 4096;
+constexpr int kPer = 8;              // table entries of a thread
+constexpr int kEntries = kPer * kN;  // of a block
+
+// How a request goes on.
+struct Goes {
+  int src;    // the request that it is a copy of; -1: it ends
+  int fills;  // pages of src
+  int dst;    // the page that its last one is copied to
+  int used;   // pages that it had
+  int copy;   // its place among the copies; -1: none
+  int held;   // positions of src
+};
+
+struct ForkHead {
+  int status, head, count, copies;
+};
+
+struct ForkArgs {
+  moe_paged_fork f;
+  Divider per;      // by page_size
+  int columns, blocks;   // of a block, of the tables
+  ForkHead* top;    // work
+  Goes* goes;       // work [n_req]
+  int* counts;      // work [blocks] pages that come back
+  int* list;        // work [n_req * max_pages] these, a block's from n_req * its first column on
+  int* mark;        // work [n_pages]
+};
+
+__device__ __forceinline__ int mark_load(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void mark_store(int* p, int x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Sum over the block's threads up to and without this one, and of all.
+__device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  int x = v;
+#pragma unroll
+  for (int c = 1; c < kWave; c *= 2) {
+    const int y = __shfl_up(x, c);
+    if (lane >= c) x += y;
+  }
+  if (lane == kWave - 1) wave_s[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < kN / kWave; ++w) {
+    const int y = wave_s[w];
+    if (w < wave) before += y;
+    all += y;
+  }
+  __syncthreads();
+  *total = all;
+  return before + x - v;
+}
+
+// The requests: how each goes on, and whether the call can be done.
+__device__ __forceinline__ void fork_requests(const ForkArgs& a) {
+  const moe_paged_fork& f = a.f;
+  __shared__ int keep_s[kMostRequests], wave_s[kN / kWave], bad_s;
+  const int tid = threadIdx.x, n = f.n_req;
+  const int head = f.ring_at[0], count = f.ring_at[1];
+  const long long most = (long long)f.max_pages * f.page_size;
+  if (tid == 0) bad_s = head < 0 || head >= f.n_pages || count < 0 || count > f.n_pages;
+  for (int r = tid; r < n; r += kN) keep_s[r] = n;
+  __syncthreads();
+  for (int r = tid; r < n; r += kN) {
+    const int p = f.parent[r], h = f.held[r];
+    if (p < -1 || p >= n || h < 0 || h > most) bad_s = 1;
+    else if (p >= 0) atomicMin(&keep_s[p], p == r ? -1 : r);   // the page that is not full stays with the request itself, or its first copy
+  }
+  __syncthreads();
+  const bool bad = bad_s;
+  int done = 0;
+  for (int r0 = 0; r0 < n; r0 += kN) {
+    const int r = r0 + tid;
+    Goes g = {-1, 0, -1, 0, -1, 0};
+    bool copied = false;
+    if (r < n && !bad) {
+      g.used = pages_for(f.held[r], a.per);
+      g.src = f.parent[r];
+      if (g.src >= 0) {
+        g.held = f.held[g.src];
+        g.fills = pages_for(g.held, a.per);
+        const int last = g.held - (int)divide((uint32_t)g.held, a.per) * f.page_size;
+        copied = last && keep_s[g.src] != r && g.src != r;
+      }
+    }
+    int all;
+    const int at = done + block_scan(copied, wave_s, &all);
+    if (copied) {
+      g.copy = at;
+      g.dst = at < count ? f.ring[ring_place(head, at, f.n_pages)] : -1;
+    }
+    if (r < n) a.goes[r] = g;
+    done += all;
+  }
+  if (tid == 0) *a.top = ForkHead{bad ? kForkBad : done > f.max_copies ? kForkCopies : done > count ? kForkNoPages : kForkOk, head, count, done};
+}
+
+// A thread's entries of a block's columns: entry i is column i % columns of request i / columns, counted from the first.
+struct Entry {
+  int r, c;
+  bool in;
+};
+__device__ __forceinline__ Entry entry_of(const ForkArgs& a, int c0, int k) {
+  const int i = k * kN + (int)threadIdx.x, r = i / a.columns;
+  return {r, c0 + i - r * a.columns, r < a.f.n_req && c0 + i - r * a.columns < a.f.max_pages};
+}
+
+// The pages of columns c0 .. that come back, in order of the columns, then of the requests, to a.list; their number.
+__device__ __forceinline__ int fork_columns(const ForkArgs& a, int c0) {
+  const moe_paged_fork& f = a.f;
+  const int n = f.n_req, tid = threadIdx.x;
+  __shared__ uint32_t bits_s[kEntries / 32];
+  __shared__ int wave_s[kN / kWave];
+  int old[kPer];
+  for (int i = tid; i < kEntries / 32; i += kN) bits_s[i] = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const Entry e = entry_of(a, c0, k);
+    old[k] = -1;
+    if (e.in && e.c < a.goes[e.r].used) old[k] = f.tables[(size_t)e.r * f.max_pages + e.c];
+    if ((uint32_t)old[k] >= (uint32_t)f.n_pages) old[k] = -1;
+    if (old[k] >= 0) mark_store(&a.mark[old[k]], 0);
+  }
+  __threadfence();
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const Entry e = entry_of(a, c0, k);
+    if (!e.in) continue;
+    const Goes g = a.goes[e.r];
+    if (g.src < 0 || e.c >= g.fills || (g.copy >= 0 && e.c == g.fills - 1)) continue;
+    const int page = f.tables[(size_t)g.src * f.max_pages + e.c];
+    if ((uint32_t)page < (uint32_t)f.n_pages) mark_store(&a.mark[page], 1);
+  }
+  __threadfence();
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kPer; ++k)
+    if (old[k] >= 0 && mark_load(&a.mark[old[k]]) != 1) atomicMax(&a.mark[old[k]], 2 + n - 1 - entry_of(a, c0, k).r);
+  __threadfence();
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const Entry e = entry_of(a, c0, k);
+    if (old[k] >= 0 && mark_load(&a.mark[old[k]]) == 2 + n - 1 - e.r) {
+      const int bit = (e.c - c0) * n + e.r;
+      atomicOr(&bits_s[bit / 32], 1u << bit % 32);
+    } else {
+      old[k] = -1;
+    }
+  }
+  __syncthreads();
+  // a thread a word: places within the block
+  const uint32_t mine = tid < kEntries / 32 ? bits_s[tid] : 0;
+  int all;
+  const int before = block_scan(__popc(mine), wave_s, &all);
+  __shared__ int first_s[kEntries / 32];
+  if (tid < kEntries / 32) first_s[tid] = before;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    if (old[k] < 0) continue;
+    const Entry e = entry_of(a, c0, k);
+    const int bit = (e.c - c0) * n + e.r;
+    a.list[(size_t)c0 * n + first_s[bit / 32] + __popc(bits_s[bit / 32] & ((1u << bit % 32) - 1))] = old[k];
+  }
+  return all;
+}
+
+// What the call leaves: block b's columns of the tables and its pages in the ring, block 0 the rest too.
+__device__ __forceinline__ void fork_finish(const ForkArgs& a, int b, int before, int back) {
+  const moe_paged_fork& f = a.f;
+  const int tid = threadIdx.x, n = f.n_req, c0 = b * a.columns;
+  ForkHead top = *a.top;
+  if (top.status == kForkOk || top.status == kForkNoPages || top.status == kForkCopies) {
+    if ((long long)top.count + back - top.copies > f.n_pages) top.status = kForkBad;
+  }
+  const bool ok = top.status == kForkOk;
+  int now[kPer];
+  if (ok || f.tables_out != f.tables) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const Entry e = entry_of(a, c0, k);
+      if (!e.in) continue;
+      const Goes g = a.goes[e.r];
+      const bool fills = ok && g.src >= 0 && e.c < g.fills;
+      now[k] = fills && g.copy >= 0 && e.c == g.fills - 1 ? g.dst : f.tables[(size_t)(fills ? g.src : e.r) * f.max_pages + e.c];
+    }
+    // copies name their pages by the old tables
+    if (ok)
+      for (int r = tid; r < n; r += kN) {
+        const Goes g = a.goes[r];
+        if (g.copy >= 0 && g.fills - 1 >= c0 && g.fills - 1 < c0 + a.columns) {
+          f.copies[3 * g.copy] = f.tables[(size_t)g.src * f.max_pages + g.fills - 1];
+          f.copies[3 * g.copy + 1] = g.dst;
+          f.copies[3 * g.copy + 2] = g.held - (g.fills - 1) * f.page_size;
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const Entry e = entry_of(a, c0, k);
+      if (e.in) f.tables_out[(size_t)e.r * f.max_pages + e.c] = now[k];
+    }
+  }
+  if (ok) {
+    const int tail = ring_place(top.head, top.count, f.n_pages);
+    for (int i = tid; i < a.counts[b]; i += kN) f.ring[ring_place(tail, before + i, f.n_pages)] = a.list[(size_t)c0 * n + i];
+  }
+  if (b == 0) {
+    for (int i = 3 * (ok ? top.copies : 0) + tid; i < 3 * f.max_copies; i += kN) f.copies[i] = -1;
+    for (int r = tid; r < n; r += kN) f.held_out[r] = ok ? a.goes[r].held : f.held[r];
+    if (tid == 0) {
+      f.ring_at_out[0] = ok ? ring_place(top.head, top.copies, f.n_pages) : top.head;
+      f.ring_at_out[1] = ok ? top.count - top.copies + back : top.count;
+      *f.status = top.status;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kN) void fork_requests_kernel(ForkArgs a) { fork_requests(a); }
+
+__global__ __launch_bounds__(kN) void fork_columns_kernel(ForkArgs a) {
+  const int back = fork_columns(a, (int)blockIdx.x * a.columns);
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = back;
+}
+
+__global__ __launch_bounds__(kN) void fork_finish_kernel(ForkArgs a) {
+  __shared__ int wave_s[kN / kWave], before_s;
+  int before = 0, back = 0;
+  for (int b0 = 0; b0 < a.blocks; b0 += kN) {
+    const int b = b0 + (int)threadIdx.x;
+    int all;
+    const int at = block_scan(b < a.blocks ? a.counts[b] : 0, wave_s, &all);
+    if (b == (int)blockIdx.x) before_s = back + at;
+    back += all;
+  }
+  __syncthreads();
+  before = before_s;
+  fork_finish(a, (int)blockIdx.x, before, back);
+}
+
+// ------------------------------------------------------------ copies
+
+constexpr int kLayers = 64;   // of a launch
+
+struct CopyArgs {
+  PageMap map;
+  int row;       // 16-byte pieces of a row (one head's position)
+  Divider by_row;
+  long long page, head, slot;   // strides in bytes
+  const int32_t* copies;
+  char* side[2 * kLayers];
+};
+
+// A block a (copy, pool): the first n positions of every head of a page.  All bytes are read once and written once.
+__global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
+  const int32_t* c = a.copies + 3 * (size_t)blockIdx.x;
+  const int src = c[0], dst = c[1], n = min(c[2], a.map.page_size);
+  if (!page_ok(a.map, src) || !page_ok(a.map, dst) || n <= 0) return;
+  char* pool = a.side[blockIdx.y];
+  const int head = (int)blockIdx.z;
+  const char* from = pool + (long long)src * a.page + (long long)head * a.head;
+  char* to = pool + (long long)dst * a.page + (long long)head * a.head;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const int all = n * a.row;
+  for (int i = threadIdx.x; i < all; i += 256) {
+    const int off = (int)divide((uint32_t)i, a.by_row);
+    const long long at = (long long)off * a.slot + (long long)(i - off * a.row) * 16;
+    *(u32x4*)(to + at) = *(const u32x4*)(from + at);
+  }
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+size_t moe_paged_fork_work_bytes(int n_req, int max_pages, int n_pages) {
+  if (n_req < 0 || n_req > kMostRequests || max_pages < 1 || n_pages < 1) return 0;
+  return sizeof(ForkHead) + (size_t)n_req * sizeof(Goes) + 4 * ((size_t)n_req * max_pages + max_pages + n_pages) + 64;
+}
+
+moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
+  if (!f) return set_error(MOE_ERR_ARG, "paged_fork: null argument");
+  if (f->n_req < 0 || f->max_pages < 1 || f->n_pages < 1 || f->page_size < 1 || f->max_copies < 0)
+    return set_error(MOE_ERR_ARG, "paged_fork: %d requests of %d pages, %d pages of %d, %d copies", f->n_req, f->max_pages, f->n_pages,
+                     f->page_size, f->max_copies);
+  if ((long long)f->n_pages * f->page_size > 0x7fffffffll || (long long)f->max_pages * f->page_size > kMostPositions)
+    return set_error(MOE_ERR_ARG, "paged_fork: %d pages of %d, %d a request: past 2^31 slots or 2^30 positions", f->n_pages, f->page_size,
+                     f->max_pages);
+  if (f->n_req > kMostRequests || f->max_copies > kMostRows)
+    return set_error(MOE_ERR_UNSUPPORTED, "paged_fork: %d requests, %d copies (at most %d, %d)", f->n_req, f->max_copies, kMostRequests, kMostRows);
+  for (const void* p : {(const void*)f->ring_at, (const void*)f->ring, (const void*)f->ring_at_out, (const void*)f->status, (const void*)f->work})
+    if (!p) return set_error(MOE_ERR_ARG, "paged_fork: null pointer");
+  if ((f->n_req && (!f->parent || !f->held || !f->tables || !f->held_out || !f->tables_out)) || (f->max_copies && !f->copies)) return set_error(MOE_ERR_ARG, "paged_fork: null pointer");
+  const size_t need = moe_paged_fork_work_bytes(f->n_req, f->max_pages, f->n_pages);
+  if (f->work_bytes < need || (uintptr_t)f->work % 16)
+    return set_error(MOE_ERR_ARG, "paged_fork: %zu bytes of work at %p, %zu needed, 16-byte aligned", f->work_bytes, f->work, need);
+  moe_status st = ensure_init();
+  if (st) return st;
+  OnDevice on;
+  if ((st = on.enter())) return st;
+  ForkArgs a;
+  a.f = *f;
+  a.per = make_divider((uint32_t)f->page_size);
+  a.columns = kEntries / (f->n_req ? f->n_req : 1);
+  if (a.columns > f->max_pages) a.columns = f->max_pages;
+  a.blocks = (f->max_pages + a.columns - 1) / a.columns;
+  a.top = (ForkHead*)f->work;
+  a.goes = (Goes*)(a.top + 1);
+  a.counts = (int*)(a.goes + f->n_req);
+  a.list = a.counts + f->max_pages;
+  a.mark = a.list + (size_t)f->n_req * f->max_pages;
+  hipLaunchKernelGGL(fork_requests_kernel, dim3(1), dim3(kN), 0, stream(), a);
+  if ((st = check_hip(hipGetLastError(), "paged_fork launch"))) return st;
+  hipLaunchKernelGGL(fork_columns_kernel, dim3((unsigned)a.blocks), dim3(kN), 0, stream(), a);
+  if ((st = check_hip(hipGetLastError(), "paged_fork launch"))) return st;
+  hipLaunchKernelGGL(fork_finish_kernel, dim3((unsigned)a.blocks), dim3(kN), 0, stream(), a);
+  return check_hip(hipGetLastError(), "paged_fork launch");
+}
+
+moe_status moe_paged_copy_dev(const int32_t* copies, int n, const moe_pages* layers, int n_layers) {
+  if (n < 0 || n_layers < 0 || n > kMostRows) return set_error(MOE_ERR_ARG, "paged_copy: %d copies in %d layers", n, n_layers);
+  if (n == 0 || n_layers == 0) return MOE_OK;
+  if (!copies || !layers) return set_error(MOE_ERR_ARG, "paged_copy: null pointer");
+  PageMap map;
+  moe_status st;
+  for (int l = 0; l < n_layers; ++l) {
+    if ((st = check_pages(&layers[l], "paged_copy", &map))) return st;
+    const moe_pages &x = layers[l], &y = layers[0];
+    if (x.dtype != y.dtype || x.n_pages != y.n_pages || x.page_size != y.page_size || x.n_kv != y.n_kv || x.head_dim != y.head_dim ||
+        x.page_stride != y.page_stride || x.head_stride != y.head_stride || x.slot_stride != y.slot_stride)
+      return set_error(MOE_ERR_UNSUPPORTED, "paged_copy: layer %d's pages are laid out otherwise than layer 0's", l);
+  }
+  if (map.n_kv > 65535) return set_error(MOE_ERR_ARG, "paged_copy: %d heads", map.n_kv);
+  if ((st = ensure_init())) return st;
+  OnDevice on;
+  if ((st = on.enter())) return st;
+  const int size = type_bytes(layers[0].dtype);
+  CopyArgs a;
+  a.map = map;
+  a.row = map.head_dim * size / 16;
+  a.by_row = make_divider((uint32_t)a.row);
+  a.page = map.page_stride * size, a.head = map.head_stride * size, a.slot = map.slot_stride * size;
+  a.copies = copies;
+  for (int l0 = 0; l0 < n_layers; l0 += kLayers) {
+    const int m = n_layers - l0 < kLayers ? n_layers - l0 : kLayers;
+    for (int l = 0; l < m; ++l) {
+      a.side[2 * l] = (char*)layers[l0 + l].k;
+      a.side[2 * l + 1] = (char*)layers[l0 + l].v;
+    }
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)n, (unsigned)(2 * m), (unsigned)map.n_kv), dim3(256), 0, stream(), a);
+    if ((st = check_hip(hipGetLastError(), "paged_copy launch"))) return st;
+  }
+  return MOE_OK;
+}
+
+}  // extern "C"

@@ -89,6 +89,32 @@ class PagedAttn(ctypes.Structure):
                 ("ldo", _LL), ("work", _P), ("work_bytes", _SZ)]
 
 
+class BeamSelect(ctypes.Structure):
+    """moe_beam_select: the best candidates of each group of beams."""
+
+    _fields_ = [("n_groups", _I), ("n_beam", _I), ("vocab", _I), ("logits", _P), ("ld", _LL),
+                ("score", _P), ("done", _P), ("weight", _P), ("eos", _I), ("pad", _I)] + \
+               [(n, _P) for n in ("parent", "token", "score_out", "done_out", "fresh", "work")] + \
+               [("work_bytes", _SZ)]
+
+
+class PagedFork(ctypes.Structure):
+    """moe_paged_fork: requests that go on as copies of others."""
+
+    _fields_ = [(n, _I) for n in ("n_req", "max_pages", "n_pages", "page_size", "max_copies")] + \
+               [(n, _P) for n in ("parent", "held", "ring_at", "ring", "tables", "held_out",
+                                  "ring_at_out", "tables_out", "copies", "status", "work")] + \
+               [("work_bytes", _SZ)]
+
+
+class PagedShare(ctypes.Structure):
+    """moe_paged_share: the positions that neighbouring rows have in common."""
+
+    _fields_ = [(n, _I) for n in ("T", "n_req", "max_pages", "page_size", "n_q", "n_kv", "head_dim")] + \
+               [("req", _P), ("pos", _P), ("tables", _P), ("n_groups", _I), ("first", _P),
+                ("prefix", _P), ("plan", _P), ("plan_bytes", _SZ)]
+
+
 _SIGS = {
     "matmul_adaptive": (None, [_P, _P, _P, _P, _I, _I, _I]),
     "moe_init": (_I, [_I]),
@@ -141,6 +167,15 @@ _SIGS = {
     "moe_paged_heads_dev": (_I, [_P, _P]),
     "moe_paged_attn_work_bytes": (_SZ, [_I, _I, _I, _I]),
     "moe_paged_attn_dev": (_I, [_P, _P]),
+    "moe_beam_select_work_bytes": (_SZ, [_I, _I, _I]),
+    "moe_beam_select_dev": (_I, [_P]),
+    "moe_paged_fork_work_bytes": (_SZ, [_I, _I, _I]),
+    "moe_paged_fork_dev": (_I, [_P]),
+    "moe_paged_copy_dev": (_I, [_P, _I, _P, _I]),
+    "moe_paged_share_plan_bytes": (_SZ, [_I] * 5),
+    "moe_paged_share_dev": (_I, [_P]),
+    "moe_paged_attn_shared_work_bytes": (_SZ, [_I] * 5),
+    "moe_paged_attn_shared_dev": (_I, [_P, _P, _P]),
     "moe_layer_debug_buffers": (_I, [_P, ctypes.POINTER(_P), ctypes.POINTER(_P),
                                      ctypes.POINTER(_P)]),
     "moe_model_create": (_I, [_P, _P, _I, ctypes.POINTER(_P)]),
