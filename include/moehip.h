@@ -605,7 +605,7 @@ moe_status moe_paged_copy_dev(const int32_t* copies, int n, const moe_pages* lay
  * leaves 0 .. T, makes every prefix 0.  plan: moe_paged_share_plan_bytes,
  * 16-byte aligned: what moe_paged_attn_shared_dev reads of it, in every layer of
  * the step; req, pos and tables stay as they are until then.  T and n_groups
- * at most 65536. */
+ * at most 16384. */
 typedef struct {
   int T, n_req, max_pages, page_size;
   int n_q, n_kv, head_dim;

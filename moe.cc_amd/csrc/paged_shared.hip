@@ -1,27 +1,114 @@
 // paged_shared.hip - attention of rows whose requests begin in the same pages
 // (moe_paged_share_dev, moe_paged_attn_shared_dev, include/moehip.h).
+//
+// out_t = softmax(scale q_t . k) v over positions 0 .. pos[t], in two parts that
+// a last kernel joins by their maxima and sums: the positions that a group of
+// rows shares, with the query heads of all its rows as columns of one product,
+// and the rest of each row for itself.  Which positions those are, and how they
+// are cut into blocks, is the same in every layer of a step, so
+// moe_paged_share_dev writes it down once: a list of items, each some columns
+// against some positions of one request's table, a block each.
+//
+// A column is a (row, query head) of one key-value head: column c of a group
+// is head c % G of its row c / G, G = n_q / n_kv.
 #include <math.h>
 
 #include <type_traits>
 
 #include "moe_device.h"
 #include "paged_attn.h"
+#include "paged_tile.h"
 
 namespace moe {
 namespace {
 
-enum { F32 = MOE_PAGE_F32, F16 = MOE_PAGE_F16, BF16 = MOE_PAGE_BF16, E4M3 = MOE_PAGE_E4M3 };
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kMostShared = 1 << 14;   // rows, groups of a call
+constexpr int kN = 1024;               // threads of the plan's block
 
-constexpr int kMostShared = 1 << 16;   // rows, groups of a call
+// ---------------------------------------------------------------- the plan
 
-// ---------------------------------------------------------------- which positions groups share
+// Columns `col0` .. of the rows from row0 on, against positions begin .. end - 1 of request req.
+struct Item {
+  int row0, col0, cols, req;
+  int begin, end;
+  int part;     // where its sums go
+  int direct;   // 1: it is all that its row has
+};
+
+// A row's parts: of column c of its group tile c / columns, pieces part0 + tile * pieces ..; of its own own0 + tile * owns ..
+struct RowPlan {
+  int state, group, row0;
+  int part0, pieces;
+  int own0, owns, pad;
+};
+enum RowState { kLeave, kZero, kNan, kDone, kJoin };
+
+struct GroupPlan {
+  int row0, rows, req, prefix;   // prefix: positions taken together, 0: none
+  int tiles, units, part0, pieces;
+};
+
+struct PlanHead {
+  int prefix_items, own_items, pad[2];
+};
+
+// How a call is cut: the same for moe_paged_share_dev and moe_paged_attn_shared_dev.
+struct ShareCut {
+  int group;          // query heads of a key-value head
+  int columns;        // of a prefix item
+  int own_columns;    // of a row's own
+  int own_tiles;      // of a row
+  int slots;          // items that are resident at once, about
+  int prefix_items, own_items;   // at most
+};
+
+ShareCut share_cut(int T, int n_groups, int n_q, int n_kv, int head_dim) {
+  ShareCut c;
+  c.group = n_q / n_kv;
+  const long long mean = n_groups ? ((long long)T + n_groups - 1) / n_groups * c.group : 0;
+  c.columns = 16;
+  while (c.columns < mean && c.columns < (head_dim > 128 ? 64 : 128)) c.columns *= 2;
+  c.own_columns = c.group < 16 ? c.group : 16;
+  c.own_tiles = (c.group + 15) / 16;
+  const int resident = kCUs * (head_dim <= 128 ? 2 : 1);
+  c.slots = resident > n_kv ? resident / n_kv : 1;
+  c.prefix_items = c.slots + (int)((long long)T * c.group / c.columns) + n_groups;
+  c.own_items = c.slots + T * c.own_tiles;
+  return c;
+}
+
+struct PlanParts {
+  PlanHead* head;
+  int* common;       // [T] leading pages that a row and its group's first share; kNotLive: no row to count
+  RowPlan* rows;     // [T]
+  GroupPlan* groups; // [n_groups]
+  Item* prefix;      // [prefix_items]
+  Item* own;         // [own_items]
+};
+constexpr int kNotLive = 0x7fffffff;
+
+size_t plan_parts(const ShareCut& c, int T, int n_groups, void* base, PlanParts* p) {
+  char* at = (char*)base;
+  auto take = [&](auto** q, size_t n) {
+    *q = (std::remove_reference_t<decltype(*q)>)at;
+    at += (n * sizeof(**q) + 15) / 16 * 16;
+  };
+  take(&p->head, 1);
+  take(&p->common, (size_t)T);
+  take(&p->rows, (size_t)T);
+  take(&p->groups, (size_t)n_groups);
+  take(&p->prefix, (size_t)c.prefix_items);
+  take(&p->own, (size_t)c.own_items);
+  return (size_t)(at - (char*)base);
+}
 
 struct ShareArgs {
   moe_paged_share s;
   Divider per;    // by page_size
-  int* common;    // plan [T] leading pages that a row and its group's first share; kNotLive: no row to count
+  ShareCut cut;
+  PlanParts p;
 };
-constexpr int kNotLive = 0x7fffffff;
 
 // A wave a row: the group that holds it, that group's first live row, and how many leading pages the two have in common.
 __global__ __launch_bounds__(256) void share_rows_kernel(ShareArgs a) {
@@ -31,19 +118,21 @@ __global__ __launch_bounds__(256) void share_rows_kernel(ShareArgs a) {
   const int positions = s.max_pages * s.page_size;
   auto length = [&](int r) { return row_length(s.req ? s.req[r] : r, s.pos[r], s.n_req, positions); };
   const int len = length(t);
-  if (len <= 0) {
-    if (lane == 0) a.common[t] = kNotLive;
-    return;
-  }
   int lo = 0, hi = s.n_groups;   // the last group that starts at or before t
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (s.first[mid] <= t) lo = mid + 1;
     else hi = mid;
   }
+  const int group = lo > 0 && t < s.first[lo] ? lo - 1 : -1;
+  if (lane == 0) a.p.rows[t].group = group;
+  if (len <= 0) {
+    if (lane == 0) a.p.common[t] = kNotLive;
+    return;
+  }
   int lead = t;
-  if (lo > 0 && t < s.first[lo]) {
-    for (int r0 = max(s.first[lo - 1], 0); r0 < t; r0 += kWave) {
+  if (group >= 0) {
+    for (int r0 = max(s.first[group], 0); r0 < t; r0 += kWave) {
       const int r = r0 + lane;
       const uint64_t live = __ballot(r < t && length(r) > 0);
       if (live) {
@@ -64,24 +153,153 @@ __global__ __launch_bounds__(256) void share_rows_kernel(ShareArgs a) {
         break;
       }
     }
-  if (lane == 0) a.common[t] = same;
+  if (lane == 0) a.p.common[t] = same;
 }
 
-// One block, a wave a group.
-__global__ __launch_bounds__(1024) void share_groups_kernel(ShareArgs a) {
-  const moe_paged_share& s = a.s;
-  const int tid = threadIdx.x, lane = tid % kWave;
-  bool bad = false;
-  for (int g = tid; g < s.n_groups; g += 1024) bad |= s.first[g] < 0 || s.first[g] > s.first[g + 1] || s.first[g + 1] > s.T;
-  bad = __syncthreads_or(bad);
-  for (int g = tid / kWave; g < s.n_groups; g += 1024 / kWave) {
-    int least = kNotLive;
-    if (!bad)
-      for (int r = s.first[g] + lane; r < s.first[g + 1]; r += kWave) least = min(least, a.common[r]);
+// Sum over the block's threads up to and without this one, and of all.
+__device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int x = v;
 #pragma unroll
-    for (int c = 32; c; c /= 2) least = min(least, __shfl_xor(least, c));
-    if (lane == 0) s.prefix[g] = least == kNotLive ? 0 : least * s.page_size;
+  for (int c = 1; c < kWave; c *= 2) {
+    const int y = __shfl_up(x, c);
+    if (lane >= c) x += y;
   }
+  if (lane == kWave - 1) wave_s[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < kN / kWave; ++w) {
+    const int y = wave_s[w];
+    if (w < wave) before += y;
+    all += y;
+  }
+  __syncthreads();
+  *total = all;
+  return before + x - v;
+}
+
+__device__ __forceinline__ int units_in_all(int positions) { return (positions + kUnit - 1) / kUnit; }
+
+// One block: the groups' prefixes, and the items.  Prefix tiles' units (128 positions) and rows' own are each cut so that
+// their items are about as many as are resident at once: pieces of ceil(all units / slots), at least one an item, so no
+// more items than `slots` and one for each tile or row.
+__global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
+  const moe_paged_share& s = a.s;
+  const ShareCut& cut = a.cut;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, positions = s.max_pages * s.page_size;
+  __shared__ int wave_s[kN / kWave];
+  __shared__ unsigned long long units_s, own_s;
+  if (tid == 0) units_s = own_s = 0;
+  bool bad = false;
+  for (int g = tid; g < s.n_groups; g += kN) bad |= s.first[g] < 0 || s.first[g] > s.first[g + 1] || s.first[g + 1] > s.T;
+  bad = __syncthreads_or(bad);
+  auto request = [&](int r) { return s.req ? s.req[r] : r; };
+  // ---- the groups: a wave each
+  for (int g = wave; g < s.n_groups; g += kN / kWave) {
+    const int r0 = s.first[g], r1 = bad ? r0 : s.first[g + 1];
+    int least = kNotLive, live = 0, lead = kNotLive;
+    for (int r = r0 + lane; r < r1; r += kWave) {
+      const int c = a.p.common[r];
+      least = min(least, c);
+      if (c != kNotLive) ++live, lead = min(lead, r);
+    }
+#pragma unroll
+    for (int c = 32; c; c /= 2) {
+      least = min(least, __shfl_xor(least, c));
+      lead = min(lead, __shfl_xor(lead, c));
+      live += __shfl_xor(live, c);
+    }
+    if (lane == 0) {
+      const int prefix = least == kNotLive ? 0 : least * s.page_size;
+      s.prefix[g] = prefix;
+      GroupPlan p = {r0, r1 - r0, 0, 0, 0, 0, 0, 0};
+      if (live > 1 && prefix > 0) {   // one row alone reads its positions as its own
+        p.req = request(lead);
+        p.prefix = prefix;
+        p.tiles = (int)(((long long)p.rows * cut.group + cut.columns - 1) / cut.columns);
+        p.units = units_in_all(prefix);
+        atomicAdd(&units_s, (unsigned long long)p.tiles * p.units);
+      }
+      a.p.groups[g] = p;
+    }
+  }
+  __threadfence_block();
+  __syncthreads();
+  auto piece = [&](unsigned long long all) {
+    const unsigned long long n = (all + cut.slots - 1) / cut.slots;
+    return n ? (int)(n < 0x40000000 ? n : 0x40000000) : 1;
+  };
+  const int per = piece(units_s);
+  int done = 0;
+  for (int g0 = 0; g0 < s.n_groups; g0 += kN) {
+    const int g = g0 + tid;
+    int pieces = 0, tiles = 0;
+    if (g < s.n_groups) {
+      pieces = (a.p.groups[g].units + per - 1) / per;
+      tiles = a.p.groups[g].tiles;
+    }
+    int all;
+    const int at = done + block_scan(tiles * pieces, wave_s, &all);
+    if (g < s.n_groups) a.p.groups[g].part0 = at, a.p.groups[g].pieces = pieces;
+    done += all;
+  }
+  if (tid == 0) a.p.head->prefix_items = done;
+  __threadfence_block();
+  __syncthreads();
+  for (int g = wave; g < s.n_groups; g += kN / kWave) {
+    const GroupPlan p = a.p.groups[g];
+    for (int i = lane; i < p.tiles * p.pieces; i += kWave) {
+      const int tile = i / p.pieces, j = i - tile * p.pieces;
+      Item x = {p.row0, tile * cut.columns, min(cut.columns, p.rows * cut.group - tile * cut.columns), p.req, 0, 0, p.part0 + i, 0};
+      x.begin = (int)((long long)p.units * j / p.pieces) * kUnit;
+      x.end = min((int)((long long)p.units * (j + 1) / p.pieces) * kUnit, p.prefix);
+      a.p.prefix[p.part0 + i] = x;
+    }
+  }
+  // ---- the rows: a thread each
+  auto own_of = [&](int r, int* len, int* group) {
+    const int g = a.p.rows[r].group;
+    *len = row_length(request(r), s.pos[r], s.n_req, positions);
+    *group = !bad && g >= 0 && *len > 0 && a.p.groups[g].prefix ? g : -1;
+    return *len > 0 ? *len - (*group >= 0 ? a.p.groups[*group].prefix : 0) : 0;
+  };
+  unsigned long long mine = 0;
+  for (int r = tid; r < s.T; r += kN) {
+    int len, group;
+    mine += (unsigned long long)units_in_all(own_of(r, &len, &group)) * cut.own_tiles;
+  }
+  if (mine) atomicAdd(&own_s, mine);
+  __syncthreads();
+  const int per_own = piece(own_s);
+  done = 0;
+  for (int r0 = 0; r0 < s.T; r0 += kN) {
+    const int r = r0 + tid;
+    int len = 0, group = -1, own = 0, owns = 0;
+    if (r < s.T) {
+      own = own_of(r, &len, &group);
+      owns = (units_in_all(own) + per_own - 1) / per_own;
+    }
+    int all;
+    const int at = done + block_scan(owns * cut.own_tiles, wave_s, &all);
+    if (r < s.T) {
+      RowPlan p = {kJoin, group, r, 0, 0, at, owns, 0};
+      const int prefix = group >= 0 ? a.p.groups[group].prefix : 0, units = units_in_all(own);
+      if (group >= 0) p.row0 = a.p.groups[group].row0, p.part0 = a.p.groups[group].part0, p.pieces = a.p.groups[group].pieces;
+      if (len <= 0) p.state = len == kPadding ? kLeave : len == kOutside ? kNan : kZero;
+      else if (group < 0 && owns == 1) p.state = kDone;
+      a.p.rows[r] = p;
+      for (int tile = 0; tile < cut.own_tiles; ++tile)
+        for (int j = 0; j < owns; ++j) {
+          const int i = at + tile * owns + j;
+          Item x = {r, tile * 16, min(16, cut.group - tile * 16), request(r), 0, 0, i, p.state == kDone};
+          x.begin = prefix + (int)((long long)units * j / owns) * kUnit;
+          x.end = prefix + min((int)((long long)units * (j + 1) / owns) * kUnit, own);
+          a.p.own[i] = x;
+        }
+    }
+    done += all;
+  }
+  if (tid == 0) a.p.head->own_items = done;
 }
 
 moe_status check_share(const moe_paged_share* s, const char* who) {
@@ -105,83 +323,468 @@ moe_status check_share(const moe_paged_share* s, const char* who) {
 
 // ---------------------------------------------------------------- attention
 
-template <int CT>
-__device__ __forceinline__ float value_at(const char* p, long long i) {
-  if constexpr (CT == F32) return ((const float*)p)[i];
-  else if constexpr (CT == F16) return (float)((const _Float16*)p)[i];
-  else if constexpr (CT == BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
-  else return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)p)[i], 0);
+struct SharedLaunch {
+  AttnPages g;
+  ShareCut cut;
+  PlanParts p;
+  Divider by_group;
+  // work: [n_kv][items][columns] maxima and sums, [n_kv][items][columns][head_dim] values
+  float* prefix_ml;
+  float* prefix_o;
+  float* own_ml;
+  float* own_o;
+};
+
+size_t shared_work(const ShareCut& c, int n_kv, int head_dim, void* base, SharedLaunch* L) {
+  const size_t prefix = (size_t)n_kv * c.prefix_items * c.columns, own = (size_t)n_kv * c.own_items * c.own_columns;
+  if (L) {
+    L->prefix_o = (float*)base;
+    L->own_o = L->prefix_o + prefix * head_dim;
+    L->prefix_ml = L->own_o + own * head_dim;
+    L->own_ml = L->prefix_ml + 2 * prefix;
+  }
+  return (prefix + own) * (head_dim + 2) * 4 + 16;
 }
 
-// A wave a (row, query head): 64 positions a step, a lane each for the scores, then a lane a dimension for the values.
+// What an item says must lie in the call's rows and tables, whatever the plan holds.
+__device__ __forceinline__ bool item_ok(const SharedLaunch& L, const Item& x, int parts, int columns) {
+  const moe_paged_attn& a = L.g.a;
+  return x.row0 >= 0 && x.col0 >= 0 && x.cols > 0 && x.cols <= columns && x.col0 <= (1 << 29) &&
+         x.row0 <= a.T - 1 - (int)divide((uint32_t)(x.col0 + x.cols - 1), L.by_group) && (uint32_t)x.req < (uint32_t)a.n_req &&
+         x.begin >= 0 && x.begin < x.end && x.end <= a.max_pages * L.g.map.page_size && (uint32_t)x.part < (uint32_t)parts;
+}
+
 template <int CT>
-__global__ __launch_bounds__(kWave) void shared_attn_kernel(AttnPages g) {
+__device__ __forceinline__ u32x2 widen16(uint32_t x) {   // four 8-bit values -> two dwords of f16 pairs (exact)
+  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true))};
+}
+
+// Two fp32 values into the same place of NP operands: three bf16 parts, whose sum they are, or two f16 parts, each rounded
+// to nearest even, whose sum is off by at most 2^-23 of the value (twice an fp32 rounding, at the worst bits) and by 2^-25.
+template <bool HALF, int NP>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&p)[NP]) {
+  if constexpr (HALF) {
+    const f16x2 h = {(_Float16)x, (_Float16)y};
+    const f16x2 l = {(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])};
+    p[0] = __builtin_bit_cast(uint32_t, h);
+    p[1] = __builtin_bit_cast(uint32_t, l);
+  } else {
+    split2<false>(x, y, &p[0], &p[1], &p[2]);
+  }
+}
+
+// Row and query head of an item's column.
+struct Column {
+  int row, head;
+};
+__device__ __forceinline__ Column column_of(const SharedLaunch& L, const Item& x, int kv, int c) {
+  const int at = x.col0 + c, r = (int)divide((uint32_t)at, L.by_group);
+  return {x.row0 + r, kv * L.cut.group + at - r * L.cut.group};
+}
+
+// ---------------------------------------------------------------- sixteen columns
+
+// A block an item, or sixteen columns of it (blockIdx.z); its waves take every fourth step of 32 positions and are joined
+// in LDS at the end.  K and V go straight into the registers that the matrix instructions read, 16 bytes a lane, keys and
+// values requested a step ahead:
+//   scores   16 keys x 16 columns a tile: lane l holds 16-byte pieces of key l % 16 and the matching query values of column l % 16
+//   weights  come out as keys 4 (l / 16) + i of column l % 16 and go back in as the second operand from the same lane
+//   values   lane l holds the keys 4 (l / 16) + i of both tiles at its 1 / 16 of the dimensions; pairs of keys are put side by
+//            side by byte permutes
+// 16-bit operands: bf16 pages with queries and weights in three parts; f16 and 8-bit pages (exact in f16) in two f16 parts.
+// fp32 pages use the fp32 instruction.
+template <int CT, int HDP, bool WHOLE>
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_kernel(SharedLaunch L, int own) {
+  constexpr bool HALF = CT == F16 || CT == E4M3;
+  constexpr int NP = HALF ? 2 : 3;                 // parts of an fp32 value
   constexpr int S = CT == F32 ? 4 : CT == E4M3 ? 1 : 2;
+  constexpr int E = 16 / S;                        // elements of a 16-byte piece
+  constexpr int NK = HDP / E / 4;                  // a lane's pieces of a key
+  constexpr int VE = HDP / 16;                     // a lane's dimensions of a value
+  constexpr int EV = VE < E ? VE : E, NV = VE / EV, VW = EV * S / 4;   // its pieces: elements, number, dwords
+  constexpr int KT = CT == F32 && HDP == 256 ? 1 : 2;                  // tiles of 16 positions a step
+  constexpr int NQ = CT == F32 ? 1 : HDP / 32;     // query operands of 8 values
+  constexpr int STEP = 16 * KT;
+  constexpr float kLift = HALF ? 14.0f : 0.0f;     // weights are held times 2^14 where their parts are f16
+
+  const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
-  const int t = (int)blockIdx.x, head = (int)blockIdx.y, lane = threadIdx.x, hd = g.map.head_dim;
-  const int req = a.req ? a.req[t] : t;
-  const int len = row_length(req, a.pos[t], a.n_req, a.max_pages * g.map.page_size);
-  if (len == kPadding) return;
-  const int kv = head / (a.n_q / g.map.n_kv);
-  const float* q = a.q + (size_t)t * a.ldq + (size_t)head * hd;
-  float* out = a.out + (size_t)t * a.ldo + (size_t)head * hd;
-  __shared__ float q_s[256], p_s[kWave];
-  __shared__ long long at_s[kWave];
-  const float scale = a.scale * (g.k_scale ? g.k_scale[kv] : 1.0f), vs = g.v_scale ? g.v_scale[kv] : 1.0f;
-  for (int d = lane; d < hd; d += kWave) q_s[d] = q[d] * scale;
-  __syncthreads();
-  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-  bool bad = len == kOutside;
-  for (int p0 = 0; p0 < len; p0 += kWave) {
-    const int p = p0 + lane;
-    float s = -INFINITY;
-    long long at = 0;
-    if (p < len) {
-      const int page = a.tables[(size_t)req * a.max_pages + divide((uint32_t)p, g.map.per)];
-      if (page_ok(g.map, page)) {
-        at = page_row(g.map, page, kv, p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size);
-        s = 0.0f;
-        for (int d = 0; d < hd; ++d) s = fmaf(q_s[d], value_at<CT>((const char*)g.k + at * S, d), s);
-      } else {
-        bad = true;
+  const int limit = own ? L.p.head->own_items : L.p.head->prefix_items, parts = own ? L.cut.own_items : L.cut.prefix_items;
+  if ((int)blockIdx.x >= min(limit, parts)) return;
+  Item it = (own ? L.p.own : L.p.prefix)[blockIdx.x];
+  const int columns = own ? L.cut.own_columns : L.cut.columns;
+  if (!item_ok(L, it, parts, columns)) return;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int hd = g.map.head_dim, kv = (int)blockIdx.y, sub = (int)blockIdx.z * 16;
+  const int heads = min(16, it.cols - sub);
+  if (heads <= 0) return;
+  const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
+  const float vs = g.v_scale ? scalar_load(g.v_scale, kv) : 1.0f;
+  const long long head_at = (long long)kv * g.map.head_stride;
+  const char* kbase = (const char*)g.k + head_at * S;
+  const char* vbase = (const char*)g.v + head_at * S;
+  const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: below 2^24
+  const int col = lane % 16, quad = lane / 16;
+  const int first = it.begin, end = it.end;
+
+  uint32_t kpiece[NK], vpiece[NV];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) kpiece[j] = (uint32_t)min((4 * j + quad) * 16, hd * S - 16);
+#pragma unroll
+  for (int h = 0; h < NV; ++h) vpiece[h] = (uint32_t)min((16 * h + col) * EV * S, hd * S - EV * S);
+
+  const Column mine = column_of(L, it, kv, sub + min(col, heads - 1));
+  const float* q = a.q + (size_t)mine.row * a.ldq + (size_t)mine.head * hd;
+  constexpr int NX = CT == F32 ? NK : 2 * NQ;
+  f32x4 x[NX];
+  auto query_dim = [&](int s) {   // of x[s]
+    return CT == F32 ? (4 * s + quad) * 4 : CT == E4M3 ? (4 * (s / 4) + quad) * 16 + 4 * (s % 4) : (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
+  };
+#pragma unroll
+  for (int s = 0; s < NX; ++s) x[s] = *(const f32x4u*)(q + min(query_dim(s), hd - 4));
+
+  const int* table = a.tables + (size_t)it.req * a.max_pages;
+  bool bad = false;
+  auto base_of = [&](int step) { return first + (step * kWaves + wave) * STEP; };
+  struct Look { int p[WHOLE ? KT : 1]; };
+  auto look = [&](int step) {
+    Look r;
+    const int base = base_of(step);
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) r.p[t] = scalar_load(table, divide((uint32_t)min(base + 16 * t, (end - 1) & ~15), g.map.per));
+    } else {
+      r.p[0] = table[divide((uint32_t)min(base + lane, end - 1), g.map.per)];
+    }
+    return r;
+  };
+  // WHOLE (a tile of 16 positions lies in one page): byte offsets of a step's tiles and the last position of each that
+  // counts; else of the lane's position.  Positions past the end take the last one's row
+  struct At { long long tile[WHOLE ? KT : 1]; int lim[WHOLE ? KT : 1]; };
+  auto place = [&](int step, const Look& r) {
+    At o;
+    const int base = base_of(step);
+#pragma unroll
+    for (int t = 0; t < (WHOLE ? KT : 1); ++t) {
+      const int p = WHOLE ? min(base + 16 * t, (end - 1) & ~15) : min(base + lane, end - 1);
+      int pg = r.p[t];
+      if (!page_ok(g.map, pg)) bad = true, pg = 0;
+      const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
+      o.tile[t] = ((long long)pg * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
+      o.lim[t] = WHOLE ? min(end - 1 - p, 15) : 15;
+    }
+    return o;
+  };
+  uint32_t kr[KT][NK][4], vr[4 * KT][NV][VW];
+  auto load_k = [&](const At& o) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const char* base = WHOLE ? kbase + o.tile[t] : kbase + __shfl(o.tile[0], 16 * t + col);
+      const uint32_t off = WHOLE ? __umul24((uint32_t)min(col, o.lim[t]), slot_bytes) : 0;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) load_piece<16, false>(base + (off + kpiece[j]), kr[t][j]);
+    }
+  };
+  auto load_v = [&](const At& o) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const char* base = WHOLE ? vbase + o.tile[t] : vbase + __shfl(o.tile[0], 16 * t + 4 * quad + i);
+        const uint32_t off = WHOLE ? __umul24((uint32_t)min(4 * quad + i, o.lim[t]), slot_bytes) : 0;
+#pragma unroll
+        for (int h = 0; h < NV; ++h) load_piece<EV * S, false>(base + (off + vpiece[h]), vr[4 * t + i][h]);
+      }
+  };
+
+  f32x4 o[VE];
+#pragma unroll
+  for (int c = 0; c < VE; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;
+  f32x4 s[KT];
+  u32x4 qp[NP][NQ];
+  float unlift = 1.0f;
+  auto score = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        if constexpr (CT == F32) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][j][c]), x[j][c], s[t], 0, 0, 0);
+        } else if constexpr (CT == E4M3) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x2 y = widen16<CT>(kr[t][j][2 * u]), z = widen16<CT>(kr[t][j][2 * u + 1]);
+            const u32x4 k = {y[0], y[1], z[0], z[1]};
+#pragma unroll
+            for (int n = 0; n < NP; ++n) s[t] = mfma32<HALF>(k, qp[n][2 * j + u], s[t]);
+          }
+        } else {
+          const u32x4 k = {kr[t][j][0], kr[t][j][1], kr[t][j][2], kr[t][j][3]};
+#pragma unroll
+          for (int n = 0; n < NP; ++n) s[t] = mfma32<HALF>(k, qp[n][j], s[t]);
+        }
+      }
+  };
+  auto gather = [&](int base) __attribute__((always_inline)) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (HALF) s[t][i] *= unlift;
+        if (base + STEP > end && base + 16 * t + 4 * quad + i >= end) s[t][i] = -INFINITY;
+        top = fmaxf(top, s[t][i]);
+      }
+    top = fmaxf(m, head_max(top));
+    if (__any(top > m)) {
+      const float keep = top == -INFINITY ? 1.0f : exp2_hw(m - top);
+      l *= keep;
+#pragma unroll
+      for (int c = 0; c < VE; ++c) o[c] *= keep;
+      m = top;
+    }
+    const float from = (m == -INFINITY ? 0.0f : m) - kLift;
+    float p[KT][4];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[t][i] = exp2_hw(s[t][i] - from);
+        l += p[t][i];
+      }
+    if constexpr (CT == F32) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < VE; ++c)
+            o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * t + i][c / EV][c % EV]), p[t][i], o[c], 0, 0, 0);
+    } else {
+      u32x4 pp[NP];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t u[NP];
+        split_pair<HALF, NP>(p[c / 2][2 * (c % 2)], p[c / 2][2 * (c % 2) + 1], u);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) pp[n][c] = u[n];
+      }
+#pragma unroll
+      for (int h = 0; h < NV; ++h) {
+        uint32_t w16[8][EV / 2];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int d = 0; d < VW; ++d) {
+            if constexpr (CT == E4M3) {
+              const u32x2 y = widen16<CT>(vr[k][h][d]);
+              w16[k][2 * d] = y[0], w16[k][2 * d + 1] = y[1];
+            } else {
+              w16[k][d] = vr[k][h][d];
+            }
+          }
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          u32x4 y;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            y[c] = __builtin_amdgcn_perm(w16[2 * c + 1][e / 2], w16[2 * c][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int n = 0; n < NP; ++n) o[h * EV + e] = mfma32<HALF>(y, pp[n], o[h * EV + e]);
+        }
       }
     }
-    float top = s;
+  };
+
+  if (base_of(0) < end) {
+    At at = place(0, look(0));
+    load_k(at);
+    load_v(at);
+    Look next = look(1);
+    // ---- queries times scale and log2(e): scores are powers of two
+    float lift = 1.0f;
 #pragma unroll
-    for (int c = 32; c; c /= 2) top = fmaxf(top, __shfl_xor(top, c));
-    top = fmaxf(top, m);
-    const float from = top == -INFINITY ? 0.0f : top, keep = expf(m - from), w = expf(s - from);
-    m = top;
-    float sum = w;
+    for (int s = 0; s < NX; ++s) x[s] *= query_dim(s) < hd && col < heads ? scale : 0.0f;
+    if constexpr (HALF) {   // the column's largest value to 2^14 .. 2^15, so that f16 parts hold the others against it
+      float big = 0.0f;
 #pragma unroll
-    for (int c = 32; c; c /= 2) sum += __shfl_xor(sum, c);
-    l = l * keep + sum;
-    p_s[lane] = w;
-    at_s[lane] = at;
-    __syncthreads();
+      for (int s = 0; s < NX; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i] *= keep;
-      const int d = lane + kWave * i;
-      if (d < hd)
-        for (int j = 0; j < kWave && p0 + j < len; ++j) o[i] = fmaf(p_s[j], value_at<CT>((const char*)g.v + at_s[j] * S, d), o[i]);
+        for (int c = 0; c < 4; ++c) big = fmaxf(big, fabsf(x[s][c]));
+      big = head_max(big);
+      if (big > 0.0f && big < INFINITY) {
+        const int e = max((int)(__float_as_uint(big) >> 23) - 127, -100);
+        lift = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+        unlift = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+      }
     }
-    __syncthreads();
-  }
-  if (__any(bad)) l = NAN;
+    if constexpr (CT != F32)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + kWave * i;
-    if (d < hd) out[d] = l == 0.0f ? 0.0f : o[i] / l * vs;
+      for (int s = 0; s < NQ; ++s)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4 y = x[2 * s + c / 2];
+          uint32_t u[NP];
+          split_pair<HALF, NP>(y[2 * (c % 2)] * lift, y[2 * (c % 2) + 1] * lift, u);
+#pragma unroll
+          for (int n = 0; n < NP; ++n) qp[n][s][c] = u[n];
+        }
+    int step = 0;
+    for (; base_of(step + 1) < end; ++step) {
+      score();
+      at = place(step + 1, next);
+      load_k(at);
+      next = look(step + 2);
+      gather(base_of(step));
+      load_v(at);
+    }
+    score();
+    gather(base_of(step));
+  }
+  l = head_sum(l);
+  if (__any(bad)) l = NAN;
+
+  // ---- the waves' sums joined, 128 dimensions at a time
+  constexpr int PASS = HDP > 128 ? 2 : 1, VP = VE / PASS;
+  __shared__ float o_s[kWaves][16 * VP][17], m_s[kWaves][16], l_s[kWaves][16];
+  if (quad == 0) m_s[wave][col] = m, l_s[wave][col] = l;
+  __syncthreads();
+  float top = m_s[0][col];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_s[w][col]);
+  const float from = top == -INFINITY ? 0.0f : top;
+  const float by = exp2_hw(m - from);
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sum += l_s[w][col] * exp2_hw(m_s[w][col] - from);
+  __shared__ float div_s[16];
+  const size_t part = ((size_t)kv * parts + it.part) * columns + sub;
+  float* part_o = own ? L.own_o : L.prefix_o;
+  if (wave == 0 && quad == 0) {
+    div_s[col] = sum == 0.0f ? 0.0f : vs / sum;
+    if (!it.direct && col < heads) {
+      float* ml = (own ? L.own_ml : L.prefix_ml) + (part + col) * 2;
+      ml[0] = top;
+      ml[1] = sum;
+    }
+  }
+#pragma unroll
+  for (int ps = 0; ps < PASS; ++ps) {
+#pragma unroll
+    for (int c = 0; c < VP; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o_s[wave][(4 * quad + i) * VP + c][col] = o[ps * VP + c][i] * by;
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * 16 * VP; i += kThreads) {
+      const int h = i / (16 * VP), at = i % (16 * VP), c = ps * VP + at % VP;
+      const int d = c / EV * 16 * EV + at / VP * EV + c % EV;
+      if (d >= hd) continue;
+      float y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) y += o_s[w][at][h];
+      if (it.direct) {
+        const Column to = column_of(L, it, kv, sub + h);
+        a.out[(size_t)to.row * a.ldo + (size_t)to.head * hd + d] = y * div_s[h];
+      } else {
+        part_o[(part + h) * hd + d] = y;
+      }
+    }
+    if (ps + 1 < PASS) __syncthreads();
   }
 }
 
-hipError_t launch_shared(const AttnPages& g, int dtype, hipStream_t s) {
-  const dim3 grid((unsigned)g.a.T, (unsigned)g.a.n_q), block(kWave);
-  if (dtype == F32) hipLaunchKernelGGL(shared_attn_kernel<F32>, grid, block, 0, s, g);
-  else if (dtype == F16) hipLaunchKernelGGL(shared_attn_kernel<F16>, grid, block, 0, s, g);
-  else if (dtype == BF16) hipLaunchKernelGGL(shared_attn_kernel<BF16>, grid, block, 0, s, g);
-  else hipLaunchKernelGGL(shared_attn_kernel<E4M3>, grid, block, 0, s, g);
+// ---------------------------------------------------------------- the join
+
+// A block a (row, query head): its parts joined, four dimensions a thread, so that several parts are read side by side.
+__global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
+  const AttnPages& g = L.g;
+  const moe_paged_attn& a = g.a;
+  const int t = (int)blockIdx.x, head = (int)blockIdx.y, hd = g.map.head_dim, tid = threadIdx.x;
+  const RowPlan r = L.p.rows[t];
+  if (r.state == kLeave || r.state == kDone) return;
+  float* out = a.out + (size_t)t * a.ldo + (size_t)head * hd;
+  if (r.state != kJoin) {
+    for (int d = tid; d < hd; d += kThreads) out[d] = r.state == kZero ? 0.0f : NAN;
+    return;
+  }
+  const int G = L.cut.group, kv = (int)divide((uint32_t)head, L.by_group), h = head - kv * G;
+  const int c = (t - r.row0) * G + h, tile = c / L.cut.columns;
+  const int np = r.pieces, n = np + r.owns;
+  const long long at0 = (long long)kv * L.cut.prefix_items + r.part0 + (long long)tile * np;
+  const long long at1 = (long long)kv * L.cut.own_items + r.own0 + (long long)(h / 16) * r.owns;
+  // (a plan that is none leads to no place outside the work)
+  if (r.row0 < 0 || r.row0 > t || np < 0 || r.owns < 0 || r.part0 < 0 || r.own0 < 0 || (np && r.part0 + (long long)(tile + 1) * np > L.cut.prefix_items) ||
+      (r.owns && r.own0 + (long long)(h / 16 + 1) * r.owns > L.cut.own_items))
+    return;
+  auto place = [&](int i, const float** ml, const float** o) {
+    const long long at = i < np ? (at0 + i) * L.cut.columns + c % L.cut.columns : (at1 + i - np) * L.cut.own_columns + h % 16;
+    *ml = (i < np ? L.prefix_ml : L.own_ml) + at * 2;
+    *o = (i < np ? L.prefix_o : L.own_o) + at * hd;
+  };
+  const int width = hd / 4, rows = kThreads / width, row = tid / width, d = tid % width * 4, lane = tid % kWave;
+  float top = -INFINITY;
+  const float *ml, *o;
+  for (int i = lane; i < n; i += kWave) place(i, &ml, &o), top = fmaxf(top, ml[0]);
+#pragma unroll
+  for (int x = 32; x; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
+  if (top == -INFINITY) top = 0.0f;
+  float sum = 0.0f;
+  for (int i = lane; i < n; i += kWave) place(i, &ml, &o), sum += ml[1] * exp2_hw(ml[0] - top);
+#pragma unroll
+  for (int x = 32; x; x /= 2) sum += __shfl_xor(sum, x);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (row < rows)
+    for (int i = row; i < n; i += rows) {
+      place(i, &ml, &o);
+      acc += *(const f32x4*)(o + d) * exp2_hw(ml[0] - top);
+    }
+  __shared__ f32x4 acc_s[kThreads];
+  acc_s[tid] = acc;
+  __syncthreads();
+  if (row == 0) {
+    for (int i = 1; i < rows; ++i) acc += acc_s[i * width + tid];
+    const float vs = g.v_scale ? g.v_scale[kv] : 1.0f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) out[d + x] = sum == 0.0f ? 0.0f : acc[x] / sum * vs;
+  }
+}
+
+template <int CT, int HDP>
+hipError_t launch(const SharedLaunch& L, bool whole, int own, dim3 grid, hipStream_t s) {
+  if (whole) hipLaunchKernelGGL((shared_columns_kernel<CT, HDP, true>), grid, dim3(kThreads), 0, s, L, own);
+  else hipLaunchKernelGGL((shared_columns_kernel<CT, HDP, false>), grid, dim3(kThreads), 0, s, L, own);
+  return hipGetLastError();
+}
+
+template <int CT>
+hipError_t launch(const SharedLaunch& L, bool whole, int own, dim3 grid, hipStream_t s) {
+  const int hd = L.g.map.head_dim;
+  return hd <= 64 ? launch<CT, 64>(L, whole, own, grid, s) : hd <= 128 ? launch<CT, 128>(L, whole, own, grid, s) : launch<CT, 256>(L, whole, own, grid, s);
+}
+
+hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtype, hipStream_t s) {
+  SharedLaunch L;
+  L.g = g;
+  L.cut = share_cut(g.a.T, sh.n_groups, g.a.n_q, g.map.n_kv, g.map.head_dim);
+  plan_parts(L.cut, g.a.T, sh.n_groups, sh.plan, &L.p);
+  shared_work(L.cut, g.map.n_kv, g.map.head_dim, g.a.work, &L);
+  L.by_group = make_divider((uint32_t)L.cut.group);
+  const bool whole = g.map.page_size % 16 == 0 && g.map.slot_stride < (1 << 22);
+  for (int own = 0; own < 2; ++own) {
+    const dim3 grid((unsigned)(own ? L.cut.own_items : L.cut.prefix_items), (unsigned)g.map.n_kv, own ? 1 : (unsigned)(L.cut.columns / 16));
+    const hipError_t e = dtype == F32    ? launch<F32>(L, whole, own, grid, s)
+                         : dtype == F16  ? launch<F16>(L, whole, own, grid, s)
+                         : dtype == BF16 ? launch<BF16>(L, whole, own, grid, s)
+                                         : launch<E4M3>(L, whole, own, grid, s);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(shared_join_kernel, dim3((unsigned)g.a.T, (unsigned)g.a.n_q), dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
 
@@ -194,7 +797,8 @@ extern "C" {
 
 size_t moe_paged_share_plan_bytes(int T, int n_groups, int n_q, int n_kv, int head_dim) {
   if (T < 0 || T > kMostShared || n_groups < 0 || n_groups > kMostShared || n_q < 1 || n_kv < 1 || n_q % n_kv || head_dim < 1) return 0;
-  return 16 + 4 * (size_t)T;
+  PlanParts p;
+  return plan_parts(share_cut(T, n_groups, n_q, n_kv, head_dim), T, n_groups, nullptr, &p);
 }
 
 moe_status moe_paged_share_dev(const moe_paged_share* s) {
@@ -202,18 +806,22 @@ moe_status moe_paged_share_dev(const moe_paged_share* s) {
   if (st || (st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
-  const ShareArgs a{*s, make_divider((uint32_t)s->page_size), (int*)s->plan};
+  ShareArgs a;
+  a.s = *s;
+  a.per = make_divider((uint32_t)s->page_size);
+  a.cut = share_cut(s->T, s->n_groups, s->n_q, s->n_kv, s->head_dim);
+  plan_parts(a.cut, s->T, s->n_groups, s->plan, &a.p);
   if (s->T) {
     hipLaunchKernelGGL(share_rows_kernel, dim3((unsigned)(s->T + 3) / 4), dim3(256), 0, stream(), a);
     if ((st = check_hip(hipGetLastError(), "paged_share launch"))) return st;
   }
-  hipLaunchKernelGGL(share_groups_kernel, dim3(1), dim3(1024), 0, stream(), a);
+  hipLaunchKernelGGL(share_plan_kernel, dim3(1), dim3(kN), 0, stream(), a);
   return check_hip(hipGetLastError(), "paged_share launch");
 }
 
 size_t moe_paged_attn_shared_work_bytes(int T, int n_groups, int n_q, int n_kv, int head_dim) {
   if (T < 0 || T > kMostShared || n_groups < 0 || n_groups > kMostShared || n_q < 1 || n_kv < 1 || n_q % n_kv || head_dim < 1) return 0;
-  return 16;
+  return shared_work(share_cut(T, n_groups, n_q, n_kv, head_dim), n_kv, head_dim, nullptr, nullptr);
 }
 
 moe_status moe_paged_attn_shared_dev(const moe_paged_attn* a, const moe_pages* g, const moe_paged_share* s) {
@@ -231,7 +839,7 @@ moe_status moe_paged_attn_shared_dev(const moe_paged_attn* a, const moe_pages* g
   if ((st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
-  return check_hip(launch_shared(AttnPages{*a, map, g->k, g->v, g->k_scale, g->v_scale}, g->dtype, stream()), "paged_attn_shared launch");
+  return check_hip(launch_shared(AttnPages{*a, map, g->k, g->v, g->k_scale, g->v_scale}, *s, g->dtype, stream()), "paged_attn_shared launch");
 }
 
 }  // extern "C"
