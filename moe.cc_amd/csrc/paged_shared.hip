@@ -354,7 +354,6 @@ __device__ __forceinline__ bool item_ok(const SharedLaunch& L, const Item& x, in
          x.begin >= 0 && x.begin < x.end && x.end <= a.max_pages * L.g.map.page_size && (uint32_t)x.part < (uint32_t)parts;
 }
 
-template <int CT>
 __device__ __forceinline__ u32x2 widen16(uint32_t x) {   // four 8-bit values -> two dwords of f16 pairs (exact)
   return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true))};
@@ -385,8 +384,8 @@ __device__ __forceinline__ Column column_of(const SharedLaunch& L, const Item& x
 
 // ---------------------------------------------------------------- sixteen columns
 
-// A block an item, or sixteen columns of it (blockIdx.z); its waves take every fourth step of 32 positions and are joined
-// in LDS at the end.  K and V go straight into the registers that the matrix instructions read, 16 bytes a lane, keys and
+// A block takes sixteen columns of an item, those from `sub` on; its waves take every fourth step of 32 positions and are
+// joined in LDS at the end.  K and V go straight into the registers that the matrix instructions read, 16 bytes a lane, keys and
 // values requested a step ahead:
 //   scores   16 keys x 16 columns a tile: lane l holds 16-byte pieces of key l % 16 and the matching query values of column l % 16
 //   weights  come out as keys 4 (l / 16) + i of column l % 16 and go back in as the second operand from the same lane
@@ -394,8 +393,13 @@ __device__ __forceinline__ Column column_of(const SharedLaunch& L, const Item& x
 //            side by byte permutes
 // 16-bit operands: bf16 pages with queries and weights in three parts; f16 and 8-bit pages (exact in f16) in two f16 parts.
 // fp32 pages use the fp32 instruction.
-template <int CT, int HDP, bool WHOLE>
-__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_kernel(SharedLaunch L, int own) {
+template <int HDP>
+struct ColumnsShared {   // 128 dimensions at a time
+  float o[kWaves][HDP > 128 ? HDP / 2 : HDP][17], m[kWaves][16], l[kWaves][16], div[16];
+};
+
+template <int CT, int HDP>
+__device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item& it, int kv, int sub, bool own, ColumnsShared<HDP>& sh) {
   constexpr bool HALF = CT == F16 || CT == E4M3;
   constexpr int NP = HALF ? 2 : 3;                 // parts of an fp32 value
   constexpr int S = CT == F32 ? 4 : CT == E4M3 ? 1 : 2;
@@ -410,13 +414,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
 
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
-  const int limit = own ? L.p.head->own_items : L.p.head->prefix_items, parts = own ? L.cut.own_items : L.cut.prefix_items;
-  if ((int)blockIdx.x >= min(limit, parts)) return;
-  Item it = (own ? L.p.own : L.p.prefix)[blockIdx.x];
-  const int columns = own ? L.cut.own_columns : L.cut.columns;
-  if (!item_ok(L, it, parts, columns)) return;
+  const int parts = own ? L.cut.own_items : L.cut.prefix_items, columns = own ? L.cut.own_columns : L.cut.columns;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int hd = g.map.head_dim, kv = (int)blockIdx.y, sub = (int)blockIdx.z * 16;
+  const int hd = g.map.head_dim;
   const int heads = min(16, it.cols - sub);
   if (heads <= 0) return;
   const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
@@ -424,7 +424,6 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
   const long long head_at = (long long)kv * g.map.head_stride;
   const char* kbase = (const char*)g.k + head_at * S;
   const char* vbase = (const char*)g.v + head_at * S;
-  const uint32_t slot_bytes = (uint32_t)(g.map.slot_stride * S);   // WHOLE: below 2^24
   const int col = lane % 16, quad = lane / 16;
   const int first = it.begin, end = it.end;
 
@@ -447,54 +446,31 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
   const int* table = a.tables + (size_t)it.req * a.max_pages;
   bool bad = false;
   auto base_of = [&](int step) { return first + (step * kWaves + wave) * STEP; };
-  struct Look { int p[WHOLE ? KT : 1]; };
-  auto look = [&](int step) {
-    Look r;
-    const int base = base_of(step);
-    if constexpr (WHOLE) {
-#pragma unroll
-      for (int t = 0; t < KT; ++t) r.p[t] = scalar_load(table, divide((uint32_t)min(base + 16 * t, (end - 1) & ~15), g.map.per));
-    } else {
-      r.p[0] = table[divide((uint32_t)min(base + lane, end - 1), g.map.per)];
-    }
-    return r;
-  };
-  // WHOLE (a tile of 16 positions lies in one page): byte offsets of a step's tiles and the last position of each that
-  // counts; else of the lane's position.  Positions past the end take the last one's row
-  struct At { long long tile[WHOLE ? KT : 1]; int lim[WHOLE ? KT : 1]; };
-  auto place = [&](int step, const Look& r) {
-    At o;
-    const int base = base_of(step);
-#pragma unroll
-    for (int t = 0; t < (WHOLE ? KT : 1); ++t) {
-      const int p = WHOLE ? min(base + 16 * t, (end - 1) & ~15) : min(base + lane, end - 1);
-      int pg = r.p[t];
-      if (!page_ok(g.map, pg)) bad = true, pg = 0;
-      const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
-      o.tile[t] = ((long long)pg * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
-      o.lim[t] = WHOLE ? min(end - 1 - p, 15) : 15;
-    }
-    return o;
+  // of the lane's position of a step (positions past the end take the last one's row): its page, its byte offset
+  auto look = [&](int step) { return table[divide((uint32_t)min(base_of(step) + lane, end - 1), g.map.per)]; };
+  auto place = [&](int step, int page) {
+    const int p = min(base_of(step) + lane, end - 1);
+    if (!page_ok(g.map, page)) bad = true, page = 0;
+    const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
+    return ((long long)page * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
   };
   uint32_t kr[KT][NK][4], vr[4 * KT][NV][VW];
-  auto load_k = [&](const At& o) {
+  auto load_k = [&](long long at) {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const char* base = WHOLE ? kbase + o.tile[t] : kbase + __shfl(o.tile[0], 16 * t + col);
-      const uint32_t off = WHOLE ? __umul24((uint32_t)min(col, o.lim[t]), slot_bytes) : 0;
+      const char* base = kbase + __shfl(at, 16 * t + col);
 #pragma unroll
-      for (int j = 0; j < NK; ++j) load_piece<16, false>(base + (off + kpiece[j]), kr[t][j]);
+      for (int j = 0; j < NK; ++j) load_piece<16, false>(base + kpiece[j], kr[t][j]);
     }
   };
-  auto load_v = [&](const At& o) {
+  auto load_v = [&](long long at) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const char* base = WHOLE ? vbase + o.tile[t] : vbase + __shfl(o.tile[0], 16 * t + 4 * quad + i);
-        const uint32_t off = WHOLE ? __umul24((uint32_t)min(4 * quad + i, o.lim[t]), slot_bytes) : 0;
+        const char* base = vbase + __shfl(at, 16 * t + 4 * quad + i);
 #pragma unroll
-        for (int h = 0; h < NV; ++h) load_piece<EV * S, false>(base + (off + vpiece[h]), vr[4 * t + i][h]);
+        for (int h = 0; h < NV; ++h) load_piece<EV * S, false>(base + vpiece[h], vr[4 * t + i][h]);
       }
   };
 
@@ -519,7 +495,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
         } else if constexpr (CT == E4M3) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const u32x2 y = widen16<CT>(kr[t][j][2 * u]), z = widen16<CT>(kr[t][j][2 * u + 1]);
+            const u32x2 y = widen16(kr[t][j][2 * u]), z = widen16(kr[t][j][2 * u + 1]);
             const u32x4 k = {y[0], y[1], z[0], z[1]};
 #pragma unroll
             for (int n = 0; n < NP; ++n) s[t] = mfma32<HALF>(k, qp[n][2 * j + u], s[t]);
@@ -583,7 +559,7 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
 #pragma unroll
           for (int d = 0; d < VW; ++d) {
             if constexpr (CT == E4M3) {
-              const u32x2 y = widen16<CT>(vr[k][h][d]);
+              const u32x2 y = widen16(vr[k][h][d]);
               w16[k][2 * d] = y[0], w16[k][2 * d + 1] = y[1];
             } else {
               w16[k][d] = vr[k][h][d];
@@ -603,10 +579,10 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
   };
 
   if (base_of(0) < end) {
-    At at = place(0, look(0));
+    long long at = place(0, look(0));
     load_k(at);
     load_v(at);
-    Look next = look(1);
+    int next = look(1);
     // ---- queries times scale and log2(e): scores are powers of two
     float lift = 1.0f;
 #pragma unroll
@@ -652,7 +628,9 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
 
   // ---- the waves' sums joined, 128 dimensions at a time
   constexpr int PASS = HDP > 128 ? 2 : 1, VP = VE / PASS;
-  __shared__ float o_s[kWaves][16 * VP][17], m_s[kWaves][16], l_s[kWaves][16];
+  auto& o_s = sh.o;
+  auto& m_s = sh.m;
+  auto& l_s = sh.l;
   if (quad == 0) m_s[wave][col] = m, l_s[wave][col] = l;
   __syncthreads();
   float top = m_s[0][col];
@@ -663,14 +641,14 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
   float sum = 0.0f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) sum += l_s[w][col] * exp2_hw(m_s[w][col] - from);
-  __shared__ float div_s[16];
+  auto& div_s = sh.div;
   const size_t part = ((size_t)kv * parts + it.part) * columns + sub;
   float* part_o = own ? L.own_o : L.prefix_o;
   if (wave == 0 && quad == 0) {
     div_s[col] = sum == 0.0f ? 0.0f : vs / sum;
     if (!it.direct && col < heads) {
       float* ml = (own ? L.own_ml : L.prefix_ml) + (part + col) * 2;
-      ml[0] = top;
+      ml[0] = top - kLift;   // what the weights are powers from
       ml[1] = sum;
     }
   }
@@ -697,6 +675,307 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_columns_k
     }
     if (ps + 1 < PASS) __syncthreads();
   }
+}
+
+// ---------------------------------------------------------------- many columns
+
+// A block takes an item of up to 64 or 128 columns: WC waves lie beside each other over the columns, 32 each (16 where
+// head_dim is past 128), the others over the positions, 32 each of a step.  K and V of a step's positions go straight
+// from memory into LDS, a step ahead, where the waves over the columns share them; rows are swizzled so that the reads of
+// both operands are free of bank conflicts.  One barrier a step.  Layouts and operands as in columns_block; e4m3 pages
+// lie in LDS as they are.  The largest score of a column is raised only when a new one is more than 2^kSlack above it.
+template <int CT, int HDP, int WC>
+struct TileShape {
+  static constexpr int S = CT == E4M3 ? 1 : 2, WP = kWaves / WC, CPW = HDP > 128 ? 1 : 2;
+  static constexpr int ROWS = 32 * WP;                    // positions of a step
+  static constexpr int RB = HDP * S, PIECES = RB / 16;    // bytes of a row, 16-byte pieces
+  static constexpr int STAGE = 2 * ROWS * RB;             // K and V
+  static constexpr int JOIN = (WP - 1) * WC * CPW * kWave * (HDP + 8);
+  static constexpr int BYTES = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
+};
+
+template <int CT, int HDP, int WC>
+__device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it, int kv, uint8_t* lds) {
+  using T = TileShape<CT, HDP, WC>;
+  constexpr bool HALF = CT != BF16;
+  constexpr int NP = HALF ? 2 : 3, S = T::S, CPW = T::CPW, PIECES = T::PIECES, RB = T::RB;
+  constexpr int E = 16 / S, NK = HDP / E / 4, VE = HDP / 16, EV = VE < E ? VE : E, NV = VE / EV, VW = EV * S / 4, NQ = HDP / 32;
+  constexpr int LOADS = T::ROWS * PIECES / kWave, NL = (LOADS + kWaves - 1) / kWaves;   // of K; a wave's
+  constexpr int PER = PIECES < 16 ? 16 / PIECES : 1, MASK = (PIECES < 16 ? PIECES : 16) - 1;
+  constexpr float kSlack = 4.0f, kLift = HALF ? 10.0f : 0.0f;   // weights reach 2^(kSlack + kLift)
+  const AttnPages& g = L.g;
+  const moe_paged_attn& a = g.a;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wc = wave % WC, wp = wave / WC, hd = g.map.head_dim, col = lane % 16, quad = lane / 16, end = it.end;
+  const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
+  const long long head_at = (long long)kv * g.map.head_stride;
+  const char* kbase = (const char*)g.k + head_at * S;
+  const char* vbase = (const char*)g.v + head_at * S;
+  const int* table = a.tables + (size_t)it.req * a.max_pages;
+  bool bad = false;
+
+  // ---- a step's rows into LDS: a load is 64 pieces, PIECES a row, the piece p of row r at p ^ swizzle(r)
+  auto swizzle = [](int row) { return row / PER & MASK; };
+  auto row_of = [&](int n) { return (wave + n * kWaves) * (kWave / PIECES) + lane / PIECES; };
+  struct Look { int p[NL]; };
+  auto look = [&](int step) {
+    Look k;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) k.p[n] = table[divide((uint32_t)min(it.begin + step * T::ROWS + row_of(n), end - 1), g.map.per)];
+    return k;
+  };
+  auto load = [&](int step, const Look& k) {
+    uint8_t* to = lds + (step & 1) * T::STAGE;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      if (LOADS % kWaves && wave + n * kWaves >= LOADS) break;
+      const int row = row_of(n), p = min(it.begin + step * T::ROWS + row, end - 1);
+      int page = k.p[n];
+      if (!page_ok(g.map, page)) bad = true, page = 0;
+      const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
+      const int piece = min(((lane % PIECES) ^ swizzle(row)) * 16, hd * S - 16);
+      const long long at = ((long long)page * g.map.page_stride + (long long)off * g.map.slot_stride) * S + piece;
+      lds_load16(kbase + at, to + (wave + n * kWaves) * 1024);
+      lds_load16(vbase + at, to + T::ROWS * RB + (wave + n * kWaves) * 1024);
+    }
+  };
+  const int steps = (end - it.begin + T::ROWS - 1) / T::ROWS;
+  Look next = look(0);
+  load(0, next);
+  next = look(1);
+
+  // ---- queries times scale and log2(e), in parts
+  u32x4 qp[CPW][NP][NQ];
+  float unlift[CPW];
+#pragma unroll
+  for (int ct = 0; ct < CPW; ++ct) {
+    const int c = (wc * CPW + ct) * 16 + col;
+    const Column mine = column_of(L, it, kv, min(c, it.cols - 1));
+    const float* q = a.q + (size_t)mine.row * a.ldq + (size_t)mine.head * hd;
+    f32x4 x[2 * NQ];
+#pragma unroll
+    for (int s = 0; s < 2 * NQ; ++s) {
+      const int d = CT == E4M3 ? (4 * (s / 4) + quad) * 16 + 4 * (s % 4) : (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
+      x[s] = *(const f32x4u*)(q + min(d, hd - 4));
+      x[s] *= d < hd && c < it.cols ? scale : 0.0f;
+    }
+    float lift = 1.0f;
+    unlift[ct] = 1.0f;
+    if constexpr (HALF) {
+      float big = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 2 * NQ; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(x[s][i]));
+      big = head_max(big);
+      if (big > 0.0f && big < INFINITY) {
+        const int e = max((int)(__float_as_uint(big) >> 23) - 127, -100);
+        lift = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+        unlift[ct] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < NQ; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 y = x[2 * s + i / 2];
+        uint32_t u[NP];
+        split_pair<HALF, NP>(y[2 * (i % 2)] * lift, y[2 * (i % 2) + 1] * lift, u);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) qp[ct][n][s][i] = u[n];
+      }
+  }
+
+  f32x4 o[CPW][VE];
+  float m[CPW], l[CPW];
+#pragma unroll
+  for (int ct = 0; ct < CPW; ++ct) {
+    m[ct] = -INFINITY, l[ct] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < VE; ++c) o[ct][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  for (int step = 0; step < steps; ++step) {
+    stage_sync<0>();
+    if (step + 1 < steps) {
+      load(step + 1, next);
+      next = look(step + 2);
+    }
+    const int base = it.begin + step * T::ROWS + wp * 32;
+    if (base >= end) continue;
+    const uint8_t* ks = lds + (step & 1) * T::STAGE + wp * 32 * RB;
+    const uint8_t* vs = ks + T::ROWS * RB;
+    // ---- scores
+    f32x4 s[CPW][2];
+#pragma unroll
+    for (int ct = 0; ct < CPW; ++ct) s[ct][0] = s[ct][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int row = 16 * t + col;
+        const u32x4 kr = *(const u32x4*)(ks + row * RB + ((4 * j + quad) ^ swizzle(row)) * 16);
+        if constexpr (CT == E4M3) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x2 y = widen16(kr[2 * u]), z = widen16(kr[2 * u + 1]);
+            const u32x4 k = {y[0], y[1], z[0], z[1]};
+#pragma unroll
+            for (int n = 0; n < NP; ++n)
+#pragma unroll
+              for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(k, qp[ct][n][2 * j + u], s[ct][t]);
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < NP; ++n)
+#pragma unroll
+            for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(kr, qp[ct][n][j], s[ct][t]);
+        }
+      }
+    // ---- weights
+    u32x4 pp[CPW][NP];
+#pragma unroll
+    for (int ct = 0; ct < CPW; ++ct) {
+      if (base + 32 > end) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (base + 16 * t + 4 * quad + i >= end) s[ct][t][i] = -INFINITY;
+      }
+      float top = s[ct][0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[ct][i / 4][i % 4]);
+      top = head_max(top) * unlift[ct];
+      if (__any(top > m[ct] + kSlack)) {
+        const float now = fmaxf(m[ct], top), keep = now == -INFINITY ? 1.0f : exp2_hw(m[ct] - now);
+        l[ct] *= keep;
+#pragma unroll
+        for (int c = 0; c < VE; ++c) o[ct][c] *= keep;
+        m[ct] = now;
+      }
+      const float from = (m[ct] == -INFINITY ? 0.0f : m[ct]) - kLift;
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = exp2_hw(HALF ? fmaf(s[ct][i / 4][i % 4], unlift[ct], -from) : s[ct][i / 4][i % 4] - from);
+        l[ct] += p[i];
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t u[NP];
+        split_pair<HALF, NP>(p[2 * c], p[2 * c + 1], u);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) pp[ct][n][c] = u[n];
+      }
+    }
+    // ---- values
+#pragma unroll
+    for (int h = 0; h < NV; ++h) {
+      uint32_t w16[8][EV / 2];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int row = 16 * (k / 4) + 4 * quad + k % 4, at = (16 * h + col) * EV * S;
+        uint32_t raw[VW];
+        const uint8_t* from = vs + row * RB + ((at / 16) ^ swizzle(row)) * 16 + at % 16;
+        load_piece<EV * S, false>((const char*)from, raw);
+#pragma unroll
+        for (int d = 0; d < VW; ++d) {
+          if constexpr (CT == E4M3) {
+            const u32x2 y = widen16(raw[d]);
+            w16[k][2 * d] = y[0], w16[k][2 * d + 1] = y[1];
+          } else {
+            w16[k][d] = raw[d];
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        u32x4 y;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          y[c] = __builtin_amdgcn_perm(w16[2 * c + 1][e / 2], w16[2 * c][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+#pragma unroll
+          for (int ct = 0; ct < CPW; ++ct) o[ct][h * EV + e] = mfma32<HALF>(y, pp[ct][n], o[ct][h * EV + e]);
+      }
+    }
+  }
+  bad = __syncthreads_or(bad);   // (every wave is done with the rows in LDS)
+#pragma unroll
+  for (int ct = 0; ct < CPW; ++ct) {
+    l[ct] = head_sum(l[ct]);
+    if (bad) l[ct] = NAN;
+  }
+  // ---- waves over the positions joined
+  if constexpr (T::WP > 1) {
+    f32x4* o_s = (f32x4*)lds;
+    float2* ml_s = (float2*)(lds + (T::WP - 1) * WC * CPW * kWave * HDP);
+    const int at = ((wp - 1) * WC + wc) * CPW;
+    if (wp) {
+#pragma unroll
+      for (int ct = 0; ct < CPW; ++ct) {
+        ml_s[(at + ct) * kWave + lane] = float2{m[ct], l[ct]};
+#pragma unroll
+        for (int c = 0; c < VE; ++c) o_s[((at + ct) * VE + c) * kWave + lane] = o[ct][c];
+      }
+    }
+    __syncthreads();
+    if (wp) return;
+    for (int w = 0; w < T::WP - 1; ++w)
+#pragma unroll
+      for (int ct = 0; ct < CPW; ++ct) {
+        const int from = (w * WC + wc) * CPW + ct;
+        const float2 ml = ml_s[from * kWave + lane];
+        const float top = fmaxf(m[ct], ml.x), least = top == -INFINITY ? 0.0f : top;
+        const float x = exp2_hw(m[ct] - least), y = exp2_hw(ml.x - least);
+        m[ct] = top;
+        l[ct] = l[ct] * x + ml.y * y;
+#pragma unroll
+        for (int c = 0; c < VE; ++c) o[ct][c] = o[ct][c] * x + o_s[(from * VE + c) * kWave + lane] * y;
+      }
+  }
+#pragma unroll
+  for (int ct = 0; ct < CPW; ++ct) {
+    const int c = (wc * CPW + ct) * 16 + col;
+    if (c >= it.cols) continue;
+    const size_t part = ((size_t)kv * L.cut.prefix_items + it.part) * L.cut.columns + c;
+    if (quad == 0) L.prefix_ml[part * 2] = m[ct] - kLift, L.prefix_ml[part * 2 + 1] = l[ct];
+#pragma unroll
+    for (int h = 0; h < NV; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = (16 * h + 4 * quad + i) * EV;
+        if (d >= hd) continue;
+#pragma unroll
+        for (int e = 0; e < EV; e += 4)
+          *(f32x4*)(L.prefix_o + part * hd + d + e) = f32x4{o[ct][h * EV + e][i], o[ct][h * EV + e + 1][i], o[ct][h * EV + e + 2][i], o[ct][h * EV + e + 3][i]};
+      }
+  }
+}
+
+// WC: waves over a prefix item's columns; 0: the item in sixteens.  Prefix items first, then the rows' own, which lie
+// beside the last of them.
+template <int CT, int HDP, int WC>
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
+  using Tile = TileShape<CT == F32 ? BF16 : CT, HDP, WC ? WC : 4>;
+  constexpr int BYTES = WC && Tile::BYTES > (int)sizeof(ColumnsShared<HDP>) ? Tile::BYTES : (int)sizeof(ColumnsShared<HDP>);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
+  const int subs = WC ? 1 : L.cut.columns / 16, kv = (int)blockIdx.y;
+  int b = (int)blockIdx.x;
+  const bool own = b >= L.cut.prefix_items * subs;
+  b = own ? b - L.cut.prefix_items * subs : b / subs;
+  const int parts = own ? L.cut.own_items : L.cut.prefix_items;
+  if (b >= min(own ? L.p.head->own_items : L.p.head->prefix_items, parts)) return;
+  const Item it = (own ? L.p.own : L.p.prefix)[b];
+  if (!item_ok(L, it, parts, own ? L.cut.own_columns : L.cut.columns)) return;
+  if constexpr (WC != 0) {
+    if (!own) {
+      tile_block<CT, HDP, WC>(L, it, kv, lds);
+      return;
+    }
+  }
+  columns_block<CT, HDP>(L, it, kv, own ? 0 : (int)blockIdx.x % subs * 16, own, *(ColumnsShared<HDP>*)lds);
 }
 
 // ---------------------------------------------------------------- the join
@@ -756,16 +1035,21 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
 }
 
 template <int CT, int HDP>
-hipError_t launch(const SharedLaunch& L, bool whole, int own, dim3 grid, hipStream_t s) {
-  if (whole) hipLaunchKernelGGL((shared_columns_kernel<CT, HDP, true>), grid, dim3(kThreads), 0, s, L, own);
-  else hipLaunchKernelGGL((shared_columns_kernel<CT, HDP, false>), grid, dim3(kThreads), 0, s, L, own);
+hipError_t launch(const SharedLaunch& L, hipStream_t s) {
+  const int waves = CT == F32 || L.cut.columns < 64 / (HDP > 128 ? 2 : 1) ? 0 : L.cut.columns / (HDP > 128 ? 16 : 32);
+  const dim3 grid((unsigned)(L.cut.prefix_items * (waves ? 1 : L.cut.columns / 16) + L.cut.own_items), (unsigned)L.g.map.n_kv);
+  if constexpr (CT != F32) {
+    if (waves == 4) hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, 4>), grid, dim3(kThreads), 0, s, L);
+    if (waves == 2) hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, 2>), grid, dim3(kThreads), 0, s, L);
+  }
+  if (waves == 0) hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, 0>), grid, dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
 
 template <int CT>
-hipError_t launch(const SharedLaunch& L, bool whole, int own, dim3 grid, hipStream_t s) {
+hipError_t launch(const SharedLaunch& L, hipStream_t s) {
   const int hd = L.g.map.head_dim;
-  return hd <= 64 ? launch<CT, 64>(L, whole, own, grid, s) : hd <= 128 ? launch<CT, 128>(L, whole, own, grid, s) : launch<CT, 256>(L, whole, own, grid, s);
+  return hd <= 64 ? launch<CT, 64>(L, s) : hd <= 128 ? launch<CT, 128>(L, s) : launch<CT, 256>(L, s);
 }
 
 hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtype, hipStream_t s) {
@@ -775,15 +1059,11 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
   plan_parts(L.cut, g.a.T, sh.n_groups, sh.plan, &L.p);
   shared_work(L.cut, g.map.n_kv, g.map.head_dim, g.a.work, &L);
   L.by_group = make_divider((uint32_t)L.cut.group);
-  const bool whole = g.map.page_size % 16 == 0 && g.map.slot_stride < (1 << 22);
-  for (int own = 0; own < 2; ++own) {
-    const dim3 grid((unsigned)(own ? L.cut.own_items : L.cut.prefix_items), (unsigned)g.map.n_kv, own ? 1 : (unsigned)(L.cut.columns / 16));
-    const hipError_t e = dtype == F32    ? launch<F32>(L, whole, own, grid, s)
-                         : dtype == F16  ? launch<F16>(L, whole, own, grid, s)
-                         : dtype == BF16 ? launch<BF16>(L, whole, own, grid, s)
-                                         : launch<E4M3>(L, whole, own, grid, s);
-    if (e != hipSuccess) return e;
-  }
+  const hipError_t e = dtype == F32    ? launch<F32>(L, s)
+                       : dtype == F16  ? launch<F16>(L, s)
+                       : dtype == BF16 ? launch<BF16>(L, s)
+                                       : launch<E4M3>(L, s);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL(shared_join_kernel, dim3((unsigned)g.a.T, (unsigned)g.a.n_q), dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
