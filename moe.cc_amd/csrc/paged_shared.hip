@@ -59,7 +59,7 @@ struct ShareCut {
   int columns;        // of a prefix item
   int own_columns;    // of a row's own
   int own_tiles;      // of a row
-  int slots;          // items that are resident at once, about
+  int slots, own_slots;   // items that are resident at once, about
   int prefix_items, own_items;   // at most
 };
 
@@ -71,10 +71,11 @@ ShareCut share_cut(int T, int n_groups, int n_q, int n_kv, int head_dim) {
   while (c.columns < mean && c.columns < (head_dim > 128 ? 64 : 128)) c.columns *= 2;
   c.own_columns = c.group < 16 ? c.group : 16;
   c.own_tiles = (c.group + 15) / 16;
-  const int resident = kCUs * (head_dim <= 128 ? 2 : 1);
+  const int resident = kCUs * (head_dim <= 128 && c.columns < 64 ? 2 : 1);
   c.slots = resident > n_kv ? resident / n_kv : 1;
   c.prefix_items = c.slots + (int)((long long)T * c.group / c.columns) + n_groups;
-  c.own_items = c.slots + T * c.own_tiles;
+  c.own_slots = 2 * kCUs > n_kv ? 2 * kCUs / n_kv : 1;
+  c.own_items = c.own_slots + T * c.own_tiles;
   return c;
 }
 
@@ -225,11 +226,11 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
   }
   __threadfence_block();
   __syncthreads();
-  auto piece = [&](unsigned long long all) {
-    const unsigned long long n = (all + cut.slots - 1) / cut.slots;
+  auto piece = [&](unsigned long long all, int slots) {
+    const unsigned long long n = (all + slots - 1) / slots;
     return n ? (int)(n < 0x40000000 ? n : 0x40000000) : 1;
   };
-  const int per = piece(units_s);
+  const int per = piece(units_s, cut.slots);
   int done = 0;
   for (int g0 = 0; g0 < s.n_groups; g0 += kN) {
     const int g = g0 + tid;
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
   }
   if (mine) atomicAdd(&own_s, mine);
   __syncthreads();
-  const int per_own = piece(own_s);
+  const int per_own = piece(own_s, cut.own_slots);
   done = 0;
   for (int r0 = 0; r0 < s.T; r0 += kN) {
     const int r = r0 + tid;
@@ -327,7 +328,8 @@ struct SharedLaunch {
   AttnPages g;
   ShareCut cut;
   PlanParts p;
-  Divider by_group;
+  Divider by_group, by_kv;
+  int prefix_blocks;   // of a launch; the rest are rows' own
   // work: [n_kv][items][columns] maxima and sums, [n_kv][items][columns][head_dim] values
   float* prefix_ml;
   float* prefix_o;
@@ -359,13 +361,15 @@ __device__ __forceinline__ u32x2 widen16(uint32_t x) {   // four 8-bit values ->
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true))};
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 // Two fp32 values into the same place of NP operands: three bf16 parts, whose sum they are, or two f16 parts, each rounded
 // to nearest even, whose sum is off by at most 2^-23 of the value (twice an fp32 rounding, at the worst bits) and by 2^-25.
 template <bool HALF, int NP>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&p)[NP]) {
   if constexpr (HALF) {
-    const f16x2 h = {(_Float16)x, (_Float16)y};
-    const f16x2 l = {(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])};
+    const f16x2 h = __builtin_convertvector(f32x2{x, y}, f16x2);
+    const f16x2 l = __builtin_convertvector(f32x2{x - (float)h[0], y - (float)h[1]}, f16x2);
     p[0] = __builtin_bit_cast(uint32_t, h);
     p[1] = __builtin_bit_cast(uint32_t, l);
   } else {
@@ -407,7 +411,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
   constexpr int NK = HDP / E / 4;                  // a lane's pieces of a key
   constexpr int VE = HDP / 16;                     // a lane's dimensions of a value
   constexpr int EV = VE < E ? VE : E, NV = VE / EV, VW = EV * S / 4;   // its pieces: elements, number, dwords
-  constexpr int KT = CT == F32 && HDP == 256 ? 1 : 2;                  // tiles of 16 positions a step
+  constexpr int KT = CT == F32 && HDP == 256 ? 1 : 2;   // tiles of 16 positions a step
   constexpr int NQ = CT == F32 ? 1 : HDP / 32;     // query operands of 8 values
   constexpr int STEP = 16 * KT;
   constexpr float kLift = HALF ? 14.0f : 0.0f;     // weights are held times 2^14 where their parts are f16
@@ -415,17 +419,16 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
   const int parts = own ? L.cut.own_items : L.cut.prefix_items, columns = own ? L.cut.own_columns : L.cut.columns;
-  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int tid = threadIdx.x % kThreads, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int hd = g.map.head_dim;
-  const int heads = min(16, it.cols - sub);
-  if (heads <= 0) return;
+  const int heads = min(16, it.cols - sub);   // (none: a half block without an item)
   const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
   const float vs = g.v_scale ? scalar_load(g.v_scale, kv) : 1.0f;
   const long long head_at = (long long)kv * g.map.head_stride;
   const char* kbase = (const char*)g.k + head_at * S;
   const char* vbase = (const char*)g.v + head_at * S;
   const int col = lane % 16, quad = lane / 16;
-  const int first = it.begin, end = it.end;
+  const int first = it.begin, end = heads > 0 ? it.end : it.begin;
 
   uint32_t kpiece[NK], vpiece[NV];
 #pragma unroll
@@ -433,7 +436,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 #pragma unroll
   for (int h = 0; h < NV; ++h) vpiece[h] = (uint32_t)min((16 * h + col) * EV * S, hd * S - EV * S);
 
-  const Column mine = column_of(L, it, kv, sub + min(col, heads - 1));
+  const Column mine = column_of(L, it, kv, sub + max(min(col, heads - 1), 0));
   const float* q = a.q + (size_t)mine.row * a.ldq + (size_t)mine.head * hd;
   constexpr int NX = CT == F32 ? NK : 2 * NQ;
   f32x4 x[NX];
@@ -659,7 +662,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 #pragma unroll
       for (int i = 0; i < 4; ++i) o_s[wave][(4 * quad + i) * VP + c][col] = o[ps * VP + c][i] * by;
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * 16 * VP; i += kThreads) {
+    for (int i = tid; i < heads * 16 * VP; i += kThreads) {
       const int h = i / (16 * VP), at = i % (16 * VP), c = ps * VP + at % VP;
       const int d = c / EV * 16 * EV + at / VP * EV + c % EV;
       if (d >= hd) continue;
@@ -679,17 +682,24 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 
 // ---------------------------------------------------------------- many columns
 
-// A block takes an item of up to 64 or 128 columns: WC waves lie beside each other over the columns, 32 each (16 where
-// head_dim is past 128), the others over the positions, 32 each of a step.  K and V of a step's positions go straight
-// from memory into LDS, a step ahead, where the waves over the columns share them; rows are swizzled so that the reads of
-// both operands are free of bank conflicts.  One barrier a step.  Layouts and operands as in columns_block; e4m3 pages
-// lie in LDS as they are.  The largest score of a column is raised only when a new one is more than 2^kSlack above it.
+// A block of eight waves takes an item of up to 64 or 128 columns: WC waves lie beside each other over the columns, 32 each
+// (16 where head_dim is past 128), the others over the positions, 32 each of a step.  K and V of a step go through LDS, a
+// step ahead, where the waves over the columns share them, in the layouts that the matrix instructions take:
+//   keys     rows of 16-bit values, 16-byte pieces; piece p of row r at p ^ swizzle(r), so that the 16 rows of a read lie in
+//            all banks; 16-bit pages go straight from memory into LDS
+//   values   cells of a dimension's 8 keys 4 q + i and 16 + 4 q + i (q: the quad of lanes that reads it), in registers put
+//            together from 8 rows' pairs of dimensions: an operand is one 16-byte read
+// 8-bit pages become f16 on the way.  A wave stages the 8 rows of one (32 positions, q): their addresses lie in its lanes,
+// found once for K and V.  One barrier a step.  A column's largest score is raised only when one is more than 2^kSlack above
+// it, so that most steps need no sums across lanes.
+constexpr int kTileThreads = 512, kTileWaves = kTileThreads / kWave;
+
 template <int CT, int HDP, int WC>
 struct TileShape {
-  static constexpr int S = CT == E4M3 ? 1 : 2, WP = kWaves / WC, CPW = HDP > 128 ? 1 : 2;
-  static constexpr int ROWS = 32 * WP;                    // positions of a step
-  static constexpr int RB = HDP * S, PIECES = RB / 16;    // bytes of a row, 16-byte pieces
-  static constexpr int STAGE = 2 * ROWS * RB;             // K and V
+  static constexpr int S = CT == E4M3 ? 1 : 2, WP = kTileWaves / WC, CPW = HDP > 128 ? 1 : 2;
+  static constexpr int ROWS = 32 * WP;             // positions of a step
+  static constexpr int RB = HDP * 2;               // bytes of a row in LDS
+  static constexpr int STAGE = 2 * ROWS * RB;      // K and V
   static constexpr int JOIN = (WP - 1) * WC * CPW * kWave * (HDP + 8);
   static constexpr int BYTES = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
 };
@@ -698,45 +708,111 @@ template <int CT, int HDP, int WC>
 __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it, int kv, uint8_t* lds) {
   using T = TileShape<CT, HDP, WC>;
   constexpr bool HALF = CT != BF16;
-  constexpr int NP = HALF ? 2 : 3, S = T::S, CPW = T::CPW, PIECES = T::PIECES, RB = T::RB;
-  constexpr int E = 16 / S, NK = HDP / E / 4, VE = HDP / 16, EV = VE < E ? VE : E, NV = VE / EV, VW = EV * S / 4, NQ = HDP / 32;
-  constexpr int LOADS = T::ROWS * PIECES / kWave, NL = (LOADS + kWaves - 1) / kWaves;   // of K; a wave's
-  constexpr int PER = PIECES < 16 ? 16 / PIECES : 1, MASK = (PIECES < 16 ? PIECES : 16) - 1;
-  constexpr float kSlack = 4.0f, kLift = HALF ? 10.0f : 0.0f;   // weights reach 2^(kSlack + kLift)
+  constexpr int NP = HALF ? 2 : 3, S = T::S, CPW = T::CPW, RB = T::RB;
+  constexpr int NK = HDP / 32, VE = HDP / 16;
+  constexpr int SETS = T::WP / 2;                              // (32 positions, q) that a wave stages
+  constexpr int KL = (8 * HDP * S + 1023) / 1024;              // 16-byte loads of a lane for their K
+  constexpr int KP = HDP * S / 16;                             // such pieces of a row
+  constexpr int VL = (HDP / 2 + kWave - 1) / kWave;            // pairs of dimensions of a lane
+  constexpr float kSlack = 4.0f, kLift = HALF ? 10.0f : 0.0f;  // weights reach 2^(kSlack + kLift)
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wc = wave % WC, wp = wave / WC, hd = g.map.head_dim, col = lane % 16, quad = lane / 16, end = it.end;
   const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
-  const long long head_at = (long long)kv * g.map.head_stride;
-  const char* kbase = (const char*)g.k + head_at * S;
-  const char* vbase = (const char*)g.v + head_at * S;
+  const long long head_at = (long long)kv * g.map.head_stride * S;
+  const char* kbase = (const char*)g.k + head_at;
+  const char* vbase = (const char*)g.v + head_at;
   const int* table = a.tables + (size_t)it.req * a.max_pages;
   bool bad = false;
 
-  // ---- a step's rows into LDS: a load is 64 pieces, PIECES a row, the piece p of row r at p ^ swizzle(r)
-  auto swizzle = [](int row) { return row / PER & MASK; };
-  auto row_of = [&](int n) { return (wave + n * kWaves) * (kWave / PIECES) + lane / PIECES; };
-  struct Look { int p[NL]; };
-  auto look = [&](int step) {
-    Look k;
-#pragma unroll
-    for (int n = 0; n < NL; ++n) k.p[n] = table[divide((uint32_t)min(it.begin + step * T::ROWS + row_of(n), end - 1), g.map.per)];
-    return k;
+  // ---- staging: set n of a wave is quad set % 4 of positions 32 (set / 4) .. of the step, set = wave + 8 n; row k (lane % 8)
+  // of it position 16 (k / 4) + 4 q + k % 4, which is row 8 q + k of its 32 in LDS
+  auto swizzle = [](int row) {
+    return HDP == 64 ? (row >> 1 & 1) | (row >> 3 & 3) << 1 : (row & 3) | (row >> 3 & 3) << 2;
   };
-  auto load = [&](int step, const Look& k) {
-    uint8_t* to = lds + (step & 1) * T::STAGE;
+  auto position = [&](int step, int n) {
+    const int set = wave + n * kTileWaves, k = lane % 8;
+    return min(it.begin + step * T::ROWS + set / 4 * 32 + 16 * (k / 4) + 4 * (set % 4) + k % 4, end - 1);
+  };
+  struct Look { int p[SETS]; };
+  auto look = [&](int step) {
+    Look x;
 #pragma unroll
-    for (int n = 0; n < NL; ++n) {
-      if (LOADS % kWaves && wave + n * kWaves >= LOADS) break;
-      const int row = row_of(n), p = min(it.begin + step * T::ROWS + row, end - 1);
-      int page = k.p[n];
+    for (int n = 0; n < SETS; ++n) x.p[n] = table[divide((uint32_t)position(step, n), g.map.per)];
+    return x;
+  };
+  uint32_t vraw[SETS][VL][8];
+  u32x4 kraw[CT == E4M3 ? SETS : 1][KL];
+  auto load = [&](int step, const Look& x) {
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+      const int set = wave + n * kTileWaves, p = position(step, n);
+      int page = x.p[n];
       if (!page_ok(g.map, page)) bad = true, page = 0;
       const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
-      const int piece = min(((lane % PIECES) ^ swizzle(row)) * 16, hd * S - 16);
-      const long long at = ((long long)page * g.map.page_stride + (long long)off * g.map.slot_stride) * S + piece;
-      lds_load16(kbase + at, to + (wave + n * kWaves) * 1024);
-      lds_load16(vbase + at, to + T::ROWS * RB + (wave + n * kWaves) * 1024);
+      const long long at = ((long long)page * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
+      uint8_t* to = lds + (step & 1) * T::STAGE + (set * 8) * RB;
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const int k = (lane + i * kWave) / KP;
+        if (KP * 8 < kWave && lane >= KP * 8) break;
+        const long long row = __shfl(at, k);
+        if constexpr (CT == E4M3) {
+          kraw[n][i] = *(const u32x4*)(kbase + row + min((lane + i * kWave) % KP * 16, hd - 16));
+        } else {
+          const int piece = (lane + i * kWave) % KP ^ swizzle(set % 4 * 8 + k);
+          lds_load16(kbase + row + min(piece * 16, hd * S - 16), to + i * 1024);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)at, k), hi = (uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), k);
+        const char* row = vbase + (long long)((unsigned long long)hi << 32 | lo);
+#pragma unroll
+        for (int i = 0; i < VL; ++i) {
+          const uint32_t d = (uint32_t)min(2 * (lane + i * kWave), hd - 2) * S;
+          if constexpr (CT == E4M3) vraw[n][i][k] = *(const uint16_t*)(row + d);
+          else vraw[n][i][k] = *(const uint32_t*)(row + d);
+        }
+      }
+    }
+  };
+  auto store = [&](int step) {
+    uint8_t* to = lds + (step & 1) * T::STAGE;
+#pragma unroll
+    for (int n = 0; n < SETS; ++n) {
+      const int set = wave + n * kTileWaves;
+      if constexpr (CT == E4M3) {
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          if (KP * 8 < kWave && lane >= KP * 8) break;
+          const int k = (lane + i * kWave) / KP, piece = (lane + i * kWave) % KP * 2, row = set * 8 + k, sw = swizzle(set % 4 * 8 + k);
+          const u32x4 x = kraw[n][i];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x2 y = widen16(x[2 * u]), z = widen16(x[2 * u + 1]);
+            *(u32x4*)(to + row * RB + ((piece + u) ^ sw) * 16) = u32x4{y[0], y[1], z[0], z[1]};
+          }
+        }
+      }
+      uint8_t* cells = to + T::ROWS * RB + set * HDP * 16;
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        if (HDP / 2 < kWave && lane >= HDP / 2) break;
+        uint32_t x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          x[k] = CT == E4M3 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(vraw[n][i][k], 1.0f, false)) : vraw[n][i][k];
+        u32x4 y, z;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          y[c] = __builtin_amdgcn_perm(x[2 * c + 1], x[2 * c], 0x05040100u);
+          z[c] = __builtin_amdgcn_perm(x[2 * c + 1], x[2 * c], 0x07060302u);
+        }
+        *(u32x4*)(cells + (lane + i * kWave) * 16) = y;
+        *(u32x4*)(cells + (HDP / 2 + lane + i * kWave) * 16) = z;
+      }
     }
   };
   const int steps = (end - it.begin + T::ROWS - 1) / T::ROWS;
@@ -745,17 +821,17 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   next = look(1);
 
   // ---- queries times scale and log2(e), in parts
-  u32x4 qp[CPW][NP][NQ];
+  u32x4 qp[CPW][NP][NK];
   float unlift[CPW];
 #pragma unroll
   for (int ct = 0; ct < CPW; ++ct) {
     const int c = (wc * CPW + ct) * 16 + col;
     const Column mine = column_of(L, it, kv, min(c, it.cols - 1));
     const float* q = a.q + (size_t)mine.row * a.ldq + (size_t)mine.head * hd;
-    f32x4 x[2 * NQ];
+    f32x4 x[2 * NK];
 #pragma unroll
-    for (int s = 0; s < 2 * NQ; ++s) {
-      const int d = CT == E4M3 ? (4 * (s / 4) + quad) * 16 + 4 * (s % 4) : (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
+    for (int s = 0; s < 2 * NK; ++s) {
+      const int d = (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
       x[s] = *(const f32x4u*)(q + min(d, hd - 4));
       x[s] *= d < hd && c < it.cols ? scale : 0.0f;
     }
@@ -764,7 +840,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     if constexpr (HALF) {
       float big = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 2 * NQ; ++s)
+      for (int s = 0; s < 2 * NK; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(x[s][i]));
       big = head_max(big);
@@ -775,7 +851,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       }
     }
 #pragma unroll
-    for (int s = 0; s < NQ; ++s)
+    for (int s = 0; s < NK; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f32x4 y = x[2 * s + i / 2];
@@ -785,6 +861,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
         for (int n = 0; n < NP; ++n) qp[ct][n][s][i] = u[n];
       }
   }
+  store(0);
 
   f32x4 o[CPW][VE];
   float m[CPW], l[CPW];
@@ -801,105 +878,76 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       next = look(step + 2);
     }
     const int base = it.begin + step * T::ROWS + wp * 32;
-    if (base >= end) continue;
-    const uint8_t* ks = lds + (step & 1) * T::STAGE + wp * 32 * RB;
-    const uint8_t* vs = ks + T::ROWS * RB;
-    // ---- scores
-    f32x4 s[CPW][2];
+    if (base < end) {
+      const uint8_t* ks = lds + (step & 1) * T::STAGE + wp * 32 * RB;
+      const uint8_t* vs = lds + (step & 1) * T::STAGE + T::ROWS * RB + (wp * 4 + quad) * HDP * 16 + col * 16;
+      // ---- scores
+      f32x4 s[CPW][2];
 #pragma unroll
-    for (int ct = 0; ct < CPW; ++ct) s[ct][0] = s[ct][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int ct = 0; ct < CPW; ++ct) s[ct][0] = s[ct][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < NK; ++j)
+      for (int j = 0; j < NK; ++j) {
+        u32x4 k[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int row = 16 * t + col;
-        const u32x4 kr = *(const u32x4*)(ks + row * RB + ((4 * j + quad) ^ swizzle(row)) * 16);
-        if constexpr (CT == E4M3) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const u32x2 y = widen16(kr[2 * u]), z = widen16(kr[2 * u + 1]);
-            const u32x4 k = {y[0], y[1], z[0], z[1]};
-#pragma unroll
-            for (int n = 0; n < NP; ++n)
-#pragma unroll
-              for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(k, qp[ct][n][2 * j + u], s[ct][t]);
-          }
-        } else {
-#pragma unroll
-          for (int n = 0; n < NP; ++n)
-#pragma unroll
-            for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(kr, qp[ct][n][j], s[ct][t]);
+        for (int t = 0; t < 2; ++t) {
+          const int row = 8 * (col / 4) + 4 * t + col % 4;
+          k[t] = *(const u32x4*)(ks + row * RB + ((4 * j + quad) ^ swizzle(row)) * 16);
         }
-      }
-    // ---- weights
-    u32x4 pp[CPW][NP];
-#pragma unroll
-    for (int ct = 0; ct < CPW; ++ct) {
-      if (base + 32 > end) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (base + 16 * t + 4 * quad + i >= end) s[ct][t][i] = -INFINITY;
-      }
-      float top = s[ct][0][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[ct][i / 4][i % 4]);
-      top = head_max(top) * unlift[ct];
-      if (__any(top > m[ct] + kSlack)) {
-        const float now = fmaxf(m[ct], top), keep = now == -INFINITY ? 1.0f : exp2_hw(m[ct] - now);
-        l[ct] *= keep;
-#pragma unroll
-        for (int c = 0; c < VE; ++c) o[ct][c] *= keep;
-        m[ct] = now;
-      }
-      const float from = (m[ct] == -INFINITY ? 0.0f : m[ct]) - kLift;
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = exp2_hw(HALF ? fmaf(s[ct][i / 4][i % 4], unlift[ct], -from) : s[ct][i / 4][i % 4] - from);
-        l[ct] += p[i];
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t u[NP];
-        split_pair<HALF, NP>(p[2 * c], p[2 * c + 1], u);
-#pragma unroll
-        for (int n = 0; n < NP; ++n) pp[ct][n][c] = u[n];
-      }
-    }
-    // ---- values
-#pragma unroll
-    for (int h = 0; h < NV; ++h) {
-      uint32_t w16[8][EV / 2];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int row = 16 * (k / 4) + 4 * quad + k % 4, at = (16 * h + col) * EV * S;
-        uint32_t raw[VW];
-        const uint8_t* from = vs + row * RB + ((at / 16) ^ swizzle(row)) * 16 + at % 16;
-        load_piece<EV * S, false>((const char*)from, raw);
-#pragma unroll
-        for (int d = 0; d < VW; ++d) {
-          if constexpr (CT == E4M3) {
-            const u32x2 y = widen16(raw[d]);
-            w16[k][2 * d] = y[0], w16[k][2 * d + 1] = y[1];
-          } else {
-            w16[k][d] = raw[d];
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < EV; ++e) {
-        u32x4 y;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          y[c] = __builtin_amdgcn_perm(w16[2 * c + 1][e / 2], w16[2 * c][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
         for (int n = 0; n < NP; ++n)
 #pragma unroll
-          for (int ct = 0; ct < CPW; ++ct) o[ct][h * EV + e] = mfma32<HALF>(y, pp[ct][n], o[ct][h * EV + e]);
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(k[t], qp[ct][n][j], s[ct][t]);
+      }
+      // ---- weights
+      u32x4 pp[CPW][NP];
+#pragma unroll
+      for (int ct = 0; ct < CPW; ++ct) {
+        if (base + 32 > end) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (base + 16 * t + 4 * quad + i >= end) s[ct][t][i] = -INFINITY;
+        }
+        float top = s[ct][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[ct][i / 4][i % 4]);
+        if (HALF) top *= unlift[ct];
+        if (__any(top > m[ct] + kSlack)) {
+          const float now = fmaxf(m[ct], head_max(top)), keep = now == -INFINITY ? 1.0f : exp2_hw(m[ct] - now);
+          l[ct] *= keep;
+#pragma unroll
+          for (int c = 0; c < VE; ++c) o[ct][c] *= keep;
+          m[ct] = now;
+        }
+        const float from = (m[ct] == -INFINITY ? 0.0f : m[ct]) - kLift;
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = exp2_hw(HALF ? fmaf(s[ct][i / 4][i % 4], unlift[ct], -from) : s[ct][i / 4][i % 4] - from);
+          l[ct] += p[i];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t u[NP];
+          split_pair<HALF, NP>(p[2 * c], p[2 * c + 1], u);
+#pragma unroll
+          for (int n = 0; n < NP; ++n) pp[ct][n][c] = u[n];
+        }
+      }
+      // ---- values
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const u32x4 v = *(const u32x4*)(vs + e * 256);
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+#pragma unroll
+          for (int ct = 0; ct < CPW; ++ct) o[ct][e] = mfma32<HALF>(v, pp[ct][n], o[ct][e]);
       }
     }
+    if (step + 1 < steps) store(step + 1);
   }
   bad = __syncthreads_or(bad);   // (every wave is done with the rows in LDS)
 #pragma unroll
@@ -922,6 +970,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     }
     __syncthreads();
     if (wp) return;
+#pragma unroll 1
     for (int w = 0; w < T::WP - 1; ++w)
 #pragma unroll
       for (int ct = 0; ct < CPW; ++ct) {
@@ -941,109 +990,140 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     if (c >= it.cols) continue;
     const size_t part = ((size_t)kv * L.cut.prefix_items + it.part) * L.cut.columns + c;
     if (quad == 0) L.prefix_ml[part * 2] = m[ct] - kLift, L.prefix_ml[part * 2 + 1] = l[ct];
+    // operand e holds cells 16 e ..: dimensions 2 c and, from HDP / 2 on, 2 c + 1
 #pragma unroll
-    for (int h = 0; h < NV; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = (16 * h + 4 * quad + i) * EV;
-        if (d >= hd) continue;
-#pragma unroll
-        for (int e = 0; e < EV; e += 4)
-          *(f32x4*)(L.prefix_o + part * hd + d + e) = f32x4{o[ct][h * EV + e][i], o[ct][h * EV + e + 1][i], o[ct][h * EV + e + 2][i], o[ct][h * EV + e + 3][i]};
-      }
+    for (int e = 0; e < VE / 2; ++e) {
+      const int d = 32 * e + 8 * quad;
+      if (d >= hd) continue;
+      const f32x4 x = o[ct][e], y = o[ct][e + VE / 2];
+      *(f32x4*)(L.prefix_o + part * hd + d) = f32x4{x[0], y[0], x[1], y[1]};
+      *(f32x4*)(L.prefix_o + part * hd + d + 4) = f32x4{x[2], y[2], x[3], y[3]};
+    }
   }
 }
 
-// WC: waves over a prefix item's columns; 0: the item in sixteens.  Prefix items first, then the rows' own, which lie
-// beside the last of them.
+// WC: waves over a prefix item's columns; 0: the item in sixteens.  Prefix items first, of all heads, then the rows' own, a
+// half of a tile block each: the long ones start together.
 template <int CT, int HDP, int WC>
-__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
-  using Tile = TileShape<CT == F32 ? BF16 : CT, HDP, WC ? WC : 4>;
-  constexpr int BYTES = WC && Tile::BYTES > (int)sizeof(ColumnsShared<HDP>) ? Tile::BYTES : (int)sizeof(ColumnsShared<HDP>);
+__global__ __launch_bounds__(WC ? kTileThreads : kThreads, WC || HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
+  constexpr int HALVES = WC ? kTileThreads / kThreads : 1;
+  constexpr int TILE = TileShape<CT == F32 ? BF16 : CT, HDP, WC ? WC : 4>::BYTES, COLUMNS = HALVES * (int)sizeof(ColumnsShared<HDP>);
+  constexpr int BYTES = WC && TILE > COLUMNS ? TILE : COLUMNS;
   __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
-  const int subs = WC ? 1 : L.cut.columns / 16, kv = (int)blockIdx.y;
-  int b = (int)blockIdx.x;
-  const bool own = b >= L.cut.prefix_items * subs;
-  b = own ? b - L.cut.prefix_items * subs : b / subs;
-  const int parts = own ? L.cut.own_items : L.cut.prefix_items;
-  if (b >= min(own ? L.p.head->own_items : L.p.head->prefix_items, parts)) return;
-  const Item it = (own ? L.p.own : L.p.prefix)[b];
-  if (!item_ok(L, it, parts, own ? L.cut.own_columns : L.cut.columns)) return;
+  const int subs = WC ? 1 : L.cut.columns / 16, half = (int)threadIdx.x / kThreads;
+  int b = (int)divide(blockIdx.x, L.by_kv);
+  const int kv = (int)blockIdx.x - b * L.g.map.n_kv;
+  const bool own = b >= L.prefix_blocks;
+  const int sub = own ? 0 : b % subs * 16;
+  b = own ? (b - L.prefix_blocks) * HALVES : b / subs;
+  const int parts = own ? L.cut.own_items : L.cut.prefix_items, some = min(own ? L.p.head->own_items : L.p.head->prefix_items, parts);
+  if (b >= some) return;
+  const bool there = b + (own ? half : 0) < some;   // (both halves come to the barriers)
+  Item it = (own ? L.p.own : L.p.prefix)[min(b + (own ? half : 0), some - 1)];
+  const bool ok = item_ok(L, it, parts, own ? L.cut.own_columns : L.cut.columns);
+  if (!own && !ok) return;
   if constexpr (WC != 0) {
     if (!own) {
       tile_block<CT, HDP, WC>(L, it, kv, lds);
       return;
     }
   }
-  columns_block<CT, HDP>(L, it, kv, own ? 0 : (int)blockIdx.x % subs * 16, own, *(ColumnsShared<HDP>*)lds);
+  if constexpr (WC && HDP > 128) return;   // (its registers would not do: launched by themselves)
+  if (!there || !ok) it.cols = 0;
+  columns_block<CT, HDP>(L, it, kv, sub, own, ((ColumnsShared<HDP>*)lds)[WC ? half : 0]);
 }
 
 // ---------------------------------------------------------------- the join
 
-// A block a (row, query head): its parts joined, four dimensions a thread, so that several parts are read side by side.
+// A wave a (row, query head): its parts joined, four dimensions a lane, so that 64 / (head_dim / 4) parts are read side by
+// side.  Latency: the parts' first rows are requested with their maxima.
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
+  constexpr int U = 4;
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
-  const int t = (int)blockIdx.x, head = (int)blockIdx.y, hd = g.map.head_dim, tid = threadIdx.x;
+  const int t = (int)blockIdx.x, head = __builtin_amdgcn_readfirstlane((int)blockIdx.y * kWaves + (int)threadIdx.x / kWave);
+  const int hd = g.map.head_dim, lane = threadIdx.x % kWave;
+  if (head >= a.n_q) return;
   const RowPlan r = L.p.rows[t];
   if (r.state == kLeave || r.state == kDone) return;
   float* out = a.out + (size_t)t * a.ldo + (size_t)head * hd;
   if (r.state != kJoin) {
-    for (int d = tid; d < hd; d += kThreads) out[d] = r.state == kZero ? 0.0f : NAN;
+    for (int d = lane; d < hd; d += kWave) out[d] = r.state == kZero ? 0.0f : NAN;
     return;
   }
   const int G = L.cut.group, kv = (int)divide((uint32_t)head, L.by_group), h = head - kv * G;
   const int c = (t - r.row0) * G + h, tile = c / L.cut.columns;
   const int np = r.pieces, n = np + r.owns;
-  const long long at0 = (long long)kv * L.cut.prefix_items + r.part0 + (long long)tile * np;
-  const long long at1 = (long long)kv * L.cut.own_items + r.own0 + (long long)(h / 16) * r.owns;
   // (a plan that is none leads to no place outside the work)
-  if (r.row0 < 0 || r.row0 > t || np < 0 || r.owns < 0 || r.part0 < 0 || r.own0 < 0 || (np && r.part0 + (long long)(tile + 1) * np > L.cut.prefix_items) ||
-      (r.owns && r.own0 + (long long)(h / 16 + 1) * r.owns > L.cut.own_items))
+  if (r.row0 < 0 || r.row0 > t || np < 0 || r.owns < 0 || n == 0 || r.part0 < 0 || r.own0 < 0 ||
+      (np && r.part0 + (long long)(tile + 1) * np > L.cut.prefix_items) || (r.owns && r.own0 + (long long)(h / 16 + 1) * r.owns > L.cut.own_items))
     return;
-  auto place = [&](int i, const float** ml, const float** o) {
-    const long long at = i < np ? (at0 + i) * L.cut.columns + c % L.cut.columns : (at1 + i - np) * L.cut.own_columns + h % 16;
-    *ml = (i < np ? L.prefix_ml : L.own_ml) + at * 2;
-    *o = (i < np ? L.prefix_o : L.own_o) + at * hd;
-  };
-  const int width = hd / 4, rows = kThreads / width, row = tid / width, d = tid % width * 4, lane = tid % kWave;
-  float top = -INFINITY;
-  const float *ml, *o;
-  for (int i = lane; i < n; i += kWave) place(i, &ml, &o), top = fmaxf(top, ml[0]);
+  const size_t at0 = ((size_t)kv * L.cut.prefix_items + r.part0 + (size_t)tile * np) * L.cut.columns + c % L.cut.columns;
+  const size_t at1 = ((size_t)kv * L.cut.own_items + r.own0 + (size_t)(h / 16) * r.owns) * L.cut.own_columns + h % 16;
+  auto ml_of = [&](int i) { return *(const float2*)(i < np ? L.prefix_ml + (at0 + (size_t)i * L.cut.columns) * 2 : L.own_ml + (at1 + (size_t)(i - np) * L.cut.own_columns) * 2); };
+  auto o_of = [&](int i, int d) { return *(const f32x4*)((i < np ? L.prefix_o + (at0 + (size_t)i * L.cut.columns) * hd : L.own_o + (at1 + (size_t)(i - np) * L.cut.own_columns) * hd) + d); };
+  const int width = hd / 4, rows = kWave / width, row = lane / width, d = lane % width * 4;
+  f32x4 y[U];
+#pragma unroll
+  for (int x = 0; x < U; ++x) y[x] = o_of(min(row + x * rows, n - 1), d);
+  const float2 first = ml_of(min(lane, n - 1));
+  float top = first.x;
+  for (int i = lane + kWave; i < n; i += kWave) top = fmaxf(top, ml_of(i).x);
 #pragma unroll
   for (int x = 32; x; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
   if (top == -INFINITY) top = 0.0f;
-  float sum = 0.0f;
-  for (int i = lane; i < n; i += kWave) place(i, &ml, &o), sum += ml[1] * exp2_hw(ml[0] - top);
+  const float by = exp2_hw(first.x - top);   // lane's part, of the first 64
+  float sum = lane < n ? first.y * by : 0.0f;
+  for (int i = lane + kWave; i < n; i += kWave) {
+    const float2 ml = ml_of(i);
+    sum += ml.y * exp2_hw(ml.x - top);
+  }
 #pragma unroll
   for (int x = 32; x; x /= 2) sum += __shfl_xor(sum, x);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (row < rows)
-    for (int i = row; i < n; i += rows) {
-      place(i, &ml, &o);
-      acc += *(const f32x4*)(o + d) * exp2_hw(ml[0] - top);
+  for (int i0 = 0; i0 < n; i0 += U * rows) {
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const int i = i0 + row + x * rows;
+      if (i0) y[x] = o_of(min(i, n - 1), d);
+      const float f = __shfl(by, i % kWave), w = i < kWave ? f : exp2_hw(ml_of(min(i, n - 1)).x - top);
+      if (row < rows && i < n) acc += y[x] * w;
     }
-  __shared__ f32x4 acc_s[kThreads];
-  acc_s[tid] = acc;
-  __syncthreads();
-  if (row == 0) {
-    for (int i = 1; i < rows; ++i) acc += acc_s[i * width + tid];
+  }
+  // the lanes of a dimension: row by row
+  f32x4 all = acc;
+  for (int x = 1; x < rows; ++x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) all[e] += __shfl(acc[e], lane + x * width);
+  }
+  if (lane < width) {
     const float vs = g.v_scale ? g.v_scale[kv] : 1.0f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) out[d + x] = sum == 0.0f ? 0.0f : acc[x] / sum * vs;
+    for (int x = 0; x < 4; ++x) out[d + x] = sum == 0.0f ? 0.0f : all[x] / sum * vs;
   }
+}
+
+template <int CT, int HDP, int WC>
+hipError_t launch(SharedLaunch L, unsigned prefix, unsigned own, hipStream_t s) {
+  L.prefix_blocks = (int)prefix;
+  hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, WC>), dim3((prefix + own) * (unsigned)L.g.map.n_kv), dim3(WC ? kTileThreads : kThreads), 0, s, L);
+  return hipGetLastError();
 }
 
 template <int CT, int HDP>
 hipError_t launch(const SharedLaunch& L, hipStream_t s) {
-  const int waves = CT == F32 || L.cut.columns < 64 / (HDP > 128 ? 2 : 1) ? 0 : L.cut.columns / (HDP > 128 ? 16 : 32);
-  const dim3 grid((unsigned)(L.cut.prefix_items * (waves ? 1 : L.cut.columns / 16) + L.cut.own_items), (unsigned)L.g.map.n_kv);
-  if constexpr (CT != F32) {
-    if (waves == 4) hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, 4>), grid, dim3(kThreads), 0, s, L);
-    if (waves == 2) hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, 2>), grid, dim3(kThreads), 0, s, L);
+  const unsigned prefix = (unsigned)L.cut.prefix_items, own = (unsigned)L.cut.own_items;
+  if constexpr (CT != F32 && HDP <= 128) {
+    if (L.cut.columns == 128) return launch<CT, HDP, 4>(L, prefix, (own + 1) / 2, s);
+    if (L.cut.columns == 64) return launch<CT, HDP, 2>(L, prefix, (own + 1) / 2, s);
   }
-  if (waves == 0) hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, 0>), grid, dim3(kThreads), 0, s, L);
-  return hipGetLastError();
+  if constexpr (CT != F32 && HDP > 128) {
+    if (L.cut.columns == 64) {
+      const hipError_t e = launch<CT, HDP, 4>(L, prefix, 0, s);
+      return e == hipSuccess ? launch<CT, HDP, 0>(L, 0, own, s) : e;
+    }
+  }
+  return launch<CT, HDP, 0>(L, prefix * (unsigned)(L.cut.columns / 16), own, s);
 }
 
 template <int CT>
@@ -1059,12 +1139,13 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
   plan_parts(L.cut, g.a.T, sh.n_groups, sh.plan, &L.p);
   shared_work(L.cut, g.map.n_kv, g.map.head_dim, g.a.work, &L);
   L.by_group = make_divider((uint32_t)L.cut.group);
+  L.by_kv = make_divider((uint32_t)g.map.n_kv);
   const hipError_t e = dtype == F32    ? launch<F32>(L, s)
                        : dtype == F16  ? launch<F16>(L, s)
                        : dtype == BF16 ? launch<BF16>(L, s)
                                        : launch<E4M3>(L, s);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(shared_join_kernel, dim3((unsigned)g.a.T, (unsigned)g.a.n_q), dim3(kThreads), 0, s, L);
+  hipLaunchKernelGGL(shared_join_kernel, dim3((unsigned)g.a.T, (unsigned)(g.a.n_q + kWaves - 1) / kWaves), dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
 
