@@ -71,7 +71,7 @@ ShareCut share_cut(int T, int n_groups, int n_q, int n_kv, int head_dim) {
   while (c.columns < mean && c.columns < (head_dim > 128 ? 64 : 128)) c.columns *= 2;
   c.own_columns = c.group < 16 ? c.group : 16;
   c.own_tiles = (c.group + 15) / 16;
-  const int resident = kCUs * (head_dim <= 128 && c.columns < 64 ? 2 : 1);
+  const int resident = kCUs * (head_dim <= 128 ? 2 : 1);
   c.slots = resident > n_kv ? resident / n_kv : 1;
   c.prefix_items = c.slots + (int)((long long)T * c.group / c.columns) + n_groups;
   c.own_slots = 2 * kCUs > n_kv ? 2 * kCUs / n_kv : 1;
@@ -419,16 +419,17 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
   const int parts = own ? L.cut.own_items : L.cut.prefix_items, columns = own ? L.cut.own_columns : L.cut.columns;
-  const int tid = threadIdx.x % kThreads, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int hd = g.map.head_dim;
-  const int heads = min(16, it.cols - sub);   // (none: a half block without an item)
+  const int heads = min(16, it.cols - sub);
+  if (heads <= 0) return;
   const float scale = a.scale * (g.k_scale ? scalar_load(g.k_scale, kv) : 1.0f) * 1.44269504088896340736f;
   const float vs = g.v_scale ? scalar_load(g.v_scale, kv) : 1.0f;
   const long long head_at = (long long)kv * g.map.head_stride;
   const char* kbase = (const char*)g.k + head_at * S;
   const char* vbase = (const char*)g.v + head_at * S;
   const int col = lane % 16, quad = lane / 16;
-  const int first = it.begin, end = heads > 0 ? it.end : it.begin;
+  const int first = it.begin, end = it.end;
 
   uint32_t kpiece[NK], vpiece[NV];
 #pragma unroll
@@ -436,7 +437,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 #pragma unroll
   for (int h = 0; h < NV; ++h) vpiece[h] = (uint32_t)min((16 * h + col) * EV * S, hd * S - EV * S);
 
-  const Column mine = column_of(L, it, kv, sub + max(min(col, heads - 1), 0));
+  const Column mine = column_of(L, it, kv, sub + min(col, heads - 1));
   const float* q = a.q + (size_t)mine.row * a.ldq + (size_t)mine.head * hd;
   constexpr int NX = CT == F32 ? NK : 2 * NQ;
   f32x4 x[NX];
@@ -682,7 +683,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 
 // ---------------------------------------------------------------- many columns
 
-// A block of eight waves takes an item of up to 64 or 128 columns: WC waves lie beside each other over the columns, 32 each
+// A block takes an item of up to 64 or 128 columns: WC waves lie beside each other over the columns, 32 each
 // (16 where head_dim is past 128), the others over the positions, 32 each of a step.  K and V of a step go through LDS, a
 // step ahead, where the waves over the columns share them, in the layouts that the matrix instructions take:
 //   keys     rows of 16-bit values, 16-byte pieces; piece p of row r at p ^ swizzle(r), so that the 16 rows of a read lie in
@@ -692,11 +693,10 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 // 8-bit pages become f16 on the way.  A wave stages the 8 rows of one (32 positions, q): their addresses lie in its lanes,
 // found once for K and V.  One barrier a step.  A column's largest score is raised only when one is more than 2^kSlack above
 // it, so that most steps need no sums across lanes.
-constexpr int kTileThreads = 512, kTileWaves = kTileThreads / kWave;
 
 template <int CT, int HDP, int WC>
 struct TileShape {
-  static constexpr int S = CT == E4M3 ? 1 : 2, WP = kTileWaves / WC, CPW = HDP > 128 ? 1 : 2;
+  static constexpr int S = CT == E4M3 ? 1 : 2, WP = kWaves / WC, CPW = HDP > 128 ? 1 : 2;
   static constexpr int ROWS = 32 * WP;             // positions of a step
   static constexpr int RB = HDP * 2;               // bytes of a row in LDS
   static constexpr int STAGE = 2 * ROWS * RB;      // K and V
@@ -710,7 +710,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   constexpr bool HALF = CT != BF16;
   constexpr int NP = HALF ? 2 : 3, S = T::S, CPW = T::CPW, RB = T::RB;
   constexpr int NK = HDP / 32, VE = HDP / 16;
-  constexpr int SETS = T::WP / 2;                              // (32 positions, q) that a wave stages
+  constexpr int SETS = T::WP * 4 / kWaves;                              // (32 positions, q) that a wave stages
   constexpr int KL = (8 * HDP * S + 1023) / 1024;              // 16-byte loads of a lane for their K
   constexpr int KP = HDP * S / 16;                             // such pieces of a row
   constexpr int VL = (HDP / 2 + kWave - 1) / kWave;            // pairs of dimensions of a lane
@@ -726,13 +726,13 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   const int* table = a.tables + (size_t)it.req * a.max_pages;
   bool bad = false;
 
-  // ---- staging: set n of a wave is quad set % 4 of positions 32 (set / 4) .. of the step, set = wave + 8 n; row k (lane % 8)
+  // ---- staging: set n of a wave is quad set % 4 of positions 32 (set / 4) .. of the step, set = wave + 4 n; row k (lane % 8)
   // of it position 16 (k / 4) + 4 q + k % 4, which is row 8 q + k of its 32 in LDS
   auto swizzle = [](int row) {
     return HDP == 64 ? (row >> 1 & 1) | (row >> 3 & 3) << 1 : (row & 3) | (row >> 3 & 3) << 2;
   };
   auto position = [&](int step, int n) {
-    const int set = wave + n * kTileWaves, k = lane % 8;
+    const int set = wave + n * kWaves, k = lane % 8;
     return min(it.begin + step * T::ROWS + set / 4 * 32 + 16 * (k / 4) + 4 * (set % 4) + k % 4, end - 1);
   };
   struct Look { int p[SETS]; };
@@ -747,7 +747,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   auto load = [&](int step, const Look& x) {
 #pragma unroll
     for (int n = 0; n < SETS; ++n) {
-      const int set = wave + n * kTileWaves, p = position(step, n);
+      const int set = wave + n * kWaves, p = position(step, n);
       int page = x.p[n];
       if (!page_ok(g.map, page)) bad = true, page = 0;
       const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
@@ -782,7 +782,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     uint8_t* to = lds + (step & 1) * T::STAGE;
 #pragma unroll
     for (int n = 0; n < SETS; ++n) {
-      const int set = wave + n * kTileWaves;
+      const int set = wave + n * kWaves;
       if constexpr (CT == E4M3) {
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
@@ -1002,26 +1002,23 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   }
 }
 
-// WC: waves over a prefix item's columns; 0: the item in sixteens.  Prefix items first, of all heads, then the rows' own, a
-// half of a tile block each: the long ones start together.
+// WC: waves over a prefix item's columns; 0: the item in sixteens.  Prefix items first, of all heads, then the rows' own:
+// the long ones start together.
 template <int CT, int HDP, int WC>
-__global__ __launch_bounds__(WC ? kTileThreads : kThreads, WC || HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
-  constexpr int HALVES = WC ? kTileThreads / kThreads : 1;
-  constexpr int TILE = TileShape<CT == F32 ? BF16 : CT, HDP, WC ? WC : 4>::BYTES, COLUMNS = HALVES * (int)sizeof(ColumnsShared<HDP>);
+__global__ __launch_bounds__(kThreads, WC || HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
+  constexpr int TILE = TileShape<CT == F32 ? BF16 : CT, HDP, WC ? WC : 4>::BYTES, COLUMNS = (int)sizeof(ColumnsShared<HDP>);
   constexpr int BYTES = WC && TILE > COLUMNS ? TILE : COLUMNS;
   __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
-  const int subs = WC ? 1 : L.cut.columns / 16, half = (int)threadIdx.x / kThreads;
+  const int subs = WC ? 1 : L.cut.columns / 16;
   int b = (int)divide(blockIdx.x, L.by_kv);
   const int kv = (int)blockIdx.x - b * L.g.map.n_kv;
   const bool own = b >= L.prefix_blocks;
   const int sub = own ? 0 : b % subs * 16;
-  b = own ? (b - L.prefix_blocks) * HALVES : b / subs;
+  b = own ? b - L.prefix_blocks : b / subs;
   const int parts = own ? L.cut.own_items : L.cut.prefix_items, some = min(own ? L.p.head->own_items : L.p.head->prefix_items, parts);
   if (b >= some) return;
-  const bool there = b + (own ? half : 0) < some;   // (both halves come to the barriers)
-  Item it = (own ? L.p.own : L.p.prefix)[min(b + (own ? half : 0), some - 1)];
-  const bool ok = item_ok(L, it, parts, own ? L.cut.own_columns : L.cut.columns);
-  if (!own && !ok) return;
+  const Item it = (own ? L.p.own : L.p.prefix)[b];
+  if (!item_ok(L, it, parts, own ? L.cut.own_columns : L.cut.columns)) return;
   if constexpr (WC != 0) {
     if (!own) {
       tile_block<CT, HDP, WC>(L, it, kv, lds);
@@ -1029,8 +1026,7 @@ __global__ __launch_bounds__(WC ? kTileThreads : kThreads, WC || HDP <= 128 ? 2 
     }
   }
   if constexpr (WC && HDP > 128) return;   // (its registers would not do: launched by themselves)
-  if (!there || !ok) it.cols = 0;
-  columns_block<CT, HDP>(L, it, kv, sub, own, ((ColumnsShared<HDP>*)lds)[WC ? half : 0]);
+  columns_block<CT, HDP>(L, it, kv, sub, own, *(ColumnsShared<HDP>*)lds);
 }
 
 // ---------------------------------------------------------------- the join
@@ -1106,7 +1102,7 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
 template <int CT, int HDP, int WC>
 hipError_t launch(SharedLaunch L, unsigned prefix, unsigned own, hipStream_t s) {
   L.prefix_blocks = (int)prefix;
-  hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, WC>), dim3((prefix + own) * (unsigned)L.g.map.n_kv), dim3(WC ? kTileThreads : kThreads), 0, s, L);
+  hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, WC>), dim3((prefix + own) * (unsigned)L.g.map.n_kv), dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
 
@@ -1114,8 +1110,8 @@ template <int CT, int HDP>
 hipError_t launch(const SharedLaunch& L, hipStream_t s) {
   const unsigned prefix = (unsigned)L.cut.prefix_items, own = (unsigned)L.cut.own_items;
   if constexpr (CT != F32 && HDP <= 128) {
-    if (L.cut.columns == 128) return launch<CT, HDP, 4>(L, prefix, (own + 1) / 2, s);
-    if (L.cut.columns == 64) return launch<CT, HDP, 2>(L, prefix, (own + 1) / 2, s);
+    if (L.cut.columns == 128) return launch<CT, HDP, 4>(L, prefix, own, s);
+    if (L.cut.columns == 64) return launch<CT, HDP, 2>(L, prefix, own, s);
   }
   if constexpr (CT != F32 && HDP > 128) {
     if (L.cut.columns == 64) {
