@@ -685,15 +685,12 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 
 // A block takes an item of up to 64 or 128 columns: WC waves lie beside each other over the columns, 32 each
 // (16 where head_dim is past 128), the others over the positions, 32 each of a step.  K and V of a step go through LDS, a
-// step ahead, where the waves over the columns share them, in the layouts that the matrix instructions take:
-//   keys     rows of 16-bit values, 16-byte pieces; piece p of row r at p ^ swizzle(r), so that the 16 rows of a read lie in
-//            all banks; 16-bit pages go straight from memory into LDS
-//   values   cells of a dimension's 8 keys 4 q + i and 16 + 4 q + i (q: the quad of lanes that reads it), in registers put
-//            together from 8 rows' pairs of dimensions: an operand is one 16-byte read
-// 8-bit pages become f16 on the way.  A wave stages the 8 rows of one (32 positions, q): their addresses lie in its lanes,
-// found once for K and V.  One barrier a step.  A column's largest score is raised only when one is more than 2^kSlack above
-// it, so that most steps need no sums across lanes.
-
+// step ahead, where the waves over the columns share them: rows of 16-bit values in 16-byte pieces, piece p of row r at
+// p ^ swizzle(r), so that the reads of both lie evenly over the banks.  Keys are read as rows; a value operand, 8 keys of one
+// dimension, is two reads that turn 4 rows x 16 dimensions around on their way.  16-bit pages go straight from memory into
+// LDS, 8-bit pages become f16 in registers.  A wave stages the 8 rows of one (32 positions, quad of lanes that reads them),
+// whose addresses lie in its lanes, found once for K and V.  One barrier a step.  A column's largest score is raised only
+// when one is more than 2^kSlack above it, so that most steps need no sums across lanes.
 template <int CT, int HDP, int WC>
 struct TileShape {
   static constexpr int S = CT == E4M3 ? 1 : 2, WP = kWaves / WC, CPW = HDP > 128 ? 1 : 2;
@@ -704,6 +701,13 @@ struct TileShape {
   static constexpr int BYTES = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
 };
 
+// Of the 16 lanes of a quad, each at 8 bytes of one of four rows (lane / 4) and 16 columns (lane % 4 * 4 ..): four 16-bit
+// values of column lane, one a row.
+__device__ __forceinline__ u32x2 read_turned(const uint8_t* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uint32_t)(uintptr_t)p));
+}
+
 template <int CT, int HDP, int WC>
 __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it, int kv, uint8_t* lds) {
   using T = TileShape<CT, HDP, WC>;
@@ -711,9 +715,8 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   constexpr int NP = HALF ? 2 : 3, S = T::S, CPW = T::CPW, RB = T::RB;
   constexpr int NK = HDP / 32, VE = HDP / 16;
   constexpr int SETS = T::WP * 4 / kWaves;                              // (32 positions, q) that a wave stages
-  constexpr int KL = (8 * HDP * S + 1023) / 1024;              // 16-byte loads of a lane for their K
+  constexpr int NL = (8 * HDP * S + 1023) / 1024;              // 16-byte loads of a lane for their keys
   constexpr int KP = HDP * S / 16;                             // such pieces of a row
-  constexpr int VL = (HDP / 2 + kWave - 1) / kWave;            // pairs of dimensions of a lane
   constexpr float kSlack = 4.0f, kLift = HALF ? 10.0f : 0.0f;  // weights reach 2^(kSlack + kLift)
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
@@ -742,8 +745,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     for (int n = 0; n < SETS; ++n) x.p[n] = table[divide((uint32_t)position(step, n), g.map.per)];
     return x;
   };
-  uint32_t vraw[SETS][VL][8];
-  u32x4 kraw[CT == E4M3 ? SETS : 1][KL];
+  u32x4 raw[CT == E4M3 ? SETS : 1][NL][2];
   auto load = [&](int step, const Look& x) {
 #pragma unroll
     for (int n = 0; n < SETS; ++n) {
@@ -752,66 +754,42 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       if (!page_ok(g.map, page)) bad = true, page = 0;
       const int off = p - (int)divide((uint32_t)p, g.map.per) * g.map.page_size;
       const long long at = ((long long)page * g.map.page_stride + (long long)off * g.map.slot_stride) * S;
-      uint8_t* to = lds + (step & 1) * T::STAGE + (set * 8) * RB;
+      uint8_t* to = lds + (step & 1) * T::STAGE + set * 8 * RB;
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int k = (lane + i * kWave) / KP;
+      for (int i = 0; i < NL; ++i) {
         if (KP * 8 < kWave && lane >= KP * 8) break;
+        const int k = (lane + i * kWave) / KP, piece = (lane + i * kWave) % KP;
         const long long row = __shfl(at, k);
         if constexpr (CT == E4M3) {
-          kraw[n][i] = *(const u32x4*)(kbase + row + min((lane + i * kWave) % KP * 16, hd - 16));
+          const int d = min(piece * 16, hd - 16);
+          raw[n][i][0] = *(const u32x4*)(kbase + row + d);
+          raw[n][i][1] = *(const u32x4*)(vbase + row + d);
         } else {
-          const int piece = (lane + i * kWave) % KP ^ swizzle(set % 4 * 8 + k);
-          lds_load16(kbase + row + min(piece * 16, hd * S - 16), to + i * 1024);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)at, k), hi = (uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), k);
-        const char* row = vbase + (long long)((unsigned long long)hi << 32 | lo);
-#pragma unroll
-        for (int i = 0; i < VL; ++i) {
-          const uint32_t d = (uint32_t)min(2 * (lane + i * kWave), hd - 2) * S;
-          if constexpr (CT == E4M3) vraw[n][i][k] = *(const uint16_t*)(row + d);
-          else vraw[n][i][k] = *(const uint32_t*)(row + d);
+          const int d = min((piece ^ swizzle(set % 4 * 8 + k)) * 16, hd * S - 16);
+          lds_load16(kbase + row + d, to + i * 1024);
+          lds_load16(vbase + row + d, to + T::ROWS * RB + i * 1024);
         }
       }
     }
   };
   auto store = [&](int step) {
-    uint8_t* to = lds + (step & 1) * T::STAGE;
+    if constexpr (CT == E4M3) {
 #pragma unroll
-    for (int n = 0; n < SETS; ++n) {
-      const int set = wave + n * kWaves;
-      if constexpr (CT == E4M3) {
+      for (int n = 0; n < SETS; ++n) {
+        const int set = wave + n * kWaves;
+        uint8_t* to = lds + (step & 1) * T::STAGE;
 #pragma unroll
-        for (int i = 0; i < KL; ++i) {
+        for (int i = 0; i < NL; ++i) {
           if (KP * 8 < kWave && lane >= KP * 8) break;
-          const int k = (lane + i * kWave) / KP, piece = (lane + i * kWave) % KP * 2, row = set * 8 + k, sw = swizzle(set % 4 * 8 + k);
-          const u32x4 x = kraw[n][i];
+          const int k = (lane + i * kWave) / KP, piece = (lane + i * kWave) % KP * 2, sw = swizzle(set % 4 * 8 + k);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const u32x2 y = widen16(x[2 * u]), z = widen16(x[2 * u + 1]);
-            *(u32x4*)(to + row * RB + ((piece + u) ^ sw) * 16) = u32x4{y[0], y[1], z[0], z[1]};
-          }
+          for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const u32x2 y = widen16(raw[n][i][side][2 * u]), z = widen16(raw[n][i][side][2 * u + 1]);
+              *(u32x4*)(to + side * T::ROWS * RB + (set * 8 + k) * RB + ((piece + u) ^ sw) * 16) = u32x4{y[0], y[1], z[0], z[1]};
+            }
         }
-      }
-      uint8_t* cells = to + T::ROWS * RB + set * HDP * 16;
-#pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        if (HDP / 2 < kWave && lane >= HDP / 2) break;
-        uint32_t x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          x[k] = CT == E4M3 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(vraw[n][i][k], 1.0f, false)) : vraw[n][i][k];
-        u32x4 y, z;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          y[c] = __builtin_amdgcn_perm(x[2 * c + 1], x[2 * c], 0x05040100u);
-          z[c] = __builtin_amdgcn_perm(x[2 * c + 1], x[2 * c], 0x07060302u);
-        }
-        *(u32x4*)(cells + (lane + i * kWave) * 16) = y;
-        *(u32x4*)(cells + (HDP / 2 + lane + i * kWave) * 16) = z;
       }
     }
   };
@@ -880,26 +858,37 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     const int base = it.begin + step * T::ROWS + wp * 32;
     if (base < end) {
       const uint8_t* ks = lds + (step & 1) * T::STAGE + wp * 32 * RB;
-      const uint8_t* vs = lds + (step & 1) * T::STAGE + T::ROWS * RB + (wp * 4 + quad) * HDP * 16 + col * 16;
+      const uint8_t* vs = ks + T::ROWS * RB + (quad * 8 + col / 4) * RB + col % 2 * 8;
       // ---- scores
       f32x4 s[CPW][2];
 #pragma unroll
       for (int ct = 0; ct < CPW; ++ct) s[ct][0] = s[ct][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      u32x4 k[NK][2];
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        u32x4 k[2];
+      for (int j = 0; j < NK; ++j)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int row = 8 * (col / 4) + 4 * t + col % 4;
-          k[t] = *(const u32x4*)(ks + row * RB + ((4 * j + quad) ^ swizzle(row)) * 16);
+          k[j][t] = *(const u32x4*)(ks + row * RB + ((4 * j + quad) ^ swizzle(row)) * 16);
         }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
 #pragma unroll
         for (int n = 0; n < NP; ++n)
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(k[t], qp[ct][n][j], s[ct][t]);
+            for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(k[j][t], qp[ct][n][j], s[ct][t]);
+      // the values' operands are requested before the weights are worked on
+      u32x4 v[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const u32x2 x = read_turned(vs + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + col / 4)) * 16);
+        const u32x2 y = read_turned(vs + 4 * RB + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + 4 + col / 4)) * 16);
+        v[e] = u32x4{x[0], x[1], y[0], y[1]};
       }
+      __builtin_amdgcn_sched_barrier(0);
       // ---- weights
       u32x4 pp[CPW][NP];
 #pragma unroll
@@ -940,11 +929,10 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       // ---- values
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const u32x4 v = *(const u32x4*)(vs + e * 256);
 #pragma unroll
         for (int n = 0; n < NP; ++n)
 #pragma unroll
-          for (int ct = 0; ct < CPW; ++ct) o[ct][e] = mfma32<HALF>(v, pp[ct][n], o[ct][e]);
+          for (int ct = 0; ct < CPW; ++ct) o[ct][e] = mfma32<HALF>(v[e], pp[ct][n], o[ct][e]);
       }
     }
     if (step + 1 < steps) store(step + 1);
@@ -990,14 +978,10 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     if (c >= it.cols) continue;
     const size_t part = ((size_t)kv * L.cut.prefix_items + it.part) * L.cut.columns + c;
     if (quad == 0) L.prefix_ml[part * 2] = m[ct] - kLift, L.prefix_ml[part * 2 + 1] = l[ct];
-    // operand e holds cells 16 e ..: dimensions 2 c and, from HDP / 2 on, 2 c + 1
 #pragma unroll
-    for (int e = 0; e < VE / 2; ++e) {
-      const int d = 32 * e + 8 * quad;
-      if (d >= hd) continue;
-      const f32x4 x = o[ct][e], y = o[ct][e + VE / 2];
-      *(f32x4*)(L.prefix_o + part * hd + d) = f32x4{x[0], y[0], x[1], y[1]};
-      *(f32x4*)(L.prefix_o + part * hd + d + 4) = f32x4{x[2], y[2], x[3], y[3]};
+    for (int e = 0; e < VE; ++e) {
+      const int d = 16 * e + 4 * quad;
+      if (d < hd) *(f32x4*)(L.prefix_o + part * hd + d) = o[ct][e];
     }
   }
 }
