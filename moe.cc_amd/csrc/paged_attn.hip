@@ -79,20 +79,6 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   return v;
 }
-__device__ __forceinline__ float wave_total(float x) {
-  auto step = [&](auto ctrl, auto mask) {
-    x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, decltype(mask)::value, 0xf, false));
-  };
-  using std::integral_constant;
-  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
-  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
-  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
-  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
-  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
-  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
-}
-
 // Where a block's piece starts: units begin .. end - 1 of all, in row `row` of request `req`, whose first unit is `at`.
 struct Piece {
   uint32_t begin, end, per;   // per: units of a piece

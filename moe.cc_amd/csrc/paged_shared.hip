@@ -56,7 +56,8 @@ struct PlanHead {
 // How a call is cut: the same for moe_paged_share_dev and moe_paged_attn_shared_dev.
 struct ShareCut {
   int group;          // query heads of a key-value head
-  int columns;        // of a prefix item
+  int columns;        // of a prefix item: 1 << shift
+  int shift;
   int own_columns;    // of a row's own
   int own_tiles;      // of a row
   int slots, own_slots;   // items that are resident at once, about
@@ -67,8 +68,9 @@ ShareCut share_cut(int T, int n_groups, int n_q, int n_kv, int head_dim) {
   ShareCut c;
   c.group = n_q / n_kv;
   const long long mean = n_groups ? ((long long)T + n_groups - 1) / n_groups * c.group : 0;
-  c.columns = 16;
-  while (c.columns < mean && c.columns < (head_dim > 128 ? 64 : 128)) c.columns *= 2;
+  c.shift = 4;
+  while (1 << c.shift < mean && 1 << c.shift < (head_dim > 128 ? 64 : 128)) ++c.shift;
+  c.columns = 1 << c.shift;
   c.own_columns = c.group < 16 ? c.group : 16;
   c.own_tiles = (c.group + 15) / 16;
   const int resident = kCUs * (head_dim <= 128 ? 2 : 1);
@@ -705,7 +707,7 @@ struct TileShape {
 // values of column lane, one a row.
 __device__ __forceinline__ u32x2 read_turned(const uint8_t* p) {
   typedef short s16x4 __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uint32_t)(uintptr_t)p));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
 template <int CT, int HDP, int WC>
@@ -1032,42 +1034,59 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
     return;
   }
   const int G = L.cut.group, kv = (int)divide((uint32_t)head, L.by_group), h = head - kv * G;
-  const int c = (t - r.row0) * G + h, tile = c / L.cut.columns;
+  const int c = (t - r.row0) * G + h, tile = c >> L.cut.shift;
   const int np = r.pieces, n = np + r.owns;
   // (a plan that is none leads to no place outside the work)
   if (r.row0 < 0 || r.row0 > t || np < 0 || r.owns < 0 || n == 0 || r.part0 < 0 || r.own0 < 0 ||
       (np && r.part0 + (long long)(tile + 1) * np > L.cut.prefix_items) || (r.owns && r.own0 + (long long)(h / 16 + 1) * r.owns > L.cut.own_items))
     return;
-  const size_t at0 = ((size_t)kv * L.cut.prefix_items + r.part0 + (size_t)tile * np) * L.cut.columns + c % L.cut.columns;
+  const size_t at0 = ((size_t)kv * L.cut.prefix_items + r.part0 + (size_t)tile * np) * L.cut.columns + (c & (L.cut.columns - 1));
   const size_t at1 = ((size_t)kv * L.cut.own_items + r.own0 + (size_t)(h / 16) * r.owns) * L.cut.own_columns + h % 16;
-  auto ml_of = [&](int i) { return *(const float2*)(i < np ? L.prefix_ml + (at0 + (size_t)i * L.cut.columns) * 2 : L.own_ml + (at1 + (size_t)(i - np) * L.cut.own_columns) * 2); };
-  auto o_of = [&](int i, int d) { return *(const f32x4*)((i < np ? L.prefix_o + (at0 + (size_t)i * L.cut.columns) * hd : L.own_o + (at1 + (size_t)(i - np) * L.cut.own_columns) * hd) + d); };
+  // (part i at a base and i steps from it: prefix parts, then the row's own)
+  const float2* const ml0 = (const float2*)L.prefix_ml + at0;
+  const float2* const ml1 = (const float2*)L.own_ml + at1 - (size_t)np * L.cut.own_columns;
+  const float* const o0 = L.prefix_o + at0 * hd;
+  const float* const o1 = L.own_o + at1 * hd - (size_t)np * L.cut.own_columns * hd;
+  const uint32_t step0 = (uint32_t)L.cut.columns, step1 = (uint32_t)L.cut.own_columns;
+  auto ml_of = [&](int i) { return (i < np ? ml0 : ml1)[(uint32_t)i * (i < np ? step0 : step1)]; };
+  auto o_of = [&](int i, int d) { return *(const f32x4*)((i < np ? o0 : o1) + (size_t)((uint32_t)i * (i < np ? step0 : step1)) * hd + d); };
   const int width = hd / 4, rows = kWave / width, row = lane / width, d = lane % width * 4;
   f32x4 y[U];
 #pragma unroll
   for (int x = 0; x < U; ++x) y[x] = o_of(min(row + x * rows, n - 1), d);
   const float2 first = ml_of(min(lane, n - 1));
   float top = first.x;
-  for (int i = lane + kWave; i < n; i += kWave) top = fmaxf(top, ml_of(i).x);
+  if (n > kWave)
+    for (int i = lane + kWave; i < n; i += kWave) top = fmaxf(top, ml_of(i).x);
 #pragma unroll
   for (int x = 32; x; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
   if (top == -INFINITY) top = 0.0f;
   const float by = exp2_hw(first.x - top);   // lane's part, of the first 64
   float sum = lane < n ? first.y * by : 0.0f;
-  for (int i = lane + kWave; i < n; i += kWave) {
-    const float2 ml = ml_of(i);
-    sum += ml.y * exp2_hw(ml.x - top);
-  }
-#pragma unroll
-  for (int x = 32; x; x /= 2) sum += __shfl_xor(sum, x);
+  if (n > kWave)
+    for (int i = lane + kWave; i < n; i += kWave) {
+      const float2 ml = ml_of(i);
+      sum += ml.y * exp2_hw(ml.x - top);
+    }
+  sum = wave_total(sum);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int i0 = 0; i0 < n; i0 += U * rows) {
+    if (i0) {
 #pragma unroll
-    for (int x = 0; x < U; ++x) {
-      const int i = i0 + row + x * rows;
-      if (i0) y[x] = o_of(min(i, n - 1), d);
-      const float f = __shfl(by, i % kWave), w = i < kWave ? f : exp2_hw(ml_of(min(i, n - 1)).x - top);
-      if (row < rows && i < n) acc += y[x] * w;
+      for (int x = 0; x < U; ++x) y[x] = o_of(min(i0 + row + x * rows, n - 1), d);
+    }
+    if (i0 + U * rows <= kWave) {
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        const int i = i0 + row + x * rows;
+        acc += y[x] * (row < rows && i < n ? __shfl(by, i) : 0.0f);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        const int i = i0 + row + x * rows;
+        if (row < rows && i < n) acc += y[x] * exp2_hw(ml_of(i).x - top);
+      }
     }
   }
   // the lanes of a dimension: row by row

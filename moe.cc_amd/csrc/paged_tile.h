@@ -1,6 +1,8 @@
 // paged_tile.h - what the attention kernels over a paged cache share: types of
 // the matrix operands, sums over a head's lanes, operands made of fp32 values.
 #pragma once
+#include <type_traits>
+
 #include "moe_device.h"
 #include "paged_attn.h"
 
@@ -37,6 +39,21 @@ __device__ __forceinline__ float head_sum(float x) {
   x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
   auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// sum over the wave's lanes, in all of them
+__device__ __forceinline__ float wave_total(float x) {
+  auto step = [&](auto ctrl, auto mask) {
+    x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, decltype(mask)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -213,6 +213,24 @@ def test_repeatable_and_graph(moehip):
     hip.destroy(graph)
 
 
+@pytest.mark.parametrize("kind", list(C.TYPES))
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0, 1e-6])
+def test_scales(moehip, kind, scale):
+    """Negative, no, sharp and flat scales."""
+    b = Batch(moehip, kind, [(9, 256, (1, 70)), (2, 64, (1, 20))], 16, 2, 128, 16, "head", seed=12)
+    b.scale = float(np.float32(scale))
+    b.run()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_large_and_small_queries(moehip, kind):
+    """Rows whose queries differ by many powers of two, in one product."""
+    b = Batch(moehip, kind, [(8, 256, (1, 40))], 8, 1, 64, 16, seed=13)
+    b.q *= (10.0 ** np.linspace(-30, 1, 8)).astype(np.float32)[:, None, None]
+    b.q[3, 2] = 0
+    b.run()
+
+
 def test_no_rows_no_groups(moehip):
     M, L = moehip, moehip.lib()
     b = Batch(M, "f32", [(3, 32, (1, 5))], 4, 2, 64, 16, seed=9, first=[0])
