@@ -6,10 +6,12 @@
 // place of all its holders' tables.  Everything about a page is therefore
 // found in one column of the tables, and columns are independent of each
 // other: a block takes some columns of all requests and finds which of their
-// pages no request holds any more by marks in `work`, a number a page:
-//   0  every page of the old tables      1  every page of the new ones
-//   2 + n - 1 - r  of the rest, by the largest: the lowest request r that held it gives it back
-// Nothing is kept from one call for the next.
+// pages no request holds any more by a number a page in `work`, the largest of
+//   0              every page of the old tables
+//   n - r          of the requests r that held it: the lowest gives it back, unless
+//   kStays         a request holds it now
+// Nothing is kept from one call for the next.  Latency bounds it: launch, the
+// requests' numbers, the tables, three rounds at the pages' numbers.
 #include <initializer_list>
 
 #include "moe_device.h"
@@ -21,17 +23,14 @@ namespace {
 
 constexpr int kN = 1024;             // threads of a block
 constexpr int kMostRequests = 4096;
-constexpr int kPer = 8;              // table entries of a thread
-constexpr int kEntries = kPer * kN;  // of a block
+constexpr int kStays = 1 << 30;
 
 // How a request goes on.
 struct Goes {
   int src;    // the request that it is a copy of; -1: it ends
-  int fills;  // pages of src
-  int dst;    // the page that its last one is copied to
-  int used;   // pages that it had
-  int copy;   // its place among the copies; -1: none
   int held;   // positions of src
+  int copy;   // its place among the copies; -1: none
+  int used;   // pages that it had
 };
 
 struct ForkHead {
@@ -42,6 +41,7 @@ struct ForkArgs {
   moe_paged_fork f;
   Divider per;      // by page_size
   int columns, blocks;   // of a block, of the tables
+  Divider by_columns;
   ForkHead* top;    // work
   Goes* goes;       // work [n_req]
   int* counts;      // work [blocks] pages that come back
@@ -49,12 +49,13 @@ struct ForkArgs {
   int* mark;        // work [n_pages]
 };
 
+// Past the L1: what the block's other waves wrote there is seen after a stage_sync<0>.
 __device__ __forceinline__ int mark_load(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void mark_store(int* p, int x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // Sum over the block's threads up to and without this one, and of all.
 __device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int x = v;
 #pragma unroll
   for (int c = 1; c < kWave; c *= 2) {
@@ -64,6 +65,7 @@ __device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
   if (lane == kWave - 1) wave_s[wave] = x;
   __syncthreads();
   int before = 0, all = 0;
+#pragma unroll
   for (int w = 0; w < kN / kWave; ++w) {
     const int y = wave_s[w];
     if (w < wave) before += y;
@@ -74,48 +76,67 @@ __device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
   return before + x - v;
 }
 
-// The requests: how each goes on, and whether the call can be done.
-__device__ __forceinline__ void fork_requests(const ForkArgs& a) {
+template <int MOST>
+struct ForkShared {
+  int parent[MOST], held[MOST], copy[MOST];
+  int wave[kN / kWave], bad;
+};
+
+// The requests, into sh: how each goes on, and whether the call can be done.  Every block of a call finds the same.
+template <int MOST>
+__device__ __forceinline__ ForkHead fork_requests(const ForkArgs& a, ForkShared<MOST>& sh) {
   const moe_paged_fork& f = a.f;
-  __shared__ int keep_s[kMostRequests], wave_s[kN / kWave], bad_s;
   const int tid = threadIdx.x, n = f.n_req;
-  const int head = f.ring_at[0], count = f.ring_at[1];
   const long long most = (long long)f.max_pages * f.page_size;
-  if (tid == 0) bad_s = head < 0 || head >= f.n_pages || count < 0 || count > f.n_pages;
-  for (int r = tid; r < n; r += kN) keep_s[r] = n;
-  __syncthreads();
+  const int head = f.ring_at[0], count = f.ring_at[1];
+  if (tid == 0) sh.bad = head < 0 || head >= f.n_pages || count < 0 || count > f.n_pages;
   for (int r = tid; r < n; r += kN) {
-    const int p = f.parent[r], h = f.held[r];
-    if (p < -1 || p >= n || h < 0 || h > most) bad_s = 1;
-    else if (p >= 0) atomicMin(&keep_s[p], p == r ? -1 : r);   // the page that is not full stays with the request itself, or its first copy
+    sh.parent[r] = f.parent[r];
+    sh.held[r] = f.held[r];
+    sh.copy[r] = n;
   }
   __syncthreads();
-  const bool bad = bad_s;
+  // the page that is not full stays with the request itself, or its first copy
+  for (int r = tid; r < n; r += kN) {
+    const int p = sh.parent[r], h = sh.held[r];
+    if (p < -1 || p >= n || h < 0 || h > most) sh.bad = 1;
+    else if (p >= 0) atomicMin(&sh.copy[p], p == r ? -1 : r);
+  }
+  __syncthreads();
+  const bool bad = sh.bad;
   int done = 0;
   for (int r0 = 0; r0 < n; r0 += kN) {
     const int r = r0 + tid;
-    Goes g = {-1, 0, -1, 0, -1, 0};
     bool copied = false;
     if (r < n && !bad) {
-      g.used = pages_for(f.held[r], a.per);
-      g.src = f.parent[r];
-      if (g.src >= 0) {
-        g.held = f.held[g.src];
-        g.fills = pages_for(g.held, a.per);
-        const int last = g.held - (int)divide((uint32_t)g.held, a.per) * f.page_size;
-        copied = last && keep_s[g.src] != r && g.src != r;
+      const int p = sh.parent[r];
+      if (p >= 0) {
+        const int h = sh.held[p];
+        copied = h != (int)divide((uint32_t)h, a.per) * f.page_size && sh.copy[p] != r && p != r;
       }
     }
     int all;
-    const int at = done + block_scan(copied, wave_s, &all);
-    if (copied) {
-      g.copy = at;
-      g.dst = at < count ? f.ring[ring_place(head, at, f.n_pages)] : -1;
-    }
-    if (r < n) a.goes[r] = g;
+    const int at = done + block_scan(copied, sh.wave, &all);
+    // (the keepers of the requests behind these are still to be read)
+    if (r < n) sh.parent[r] = bad ? -1 : copied ? sh.parent[r] | at << 12 | 1 << 30 : sh.parent[r];
     done += all;
   }
-  if (tid == 0) *a.top = ForkHead{bad ? kForkBad : done > f.max_copies ? kForkCopies : done > count ? kForkNoPages : kForkOk, head, count, done};
+  __syncthreads();
+  for (int r = tid; r < n; r += kN) {
+    const int x = sh.parent[r];
+    const bool copied = x >= 0 && x >> 30;
+    sh.copy[r] = copied ? x >> 12 & 0xfff : -1;
+    if (copied) sh.parent[r] = x & 0xfff;
+    if (bad) sh.held[r] = 0;
+  }
+  __syncthreads();
+  return ForkHead{bad ? kForkBad : done > f.max_copies ? kForkCopies : done > count ? kForkNoPages : kForkOk, head, count, done};
+}
+
+template <int MOST>
+__device__ __forceinline__ Goes goes_of(const ForkArgs& a, const ForkShared<MOST>& sh, int r) {
+  const int p = sh.parent[r];
+  return Goes{p, p >= 0 ? sh.held[p] : 0, sh.copy[r], pages_for(sh.held[r], a.per)};
 }
 
 // A thread's entries of a block's columns: entry i is column i % columns of request i / columns, counted from the first.
@@ -124,48 +145,59 @@ struct Entry {
   bool in;
 };
 __device__ __forceinline__ Entry entry_of(const ForkArgs& a, int c0, int k) {
-  const int i = k * kN + (int)threadIdx.x, r = i / a.columns;
-  return {r, c0 + i - r * a.columns, r < a.f.n_req && c0 + i - r * a.columns < a.f.max_pages};
+  const int i = k * kN + (int)threadIdx.x, r = (int)divide((uint32_t)i, a.by_columns), c = c0 + i - r * a.columns;
+  return {r, c, r < a.f.n_req && c < a.f.max_pages};
 }
 
-// The pages of columns c0 .. that come back, in order of the columns, then of the requests, to a.list; their number.
-__device__ __forceinline__ int fork_columns(const ForkArgs& a, int c0) {
+// The pages of columns c0 .. that come back, in order of the columns, then of the requests, to `list`; their number.
+template <int PER, int MOST>
+__device__ __forceinline__ int fork_columns(const ForkArgs& a, ForkShared<MOST>& sh, int c0, int* list) {
   const moe_paged_fork& f = a.f;
   const int n = f.n_req, tid = threadIdx.x;
-  __shared__ uint32_t bits_s[kEntries / 32];
-  __shared__ int wave_s[kN / kWave];
-  int old[kPer];
-  for (int i = tid; i < kEntries / 32; i += kN) bits_s[i] = 0;
+  constexpr int WORDS = PER * kN / 32;
+  __shared__ uint32_t bits_s[WORDS];
+  __shared__ int first_s[WORDS];
+  int old[PER], now[PER];
+  for (int i = tid; i < WORDS; i += kN) bits_s[i] = 0;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
+  for (int k = 0; k < PER; ++k) {
     const Entry e = entry_of(a, c0, k);
-    old[k] = -1;
-    if (e.in && e.c < a.goes[e.r].used) old[k] = f.tables[(size_t)e.r * f.max_pages + e.c];
-    if ((uint32_t)old[k] >= (uint32_t)f.n_pages) old[k] = -1;
-    if (old[k] >= 0) mark_store(&a.mark[old[k]], 0);
-  }
-  __threadfence();
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const Entry e = entry_of(a, c0, k);
+    old[k] = now[k] = -1;
     if (!e.in) continue;
-    const Goes g = a.goes[e.r];
-    if (g.src < 0 || e.c >= g.fills || (g.copy >= 0 && e.c == g.fills - 1)) continue;
-    const int page = f.tables[(size_t)g.src * f.max_pages + e.c];
-    if ((uint32_t)page < (uint32_t)f.n_pages) mark_store(&a.mark[page], 1);
+    const Goes g = goes_of(a, sh, e.r);
+    const int* row = f.tables + e.c;
+    if (e.c < g.used) old[k] = row[(size_t)e.r * f.max_pages];
+    const int fills = pages_for(g.held, a.per);
+    if (g.src >= 0 && e.c < fills && !(g.copy >= 0 && e.c == fills - 1)) now[k] = row[(size_t)g.src * f.max_pages];
   }
-  __threadfence();
-  __syncthreads();
+  // what the request before does for the same page, in a neighbouring lane, need not be done again
+  const int lane = tid % kWave, from = lane - a.columns;
+  auto again = [&](int x) {
+    const int y = __shfl(x, max(from, 0));
+    return from >= 0 && x == y;
+  };
 #pragma unroll
-  for (int k = 0; k < kPer; ++k)
-    if (old[k] >= 0 && mark_load(&a.mark[old[k]]) != 1) atomicMax(&a.mark[old[k]], 2 + n - 1 - entry_of(a, c0, k).r);
-  __threadfence();
-  __syncthreads();
+  for (int k = 0; k < PER; ++k) {
+    if ((uint32_t)old[k] >= (uint32_t)f.n_pages) old[k] = -1;
+    if ((uint32_t)now[k] >= (uint32_t)f.n_pages) now[k] = -1;
+    const bool twice = again(old[k]), stays = old[k] == now[k];
+    if (again(now[k])) now[k] = -1;
+    if (old[k] >= 0 && !twice) mark_store(&a.mark[old[k]], 0);
+    if (twice || stays) old[k] = -1;   // from here on: what this entry may give back
+  }
+  stage_sync<0>();
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
+  for (int k = 0; k < PER; ++k) {
+    if (now[k] >= 0) atomicMax(&a.mark[now[k]], kStays);
+    if (old[k] >= 0) atomicMax(&a.mark[old[k]], n - entry_of(a, c0, k).r);
+  }
+  stage_sync<0>();
+#pragma unroll
+  for (int k = 0; k < PER; ++k) now[k] = old[k] >= 0 ? mark_load(&a.mark[old[k]]) : 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
     const Entry e = entry_of(a, c0, k);
-    if (old[k] >= 0 && mark_load(&a.mark[old[k]]) == 2 + n - 1 - e.r) {
+    if (e.in && now[k] == n - e.r) {
       const int bit = (e.c - c0) * n + e.r;
       atomicOr(&bits_s[bit / 32], 1u << bit % 32);
     } else {
@@ -174,65 +206,58 @@ __device__ __forceinline__ int fork_columns(const ForkArgs& a, int c0) {
   }
   __syncthreads();
   // a thread a word: places within the block
-  const uint32_t mine = tid < kEntries / 32 ? bits_s[tid] : 0;
+  static_assert(WORDS <= kN);
   int all;
-  const int before = block_scan(__popc(mine), wave_s, &all);
-  __shared__ int first_s[kEntries / 32];
-  if (tid < kEntries / 32) first_s[tid] = before;
+  const int before = block_scan(tid < WORDS ? __popc(bits_s[tid]) : 0, sh.wave, &all);
+  if (tid < WORDS) first_s[tid] = before;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
+  for (int k = 0; k < PER; ++k) {
     if (old[k] < 0) continue;
     const Entry e = entry_of(a, c0, k);
     const int bit = (e.c - c0) * n + e.r;
-    a.list[(size_t)c0 * n + first_s[bit / 32] + __popc(bits_s[bit / 32] & ((1u << bit % 32) - 1))] = old[k];
+    list[first_s[bit / 32] + __popc(bits_s[bit / 32] & ((1u << bit % 32) - 1))] = old[k];
   }
   return all;
 }
 
 // What the call leaves: block b's columns of the tables and its pages in the ring, block 0 the rest too.
-__device__ __forceinline__ void fork_finish(const ForkArgs& a, int b, int before, int back) {
+template <int PER, class GoesOf>
+__device__ __forceinline__ void fork_finish(const ForkArgs& a, ForkHead top, int b, int before, int mine, int back, const int* list, GoesOf goes) {
   const moe_paged_fork& f = a.f;
   const int tid = threadIdx.x, n = f.n_req, c0 = b * a.columns;
-  ForkHead top = *a.top;
-  if (top.status == kForkOk || top.status == kForkNoPages || top.status == kForkCopies) {
-    if ((long long)top.count + back - top.copies > f.n_pages) top.status = kForkBad;
-  }
+  if ((long long)top.count + back > f.n_pages) top.status = kForkBad;
   const bool ok = top.status == kForkOk;
-  int now[kPer];
   if (ok || f.tables_out != f.tables) {
+    int now[PER];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
       const Entry e = entry_of(a, c0, k);
       if (!e.in) continue;
-      const Goes g = a.goes[e.r];
-      const bool fills = ok && g.src >= 0 && e.c < g.fills;
-      now[k] = fills && g.copy >= 0 && e.c == g.fills - 1 ? g.dst : f.tables[(size_t)(fills ? g.src : e.r) * f.max_pages + e.c];
-    }
-    // copies name their pages by the old tables
-    if (ok)
-      for (int r = tid; r < n; r += kN) {
-        const Goes g = a.goes[r];
-        if (g.copy >= 0 && g.fills - 1 >= c0 && g.fills - 1 < c0 + a.columns) {
-          f.copies[3 * g.copy] = f.tables[(size_t)g.src * f.max_pages + g.fills - 1];
-          f.copies[3 * g.copy + 1] = g.dst;
-          f.copies[3 * g.copy + 2] = g.held - (g.fills - 1) * f.page_size;
-        }
+      const Goes g = goes(e.r);
+      const int fills = pages_for(g.held, a.per);
+      const bool in = ok && g.src >= 0 && e.c < fills;
+      now[k] = f.tables[(size_t)(in ? g.src : e.r) * f.max_pages + e.c];
+      if (in && g.copy >= 0 && e.c == fills - 1) {   // copies name their pages by the old tables
+        f.copies[3 * g.copy] = now[k];
+        f.copies[3 * g.copy + 1] = now[k] = f.ring[ring_place(top.head, g.copy, f.n_pages)];
+        f.copies[3 * g.copy + 2] = g.held - (fills - 1) * f.page_size;
       }
-    __syncthreads();
+    }
+    stage_sync<0>();
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
       const Entry e = entry_of(a, c0, k);
       if (e.in) f.tables_out[(size_t)e.r * f.max_pages + e.c] = now[k];
     }
   }
   if (ok) {
     const int tail = ring_place(top.head, top.count, f.n_pages);
-    for (int i = tid; i < a.counts[b]; i += kN) f.ring[ring_place(tail, before + i, f.n_pages)] = a.list[(size_t)c0 * n + i];
+    for (int i = tid; i < mine; i += kN) f.ring[ring_place(tail, before + i, f.n_pages)] = list[i];
   }
   if (b == 0) {
     for (int i = 3 * (ok ? top.copies : 0) + tid; i < 3 * f.max_copies; i += kN) f.copies[i] = -1;
-    for (int r = tid; r < n; r += kN) f.held_out[r] = ok ? a.goes[r].held : f.held[r];
+    for (int r = tid; r < n; r += kN) f.held_out[r] = ok ? goes(r).held : f.held[r];
     if (tid == 0) {
       f.ring_at_out[0] = ok ? ring_place(top.head, top.copies, f.n_pages) : top.head;
       f.ring_at_out[1] = ok ? top.count - top.copies + back : top.count;
@@ -241,26 +266,42 @@ __device__ __forceinline__ void fork_finish(const ForkArgs& a, int b, int before
   }
 }
 
-__global__ __launch_bounds__(kN) void fork_requests_kernel(ForkArgs a) { fork_requests(a); }
-
-__global__ __launch_bounds__(kN) void fork_columns_kernel(ForkArgs a) {
-  const int back = fork_columns(a, (int)blockIdx.x * a.columns);
-  if (threadIdx.x == 0) a.counts[blockIdx.x] = back;
+// Few entries: all of it in one block.
+constexpr int kOnePer = 2, kFewRequests = 1024;
+__global__ __launch_bounds__(kN) void fork_one_kernel(ForkArgs a) {
+  __shared__ ForkShared<kFewRequests> sh;
+  const ForkHead top = fork_requests(a, sh);
+  const int back = fork_columns<kOnePer>(a, sh, 0, a.list);
+  stage_sync<0>();
+  fork_finish<kOnePer>(a, top, 0, 0, back, back, a.list, [&](int r) { return goes_of(a, sh, r); });
 }
 
+// Many: a block some columns, then, when the pages that come back are counted, the tables.
+template <int PER>
+__global__ __launch_bounds__(kN) void fork_columns_kernel(ForkArgs a) {
+  __shared__ ForkShared<PER == 1 ? kFewRequests : kMostRequests> sh;
+  const ForkHead top = fork_requests(a, sh);
+  const int c0 = (int)blockIdx.x * a.columns, back = fork_columns<PER>(a, sh, c0, a.list + (size_t)c0 * a.f.n_req);
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = back;
+  if (blockIdx.x == 0) {   // (held may be changed by the next kernel while its other blocks need it)
+    for (int r = threadIdx.x; r < a.f.n_req; r += kN) a.goes[r] = goes_of(a, sh, r);
+    if (threadIdx.x == 0) *a.top = top;
+  }
+}
+
+template <int PER>
 __global__ __launch_bounds__(kN) void fork_finish_kernel(ForkArgs a) {
-  __shared__ int wave_s[kN / kWave], before_s;
-  int before = 0, back = 0;
+  __shared__ int wave_s[kN / kWave], before_s, mine_s;
+  int back = 0;
   for (int b0 = 0; b0 < a.blocks; b0 += kN) {
-    const int b = b0 + (int)threadIdx.x;
+    const int b = b0 + (int)threadIdx.x, c = b < a.blocks ? a.counts[b] : 0;
     int all;
-    const int at = block_scan(b < a.blocks ? a.counts[b] : 0, wave_s, &all);
-    if (b == (int)blockIdx.x) before_s = back + at;
+    const int at = block_scan(c, wave_s, &all);
+    if (b == (int)blockIdx.x) before_s = back + at, mine_s = c;
     back += all;
   }
   __syncthreads();
-  before = before_s;
-  fork_finish(a, (int)blockIdx.x, before, back);
+  fork_finish<PER>(a, *a.top, (int)blockIdx.x, before_s, mine_s, back, a.list + (size_t)blockIdx.x * a.columns * a.f.n_req, [&](int r) { return a.goes[r]; });
 }
 
 // ------------------------------------------------------------ copies
@@ -329,19 +370,27 @@ moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
   ForkArgs a;
   a.f = *f;
   a.per = make_divider((uint32_t)f->page_size);
-  a.columns = kEntries / (f->n_req ? f->n_req : 1);
+  const bool one = f->n_req <= kFewRequests && (long long)f->n_req * f->max_pages <= kOnePer * kN;
+  const int per = f->n_req <= 256 ? 1 : 4;   // entries of a thread: four columns a block at least, up to 1024 requests
+  a.columns = one ? f->max_pages : per * kN / f->n_req;
   if (a.columns > f->max_pages) a.columns = f->max_pages;
   a.blocks = (f->max_pages + a.columns - 1) / a.columns;
+  a.by_columns = make_divider((uint32_t)a.columns);
   a.top = (ForkHead*)f->work;
   a.goes = (Goes*)(a.top + 1);
   a.counts = (int*)(a.goes + f->n_req);
   a.list = a.counts + f->max_pages;
   a.mark = a.list + (size_t)f->n_req * f->max_pages;
-  hipLaunchKernelGGL(fork_requests_kernel, dim3(1), dim3(kN), 0, stream(), a);
+  if (one) {
+    hipLaunchKernelGGL(fork_one_kernel, dim3(1), dim3(kN), 0, stream(), a);
+    return check_hip(hipGetLastError(), "paged_fork launch");
+  }
+  const dim3 grid((unsigned)a.blocks);
+  if (per == 1) hipLaunchKernelGGL(fork_columns_kernel<1>, grid, dim3(kN), 0, stream(), a);
+  else hipLaunchKernelGGL(fork_columns_kernel<4>, grid, dim3(kN), 0, stream(), a);
   if ((st = check_hip(hipGetLastError(), "paged_fork launch"))) return st;
-  hipLaunchKernelGGL(fork_columns_kernel, dim3((unsigned)a.blocks), dim3(kN), 0, stream(), a);
-  if ((st = check_hip(hipGetLastError(), "paged_fork launch"))) return st;
-  hipLaunchKernelGGL(fork_finish_kernel, dim3((unsigned)a.blocks), dim3(kN), 0, stream(), a);
+  if (per == 1) hipLaunchKernelGGL(fork_finish_kernel<1>, grid, dim3(kN), 0, stream(), a);
+  else hipLaunchKernelGGL(fork_finish_kernel<4>, grid, dim3(kN), 0, stream(), a);
   return check_hip(hipGetLastError(), "paged_fork launch");
 }
 

@@ -45,7 +45,7 @@ def fork(parent, held, tables, ring, ring_at, page_size, max_copies):
             p = int(tables[r, c])
             if c < used[r] and good(p) and p not in stays and p not in back:
                 back.append(p)
-    if count + len(back) - len(copies) > n_pages:
+    if count + len(back) > n_pages:
         return dict(same, status=BAD)
     if len(copies) > max_copies:
         return dict(same, status=TOO_MANY)
