@@ -14,11 +14,14 @@
 // 64-bit whole number holds exactly: the logit's bits as an ordered whole
 // number above, the token's complement below.  Between rows by value * weight
 // in 64 bits, so that two candidates are told apart unless they are 1e-8 close
-// to each other; that is also how exact the sums are.  Sums: exp(x - m) with
-// x - m and its product with log2(e) carried in two floats each, so that a
-// term's only error is that of the hardware's exp2 (2^-23 of it, either way);
-// four terms are added in fp32, the rest in 64 bits.
+// to each other; that is also how exact the sums are.  Sums: exp(x) = 2^(x
+// log2(e)), the product carried in two floats and split into a whole number and
+// what is left, so that a term's error is that of the hardware's exp2 on
+// [-1/2, 1/2] (2^-23 of it, either way) and 2^-25; four terms are added in fp32,
+// the rest in 64 bits.
 #include <math.h>
+
+#include <type_traits>
 
 #include "moe_device.h"
 #include "moe_lib.h"
@@ -29,19 +32,18 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostBeams = kWave;          // a list is a lane a beam
 constexpr int kStep = 16 * kWave;          // logits of a wave's step
-constexpr int kBlocks = 2048;              // blocks that rows are cut into, about
+constexpr int kBlocks = 1024;              // blocks that rows are cut into, about
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // Sum of a part of a row: sum * exp(at); nothing there: 0 at -inf.
 struct Part {
-  double sum;
-  float at, pad;
+  double sum, at;
 };
 
-__device__ __forceinline__ double part_at(const Part& p, float at) {
-  return p.at == at || p.at == -INFINITY ? p.sum : p.sum * exp((double)p.at - (double)at);
+__device__ __forceinline__ double part_at(const Part& p, double at) {
+  return p.at == at || p.at == -(double)INFINITY ? p.sum : p.sum * exp(p.at - at);
 }
 
 struct SelectArgs {
@@ -59,6 +61,8 @@ __device__ __forceinline__ float unordered(uint32_t u) {
   return __uint_as_float(u >> 31 ? u & 0x7fffffffu : ~u);
 }
 constexpr uint32_t kOrderedNone = 0x007fffffu;   // of -inf, which is no candidate
+// The float before that of an ordered number (before 0 lies -0, which is 0).
+__device__ __forceinline__ float before(uint32_t u) { return unordered(u - (u == 0x80000000u ? 2 : 1)); }
 
 __device__ __forceinline__ uint64_t read_lane(uint64_t x, int l) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
@@ -92,8 +96,22 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t x, int n) {
 }
 
 __device__ __forceinline__ float wave_max(float x) {
+  auto with = [&](auto ctrl) {
+    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, false)));
+  };
+  with(std::integral_constant<int, 0xB1>{});    // quad_perm [1,0,3,2], [2,3,0,1]
+  with(std::integral_constant<int, 0x4E>{});
+  with(std::integral_constant<int, 0x141>{});   // row_half_mirror, row_mirror
+  with(std::integral_constant<int, 0x140>{});
+  auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
+__device__ __forceinline__ double wave_max(double x) {
 #pragma unroll
-  for (int c = 32; c; c /= 2) x = fmaxf(x, __shfl_xor(x, c));
+  for (int c = 32; c; c /= 2) x = fmax(x, __shfl_xor(x, c));
   return x;
 }
 
@@ -118,6 +136,16 @@ __device__ __forceinline__ float exp_from(float x, float m) {
   return fmaf(y, lo * 0.69314718055994530942f, y);
 }
 
+// exp(x) * 2^-at, for x under `floor` that of floor; at a whole number, |at| and the product's whole part below 2^21, the
+// result a normal number.  A NaN counts as floor.
+__device__ __forceinline__ float exp_at(float x, float floor, float at) {
+  constexpr float kWhole = 12582912.0f;   // 1.5 * 2^23: a sum with it is a whole number, whose last bits are its own
+  x = fmaxf(x, floor);
+  const float p = x * kLog2eHi, low = fmaf(x, kLog2eLo, fmaf(x, kLog2eHi, -p));
+  const float u = p + (kWhole - at), rest = p - (u - (kWhole - at));
+  return __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(rest + low)) + (__float_as_uint(u) << 23));
+}
+
 // A row has candidates from its logits: it is neither ended nor none at all.
 __device__ __forceinline__ bool usable(const moe_beam_select& a, int r) {
   const float w = a.weight ? a.weight[r] : 1.0f;
@@ -133,47 +161,91 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   const int first = (int)((long long)b * steps / s.blocks), end = (int)((long long)(b + 1) * steps / s.blocks);
   const float* x0 = a.logits + (size_t)row * a.ld;
   List list;
-  float at = -INFINITY, least = -INFINITY;   // at: as Part's; least: what a logit has to pass
+  float from = -INFINITY, power = 0.0f, floor = 0.0f;   // the logit that sums are taken from, its power of two
+  double at = -(double)INFINITY;                        // as Part's
+  bool far = false;                                     // logits too far from 0 for exp_at
+  float least = -INFINITY;                              // what a logit has to pass
   double sum = 0.0;
-  for (int step = first + wave; step < end; step += kWaves) {
+  // what the block's n_beam-th has to reach at least, as an ordered number: after the first step the least of the waves'
+  // share-th (share = n_beam / 4, rounded up), then any wave's n_beam-th
+  __shared__ uint32_t share_s[kWaves], least_s;
+  f32x4 next[4];
+  auto load = [&](int step) {
     const int v0 = step * kStep + 4 * lane;
-    float x[16];
     if ((step + 1) * kStep <= a.vocab) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 y = *(const f32x4u*)(x0 + v0 + j * 4 * kWave);
-        x[4 * j] = y[0], x[4 * j + 1] = y[1], x[4 * j + 2] = y[2], x[4 * j + 3] = y[3];
-      }
+      for (int j = 0; j < 4; ++j) next[j] = *(const f32x4u*)(x0 + v0 + j * 4 * kWave);
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int v = v0 + j / 4 * 4 * kWave + j % 4;
-        x[j] = v < a.vocab ? x0[v] : -INFINITY;
+        next[j / 4][j % 4] = v < a.vocab ? x0[v] : -INFINITY;
       }
     }
+  };
+  if (threadIdx.x == 0) least_s = 0;
+  if (first + wave < end) {
+    load(first + wave);
+  } else {   // a wave without a step comes to the first one's barrier all the same
+    if (lane == 0) share_s[wave] = 0;
+    __syncthreads();
+  }
+  for (int step = first + wave; step < end; step += kWaves) {
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = next[j / 4][j % 4];
+    if (step + kWaves < end) load(step + kWaves);
     float top = x[0];
 #pragma unroll
     for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-    // ---- the sum.  What it is taken from moves only when a term would leave fp32
+    // ---- the sum.  Its power of two moves only when a term would leave fp32; terms below 2^-100 of that count as 2^-100
     const float most = wave_max(top);
-    if (most > at + 40.0f) {
-      if (at > -INFINITY) sum *= exp((double)at - (double)most);
-      at = most;
+    if (!(most < INFINITY)) sum = NAN;
+    if (most > from + 40.0f && most < INFINITY) {
+      far = fabsf(most) > 1e6f;
+      power = rintf(most * kLog2eHi);
+      const double now = far ? (double)most : (double)power * 0.693147180559945309417;
+      if (from > -INFINITY) sum *= exp(at - now);
+      at = now, from = most, floor = (power - 100.0f) * 0.693147180559945309417f;
     }
-    if (at > -INFINITY) {
+    if (far) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        sum += (double)((exp_from(x[j], at) + exp_from(x[j + 1], at)) + (exp_from(x[j + 2], at) + exp_from(x[j + 3], at)));
+      for (int j = 0; j < 16; ++j) sum += (double)exp_from(x[j], from);
+    } else if (from > -INFINITY) {
+      float check = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        check += (x[j] + x[j + 1]) + (x[j + 2] + x[j + 3]);
+        sum += (double)((exp_at(x[j], floor, power) + exp_at(x[j + 1], floor, power)) + (exp_at(x[j + 2], floor, power) + exp_at(x[j + 3], floor, power)));
+      }
+      if (check != check) sum = NAN;   // one of them is (no infinity but -inf is left)
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum += x[j] == -INFINITY ? 0.0 : (double)NAN;
     }
-    // ---- the best.  Of the lanes' largest the K-th bounds the K-th of all from below
-    const uint32_t bound = max(nth_largest(top > least ? ordered(top) : 0u, K), kOrderedNone + 1);
-    if (!__any(top > least)) continue;
+    // ---- the best
+    if (step == first + wave) {
+      const uint32_t mine = nth_largest(top > -INFINITY ? ordered(top) : 0u, (K + kWaves - 1) / kWaves);
+      if (lane == 0) share_s[wave] = mine;
+      __syncthreads();
+      uint32_t all = share_s[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) all = min(all, share_s[w]);
+      least = all > kOrderedNone ? before(all) : -INFINITY;
+      if (lane == 0) atomicMax(&least_s, all);
+    } else {
+      const uint32_t others = least_s;
+      if (others > kOrderedNone) least = fmaxf(least, before(others));   // (as good as theirs may be an earlier token)
+    }
+    const uint64_t better = __ballot(top > least);
+    if (!better) continue;
+    // of the lanes' largest the K-th bounds the K-th of all from below
+    uint32_t bound = kOrderedNone + 1;
+    if (__popcll(better) > K) bound = max(bound, nth_largest(top > least ? ordered(top) : 0u, K));
+    const float pass = fmaxf(before(bound), least);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      uint64_t who = __ballot(ordered(x[j]) >= bound && x[j] > least);
+      uint64_t who = __ballot(x[j] > pass);
       while (who) {
         const int l = __builtin_ctzll(who);
         who &= who - 1;
@@ -182,7 +254,10 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
         if (k > list.last) list.insert(k, K);
       }
     }
-    if (list.last) least = unordered((uint32_t)(list.last >> 32));
+    if (list.last) {
+      least = fmaxf(least, unordered((uint32_t)(list.last >> 32)));
+      if (lane == 0) atomicMax(&least_s, (uint32_t)(list.last >> 32));
+    }
   }
   // ---- the waves' lists and sums joined
   __shared__ uint64_t key_s[kWaves][kMostBeams], best_s[kMostBeams];
@@ -190,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   const double all = wave_sum(sum);
   key_s[wave][lane] = lane < K ? list.key : 0;
   if (wave == 0) best_s[lane] = 0;
-  if (lane == 0) part_s[wave] = Part{all, at, 0.0f};
+  if (lane == 0) part_s[wave] = Part{all, at};
   __syncthreads();
   const int mine = threadIdx.x % kWave;
   if (mine < K && key_s[wave][mine]) {
@@ -204,11 +279,11 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   __syncthreads();
   if ((int)threadIdx.x < K) s.keys[((size_t)row * K + threadIdx.x) * s.blocks + b] = best_s[threadIdx.x];
   if (threadIdx.x == 0) {
-    float most = part_s[0].at;
-    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, part_s[w].at);
+    double most = part_s[0].at;
+    for (int w = 1; w < kWaves; ++w) most = fmax(most, part_s[w].at);
     double total = 0.0;
     for (int w = 0; w < kWaves; ++w) total += part_at(part_s[w], most);
-    s.parts[(size_t)row * s.blocks + b] = Part{total, most, 0.0f};
+    s.parts[(size_t)row * s.blocks + b] = Part{total, most};
   }
 }
 
@@ -233,14 +308,14 @@ __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
       list.key = lane == 0 ? 1 : 0;
     } else if (use) {
       const Part* p = s.parts + (size_t)row * s.blocks;
-      float most = -INFINITY;
-      for (int c = lane; c < s.blocks; c += kWave) most = fmaxf(most, p[c].at);
+      double most = -(double)INFINITY;
+      for (int c = lane; c < s.blocks; c += kWave) most = fmax(most, p[c].at);
       most = wave_max(most);
       double sum = 0.0;
       for (int c = lane; c < s.blocks; c += kWave) sum += part_at(p[c], most);
       sum = wave_sum(sum);
       if (sum > 0.0 && sum < (double)INFINITY) {   // (a NaN or +inf among the logits makes it NaN)
-        base = (double)score - ((double)most + log(sum));
+        base = (double)score - (most + log(sum));
         const uint64_t* keys = s.keys + (size_t)row * K * s.blocks;
         for (int c0 = 0; c0 < K * s.blocks; c0 += kWave) {
           const uint64_t k = c0 + lane < K * s.blocks ? keys[c0 + lane] : 0;
