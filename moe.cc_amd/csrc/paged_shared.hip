@@ -185,18 +185,139 @@ __device__ __forceinline__ int units_in_all(int positions) { return (positions +
 
 // One block: the groups' prefixes, and the items.  Prefix tiles' units (128 positions) and rows' own are each cut so that
 // their items are about as many as are resident at once: pieces of ceil(all units / slots), at least one an item, so no
-// more items than `slots` and one for each tile or row.
+// more items than `slots` and one for each tile or row.  ONE: a thread a group and a row (at most kN of each), whose numbers
+// stay in its registers and LDS; else they go around through the plan, kN at a time.  Latency bounds it: 64 rows ~.
+struct PlanShared {
+  int wave[kN / kWave];
+  unsigned long long units, own;
+  int least[kN], lead[kN], live[kN];      // ONE: of the groups
+  int part0[kN], pieces[kN], prefix[kN];
+  int own0[kN];                           // ONE: of the rows
+};
+
+// The last of n ascending numbers, the first of which is 0, that is at most i.
+__device__ __forceinline__ int owner_of(const int* at, int n, int i) {
+  int lo = 0;
+  for (int hi = n; hi - lo > 1;) {
+    const int mid = (lo + hi) / 2;
+    if (at[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int piece_of(unsigned long long all, int slots) {
+  const unsigned long long n = (all + slots - 1) / slots;
+  return n ? (int)(n < 0x40000000 ? n : 0x40000000) : 1;
+}
+
+// A group of rows row0 .. row0 + rows - 1 with `live` to count and `least` leading pages in common.  One row alone reads its
+// positions as its own.
+__device__ __forceinline__ GroupPlan group_plan(const ShareArgs& a, int row0, int rows, int req, int live, int least) {
+  GroupPlan p = {row0, rows, req, 0, 0, 0, 0, 0};
+  if (live > 1 && least > 0) {
+    p.prefix = least * a.s.page_size;
+    p.tiles = (int)(((long long)rows * a.cut.group + a.cut.columns - 1) / a.cut.columns);
+    p.units = units_in_all(p.prefix);
+  }
+  return p;
+}
+
+// Item i of a group's.
+__device__ __forceinline__ Item prefix_item(const ShareArgs& a, const GroupPlan& p, int i) {
+  const int tile = i / p.pieces, j = i - tile * p.pieces;
+  Item x = {p.row0, tile * a.cut.columns, min(a.cut.columns, p.rows * a.cut.group - tile * a.cut.columns), p.req, 0, 0, p.part0 + i, 0};
+  x.begin = (int)((long long)p.units * j / p.pieces) * kUnit;
+  x.end = min((int)((long long)p.units * (j + 1) / p.pieces) * kUnit, p.prefix);
+  return x;
+}
+
+// Item i of row r's own positions, `own` from `prefix` on, in `owns` pieces.
+__device__ __forceinline__ Item own_item(const ShareArgs& a, int r, int req, int prefix, int own, int owns, int own0, int i, bool done) {
+  const int tile = i / owns, j = i - tile * owns, units = units_in_all(own);
+  Item x = {r, tile * 16, min(16, a.cut.group - tile * 16), req, 0, 0, own0 + i, done};
+  x.begin = prefix + (int)((long long)units * j / owns) * kUnit;
+  x.end = prefix + min((int)((long long)units * (j + 1) / owns) * kUnit, own);
+  return x;
+}
+
+__device__ __forceinline__ RowPlan row_plan(int len, int group, const GroupPlan& p, int r, int own0, int owns) {
+  RowPlan x = {kJoin, group, r, 0, 0, own0, owns, 0};
+  if (group >= 0) x.row0 = p.row0, x.part0 = p.part0, x.pieces = p.pieces;
+  if (len <= 0) x.state = len == kPadding ? kLeave : len == kOutside ? kNan : kZero;
+  else if (group < 0 && owns == 1) x.state = kDone;
+  return x;
+}
+
+template <bool ONE>
 __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
   const moe_paged_share& s = a.s;
   const ShareCut& cut = a.cut;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, positions = s.max_pages * s.page_size;
-  __shared__ int wave_s[kN / kWave];
-  __shared__ unsigned long long units_s, own_s;
-  if (tid == 0) units_s = own_s = 0;
+  __shared__ PlanShared sh;
+  auto request = [&](int r) { return s.req ? s.req[r] : r; };
+  if (tid == 0) sh.units = sh.own = 0;
+  if constexpr (ONE) {
+    const bool is_group = tid < s.n_groups, is_row = tid < s.T;
+    int row0 = 0, row1 = 0, common = kNotLive, group = -1, req = 0, len = 0;
+    if (is_group) row0 = s.first[tid], row1 = s.first[tid + 1];
+    if (is_row) {
+      common = a.p.common[tid];
+      group = a.p.rows[tid].group;
+      req = request(tid);
+      len = row_length(req, s.pos[tid], s.n_req, positions);
+    }
+    sh.least[tid] = sh.lead[tid] = kNotLive;
+    sh.live[tid] = 0;
+    const bool bad = __syncthreads_or(is_group && (row0 < 0 || row0 > row1 || row1 > s.T));
+    if (bad) group = -1, row1 = row0;
+    if (common != kNotLive && group >= 0) {
+      atomicMin(&sh.least[group], common);
+      atomicMin(&sh.lead[group], tid);
+      atomicAdd(&sh.live[group], 1);
+    }
+    __syncthreads();
+    GroupPlan p = {};
+    if (is_group) {
+      const int least = sh.least[tid];
+      s.prefix[tid] = least == kNotLive ? 0 : least * s.page_size;
+      p = group_plan(a, row0, row1 - row0, least == kNotLive ? 0 : request(sh.lead[tid]), sh.live[tid], least == kNotLive ? 0 : least);
+      if (p.tiles) atomicAdd(&sh.units, (unsigned long long)p.tiles * p.units);
+    }
+    __syncthreads();
+    const int per = piece_of(sh.units, cut.slots);
+    p.pieces = (p.units + per - 1) / per;
+    int all;
+    p.part0 = block_scan(p.tiles * p.pieces, sh.wave, &all);
+    sh.part0[tid] = p.part0, sh.pieces[tid] = p.pieces, sh.prefix[tid] = p.prefix;
+    if (is_group) a.p.groups[tid] = p;
+    __syncthreads();
+    // ---- the rows' own
+    const int prefix = group >= 0 && len > 0 ? sh.prefix[group] : 0, own = len > 0 ? len - prefix : 0, units = units_in_all(own);
+    if (!prefix) group = -1;
+    if (units) atomicAdd(&sh.own, (unsigned long long)units * cut.own_tiles);
+    for (int i = tid; i < all; i += kN) {
+      const int g = owner_of(sh.part0, s.n_groups, i);
+      a.p.prefix[i] = prefix_item(a, a.p.groups[g], i - sh.part0[g]);
+    }
+    if (tid == 0) a.p.head->prefix_items = all;
+    __syncthreads();
+    const int per_own = piece_of(sh.own, cut.own_slots), owns = (units + per_own - 1) / per_own;
+    int owned;
+    const int own0 = block_scan(owns * cut.own_tiles, sh.wave, &owned);
+    if (is_row) {
+      GroupPlan of = {};
+      if (group >= 0) of = a.p.groups[group];
+      const RowPlan x = row_plan(len, group, of, tid, own0, owns);
+      a.p.rows[tid] = x;
+      for (int i = 0; i < owns * cut.own_tiles; ++i) a.p.own[own0 + i] = own_item(a, tid, req, prefix, own, owns, own0, i, x.state == kDone);
+    }
+    if (tid == 0) a.p.head->own_items = owned;
+    return;
+  }
   bool bad = false;
   for (int g = tid; g < s.n_groups; g += kN) bad |= s.first[g] < 0 || s.first[g] > s.first[g + 1] || s.first[g + 1] > s.T;
   bad = __syncthreads_or(bad);
-  auto request = [&](int r) { return s.req ? s.req[r] : r; };
   // ---- the groups: a wave each
   for (int g = wave; g < s.n_groups; g += kN / kWave) {
     const int r0 = s.first[g], r1 = bad ? r0 : s.first[g + 1];
@@ -213,26 +334,14 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
       live += __shfl_xor(live, c);
     }
     if (lane == 0) {
-      const int prefix = least == kNotLive ? 0 : least * s.page_size;
-      s.prefix[g] = prefix;
-      GroupPlan p = {r0, r1 - r0, 0, 0, 0, 0, 0, 0};
-      if (live > 1 && prefix > 0) {   // one row alone reads its positions as its own
-        p.req = request(lead);
-        p.prefix = prefix;
-        p.tiles = (int)(((long long)p.rows * cut.group + cut.columns - 1) / cut.columns);
-        p.units = units_in_all(prefix);
-        atomicAdd(&units_s, (unsigned long long)p.tiles * p.units);
-      }
+      s.prefix[g] = least == kNotLive ? 0 : least * s.page_size;
+      const GroupPlan p = group_plan(a, r0, r1 - r0, least == kNotLive ? 0 : request(lead), live, least == kNotLive ? 0 : least);
+      if (p.tiles) atomicAdd(&sh.units, (unsigned long long)p.tiles * p.units);
       a.p.groups[g] = p;
     }
   }
-  __threadfence_block();
   __syncthreads();
-  auto piece = [&](unsigned long long all, int slots) {
-    const unsigned long long n = (all + slots - 1) / slots;
-    return n ? (int)(n < 0x40000000 ? n : 0x40000000) : 1;
-  };
-  const int per = piece(units_s, cut.slots);
+  const int per = piece_of(sh.units, cut.slots);
   int done = 0;
   for (int g0 = 0; g0 < s.n_groups; g0 += kN) {
     const int g = g0 + tid;
@@ -242,22 +351,15 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
       tiles = a.p.groups[g].tiles;
     }
     int all;
-    const int at = done + block_scan(tiles * pieces, wave_s, &all);
+    const int at = done + block_scan(tiles * pieces, sh.wave, &all);
     if (g < s.n_groups) a.p.groups[g].part0 = at, a.p.groups[g].pieces = pieces;
     done += all;
   }
   if (tid == 0) a.p.head->prefix_items = done;
-  __threadfence_block();
   __syncthreads();
   for (int g = wave; g < s.n_groups; g += kN / kWave) {
     const GroupPlan p = a.p.groups[g];
-    for (int i = lane; i < p.tiles * p.pieces; i += kWave) {
-      const int tile = i / p.pieces, j = i - tile * p.pieces;
-      Item x = {p.row0, tile * cut.columns, min(cut.columns, p.rows * cut.group - tile * cut.columns), p.req, 0, 0, p.part0 + i, 0};
-      x.begin = (int)((long long)p.units * j / p.pieces) * kUnit;
-      x.end = min((int)((long long)p.units * (j + 1) / p.pieces) * kUnit, p.prefix);
-      a.p.prefix[p.part0 + i] = x;
-    }
+    for (int i = lane; i < p.tiles * p.pieces; i += kWave) a.p.prefix[p.part0 + i] = prefix_item(a, p, i);
   }
   // ---- the rows: a thread each
   auto own_of = [&](int r, int* len, int* group) {
@@ -271,9 +373,9 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
     int len, group;
     mine += (unsigned long long)units_in_all(own_of(r, &len, &group)) * cut.own_tiles;
   }
-  if (mine) atomicAdd(&own_s, mine);
+  if (mine) atomicAdd(&sh.own, mine);
   __syncthreads();
-  const int per_own = piece(own_s, cut.own_slots);
+  const int per_own = piece_of(sh.own, cut.own_slots);
   done = 0;
   for (int r0 = 0; r0 < s.T; r0 += kN) {
     const int r = r0 + tid;
@@ -283,22 +385,13 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
       owns = (units_in_all(own) + per_own - 1) / per_own;
     }
     int all;
-    const int at = done + block_scan(owns * cut.own_tiles, wave_s, &all);
+    const int at = done + block_scan(owns * cut.own_tiles, sh.wave, &all);
     if (r < s.T) {
-      RowPlan p = {kJoin, group, r, 0, 0, at, owns, 0};
-      const int prefix = group >= 0 ? a.p.groups[group].prefix : 0, units = units_in_all(own);
-      if (group >= 0) p.row0 = a.p.groups[group].row0, p.part0 = a.p.groups[group].part0, p.pieces = a.p.groups[group].pieces;
-      if (len <= 0) p.state = len == kPadding ? kLeave : len == kOutside ? kNan : kZero;
-      else if (group < 0 && owns == 1) p.state = kDone;
-      a.p.rows[r] = p;
-      for (int tile = 0; tile < cut.own_tiles; ++tile)
-        for (int j = 0; j < owns; ++j) {
-          const int i = at + tile * owns + j;
-          Item x = {r, tile * 16, min(16, cut.group - tile * 16), request(r), 0, 0, i, p.state == kDone};
-          x.begin = prefix + (int)((long long)units * j / owns) * kUnit;
-          x.end = prefix + min((int)((long long)units * (j + 1) / owns) * kUnit, own);
-          a.p.own[i] = x;
-        }
+      GroupPlan of = {};
+      if (group >= 0) of = a.p.groups[group];
+      const RowPlan x = row_plan(len, group, of, r, at, owns);
+      a.p.rows[r] = x;
+      for (int i = 0; i < owns * cut.own_tiles; ++i) a.p.own[at + i] = own_item(a, r, request(r), of.prefix, own, owns, at, i, x.state == kDone);
     }
     done += all;
   }
@@ -1175,7 +1268,8 @@ moe_status moe_paged_share_dev(const moe_paged_share* s) {
     hipLaunchKernelGGL(share_rows_kernel, dim3((unsigned)(s->T + 3) / 4), dim3(256), 0, stream(), a);
     if ((st = check_hip(hipGetLastError(), "paged_share launch"))) return st;
   }
-  hipLaunchKernelGGL(share_plan_kernel, dim3(1), dim3(kN), 0, stream(), a);
+  if (s->T <= kN && s->n_groups <= kN) hipLaunchKernelGGL(share_plan_kernel<true>, dim3(1), dim3(kN), 0, stream(), a);
+  else hipLaunchKernelGGL(share_plan_kernel<false>, dim3(1), dim3(kN), 0, stream(), a);
   return check_hip(hipGetLastError(), "paged_share launch");
 }
 

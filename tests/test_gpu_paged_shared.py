@@ -263,3 +263,13 @@ def test_share_wide(moehip):
     s = M.PagedShare(T, T, width, ps, 32, 4, 128, d[0].ptr, d[1].ptr, d[2].ptr, len(sizes), d[3].ptr, d[4].ptr, d[5].ptr, need)
     M.check(L.moe_paged_share_dev(ctypes.byref(s)))
     np.testing.assert_array_equal(d[4].download((len(sizes),), np.int32), B.share(req, pos, tables, first, ps))
+
+
+@pytest.mark.parametrize("rows,groups", [(1500, 40), (1100, 1099), (400, 2000)])
+def test_many_rows_and_groups(moehip, rows, groups):
+    """More of either than the plan's block has threads."""
+    rng = np.random.default_rng(rows)
+    cuts = np.sort(rng.integers(0, rows + 1, groups - 1))
+    first = np.concatenate([[0], cuts, [rows]]).astype(np.int32)
+    sizes = [(int(b - a), 16 * int(rng.integers(0, 4)), (0, 20)) for a, b in zip(first, first[1:]) if b > a]
+    Batch(moehip, "bf16", sizes, 2, 1, 64, 16, seed=14, first=first).run()
