@@ -160,6 +160,7 @@ __global__ __launch_bounds__(256) void share_rows_kernel(ShareArgs a) {
 }
 
 // Sum over the block's threads up to and without this one, and of all.
+template <int N>
 __device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int x = v;
@@ -171,7 +172,8 @@ __device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
   if (lane == kWave - 1) wave_s[wave] = x;
   __syncthreads();
   int before = 0, all = 0;
-  for (int w = 0; w < kN / kWave; ++w) {
+#pragma unroll
+  for (int w = 0; w < N / kWave; ++w) {
     const int y = wave_s[w];
     if (w < wave) before += y;
     all += y;
@@ -185,14 +187,15 @@ __device__ __forceinline__ int units_in_all(int positions) { return (positions +
 
 // One block: the groups' prefixes, and the items.  Prefix tiles' units (128 positions) and rows' own are each cut so that
 // their items are about as many as are resident at once: pieces of ceil(all units / slots), at least one an item, so no
-// more items than `slots` and one for each tile or row.  ONE: a thread a group and a row (at most kN of each), whose numbers
-// stay in its registers and LDS; else they go around through the plan, kN at a time.  Latency bounds it: 64 rows ~.
+// more items than `slots` and one for each tile or row.  ONE: a thread a group and a row (at most N of each), whose numbers
+// stay in its registers and LDS; else they go around through the plan, N at a time.  Latency bounds it.
+template <int N>
 struct PlanShared {
-  int wave[kN / kWave];
+  int wave[N / kWave];
   unsigned long long units, own;
-  int least[kN], lead[kN], live[kN];      // ONE: of the groups
-  int part0[kN], pieces[kN], prefix[kN];
-  int own0[kN];                           // ONE: of the rows
+  int least[N], lead[N], live[N];      // ONE: of the groups
+  int part0[N], pieces[N], prefix[N];
+  int own0[N];                           // ONE: of the rows
 };
 
 // The last of n ascending numbers, the first of which is 0, that is at most i.
@@ -206,9 +209,16 @@ __device__ __forceinline__ int owner_of(const int* at, int n, int i) {
   return lo;
 }
 
+// ceil(all / slots), at least 1 (whole numbers below 2^53: the quotient is not rounded past one)
 __device__ __forceinline__ int piece_of(unsigned long long all, int slots) {
-  const unsigned long long n = (all + slots - 1) / slots;
-  return n ? (int)(n < 0x40000000 ? n : 0x40000000) : 1;
+  const double n = floor((double)(all + (unsigned long long)(slots - 1)) / (double)slots);
+  return (int)fmin(fmax(n, 1.0), 1073741824.0);
+}
+
+// Units before piece j of `pieces` even ones.
+__device__ __forceinline__ int units_before(int units, int pieces, int j) {
+  const int each = units / pieces;
+  return each * j + min(j, units - each * pieces);
 }
 
 // A group of rows row0 .. row0 + rows - 1 with `live` to count and `least` leading pages in common.  One row alone reads its
@@ -217,7 +227,7 @@ __device__ __forceinline__ GroupPlan group_plan(const ShareArgs& a, int row0, in
   GroupPlan p = {row0, rows, req, 0, 0, 0, 0, 0};
   if (live > 1 && least > 0) {
     p.prefix = least * a.s.page_size;
-    p.tiles = (int)(((long long)rows * a.cut.group + a.cut.columns - 1) / a.cut.columns);
+    p.tiles = (int)(((long long)rows * a.cut.group + a.cut.columns - 1) >> a.cut.shift);
     p.units = units_in_all(p.prefix);
   }
   return p;
@@ -227,8 +237,8 @@ __device__ __forceinline__ GroupPlan group_plan(const ShareArgs& a, int row0, in
 __device__ __forceinline__ Item prefix_item(const ShareArgs& a, const GroupPlan& p, int i) {
   const int tile = i / p.pieces, j = i - tile * p.pieces;
   Item x = {p.row0, tile * a.cut.columns, min(a.cut.columns, p.rows * a.cut.group - tile * a.cut.columns), p.req, 0, 0, p.part0 + i, 0};
-  x.begin = (int)((long long)p.units * j / p.pieces) * kUnit;
-  x.end = min((int)((long long)p.units * (j + 1) / p.pieces) * kUnit, p.prefix);
+  x.begin = units_before(p.units, p.pieces, j) * kUnit;
+  x.end = min(units_before(p.units, p.pieces, j + 1) * kUnit, p.prefix);
   return x;
 }
 
@@ -236,8 +246,8 @@ __device__ __forceinline__ Item prefix_item(const ShareArgs& a, const GroupPlan&
 __device__ __forceinline__ Item own_item(const ShareArgs& a, int r, int req, int prefix, int own, int owns, int own0, int i, bool done) {
   const int tile = i / owns, j = i - tile * owns, units = units_in_all(own);
   Item x = {r, tile * 16, min(16, a.cut.group - tile * 16), req, 0, 0, own0 + i, done};
-  x.begin = prefix + (int)((long long)units * j / owns) * kUnit;
-  x.end = prefix + min((int)((long long)units * (j + 1) / owns) * kUnit, own);
+  x.begin = prefix + units_before(units, owns, j) * kUnit;
+  x.end = prefix + min(units_before(units, owns, j + 1) * kUnit, own);
   return x;
 }
 
@@ -249,12 +259,12 @@ __device__ __forceinline__ RowPlan row_plan(int len, int group, const GroupPlan&
   return x;
 }
 
-template <bool ONE>
-__global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
+template <int N, bool ONE>
+__global__ __launch_bounds__(N) void share_plan_kernel(ShareArgs a) {
   const moe_paged_share& s = a.s;
   const ShareCut& cut = a.cut;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, positions = s.max_pages * s.page_size;
-  __shared__ PlanShared sh;
+  __shared__ PlanShared<N> sh;
   auto request = [&](int r) { return s.req ? s.req[r] : r; };
   if (tid == 0) sh.units = sh.own = 0;
   if constexpr (ONE) {
@@ -288,7 +298,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
     const int per = piece_of(sh.units, cut.slots);
     p.pieces = (p.units + per - 1) / per;
     int all;
-    p.part0 = block_scan(p.tiles * p.pieces, sh.wave, &all);
+    p.part0 = block_scan<N>(p.tiles * p.pieces, sh.wave, &all);
     sh.part0[tid] = p.part0, sh.pieces[tid] = p.pieces, sh.prefix[tid] = p.prefix;
     if (is_group) a.p.groups[tid] = p;
     __syncthreads();
@@ -296,7 +306,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
     const int prefix = group >= 0 && len > 0 ? sh.prefix[group] : 0, own = len > 0 ? len - prefix : 0, units = units_in_all(own);
     if (!prefix) group = -1;
     if (units) atomicAdd(&sh.own, (unsigned long long)units * cut.own_tiles);
-    for (int i = tid; i < all; i += kN) {
+    for (int i = tid; i < all; i += N) {
       const int g = owner_of(sh.part0, s.n_groups, i);
       a.p.prefix[i] = prefix_item(a, a.p.groups[g], i - sh.part0[g]);
     }
@@ -304,7 +314,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
     __syncthreads();
     const int per_own = piece_of(sh.own, cut.own_slots), owns = (units + per_own - 1) / per_own;
     int owned;
-    const int own0 = block_scan(owns * cut.own_tiles, sh.wave, &owned);
+    const int own0 = block_scan<N>(owns * cut.own_tiles, sh.wave, &owned);
     if (is_row) {
       GroupPlan of = {};
       if (group >= 0) of = a.p.groups[group];
@@ -316,10 +326,10 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
     return;
   }
   bool bad = false;
-  for (int g = tid; g < s.n_groups; g += kN) bad |= s.first[g] < 0 || s.first[g] > s.first[g + 1] || s.first[g + 1] > s.T;
+  for (int g = tid; g < s.n_groups; g += N) bad |= s.first[g] < 0 || s.first[g] > s.first[g + 1] || s.first[g + 1] > s.T;
   bad = __syncthreads_or(bad);
   // ---- the groups: a wave each
-  for (int g = wave; g < s.n_groups; g += kN / kWave) {
+  for (int g = wave; g < s.n_groups; g += N / kWave) {
     const int r0 = s.first[g], r1 = bad ? r0 : s.first[g + 1];
     int least = kNotLive, live = 0, lead = kNotLive;
     for (int r = r0 + lane; r < r1; r += kWave) {
@@ -343,7 +353,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
   __syncthreads();
   const int per = piece_of(sh.units, cut.slots);
   int done = 0;
-  for (int g0 = 0; g0 < s.n_groups; g0 += kN) {
+  for (int g0 = 0; g0 < s.n_groups; g0 += N) {
     const int g = g0 + tid;
     int pieces = 0, tiles = 0;
     if (g < s.n_groups) {
@@ -351,13 +361,13 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
       tiles = a.p.groups[g].tiles;
     }
     int all;
-    const int at = done + block_scan(tiles * pieces, sh.wave, &all);
+    const int at = done + block_scan<N>(tiles * pieces, sh.wave, &all);
     if (g < s.n_groups) a.p.groups[g].part0 = at, a.p.groups[g].pieces = pieces;
     done += all;
   }
   if (tid == 0) a.p.head->prefix_items = done;
   __syncthreads();
-  for (int g = wave; g < s.n_groups; g += kN / kWave) {
+  for (int g = wave; g < s.n_groups; g += N / kWave) {
     const GroupPlan p = a.p.groups[g];
     for (int i = lane; i < p.tiles * p.pieces; i += kWave) a.p.prefix[p.part0 + i] = prefix_item(a, p, i);
   }
@@ -369,7 +379,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
     return *len > 0 ? *len - (*group >= 0 ? a.p.groups[*group].prefix : 0) : 0;
   };
   unsigned long long mine = 0;
-  for (int r = tid; r < s.T; r += kN) {
+  for (int r = tid; r < s.T; r += N) {
     int len, group;
     mine += (unsigned long long)units_in_all(own_of(r, &len, &group)) * cut.own_tiles;
   }
@@ -377,7 +387,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
   __syncthreads();
   const int per_own = piece_of(sh.own, cut.own_slots);
   done = 0;
-  for (int r0 = 0; r0 < s.T; r0 += kN) {
+  for (int r0 = 0; r0 < s.T; r0 += N) {
     const int r = r0 + tid;
     int len = 0, group = -1, own = 0, owns = 0;
     if (r < s.T) {
@@ -385,7 +395,7 @@ __global__ __launch_bounds__(kN) void share_plan_kernel(ShareArgs a) {
       owns = (units_in_all(own) + per_own - 1) / per_own;
     }
     int all;
-    const int at = done + block_scan(owns * cut.own_tiles, sh.wave, &all);
+    const int at = done + block_scan<N>(owns * cut.own_tiles, sh.wave, &all);
     if (r < s.T) {
       GroupPlan of = {};
       if (group >= 0) of = a.p.groups[group];
@@ -1268,8 +1278,10 @@ moe_status moe_paged_share_dev(const moe_paged_share* s) {
     hipLaunchKernelGGL(share_rows_kernel, dim3((unsigned)(s->T + 3) / 4), dim3(256), 0, stream(), a);
     if ((st = check_hip(hipGetLastError(), "paged_share launch"))) return st;
   }
-  if (s->T <= kN && s->n_groups <= kN) hipLaunchKernelGGL(share_plan_kernel<true>, dim3(1), dim3(kN), 0, stream(), a);
-  else hipLaunchKernelGGL(share_plan_kernel<false>, dim3(1), dim3(kN), 0, stream(), a);
+  const int most = s->T > s->n_groups ? s->T : s->n_groups;
+  if (most <= 256) hipLaunchKernelGGL((share_plan_kernel<256, true>), dim3(1), dim3(256), 0, stream(), a);
+  else if (most <= kN) hipLaunchKernelGGL((share_plan_kernel<kN, true>), dim3(1), dim3(kN), 0, stream(), a);
+  else hipLaunchKernelGGL((share_plan_kernel<kN, false>), dim3(1), dim3(kN), 0, stream(), a);
   return check_hip(hipGetLastError(), "paged_share launch");
 }
 
