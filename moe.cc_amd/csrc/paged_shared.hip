@@ -1182,7 +1182,8 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
 #pragma unroll
       for (int x = 0; x < U; ++x) {
         const int i = i0 + row + x * rows;
-        acc += y[x] * (row < rows && i < n ? __shfl(by, i) : 0.0f);
+        const float f = __shfl(by, i);   // (with every lane there)
+        acc += y[x] * (row < rows && i < n ? f : 0.0f);
       }
     } else {
 #pragma unroll

@@ -135,6 +135,15 @@ def test_attention(moehip, kind, nq, nkv, hd, ps, order, groups):
     b.run(ldq=nq * hd + 5 if groups == 2 else None, ldo=nq * hd + 3 if groups == 3 else None)
 
 
+@pytest.mark.parametrize("kind", list(C.TYPES))
+@pytest.mark.parametrize("nq,nkv,hd,groups", [(4, 1, 64, [(6, 6000, (1, 300)), (2, 3000, (900, 1000))]), (8, 2, 80, [(17, 4500, (0, 140))]), (2, 1, 256, [(33, 2700, (1, 600))]),
+                                              (8, 8, 128, [(1, 9000, (5, 6))]), (32, 2, 16, [(3, 12000, (1, 2000))])])
+def test_many_parts(moehip, kind, nq, nkv, hd, groups):
+    """Prefixes and rows of their own long enough that a head's sums come in tens of parts, up to more than a wave's lanes."""
+    print("shared attention, many parts", kind, nq, nkv, hd, groups, flush=True)
+    Batch(moehip, kind, groups, nq, nkv, hd, 16, "head", seed=hd + 1).run()
+
+
 def test_rows_of_no_request_and_empty_ones(moehip):
     """In a group, at its start, and a whole group of them; rows outside every group."""
     b = Batch(moehip, "bf16", [(6, 96, (1, 40)), (3, 64, (1, 20)), (4, 48, (2, 9))], 8, 2, 64, 16, seed=2, first=[1, 6, 9, 12])
