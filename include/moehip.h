@@ -650,6 +650,25 @@ moe_status moe_paged_attn_shared_dev(const moe_paged_attn* a, const moe_pages* p
 moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
                                 const int32_t* ids, float* logits, int32_t* next);
 
+/* One step of beam searches, from the last step's logits to the next one's,
+ * without a number coming to the host: moe_beam_select_dev(select), then
+ * moe_paged_fork_dev(fork) and its copies in layers[0 .. n_layers - 1], then
+ * moe_paged_plan_dev(plan) for one token of every beam that goes on, the layers
+ * with moe_paged_attn_shared_dev (a group's beams share what they hold in the
+ * same pages), and the head: logits [n_req x vocab] of each beam's token (zeros'
+ * for one that has ended), which may be select->logits.  Beam b of search g is
+ * request g * n_beam + b.  The three descriptions hand their arrays on to each
+ * other: fork->parent is select->parent, plan->fresh select->fresh, plan->held,
+ * ring_at, ring and tables are fork->held_out, ring_at_out, ring and tables_out;
+ * the layers' pages are laid out alike.  A search starts with
+ * moe_model_step_paged on its prompts, each as its group's first request, and
+ * scores of 0 for those, -inf for the others; it ends with a last
+ * moe_beam_select_dev.  fork->status or plan->status other than 0: the step's
+ * logits are worthless, the search has lost its place.  Checks, scratch and
+ * captures as moe_model_step_paged's. */
+moe_status moe_model_step_beams(moe_model* m, const moe_beam_select* select, const moe_paged_fork* fork,
+                                const moe_paged_plan* plan, const moe_pages* layers, float* logits);
+
 /* Name of the kernel variant the GEMV entry points use for a shape. */
 const char* moe_gemv_variant(int dtype, int M, int N, int K);
 

@@ -25,6 +25,7 @@
 
 #include "moe_device.h"
 #include "moe_lib.h"
+#include "paged_attn.h"
 
 namespace moe {
 namespace {
@@ -393,9 +394,27 @@ int blocks_for(long long rows, int vocab) {
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-constexpr long long kMostRows = 65535;   // a launch's second dimension
+constexpr long long kMostSelected = 65535;   // rows: a launch's second dimension
 
 }  // namespace
+
+moe_status check_select(const moe_beam_select* a) {
+  if (!a) return set_error(MOE_ERR_ARG, "beam_select: null argument");
+  if (a->n_groups < 0 || a->n_beam < 1 || a->vocab < 1)
+    return set_error(MOE_ERR_ARG, "beam_select: %d groups of %d beams, %d tokens", a->n_groups, a->n_beam, a->vocab);
+  if (a->n_beam > kMostBeams || (long long)a->n_groups * a->n_beam > kMostSelected || a->vocab > (1 << 30))
+    return set_error(MOE_ERR_UNSUPPORTED, "beam_select: %d groups of %d beams, %d tokens (at most %d beams, %lld rows, 2^30 tokens)",
+                     a->n_groups, a->n_beam, a->vocab, kMostBeams, kMostSelected);
+  if (a->ld < a->vocab) return set_error(MOE_ERR_ARG, "beam_select: rows of %lld floats for %d tokens", a->ld, a->vocab);
+  if (a->n_groups == 0) return MOE_OK;
+  if (!a->logits || !a->score || !a->parent || !a->token || !a->score_out || !a->done_out || !a->fresh || !a->work)
+    return set_error(MOE_ERR_ARG, "beam_select: null pointer");
+  const size_t need = ::moe_beam_select_work_bytes(a->n_groups, a->n_beam, a->vocab);
+  if (a->work_bytes < need || (uintptr_t)a->work % 16)
+    return set_error(MOE_ERR_ARG, "beam_select: %zu bytes of work at %p, %zu needed, 16-byte aligned", a->work_bytes, a->work, need);
+  return MOE_OK;
+}
+
 }  // namespace moe
 
 using namespace moe;
@@ -403,27 +422,14 @@ using namespace moe;
 extern "C" {
 
 size_t moe_beam_select_work_bytes(int n_groups, int n_beam, int vocab) {
-  if (n_groups < 0 || n_beam < 1 || n_beam > kMostBeams || vocab < 1 || (long long)n_groups * n_beam > kMostRows) return 0;
+  if (n_groups < 0 || n_beam < 1 || n_beam > kMostBeams || vocab < 1 || (long long)n_groups * n_beam > kMostSelected) return 0;
   const size_t rows = (size_t)n_groups * n_beam;
   return rows ? rows * blocks_for((long long)rows, vocab) * (sizeof(Part) + 8 * (size_t)n_beam) : 16;
 }
 
 moe_status moe_beam_select_dev(const moe_beam_select* a) {
-  if (!a) return set_error(MOE_ERR_ARG, "beam_select: null argument");
-  if (a->n_groups < 0 || a->n_beam < 1 || a->vocab < 1)
-    return set_error(MOE_ERR_ARG, "beam_select: %d groups of %d beams, %d tokens", a->n_groups, a->n_beam, a->vocab);
-  if (a->n_beam > kMostBeams || (long long)a->n_groups * a->n_beam > kMostRows || a->vocab > (1 << 30))
-    return set_error(MOE_ERR_UNSUPPORTED, "beam_select: %d groups of %d beams, %d tokens (at most %d beams, %lld rows, 2^30 tokens)",
-                     a->n_groups, a->n_beam, a->vocab, kMostBeams, kMostRows);
-  if (a->ld < a->vocab) return set_error(MOE_ERR_ARG, "beam_select: rows of %lld floats for %d tokens", a->ld, a->vocab);
-  if (a->n_groups == 0) return MOE_OK;
-  if (!a->logits || !a->score || !a->parent || !a->token || !a->score_out || !a->done_out || !a->fresh || !a->work)
-    return set_error(MOE_ERR_ARG, "beam_select: null pointer");
-  const size_t need = moe_beam_select_work_bytes(a->n_groups, a->n_beam, a->vocab);
-  if (a->work_bytes < need || (uintptr_t)a->work % 16)
-    return set_error(MOE_ERR_ARG, "beam_select: %zu bytes of work at %p, %zu needed, 16-byte aligned", a->work_bytes, a->work, need);
-  moe_status st = ensure_init();
-  if (st) return st;
+  moe_status st = check_select(a);
+  if (st || a->n_groups == 0 || (st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
   const int rows = a->n_groups * a->n_beam;

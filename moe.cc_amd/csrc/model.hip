@@ -20,6 +20,7 @@
 #include <unistd.h>
 
 #include <initializer_list>
+#include <functional>
 #include <mutex>
 #include <new>
 #include <string>
@@ -69,6 +70,7 @@ struct moe_model {
   // per-forward scratch, grown on demand
   Buf x, xa, xn, qkv, H, S, ids;
   Buf last, last_logits, attn_work;   // of steps over a paged cache
+  Buf beam_rows, share_plan;          // of steps of beam searches
   float* xf = nullptr;
   float* logits = nullptr;
   float* head_part = nullptr;   // block maxima of the head's product
@@ -129,7 +131,7 @@ void free_model(moe_model* m) {
   dfree(m->rope_cos); dfree(m->rope_sin); dfree(m->xf); dfree(m->logits);
   dfree(m->head_part); dfree(m->next); dfree(m->hist_pos);
   for (Buf* b : {&m->x, &m->xa, &m->xn, &m->qkv, &m->H, &m->S, &m->ids, &m->hist, &m->last,
-                 &m->last_logits, &m->attn_work})
+                 &m->last_logits, &m->attn_work, &m->beam_rows, &m->share_plan})
     if (b->p) (void)hipFree(b->p);
   delete m;
 }
@@ -290,29 +292,32 @@ moe_status forward_checked(moe_model* m, const int32_t* ids, int T, int ids_on_d
   return forward_dev(m, ids_d, T, logits_out, next_out, false);
 }
 
-// One step over a paged cache: forward_dev's layers with each token at its
-// own request's position, K and V in the requests' pages.
-moe_status step_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* layers, const int32_t* ids,
-                      float* logits, int32_t* next) {
+// The scratch of a step over T rows and R requests, so that the step allocates none.
+moe_status reserve_paged(moe_model* m, int T, int R, size_t work, bool own_logits) {
+  const QwenConfig& c = m->cfg;
+  const size_t td = (size_t)T * c.d_model * 4, rd = (size_t)R * c.d_model * 4, had = m->H.bytes;
+  moe_status st;
+  if ((st = grow(m->x, td)) || (st = grow(m->xa, td)) || (st = grow(m->xn, td)) ||
+      (st = grow(m->qkv, (size_t)T * m->nqkv * 4)) || (st = grow(m->H, (size_t)T * m->Dq * 4)) ||
+      // (rows of no request keep what is there: numbers from the start)
+      (m->H.bytes > had && (st = check_hip(hipMemsetAsync(m->H.p, 0, m->H.bytes, stream()), "model scratch clear"))) ||
+      (st = grow(m->last, 2 * rd)) || (st = grow(m->attn_work, work)) ||
+      (own_logits && (st = grow(m->last_logits, (size_t)R * c.vocab_size * 4))))
+    return st;
+  for (DevLayer& L : m->layers)
+    if ((st = reserve_layer(L.moe, T))) return st;
+  return MOE_OK;
+}
+
+// forward_dev's layers with each token of a plan at its own request's position, K and V in the requests' pages, then the
+// head.  share: what groups of rows hold in the same pages is read once (else NULL).
+moe_status run_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* layers, const int32_t* ids,
+                     const moe_paged_share* share, float* logits, int32_t* next) {
   const QwenConfig& c = m->cfg;
   hipStream_t s = stream();
   const int D = c.d_model, T = p->max_tokens, R = p->n_req;
   const float eps = c.rms_eps;
-  const size_t td = (size_t)T * D * 4, rd = (size_t)R * D * 4;
-  const size_t work = moe_paged_attn_work_bytes(T, c.n_q, c.n_kv, c.head_dim);
   moe_status st;
-  const size_t had = m->H.bytes;
-  if ((st = grow(m->x, td)) || (st = grow(m->xa, td)) || (st = grow(m->xn, td)) ||
-      (st = grow(m->qkv, (size_t)T * m->nqkv * 4)) || (st = grow(m->H, (size_t)T * m->Dq * 4)) ||
-      // (rows of no request keep what is there: numbers from the start)
-      (m->H.bytes > had && (st = check_hip(hipMemsetAsync(m->H.p, 0, m->H.bytes, s), "model scratch clear"))) ||
-      (st = grow(m->last, 2 * rd)) || (st = grow(m->attn_work, work)) ||
-      (!logits && (st = grow(m->last_logits, (size_t)R * c.vocab_size * 4))))
-    return st;
-  // everything the step allocates is there before its plan moves the requests on
-  for (DevLayer& L : m->layers)
-    if ((st = reserve_layer(L.moe, T))) return st;
-  if ((st = moe_paged_plan_dev(p))) return st;
   float* x = (float*)m->x.p;
   float* xa = (float*)m->xa.p;
   float* xn = (float*)m->xn.p;
@@ -333,8 +338,8 @@ moe_status step_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* la
                              m->max_seq, c.head_dim, qkv, m->nqkv};
     if ((st = moe_paged_heads_dev(&ha, &layers[l]))) return st;
     const moe_paged_attn aa{qkv, m->nqkv, T, c.n_q, p->req, p->pos, p->tables, R, p->max_pages, m->scale, H, m->Dq,
-                            m->attn_work.p, work};
-    if ((st = moe_paged_attn_dev(&aa, &layers[l]))) return st;
+                            m->attn_work.p, m->attn_work.bytes};
+    if ((st = share ? moe_paged_attn_shared_dev(&aa, &layers[l], share) : moe_paged_attn_dev(&aa, &layers[l]))) return st;
     DenseArgs oa{H, m->Dq, L.wo, m->Dq, L.bo, x, D, xa, D, T, D, m->Dq};
     if ((st = dense_matmul(oa, s))) return st;
     if ((st = moe_block_forward(L.moe, xa, T, x, eps))) return st;
@@ -349,6 +354,50 @@ moe_status step_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* la
   DenseArgs ha{xf, D, m->lm_head, D, nullptr, nullptr, 0, lg, c.vocab_size, R, c.vocab_size, D};
   if ((st = dense_matmul(ha, s))) return st;
   return next ? greedy_rows(lg, c.vocab_size, R, p->starts, next, s) : MOE_OK;
+}
+
+// One step over a paged cache.
+moe_status step_paged(moe_model* m, const moe_paged_plan* p, const moe_pages* layers, const int32_t* ids,
+                      float* logits, int32_t* next) {
+  const QwenConfig& c = m->cfg;
+  // everything the step allocates is there before its plan moves the requests on
+  moe_status st = reserve_paged(m, p->max_tokens, p->n_req, moe_paged_attn_work_bytes(p->max_tokens, c.n_q, c.n_kv, c.head_dim), !logits);
+  if (st || (st = moe_paged_plan_dev(p))) return st;
+  return run_paged(m, p, layers, ids, nullptr, logits, next);
+}
+
+// The rows of a plan over beams: each row's token, and where each group's rows start.
+__global__ __launch_bounds__(256) void beam_rows_kernel(const int32_t* req, const int32_t* token, int T, int n_req, const int32_t* starts,
+                                                       int n_beam, int n_groups, int32_t* ids, int32_t* first) {
+  const int i = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  if (i < T) {
+    const int r = req[i];
+    ids[i] = r >= 0 && r < n_req ? token[r] : 0;
+  }
+  if (i <= n_groups) first[i] = starts[i * n_beam];
+}
+
+// One step of beam searches: choice, tables, copies, then a step of one token a beam that goes on.
+moe_status step_beams(moe_model* m, const moe_beam_select* b, const moe_paged_fork* f, const moe_paged_plan* p, const moe_pages* layers,
+                      float* logits) {
+  const QwenConfig& c = m->cfg;
+  const int T = p->max_tokens, G = b->n_groups;
+  const size_t plan = moe_paged_share_plan_bytes(T, G, c.n_q, c.n_kv, c.head_dim);
+  moe_status st = reserve_paged(m, T, p->n_req, moe_paged_attn_shared_work_bytes(T, G, c.n_q, c.n_kv, c.head_dim), false);
+  if (st || (st = grow(m->beam_rows, ((size_t)T + 2 * (size_t)G + 1) * 4)) || (st = grow(m->share_plan, plan))) return st;
+  int32_t* ids = (int32_t*)m->beam_rows.p;
+  int32_t* first = ids + T;
+  if ((st = moe_beam_select_dev(b)) || (st = moe_paged_fork_dev(f)) ||
+      (st = moe_paged_copy_dev(f->copies, f->max_copies, layers, c.n_layers)) || (st = moe_paged_plan_dev(p)))
+    return st;
+  const int rows = T > G + 1 ? T : G + 1;
+  hipLaunchKernelGGL(beam_rows_kernel, dim3((unsigned)(rows + 255) / 256), dim3(256), 0, stream(), p->req, b->token, T, p->n_req, p->starts,
+                     b->n_beam, G, ids, first);
+  if ((st = check_hip(hipGetLastError(), "beam rows launch"))) return st;
+  const moe_paged_share share{T, p->n_req, p->max_pages, p->page_size, c.n_q, c.n_kv, c.head_dim, p->req, p->pos, p->tables,
+                              G, first, first + G + 1, m->share_plan.p, m->share_plan.bytes};
+  if ((st = moe_paged_share_dev(&share))) return st;
+  return run_paged(m, p, layers, ids, &share, logits, nullptr);
 }
 
 // ---- QW3W file (io.c:193-285) ----
@@ -842,15 +891,15 @@ moe_status moe_model_forward(moe_model* m, const int32_t* ids, int T, int ids_on
   return forward_checked(m, ids, T, ids_on_device, logits_dev, next_dev);
 }
 
-moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
-                                const int32_t* ids, float* logits, int32_t* next) {
-  if (!m || !plan || !layers || !ids || (!logits && !next)) return set_error(MOE_ERR_ARG, "step_paged: null argument");
+// What a step of any kind asks of the plan and the layers, and of the library: `take` is run with the model held.
+static moe_status checked_step(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers, const char* who,
+                               const std::function<moe_status()>& take) {
   if (plan->n_req < 1 || plan->max_tokens < 1)
-    return set_error(MOE_ERR_ARG, "step_paged: %d requests, %d tokens", plan->n_req, plan->max_tokens);
+    return set_error(MOE_ERR_ARG, "%s: %d requests, %d tokens", who, plan->n_req, plan->max_tokens);
   for (int l = 0; l < m->cfg.n_layers; ++l)
     if (layers[l].n_kv != m->cfg.n_kv || layers[l].head_dim != m->cfg.head_dim || layers[l].n_pages != plan->n_pages ||
         layers[l].page_size != plan->page_size)
-      return set_error(MOE_ERR_ARG, "step_paged: layer %d has %d pages of %d positions, %d heads of %d", l, layers[l].n_pages,
+      return set_error(MOE_ERR_ARG, "%s: layer %d has %d pages of %d positions, %d heads of %d", who, l, layers[l].n_pages,
                        layers[l].page_size, layers[l].n_kv, layers[l].head_dim);
   moe_status st = check_paged_step(plan, layers, m->cfg.n_layers, m->cfg.n_q, m->cfg.n_kv);
   if (st || (st = ensure_init())) return st;
@@ -858,9 +907,33 @@ moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const 
   if ((st = on.enter())) return st;
   std::lock_guard<std::mutex> lk(m->mu);
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  if ((st = check_hip(hipStreamIsCapturing(stream(), &capture), "step_paged capture"))) return st;
-  if (capture != hipStreamCaptureStatusNone) return set_error(MOE_ERR_ARG, "step_paged: the stream is being captured");
-  return step_paged(m, plan, layers, ids, logits, next);
+  if ((st = check_hip(hipStreamIsCapturing(stream(), &capture), "step capture"))) return st;
+  if (capture != hipStreamCaptureStatusNone) return set_error(MOE_ERR_ARG, "%s: the stream is being captured", who);
+  return take();
+}
+
+moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
+                                const int32_t* ids, float* logits, int32_t* next) {
+  if (!m || !plan || !layers || !ids || (!logits && !next)) return set_error(MOE_ERR_ARG, "step_paged: null argument");
+  return checked_step(m, plan, layers, "step_paged", [&] { return step_paged(m, plan, layers, ids, logits, next); });
+}
+
+moe_status moe_model_step_beams(moe_model* m, const moe_beam_select* select, const moe_paged_fork* fork, const moe_paged_plan* plan,
+                                const moe_pages* layers, float* logits) {
+  if (!m || !select || !fork || !plan || !layers || !logits) return set_error(MOE_ERR_ARG, "step_beams: null argument");
+  moe_status st;
+  if ((st = check_select(select)) || (st = check_fork(fork)) || (st = check_copy(fork->copies, fork->max_copies, layers, m->cfg.n_layers)))
+    return st;
+  if (select->vocab != m->cfg.vocab_size || (long long)select->n_groups * select->n_beam != plan->n_req || fork->n_req != plan->n_req ||
+      fork->max_pages != plan->max_pages || fork->n_pages != plan->n_pages || fork->page_size != plan->page_size ||
+      plan->max_tokens > shared_rows_max())
+    return set_error(MOE_ERR_ARG, "step_beams: %d groups of %d beams, %d tokens; %d and %d requests, of %d and %d pages, %d rows",
+                     select->n_groups, select->n_beam, select->vocab, fork->n_req, plan->n_req, fork->max_pages, plan->max_pages,
+                     plan->max_tokens);
+  if (fork->parent != select->parent || plan->fresh != select->fresh || plan->held != fork->held_out || plan->ring_at != fork->ring_at_out ||
+      plan->ring != fork->ring || plan->tables != fork->tables_out)
+    return set_error(MOE_ERR_ARG, "step_beams: what the choice, the fork and the plan hand on to each other differs");
+  return checked_step(m, plan, layers, "step_beams", [&] { return step_beams(m, select, fork, plan, layers, logits); });
 }
 
 moe_status moe_model_forward_full(moe_model* m, const int32_t* ids, int T, int apply_softmax,

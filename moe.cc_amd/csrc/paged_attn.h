@@ -37,6 +37,13 @@ hipError_t launch_paged_attn(const AttnPages& p, int dtype, hipStream_t stream);
 // over these layers' pages: what its moe_paged_* calls would refuse.
 moe_status check_paged_step(const moe_paged_plan* plan, const moe_pages* layers, int n_layers, int n_q, int n_kv);
 
+// What moe_beam_select_dev, moe_paged_fork_dev and moe_paged_copy_dev refuse, without any GPU work.
+moe_status check_select(const moe_beam_select* s);
+moe_status check_fork(const moe_paged_fork* f);
+moe_status check_copy(const int32_t* copies, int n, const moe_pages* layers, int n_layers);
+// Rows of moe_paged_share_dev at most.
+int shared_rows_max();
+
 // x row of each request's last token (zeros for one without tokens): out
 // [n_req][D] from x [.][D] at starts[r + 1] - 1.
 hipError_t launch_last_rows(const float* x, const int32_t* starts, int n_req, int D, float* out, hipStream_t stream);

@@ -353,18 +353,8 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
 }
 
 }  // namespace
-}  // namespace moe
 
-using namespace moe;
-
-extern "C" {
-
-size_t moe_paged_fork_work_bytes(int n_req, int max_pages, int n_pages) {
-  if (n_req < 0 || n_req > kMostRequests || max_pages < 1 || n_pages < 1) return 0;
-  return sizeof(ForkHead) + (size_t)n_req * sizeof(Goes) + 4 * ((size_t)n_req * max_pages + max_pages) + 64;
-}
-
-moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
+moe_status check_fork(const moe_paged_fork* f) {
   if (!f) return set_error(MOE_ERR_ARG, "paged_fork: null argument");
   if (f->n_req < 0 || f->max_pages < 1 || f->n_pages < 1 || f->page_size < 1 || f->max_copies < 0)
     return set_error(MOE_ERR_ARG, "paged_fork: %d requests of %d pages, %d pages of %d, %d copies", f->n_req, f->max_pages, f->n_pages,
@@ -377,11 +367,43 @@ moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
   for (const void* p : {(const void*)f->ring_at, (const void*)f->ring, (const void*)f->ring_at_out, (const void*)f->status, (const void*)f->work})
     if (!p) return set_error(MOE_ERR_ARG, "paged_fork: null pointer");
   if ((f->n_req && (!f->parent || !f->held || !f->tables || !f->held_out || !f->tables_out)) || (f->max_copies && !f->copies)) return set_error(MOE_ERR_ARG, "paged_fork: null pointer");
-  const size_t need = moe_paged_fork_work_bytes(f->n_req, f->max_pages, f->n_pages);
+  const size_t need = ::moe_paged_fork_work_bytes(f->n_req, f->max_pages, f->n_pages);
   if (f->work_bytes < need || (uintptr_t)f->work % 16)
     return set_error(MOE_ERR_ARG, "paged_fork: %zu bytes of work at %p, %zu needed, 16-byte aligned", f->work_bytes, f->work, need);
-  moe_status st = ensure_init();
-  if (st) return st;
+  return MOE_OK;
+}
+
+moe_status check_copy(const int32_t* copies, int n, const moe_pages* layers, int n_layers) {
+  if (n < 0 || n_layers < 0 || n > kMostRows) return set_error(MOE_ERR_ARG, "paged_copy: %d copies in %d layers", n, n_layers);
+  if (n == 0 || n_layers == 0) return MOE_OK;
+  if (!copies || !layers) return set_error(MOE_ERR_ARG, "paged_copy: null pointer");
+  for (int l = 0; l < n_layers; ++l) {
+    PageMap map;
+    moe_status st = check_pages(&layers[l], "paged_copy", &map);
+    if (st) return st;
+    const moe_pages &x = layers[l], &y = layers[0];
+    if (x.dtype != y.dtype || x.n_pages != y.n_pages || x.page_size != y.page_size || x.n_kv != y.n_kv || x.head_dim != y.head_dim ||
+        x.page_stride != y.page_stride || x.head_stride != y.head_stride || x.slot_stride != y.slot_stride)
+      return set_error(MOE_ERR_UNSUPPORTED, "paged_copy: layer %d's pages are laid out otherwise than layer 0's", l);
+    if (x.n_kv > 65535) return set_error(MOE_ERR_ARG, "paged_copy: %d heads", x.n_kv);
+  }
+  return MOE_OK;
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+size_t moe_paged_fork_work_bytes(int n_req, int max_pages, int n_pages) {
+  if (n_req < 0 || n_req > kMostRequests || max_pages < 1 || n_pages < 1) return 0;
+  return sizeof(ForkHead) + (size_t)n_req * sizeof(Goes) + 4 * ((size_t)n_req * max_pages + max_pages) + 64;
+}
+
+moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
+  moe_status st = check_fork(f);
+  if (st || (st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;
   ForkArgs a;
@@ -413,19 +435,10 @@ moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
 }
 
 moe_status moe_paged_copy_dev(const int32_t* copies, int n, const moe_pages* layers, int n_layers) {
-  if (n < 0 || n_layers < 0 || n > kMostRows) return set_error(MOE_ERR_ARG, "paged_copy: %d copies in %d layers", n, n_layers);
-  if (n == 0 || n_layers == 0) return MOE_OK;
-  if (!copies || !layers) return set_error(MOE_ERR_ARG, "paged_copy: null pointer");
+  moe_status st = check_copy(copies, n, layers, n_layers);
+  if (st || n == 0 || n_layers == 0) return st;
   PageMap map;
-  moe_status st;
-  for (int l = 0; l < n_layers; ++l) {
-    if ((st = check_pages(&layers[l], "paged_copy", &map))) return st;
-    const moe_pages &x = layers[l], &y = layers[0];
-    if (x.dtype != y.dtype || x.n_pages != y.n_pages || x.page_size != y.page_size || x.n_kv != y.n_kv || x.head_dim != y.head_dim ||
-        x.page_stride != y.page_stride || x.head_stride != y.head_stride || x.slot_stride != y.slot_stride)
-      return set_error(MOE_ERR_UNSUPPORTED, "paged_copy: layer %d's pages are laid out otherwise than layer 0's", l);
-  }
-  if (map.n_kv > 65535) return set_error(MOE_ERR_ARG, "paged_copy: %d heads", map.n_kv);
+  if ((st = check_pages(&layers[0], "paged_copy", &map))) return st;
   if ((st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;

@@ -1253,6 +1253,9 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
 }
 
 }  // namespace
+
+int shared_rows_max() { return kMostShared; }
+
 }  // namespace moe
 
 using namespace moe;

@@ -190,6 +190,7 @@ _SIGS = {
     "moe_model_forward": (_I, [_P, _P, _I, _I, _P, _P]),
     "moe_model_forward_full": (_I, [_P, _P, _I, _I, _P]),
     "moe_model_step_paged": (_I, [_P] * 6),
+    "moe_model_step_beams": (_I, [_P] * 6),
     "moe_model_generate": (_I, [_P, _P, _I, _I, _P, ctypes.POINTER(ctypes.c_float),
                                 ctypes.POINTER(ctypes.c_float)]),
 }
@@ -465,6 +466,37 @@ class PagedCache:
         self._b["fresh"].upload(fresh)
         self._b["ids"].upload(ids)
 
+    def fork_args(self, parent_ptr: int) -> PagedFork:
+        """moe_paged_fork on this cache's state, in place, with the parents at parent_ptr (int32 [n_req], device)."""
+        if "copies" not in self._b:
+            need = lib().moe_paged_fork_work_bytes(self.n_req, self.plan.max_pages, self.plan.n_pages)
+            if not need:
+                raise MoeError(f"a fork of {self.n_req} requests")
+            self._b["copies"] = DeviceBuffer(12 * self.n_req)
+            self._b["fork_status"] = DeviceBuffer.from_array(np.zeros(1, np.int32))
+            self._b["fork_work"] = DeviceBuffer(need)
+        b = {n: x.ptr for n, x in self._b.items()}
+        return PagedFork(self.n_req, self.plan.max_pages, self.plan.n_pages, self.plan.page_size, self.n_req,
+                         parent_ptr, b["held"], b["ring_at"], b["ring"], b["tables"], b["held"], b["ring_at"],
+                         b["tables"], b["copies"], b["fork_status"], b["fork_work"], self._b["fork_work"].nbytes)
+
+    def fork(self, parent) -> None:
+        """Request r goes on as a copy of what request parent[r] holds (r: it stays, -1: it ends): tables, pages and,
+        in every layer, the last pages that are not full.  Raises if the pages do not suffice."""
+        parent = np.ascontiguousarray(parent, np.int32)
+        if parent.shape != (self.n_req,):
+            raise MoeError(f"{parent.size} parents of {self.n_req} requests")
+        buf = DeviceBuffer.from_array(parent)
+        args = self.fork_args(buf.ptr)
+        check(lib().moe_paged_fork_dev(ctypes.byref(args)), "moe_paged_fork_dev")
+        check(lib().moe_paged_copy_dev(args.copies, args.max_copies, self.layers, len(self.layers)), "moe_paged_copy_dev")
+        if self.fork_status:
+            raise MoeError(f"paged_fork: status {self.fork_status}")
+
+    @property
+    def fork_status(self) -> int:
+        return int(self.array("fork_status", 1)[0])
+
     def array(self, name, *shape) -> np.ndarray:
         """A copy of one of the plan's arrays."""
         return self._b[name].download(shape, np.int32)
@@ -602,6 +634,60 @@ class Model:
         check(lib().moe_model_step_paged(self.h, ctypes.byref(cache.plan), cache.layers,
                                          cache._b["ids"].ptr, lg.ptr, nx.ptr), "moe_model_step_paged")
         return lg.download((cache.n_req, self.V), np.float32), nx.download((cache.n_req,), np.int32)
+
+    def beam_search(self, prompts, n_beam, n_new, eos=-1, page_size=16, dtype=PAGE_F32, n_pages=None):
+        """Beam searches over `prompts` (lists of ids), all steps on the device.
+
+        -> (ids [len(prompts)][n_beam]: lists of up to n_new new ids, the best beam first, a list ending with `eos` where
+        it came; their log probabilities [len(prompts), n_beam])"""
+        prompts = [np.ascontiguousarray(p, np.int32) for p in prompts]
+        G, R, V = len(prompts), len(prompts) * n_beam, self.V
+        if not prompts or min(p.size for p in prompts) < 1 or n_beam < 1 or n_new < 1:
+            raise MoeError(f"a search of {n_beam} beams over {len(prompts)} prompts, {n_new} new tokens")
+        width = -(-(max(p.size for p in prompts) + n_new) // page_size)
+        cfg = self.cfg
+        cache = PagedCache(cfg.n_layers, cfg.n_kv, cfg.head_dim, R * width if n_pages is None else n_pages, page_size,
+                           R, width, max(R, sum(p.size for p in prompts)), dtype)
+        # the prompts, each its group's first request
+        fresh = np.zeros(R, np.int32)
+        fresh[::n_beam] = [p.size for p in prompts]
+        cache.set_step(fresh, np.concatenate(prompts))
+        logits = DeviceBuffer(R * V * 4)
+        check(lib().moe_model_step_paged(self.h, ctypes.byref(cache.plan), cache.layers, cache._b["ids"].ptr,
+                                         logits.ptr, None), "moe_model_step_paged")
+        if cache.status:
+            raise MoeError(f"the prompts' plan: status {cache.status}")
+        cache.plan.max_tokens = R
+        score = np.where(np.arange(R) % n_beam == 0, 0, -np.inf).astype(np.float32)
+        state = {"score": DeviceBuffer.from_array(score), "done": DeviceBuffer.from_array(np.zeros(R, np.int32))}
+        told = DeviceBuffer(n_new * 2 * R * 4)   # parents and tokens of every step
+        need = lib().moe_beam_select_work_bytes(G, n_beam, V)
+        work = DeviceBuffer(need)
+        for i in range(n_new):
+            parent, token = told.ptr + 8 * R * i, told.ptr + 8 * R * i + 4 * R
+            sel = BeamSelect(G, n_beam, V, logits.ptr, V, state["score"].ptr, state["done"].ptr, None, eos, 0, parent,
+                             token, state["score"].ptr, state["done"].ptr, cache._b["fresh"].ptr, work.ptr, need)
+            if i == n_new - 1:
+                check(lib().moe_beam_select_dev(ctypes.byref(sel)), "moe_beam_select_dev")
+                break
+            fork = cache.fork_args(parent)
+            check(lib().moe_model_step_beams(self.h, ctypes.byref(sel), ctypes.byref(fork), ctypes.byref(cache.plan),
+                                             cache.layers, logits.ptr), "moe_model_step_beams")
+            if cache.fork_status or cache.status:
+                raise MoeError(f"step {i}: fork status {cache.fork_status}, plan status {cache.status}")
+        told = told.download((n_new, 2, R), np.int32)
+        out, at = [[] for _ in range(R)], np.arange(R)
+        for parent, token in told[::-1]:
+            for r in range(R):
+                if at[r] >= 0:
+                    out[r].append(int(token[at[r]]))
+            at = np.where(at >= 0, parent[at], -1)
+        for r in range(R):
+            out[r] = out[r][::-1]
+            if eos in out[r]:
+                out[r] = out[r][:out[r].index(eos) + 1]
+        return ([out[g * n_beam:(g + 1) * n_beam] for g in range(G)],
+                state["score"].download((G, n_beam), np.float32))
 
     def generate(self, prompt, n_new):
         """-> (ids [n_new], ms_prompt, ms_decode)"""
