@@ -33,6 +33,9 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostBeams = kWave;          // a list is a lane a beam
 constexpr int kStep = 16 * kWave;          // logits of a wave's step
+// From here on the blocks' lists are merged by a kernel of their own (one group, 151936 columns, us with it and without: 16
+// beams 29.8, 27.6; 32 beams 42, 58; 64 beams 69, 147).
+constexpr int kMergedBeams = 32;
 constexpr int kBlocks = 1024;              // blocks that rows are cut into, about
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -51,7 +54,8 @@ struct SelectArgs {
   moe_beam_select a;
   int blocks;       // of a row
   Part* parts;      // work [rows][blocks]
-  uint64_t* keys;   // work [rows][n_beam][blocks]: each block's best, in order; 0: none
+  int merged;       // the blocks' lists are merged by a kernel of their own
+  uint64_t* keys;   // work [rows][n_beam][blocks], or merged [rows][blocks][n_beam]: each block's best, in order; 0: none
 };
 
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -96,21 +100,25 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t x, int n) {
   return t;
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-  auto with = [&](auto ctrl) {
-    x = fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, false)));
+// Largest of the lanes' numbers (of floats: that are numbers), in all of them.
+template <class T>
+__device__ __forceinline__ T wave_max(T x) {
+  auto larger = [](uint32_t y, uint32_t z) {
+    if constexpr (std::is_same_v<T, float>) return fmaxf(__uint_as_float(y), __uint_as_float(z));
+    else return y > z ? y : z;
   };
-  with(std::integral_constant<int, 0xB1>{});    // quad_perm [1,0,3,2], [2,3,0,1]
-  with(std::integral_constant<int, 0x4E>{});
-  with(std::integral_constant<int, 0x141>{});   // row_half_mirror, row_mirror
-  with(std::integral_constant<int, 0x140>{});
-  auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-  auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+  auto bits = [&]() { return __builtin_bit_cast(uint32_t, x); };
+  x = larger(bits(), __builtin_amdgcn_update_dpp(0, bits(), 0xB1, 0xf, 0xf, false));    // quad_perm [1,0,3,2], [2,3,0,1]
+  x = larger(bits(), __builtin_amdgcn_update_dpp(0, bits(), 0x4E, 0xf, 0xf, false));
+  x = larger(bits(), __builtin_amdgcn_update_dpp(0, bits(), 0x141, 0xf, 0xf, false));   // row_half_mirror, row_mirror
+  x = larger(bits(), __builtin_amdgcn_update_dpp(0, bits(), 0x140, 0xf, 0xf, false));
+  auto p = __builtin_amdgcn_permlane32_swap(bits(), bits(), false, false);
+  x = larger(p[0], p[1]);
+  auto q = __builtin_amdgcn_permlane16_swap(bits(), bits(), false, false);
+  return larger(q[0], q[1]);
 }
 
-__device__ __forceinline__ double wave_max(double x) {
+__device__ __forceinline__ double wave_max_f64(double x) {
 #pragma unroll
   for (int c = 32; c; c /= 2) x = fmax(x, __shfl_xor(x, c));
   return x;
@@ -278,7 +286,8 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
     if (rank < K) best_s[rank] = k;
   }
   __syncthreads();
-  if ((int)threadIdx.x < K) s.keys[((size_t)row * K + threadIdx.x) * s.blocks + b] = best_s[threadIdx.x];
+  if ((int)threadIdx.x < K)
+    s.keys[(size_t)row * K * s.blocks + (s.merged ? (size_t)b * K + threadIdx.x : (size_t)threadIdx.x * s.blocks + b)] = best_s[threadIdx.x];
   if (threadIdx.x == 0) {
     double most = part_s[0].at;
     for (int w = 1; w < kWaves; ++w) most = fmax(most, part_s[w].at);
@@ -288,14 +297,51 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   }
 }
 
-// A block a group; a wave a row, then all rows' lists against each other.
+// The 64 largest of two lists sorted over the lanes, sorted: of lane i's and the other's 63 - i'th the larger, which rise and
+// fall once, then six exchanges.
+__device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b) {
+  const int lane = threadIdx.x % kWave;
+  const uint64_t other = __shfl(b, kWave - 1 - lane);
+  uint64_t x = a > other ? a : other;
+#pragma unroll
+  for (int c = kWave / 2; c; c /= 2) {
+    const uint64_t y = __shfl_xor(x, c);
+    x = (lane & c) == 0 ? (x > y ? x : y) : (x > y ? y : x);
+  }
+  return x;
+}
+
+// Many beams: a block a row merges its blocks' lists, into the first one's place.  (Inserted one by one by the next kernel, a
+// wave a row: 64 beams 147 us.)
+__global__ __launch_bounds__(kThreads) void select_merge_kernel(SelectArgs s) {
+  const moe_beam_select& a = s.a;
+  const int row = (int)blockIdx.x, K = a.n_beam, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  if (!usable(a, row) || (a.done && a.done[row])) return;
+  uint64_t* keys = s.keys + (size_t)row * K * s.blocks;
+  auto load = [&](int b) { return lane < K && b < s.blocks ? keys[(size_t)b * K + lane] : 0; };
+  uint64_t best = load(wave), next = load(wave + kWaves);
+  for (int b = wave + kWaves; b < s.blocks; b += kWaves) {
+    const uint64_t now = next;
+    next = load(b + kWaves);
+    if (__any(now > read_lane(best, K - 1))) best = merge_lists(best, now);
+  }
+  __shared__ uint64_t list_s[kWaves][kWave];
+  list_s[wave][lane] = best;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) best = merge_lists(best, list_s[w][lane]);
+  if (lane < K) keys[lane] = best;
+}
+
+// A block a group; a wave a row, then one wave merges the rows' lists, a lane each.
 __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
   const moe_beam_select& a = s.a;
   constexpr int W = 1024 / kWave;
   const int K = a.n_beam, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, row0 = (int)blockIdx.x * K;
   __shared__ uint64_t key_s[kMostBeams][kMostBeams];
   __shared__ double base_s[kMostBeams], weight_s[kMostBeams];
-  __shared__ int count_s[kMostBeams], place_s[kMostBeams * kMostBeams], out_s[kMostBeams], done_s[kMostBeams];
+  __shared__ int count_s[kMostBeams], done_s[kMostBeams];
   for (int i = wave; i < K; i += W) {
     const int row = row0 + i;
     const bool use = usable(a, row), done = a.done && a.done[row];
@@ -311,14 +357,15 @@ __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
       const Part* p = s.parts + (size_t)row * s.blocks;
       double most = -(double)INFINITY;
       for (int c = lane; c < s.blocks; c += kWave) most = fmax(most, p[c].at);
-      most = wave_max(most);
+      most = wave_max_f64(most);
       double sum = 0.0;
       for (int c = lane; c < s.blocks; c += kWave) sum += part_at(p[c], most);
       sum = wave_sum(sum);
       if (sum > 0.0 && sum < (double)INFINITY) {   // (a NaN or +inf among the logits makes it NaN)
         base = (double)score - (most + log(sum));
         const uint64_t* keys = s.keys + (size_t)row * K * s.blocks;
-        for (int c0 = 0; c0 < K * s.blocks; c0 += kWave) {
+        if (s.merged) list.key = lane < K ? keys[lane] : 0;
+        for (int c0 = s.merged ? K * s.blocks : 0; c0 < K * s.blocks; c0 += kWave) {
           const uint64_t k = c0 + lane < K * s.blocks ? keys[c0 + lane] : 0;
           if (!__any(k > list.last)) continue;
           const uint32_t bound = nth_largest(k > list.last ? (uint32_t)(k >> 32) : 0u, K);
@@ -336,54 +383,35 @@ __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
     if (lane < K) key_s[i][lane] = list.key;
     if (lane == 0) count_s[i] = count, base_s[i] = base, done_s[i] = done, weight_s[i] = weight;
   }
-  auto value_of = [&](int row, int c) {
-    return done_s[row] ? base_s[row] : base_s[row] + (double)unordered((uint32_t)(key_s[row][c] >> 32));
-  };
-  for (int i = tid; i < K * K; i += 1024) place_s[i] = 0;
-  if (tid < K) out_s[tid] = -1;
   __syncthreads();
-  // the place of each candidate: how many of every row come before it
-  for (int i = tid; i < K * K * K; i += 1024) {
-    const int at = i / K, other = i % K, row = at / K, c = at % K;
-    if (c >= count_s[row]) continue;
-    int n;
-    if (other == row) {
-      n = c;
-    } else {
-      const double x = value_of(row, c) * weight_s[row];
-      int lo = 0, hi = count_s[other];   // equal ranks: the lower row first
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        const double y = value_of(other, mid) * weight_s[other];
-        if (y > x || (y == x && other < row)) lo = mid + 1;
-        else hi = mid;
-      }
-      n = lo;
+  if (wave) return;
+  // ---- lane i: row i's best candidate that is left; the best of all goes first, of equal ones the lowest row's
+  const int mine = min(lane, K - 1), count = lane < K ? count_s[mine] : 0;
+  const bool done = done_s[mine];
+  const double base = base_s[mine], weight = weight_s[mine];
+  int at = 0;
+  uint64_t key = key_s[mine][0];
+  auto value = [&]() { return done ? base : base + (double)unordered((uint32_t)(key >> 32)); };
+  for (int i = 0; i < K; ++i) {
+    const uint64_t bits = (uint64_t)__double_as_longlong(value() * weight + 0.0);
+    const uint64_t rank = at < count ? (bits >> 63 ? ~bits : bits | 1ull << 63) : 0;
+    const uint32_t hi = wave_max((uint32_t)(rank >> 32));
+    const uint32_t lo = wave_max((uint32_t)(rank >> 32) == hi ? (uint32_t)rank : 0u);
+    const uint64_t best = __ballot(at < count && rank == ((uint64_t)hi << 32 | lo));
+    const int to = row0 + i;
+    if (!best) {
+      if (lane == 0) a.parent[to] = a.token[to] = -1, a.score_out[to] = -INFINITY, a.done_out[to] = a.fresh[to] = 0;
+      continue;
     }
-    if (n) atomicAdd(&place_s[at], n);
-  }
-  __syncthreads();
-  for (int i = tid; i < K * K; i += 1024)
-    if (i % K < count_s[i / K] && place_s[i] < K) out_s[place_s[i]] = i;
-  __syncthreads();
-  if (tid < K) {
-    const int from = out_s[tid], to = row0 + tid;
-    int parent = -1, token = -1, done = 0;
-    double value = -(double)INFINITY;
-    if (from >= 0) {
-      const int row = from / K, c = from % K;
-      const uint64_t k = key_s[row][c];
-      parent = row0 + row;
-      done = done_s[row] != 0;
-      token = done ? a.pad : (int)(0xffffffffu - (uint32_t)k);
-      value = value_of(row, c);
-      done = done || token == a.eos;
+    if (lane == __builtin_ctzll(best)) {
+      const int token = done ? a.pad : (int)(0xffffffffu - (uint32_t)key), ends = done || token == a.eos;
+      a.parent[to] = row0 + lane;
+      a.token[to] = token;
+      a.score_out[to] = (float)value();
+      a.done_out[to] = ends;
+      a.fresh[to] = !ends;
+      if (++at < count) key = key_s[mine][at];
     }
-    a.parent[to] = parent;
-    a.token[to] = token;
-    a.score_out[to] = (float)value;
-    a.done_out[to] = done;
-    a.fresh[to] = parent >= 0 && !done;
   }
 }
 
@@ -436,10 +464,15 @@ moe_status moe_beam_select_dev(const moe_beam_select* a) {
   SelectArgs s;
   s.a = *a;
   s.blocks = blocks_for(rows, a->vocab);
+  s.merged = a->n_beam >= kMergedBeams && s.blocks > 1;
   s.parts = (Part*)a->work;
   s.keys = (uint64_t*)(s.parts + (size_t)rows * s.blocks);
   hipLaunchKernelGGL(select_rows_kernel, dim3((unsigned)s.blocks, (unsigned)rows), dim3(kThreads), 0, stream(), s);
   if ((st = check_hip(hipGetLastError(), "beam_select launch"))) return st;
+  if (s.merged) {
+    hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream(), s);
+    if ((st = check_hip(hipGetLastError(), "beam_select launch"))) return st;
+  }
   hipLaunchKernelGGL(select_groups_kernel, dim3((unsigned)a->n_groups), dim3(1024), 0, stream(), s);
   return check_hip(hipGetLastError(), "beam_select launch");
 }
