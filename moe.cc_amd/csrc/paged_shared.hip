@@ -25,6 +25,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostShared = 1 << 14;   // rows, groups of a call
 constexpr int kN = 1024;               // threads of the plan's block
+constexpr int kTile = 64;              // columns of a prefix item at most
 
 // ---------------------------------------------------------------- the plan
 
@@ -69,7 +70,7 @@ ShareCut share_cut(int T, int n_groups, int n_q, int n_kv, int head_dim) {
   c.group = n_q / n_kv;
   const long long mean = n_groups ? ((long long)T + n_groups - 1) / n_groups * c.group : 0;
   c.shift = 4;
-  while (1 << c.shift < mean && 1 << c.shift < (head_dim > 128 ? 64 : 128)) ++c.shift;
+  while (1 << c.shift < mean && 1 << c.shift < kTile) ++c.shift;
   c.columns = 1 << c.shift;
   c.own_columns = c.group < 16 ? c.group : 16;
   c.own_tiles = (c.group + 15) / 16;
@@ -434,6 +435,7 @@ struct SharedLaunch {
   ShareCut cut;
   PlanParts p;
   Divider by_group, by_kv;
+  bool tiles;          // prefix items are taken whole, not in sixteens
   int prefix_blocks;   // of a launch; the rest are rows' own
   // work: [n_kv][items][columns] maxima and sums, [n_kv][items][columns][head_dim] values
   float* prefix_ml;
@@ -788,19 +790,22 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 
 // ---------------------------------------------------------------- many columns
 
-// A block takes an item of up to 64 or 128 columns: WC waves lie beside each other over the columns, 32 each
-// (16 where head_dim is past 128), the others over the positions, 32 each of a step.  K and V of a step go through LDS, a
+// A block takes an item of up to 64 columns: WC waves lie beside each other over the columns, 32 each (16 where head_dim is
+// past 128), the others over the positions, 32 each of a step (fp32 pages: 16).  K and V of a step go through LDS, a
 // step ahead, where the waves over the columns share them: rows of 16-bit values in 16-byte pieces, piece p of row r at
 // p ^ swizzle(r), so that the reads of both lie evenly over the banks.  Keys are read as rows; a value operand, 8 keys of one
 // dimension, is two reads that turn 4 rows x 16 dimensions around on their way.  16-bit pages go straight from memory into
 // LDS, 8-bit pages become f16 in registers.  A wave stages the 8 rows of one (32 positions, quad of lanes that reads them),
 // whose addresses lie in its lanes, found once for K and V.  One barrier a step.  A column's largest score is raised only
 // when one is more than 2^kSlack above it, so that most steps need no sums across lanes.
+constexpr int type_size(int type) { return type == F32 ? 4 : type == E4M3 ? 1 : 2; }
+
 template <int CT, int HDP, int WC>
 struct TileShape {
-  static constexpr int S = CT == E4M3 ? 1 : 2, WP = kWaves / WC, CPW = HDP > 128 ? 1 : 2;
-  static constexpr int ROWS = 32 * WP;             // positions of a step
-  static constexpr int RB = HDP * 2;               // bytes of a row in LDS
+  static constexpr int S = type_size(CT), WP = kWaves / WC, CPW = HDP > 128 ? 1 : 2;
+  static constexpr int PW = CT == F32 ? 32 / WP : 32;    // positions of a step and a wave
+  static constexpr int ROWS = PW * WP;             // of a step
+  static constexpr int RB = HDP * (CT == F32 ? 4 : 2);   // bytes of a row in LDS
   static constexpr int STAGE = 2 * ROWS * RB;      // K and V
   static constexpr int JOIN = (WP - 1) * WC * CPW * kWave * (HDP + 8);
   static constexpr int BYTES = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
@@ -816,10 +821,10 @@ __device__ __forceinline__ u32x2 read_turned(const uint8_t* p) {
 template <int CT, int HDP, int WC>
 __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it, int kv, uint8_t* lds) {
   using T = TileShape<CT, HDP, WC>;
-  constexpr bool HALF = CT != BF16;
-  constexpr int NP = HALF ? 2 : 3, S = T::S, CPW = T::CPW, RB = T::RB;
-  constexpr int NK = HDP / 32, VE = HDP / 16;
-  constexpr int SETS = T::WP * 4 / kWaves;                              // (32 positions, q) that a wave stages
+  constexpr bool HALF = CT == F16 || CT == E4M3;
+  constexpr int NP = HALF ? 2 : CT == BF16 ? 3 : 1, S = T::S, CPW = T::CPW, RB = T::RB;
+  constexpr int NK = CT == F32 ? HDP / 16 : HDP / 32, VE = HDP / 16, KT = T::PW / 16;
+  constexpr int SETS = T::ROWS / 32;                              // (32 positions, q) that a wave stages
   constexpr int NL = (8 * HDP * S + 1023) / 1024;              // 16-byte loads of a lane for their keys
   constexpr int KP = HDP * S / 16;                             // such pieces of a row
   constexpr float kSlack = 4.0f, kLift = HALF ? 10.0f : 0.0f;  // weights reach 2^(kSlack + kLift)
@@ -837,7 +842,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   // ---- staging: set n of a wave is quad set % 4 of positions 32 (set / 4) .. of the step, set = wave + 4 n; row k (lane % 8)
   // of it position 16 (k / 4) + 4 q + k % 4, which is row 8 q + k of its 32 in LDS
   auto swizzle = [](int row) {
-    return HDP == 64 ? (row >> 1 & 1) | (row >> 3 & 3) << 1 : (row & 3) | (row >> 3 & 3) << 2;
+    return RB == 128 ? (row >> 1 & 1) | (row >> 3 & 3) << 1 : (row & 3) | (row >> 3 & 3) << 2;
   };
   auto position = [&](int step, int n) {
     const int set = wave + n * kWaves, k = lane % 8;
@@ -904,17 +909,18 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   next = look(1);
 
   // ---- queries times scale and log2(e), in parts
-  u32x4 qp[CPW][NP][NK];
+  u32x4 qp[CPW][NP][NK];   // (fp32: the values)
   float unlift[CPW];
+  constexpr int NX = CT == F32 ? NK : 2 * NK;
 #pragma unroll
   for (int ct = 0; ct < CPW; ++ct) {
     const int c = (wc * CPW + ct) * 16 + col;
     const Column mine = column_of(L, it, kv, min(c, it.cols - 1));
     const float* q = a.q + (size_t)mine.row * a.ldq + (size_t)mine.head * hd;
-    f32x4 x[2 * NK];
+    f32x4 x[NX];
 #pragma unroll
-    for (int s = 0; s < 2 * NK; ++s) {
-      const int d = (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
+    for (int s = 0; s < NX; ++s) {
+      const int d = CT == F32 ? (4 * s + quad) * 4 : (4 * (s / 2) + quad) * 8 + 4 * (s % 2);
       x[s] = *(const f32x4u*)(q + min(d, hd - 4));
       x[s] *= d < hd && c < it.cols ? scale : 0.0f;
     }
@@ -923,7 +929,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     if constexpr (HALF) {
       float big = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 2 * NK; ++s)
+      for (int s = 0; s < NX; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(x[s][i]));
       big = head_max(big);
@@ -934,15 +940,20 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       }
     }
 #pragma unroll
-    for (int s = 0; s < NK; ++s)
+    for (int s = 0; s < NK; ++s) {
+      if constexpr (CT == F32) {
+        qp[ct][0][s] = __builtin_bit_cast(u32x4, x[s]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 y = x[2 * s + i / 2];
-        uint32_t u[NP];
-        split_pair<HALF, NP>(y[2 * (i % 2)] * lift, y[2 * (i % 2) + 1] * lift, u);
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 y = x[2 * s + i / 2];
+          uint32_t u[NP];
+          split_pair<HALF, NP>(y[2 * (i % 2)] * lift, y[2 * (i % 2) + 1] * lift, u);
 #pragma unroll
-        for (int n = 0; n < NP; ++n) qp[ct][n][s][i] = u[n];
+          for (int n = 0; n < NP; ++n) qp[ct][n][s][i] = u[n];
+        }
       }
+    }
   }
   store(0);
 
@@ -960,54 +971,69 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       load(step + 1, next);
       next = look(step + 2);
     }
-    const int base = it.begin + step * T::ROWS + wp * 32;
+    const int base = it.begin + step * T::ROWS + wp * T::PW;
     if (base < end) {
-      const uint8_t* ks = lds + (step & 1) * T::STAGE + wp * 32 * RB;
+      // (a wave's 16 positions of 32 are rows 8 q + 4 wp .. + 3)
+      const uint8_t* ks = lds + (step & 1) * T::STAGE + wp * (KT == 2 ? 32 : 4) * RB;
       const uint8_t* vs = ks + T::ROWS * RB + (quad * 8 + col / 4) * RB + col % 2 * 8;
       // ---- scores
-      f32x4 s[CPW][2];
+      f32x4 s[CPW][KT];
 #pragma unroll
-      for (int ct = 0; ct < CPW; ++ct) s[ct][0] = s[ct][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      u32x4 k[NK][2];
+      for (int ct = 0; ct < CPW; ++ct)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      u32x4 k[NK][KT];
 #pragma unroll
       for (int j = 0; j < NK; ++j)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < KT; ++t) {
           const int row = 8 * (col / 4) + 4 * t + col % 4;
           k[j][t] = *(const u32x4*)(ks + row * RB + ((4 * j + quad) ^ swizzle(row)) * 16);
         }
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (CT != F32) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < NK; ++j)
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
+        for (int n = 0; n < (CT == F32 ? 4 : NP); ++n)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int ct = 0; ct < CPW; ++ct) s[ct][t] = mfma32<HALF>(k[j][t], qp[ct][n][j], s[ct][t]);
-      // the values' operands are requested before the weights are worked on
-      u32x4 v[VE];
+            for (int ct = 0; ct < CPW; ++ct) {
+              if constexpr (CT == F32)
+                s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[j][t][n]), __uint_as_float(qp[ct][0][j][n]), s[ct][t], 0, 0, 0);
+              else
+                s[ct][t] = mfma32<HALF>(k[j][t], qp[ct][n][j], s[ct][t]);
+            }
+      // the values' operands are requested before the weights are worked on: of fp32 pages four dimensions of keys
+      // 16 t + 4 quad + i in v[(4 t + i) HDP / 64 + h]
+      u32x4 v[CT == F32 ? KT * VE : VE];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const u32x2 x = read_turned(vs + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + col / 4)) * 16);
-        const u32x2 y = read_turned(vs + 4 * RB + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + 4 + col / 4)) * 16);
-        v[e] = u32x4{x[0], x[1], y[0], y[1]};
+      for (int e = 0; e < (CT == F32 ? KT * VE : VE); ++e) {
+        if constexpr (CT == F32) {
+          const int row = 8 * quad + e / (VE / 4), piece = 16 * (e % (VE / 4)) + col;
+          v[e] = *(const u32x4*)(ks + T::ROWS * RB + row * RB + (piece ^ swizzle(row)) * 16);
+        } else {
+          const u32x2 x = read_turned(vs + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + col / 4)) * 16);
+          const u32x2 y = read_turned(vs + 4 * RB + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + 4 + col / 4)) * 16);
+          v[e] = u32x4{x[0], x[1], y[0], y[1]};
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
       // ---- weights
       u32x4 pp[CPW][NP];
+      float p[CPW][4 * KT];
 #pragma unroll
       for (int ct = 0; ct < CPW; ++ct) {
-        if (base + 32 > end) {
+        if (base + T::PW > end) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (base + 16 * t + 4 * quad + i >= end) s[ct][t][i] = -INFINITY;
         }
         float top = s[ct][0][0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[ct][i / 4][i % 4]);
+        for (int i = 1; i < 4 * KT; ++i) top = fmaxf(top, s[ct][i / 4][i % 4]);
         if (HALF) top *= unlift[ct];
         if (__any(top > m[ct] + kSlack)) {
           const float now = fmaxf(m[ct], head_max(top)), keep = now == -INFINITY ? 1.0f : exp2_hw(m[ct] - now);
@@ -1017,27 +1043,36 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
           m[ct] = now;
         }
         const float from = (m[ct] == -INFINITY ? 0.0f : m[ct]) - kLift;
-        float p[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = exp2_hw(HALF ? fmaf(s[ct][i / 4][i % 4], unlift[ct], -from) : s[ct][i / 4][i % 4] - from);
-          l[ct] += p[i];
+        for (int i = 0; i < 4 * KT; ++i) {
+          p[ct][i] = exp2_hw(HALF ? fmaf(s[ct][i / 4][i % 4], unlift[ct], -from) : s[ct][i / 4][i % 4] - from);
+          l[ct] += p[ct][i];
         }
+        if constexpr (CT != F32)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t u[NP];
-          split_pair<HALF, NP>(p[2 * c], p[2 * c + 1], u);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t u[NP];
+            split_pair<HALF, NP>(p[ct][2 * c], p[ct][2 * c + 1], u);
 #pragma unroll
-          for (int n = 0; n < NP; ++n) pp[ct][n][c] = u[n];
-        }
+            for (int n = 0; n < NP; ++n) pp[ct][n][c] = u[n];
+          }
       }
       // ---- values
+      if constexpr (CT == F32) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
+        for (int i = 0; i < 4 * KT; ++i)
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
+          for (int e = 0; e < VE; ++e)
 #pragma unroll
-          for (int ct = 0; ct < CPW; ++ct) o[ct][e] = mfma32<HALF>(v[e], pp[ct][n], o[ct][e]);
+            for (int ct = 0; ct < CPW; ++ct)
+              o[ct][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[i * (VE / 4) + e / 4][e % 4]), p[ct][i], o[ct][e], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+#pragma unroll
+          for (int n = 0; n < NP; ++n)
+#pragma unroll
+            for (int ct = 0; ct < CPW; ++ct) o[ct][e] = mfma32<HALF>(v[e], pp[ct][n], o[ct][e]);
       }
     }
     if (step + 1 < steps) store(step + 1);
@@ -1085,8 +1120,13 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
     if (quad == 0) L.prefix_ml[part * 2] = m[ct] - kLift, L.prefix_ml[part * 2 + 1] = l[ct];
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      const int d = 16 * e + 4 * quad;
-      if (d < hd) *(f32x4*)(L.prefix_o + part * hd + d) = o[ct][e];
+      // (fp32: o[4 h + c][i] is dimension 64 h + 16 quad + 4 i + c)
+      const int d = CT == F32 ? 64 * (e / 4) + 16 * quad + 4 * (e % 4) : 16 * e + 4 * quad;
+      f32x4 y = o[ct][e];
+      if constexpr (CT == F32)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) y[x] = o[ct][e / 4 * 4 + x][e % 4];
+      if (d < hd) *(f32x4*)(L.prefix_o + part * hd + d) = y;
     }
   }
 }
@@ -1095,7 +1135,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
 // the long ones start together.
 template <int CT, int HDP, int WC>
 __global__ __launch_bounds__(kThreads, WC || HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
-  constexpr int TILE = TileShape<CT == F32 ? BF16 : CT, HDP, WC ? WC : 4>::BYTES, COLUMNS = (int)sizeof(ColumnsShared<HDP>);
+  constexpr int TILE = TileShape<CT, HDP, WC ? WC : 4>::BYTES, COLUMNS = (int)sizeof(ColumnsShared<HDP>);
   constexpr int BYTES = WC && TILE > COLUMNS ? TILE : COLUMNS;
   __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
   const int subs = WC ? 1 : L.cut.columns / 16;
@@ -1216,12 +1256,10 @@ hipError_t launch(SharedLaunch L, unsigned prefix, unsigned own, hipStream_t s) 
 template <int CT, int HDP>
 hipError_t launch(const SharedLaunch& L, hipStream_t s) {
   const unsigned prefix = (unsigned)L.cut.prefix_items, own = (unsigned)L.cut.own_items;
-  if constexpr (CT != F32 && HDP <= 128) {
-    if (L.cut.columns == 128) return launch<CT, HDP, 4>(L, prefix, own, s);
-    if (L.cut.columns == 64) return launch<CT, HDP, 2>(L, prefix, own, s);
-  }
-  if constexpr (CT != F32 && HDP > 128) {
-    if (L.cut.columns == 64) {
+  if constexpr (HDP <= 128) {
+    if (L.tiles) return launch<CT, HDP, 2>(L, prefix, own, s);
+  } else if constexpr (CT != F32) {
+    if (L.tiles) {
       const hipError_t e = launch<CT, HDP, 4>(L, prefix, 0, s);
       return e == hipSuccess ? launch<CT, HDP, 0>(L, 0, own, s) : e;
     }
@@ -1243,6 +1281,11 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
   shared_work(L.cut, g.map.n_kv, g.map.head_dim, g.a.work, &L);
   L.by_group = make_divider((uint32_t)L.cut.group);
   L.by_kv = make_divider((uint32_t)g.map.n_kv);
+  // Items of 64 columns are taken whole, but where all of them in sixteens, at their longest, would be resident at once: then
+  // only a block's latency counts (us of bf16 pages, 64 over 8 heads of 128, whole and in sixteens: 8 rows of 600 positions
+  // 14.9, 12.0; 8 groups of 8 rows of 250 16.8, 14.6, of 600 18.6, 21.1).
+  const long long all = ((long long)g.a.T * L.cut.group + kTile - 1) / kTile, units = ((long long)g.a.max_pages * g.map.page_size + kUnit - 1) / kUnit;
+  L.tiles = L.cut.columns == kTile && (all > sh.n_groups ? all : sh.n_groups) * units * (kTile / 16) * g.map.n_kv > 2 * kCUs;
   const hipError_t e = dtype == F32    ? launch<F32>(L, s)
                        : dtype == F16  ? launch<F16>(L, s)
                        : dtype == BF16 ? launch<BF16>(L, s)

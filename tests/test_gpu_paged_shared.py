@@ -14,9 +14,10 @@ pytestmark = pytest.mark.gpu
 class Batch:
     """Rows in groups whose requests begin in the same pages.
 
-    groups: [(rows, shared positions, (fewest, most) of a row's own)]; the rest of the pool holds NaNs and infinities."""
+    groups: [(rows, shared positions, (fewest, most) of a row's own)]; the rest of the pool holds NaNs and infinities.
+    wide: tables of 32768 positions, whose shared items are not taken in sixteen columns only for being few."""
 
-    def __init__(self, M, kind, groups, nq, nkv, hd, ps, order="slot", seed=0, listed=True, spare_rows=0, first=None):
+    def __init__(self, M, kind, groups, nq, nkv, hd, ps, order="slot", seed=0, listed=True, spare_rows=0, first=None, wide=False):
         self.M, self.nq, self.nkv, self.hd, self.ps = M, nq, nkv, hd, ps
         self.rng = rng = np.random.default_rng(seed)
         self.T = T = sum(g[0] for g in groups)
@@ -25,6 +26,8 @@ class Batch:
             plan.append((rows, shared // ps, [int(rng.integers(lo, hi + 1)) for _ in range(rows)]))
             pages += shared // ps + sum(-(-m // ps) for m in plan[-1][2])
         width = max(1, max(s + max(-(-m // ps) for m in mine) for _, s, mine in plan)) + 1
+        if wide:
+            width = max(width, 32768 // ps)
         self.n_pages = pages + 2
         order_of = iter(rng.permutation(self.n_pages).tolist())
         dtype = C.TYPES[kind]
@@ -129,19 +132,21 @@ GROUPS = [
 @pytest.mark.parametrize("kind", list(C.TYPES))
 @pytest.mark.parametrize("nq,nkv,hd,ps,order", [(8, 2, 64, 16, "slot"), (32, 4, 128, 16, "head"), (15, 3, 80, 24, "slot"), (6, 6, 256, 7, "shared"), (40, 1, 16, 1, "head"), (4, 1, 192, 128, "head")])
 @pytest.mark.parametrize("groups", range(len(GROUPS)))
-def test_attention(moehip, kind, nq, nkv, hd, ps, order, groups):
-    print("shared attention", kind, nq, nkv, hd, ps, order, groups, flush=True)
-    b = Batch(moehip, kind, GROUPS[groups], nq, nkv, hd, ps, order, seed=hd + groups, listed=groups % 2 == 0, spare_rows=2 if groups % 2 == 0 else 0)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention(moehip, kind, nq, nkv, hd, ps, order, groups, wide):
+    print("shared attention", kind, nq, nkv, hd, ps, order, groups, wide, flush=True)
+    b = Batch(moehip, kind, GROUPS[groups], nq, nkv, hd, ps, order, seed=hd + groups, listed=groups % 2 == 0, spare_rows=2 if groups % 2 == 0 else 0, wide=wide)
     b.run(ldq=nq * hd + 5 if groups == 2 else None, ldo=nq * hd + 3 if groups == 3 else None)
 
 
 @pytest.mark.parametrize("kind", list(C.TYPES))
 @pytest.mark.parametrize("nq,nkv,hd,groups", [(4, 1, 64, [(6, 6000, (1, 300)), (2, 3000, (900, 1000))]), (8, 2, 80, [(17, 4500, (0, 140))]), (2, 1, 256, [(33, 2700, (1, 600))]),
                                               (8, 8, 128, [(1, 9000, (5, 6))]), (32, 2, 16, [(3, 12000, (1, 2000))])])
-def test_many_parts(moehip, kind, nq, nkv, hd, groups):
+@pytest.mark.parametrize("wide", [False, True])
+def test_many_parts(moehip, kind, nq, nkv, hd, groups, wide):
     """Prefixes and rows of their own long enough that a head's sums come in tens of parts, up to more than a wave's lanes."""
-    print("shared attention, many parts", kind, nq, nkv, hd, groups, flush=True)
-    Batch(moehip, kind, groups, nq, nkv, hd, 16, "head", seed=hd + 1).run()
+    print("shared attention, many parts", kind, nq, nkv, hd, groups, wide, flush=True)
+    Batch(moehip, kind, groups, nq, nkv, hd, 16, "head", seed=hd + 1, wide=wide).run()
 
 
 def test_rows_of_no_request_and_empty_ones(moehip):
@@ -157,15 +162,16 @@ def test_rows_of_no_request_and_empty_ones(moehip):
     b.run()
 
 
-def test_outside_and_bad_pages(moehip):
+@pytest.mark.parametrize("wide", [False, True])
+def test_outside_and_bad_pages(moehip, wide):
     """A request or position outside the tables, a page that is none: NaN in the rows that attend it, none else."""
-    b = Batch(moehip, "f16", [(6, 160, (1, 40)), (5, 80, (20, 20))], 8, 2, 64, 16, seed=3, spare_rows=1)
+    b = Batch(moehip, "f16", [(6, 160, (1, 40)), (5, 80, (20, 20))], 24, 2, 64, 16, seed=3, spare_rows=1, wide=wide)
     b.req[1], b.pos[3] = b.n_req, b.tables.shape[1] * 16
     b.tables[b.req[8], 5] = b.n_pages      # a page of its own
     b.upload()
     b.calls()
     b.check(nan_rows=(1, 3, 8))
-    b = Batch(moehip, "f32", [(6, 160, (1, 40)), (5, 80, (1, 40))], 8, 2, 64, 16, seed=4)
+    b = Batch(moehip, "f32", [(6, 160, (1, 40)), (5, 80, (1, 40))], 24, 2, 64, 16, seed=4, wide=wide)
     for t in range(6):
         b.tables[b.req[t], 4] = -1         # a page that the group shares
     b.upload()
@@ -174,9 +180,11 @@ def test_outside_and_bad_pages(moehip):
 
 
 @pytest.mark.parametrize("first", [[0, 4, 2, 9], [0, 10], [-1, 9], [9, 9, 9], [0, 0, 9, 9], [3, 3]], ids=str)
-def test_firsts(moehip, first):
+@pytest.mark.parametrize("wide", [False, True])
+def test_firsts(moehip, first, wide):
     """Empty groups, groups that are none: every row has its attention all the same."""
     Batch(moehip, "bf16", [(9, 128, (1, 20))], 4, 2, 64, 16, seed=5, first=first).run()
+    Batch(moehip, "bf16", [(9, 128, (1, 20))], 48, 2, 64, 16, seed=5, first=first, wide=wide).run()
 
 
 def test_rows_of_one_request(moehip):
