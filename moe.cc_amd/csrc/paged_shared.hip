@@ -800,9 +800,9 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 // when one is more than 2^kSlack above it, so that most steps need no sums across lanes.
 constexpr int type_size(int type) { return type == F32 ? 4 : type == E4M3 ? 1 : 2; }
 
-template <int CT, int HDP, int WC>
+template <int CT, int HDP, int WC, int CPW>
 struct TileShape {
-  static constexpr int S = type_size(CT), WP = kWaves / WC, CPW = HDP > 128 ? 1 : 2;
+  static constexpr int S = type_size(CT), WP = kWaves / WC;
   static constexpr int PW = CT == F32 ? 32 / WP : 32;    // positions of a step and a wave
   static constexpr int ROWS = PW * WP;             // of a step
   static constexpr int RB = HDP * (CT == F32 ? 4 : 2);   // bytes of a row in LDS
@@ -818,11 +818,11 @@ __device__ __forceinline__ u32x2 read_turned(const uint8_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
-template <int CT, int HDP, int WC>
+template <int CT, int HDP, int WC, int CPW>
 __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it, int kv, uint8_t* lds) {
-  using T = TileShape<CT, HDP, WC>;
+  using T = TileShape<CT, HDP, WC, CPW>;
   constexpr bool HALF = CT == F16 || CT == E4M3;
-  constexpr int NP = HALF ? 2 : CT == BF16 ? 3 : 1, S = T::S, CPW = T::CPW, RB = T::RB;
+  constexpr int NP = HALF ? 2 : CT == BF16 ? 3 : 1, S = T::S, RB = T::RB;
   constexpr int NK = CT == F32 ? HDP / 16 : HDP / 32, VE = HDP / 16, KT = T::PW / 16;
   constexpr int SETS = T::ROWS / 32;                              // (32 positions, q) that a wave stages
   constexpr int NL = (8 * HDP * S + 1023) / 1024;              // 16-byte loads of a lane for their keys
@@ -1131,11 +1131,11 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
   }
 }
 
-// WC: waves over a prefix item's columns; 0: the item in sixteens.  Prefix items first, of all heads, then the rows' own:
+// WC: waves over a prefix item's columns, CPW: their sixteens; 0: the item in sixteens.  Prefix items first, of all heads, then the rows' own:
 // the long ones start together.
-template <int CT, int HDP, int WC>
+template <int CT, int HDP, int WC, int CPW>
 __global__ __launch_bounds__(kThreads, WC || HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
-  constexpr int TILE = TileShape<CT, HDP, WC ? WC : 4>::BYTES, COLUMNS = (int)sizeof(ColumnsShared<HDP>);
+  constexpr int TILE = TileShape<CT, HDP, WC ? WC : 4, 1>::BYTES, COLUMNS = (int)sizeof(ColumnsShared<HDP>);
   constexpr int BYTES = WC && TILE > COLUMNS ? TILE : COLUMNS;
   __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
   const int subs = WC ? 1 : L.cut.columns / 16;
@@ -1150,7 +1150,7 @@ __global__ __launch_bounds__(kThreads, WC || HDP <= 128 ? 2 : 1) void shared_att
   if (!item_ok(L, it, parts, own ? L.cut.own_columns : L.cut.columns)) return;
   if constexpr (WC != 0) {
     if (!own) {
-      tile_block<CT, HDP, WC>(L, it, kv, lds);
+      tile_block<CT, HDP, WC, CPW>(L, it, kv, lds);
       return;
     }
   }
@@ -1246,10 +1246,10 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
   }
 }
 
-template <int CT, int HDP, int WC>
+template <int CT, int HDP, int WC, int CPW>
 hipError_t launch(SharedLaunch L, unsigned prefix, unsigned own, hipStream_t s) {
   L.prefix_blocks = (int)prefix;
-  hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, WC>), dim3((prefix + own) * (unsigned)L.g.map.n_kv), dim3(kThreads), 0, s, L);
+  hipLaunchKernelGGL((shared_attn_kernel<CT, HDP, WC, CPW>), dim3((prefix + own) * (unsigned)L.g.map.n_kv), dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
 
@@ -1257,14 +1257,14 @@ template <int CT, int HDP>
 hipError_t launch(const SharedLaunch& L, hipStream_t s) {
   const unsigned prefix = (unsigned)L.cut.prefix_items, own = (unsigned)L.cut.own_items;
   if constexpr (HDP <= 128) {
-    if (L.tiles) return launch<CT, HDP, 2>(L, prefix, own, s);
+    if (L.tiles) return L.cut.columns == kTile ? launch<CT, HDP, 2, 2>(L, prefix, own, s) : launch<CT, HDP, 2, 1>(L, prefix, own, s);
   } else if constexpr (CT != F32) {
     if (L.tiles) {
-      const hipError_t e = launch<CT, HDP, 4>(L, prefix, 0, s);
-      return e == hipSuccess ? launch<CT, HDP, 0>(L, 0, own, s) : e;
+      const hipError_t e = launch<CT, HDP, 4, 1>(L, prefix, 0, s);
+      return e == hipSuccess ? launch<CT, HDP, 0, 0>(L, 0, own, s) : e;
     }
   }
-  return launch<CT, HDP, 0>(L, prefix * (unsigned)(L.cut.columns / 16), own, s);
+  return launch<CT, HDP, 0, 0>(L, prefix * (unsigned)(L.cut.columns / 16), own, s);
 }
 
 template <int CT>
@@ -1281,11 +1281,12 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
   shared_work(L.cut, g.map.n_kv, g.map.head_dim, g.a.work, &L);
   L.by_group = make_divider((uint32_t)L.cut.group);
   L.by_kv = make_divider((uint32_t)g.map.n_kv);
-  // Items of 64 columns are taken whole, but where all of them in sixteens, at their longest, would be resident at once: then
-  // only a block's latency counts (us of bf16 pages, 64 over 8 heads of 128, whole and in sixteens: 8 rows of 600 positions
-  // 14.9, 12.0; 8 groups of 8 rows of 250 16.8, 14.6, of 600 18.6, 21.1).
-  const long long all = ((long long)g.a.T * L.cut.group + kTile - 1) / kTile, units = ((long long)g.a.max_pages * g.map.page_size + kUnit - 1) / kUnit;
-  L.tiles = L.cut.columns == kTile && (all > sh.n_groups ? all : sh.n_groups) * units * (kTile / 16) * g.map.n_kv > 2 * kCUs;
+  // Items of 32 and 64 columns are taken whole, but where all of them in sixteens, at their longest, would be resident at once:
+  // then only a block's latency counts (us of bf16 pages, 32 heads over 4 of 128, whole and in sixteens: 8 rows of 600
+  // positions 14.9, 12.0; 8 groups of 8 rows of 250 16.8, 14.6, of 600 18.6, 21.1).
+  const long long all = ((long long)g.a.T * L.cut.group + L.cut.columns - 1) / L.cut.columns, units = ((long long)g.a.max_pages * g.map.page_size + kUnit - 1) / kUnit;
+  L.tiles = (L.cut.columns == kTile || (L.cut.columns == kTile / 2 && g.map.head_dim <= 128)) &&
+            (all > sh.n_groups ? all : sh.n_groups) * units * (L.cut.columns / 16) * g.map.n_kv > 2 * kCUs;
   const hipError_t e = dtype == F32    ? launch<F32>(L, s)
                        : dtype == F16  ? launch<F16>(L, s)
                        : dtype == BF16 ? launch<BF16>(L, s)
