@@ -624,7 +624,8 @@ moe_status moe_paged_share_dev(const moe_paged_share* s);
 /* moe_paged_attn_dev's results (a, pages: its arguments), with each group's
  * prefix read once for all its rows instead of once a row.  s: as
  * moe_paged_share_dev was given it for the same rows, tables and heads.
- * work: moe_paged_attn_shared_work_bytes, else as moe_paged_attn's. */
+ * work: moe_paged_attn_shared_work_bytes, else as moe_paged_attn's.  Few rows of
+ * short prefixes (bf16: 8 of 600 positions) are as fast by moe_paged_attn_dev. */
 size_t moe_paged_attn_shared_work_bytes(int T, int n_groups, int n_q, int n_kv, int head_dim);
 moe_status moe_paged_attn_shared_dev(const moe_paged_attn* a, const moe_pages* pages, const moe_paged_share* s);
 

@@ -8,7 +8,11 @@
 // One read of the logits bounds it.  The first kernel cuts a row into blocks;
 // a wave takes 1024 logits a step, sums their exponentials and keeps the
 // n_beam best as a list sorted over its lanes.  The second, a block a group,
-// joins the rows' sums and lists and ranks the candidates of all rows.
+// joins the rows' sums and lists and ranks the candidates of all rows.  One
+// group of 4 beams over 151936 tokens takes 13.3 us, of which the launches and
+// the chain of a block's own work are most; 24 groups of 8 (117 MB) 40 us, the
+// first kernel's 31 of them at 3.5 TB/s, where its exponentials, 64-bit sums
+// and bounds keep the vector units as busy as the memory.
 //
 // Order.  Inside a row candidates are ordered by (logit, token), which a
 // 64-bit whole number holds exactly: the logit's bits as an ordered whole
@@ -36,7 +40,9 @@ constexpr int kStep = 16 * kWave;          // logits of a wave's step
 // From here on the blocks' lists are merged by a kernel of their own (one group, 151936 columns, us with it and without: 16
 // beams 29.8, 27.6; 32 beams 42, 58; 64 beams 69, 147).
 constexpr int kMergedBeams = 32;
-constexpr int kBlocks = 1024;              // blocks that rows are cut into, about
+// Blocks that rows are cut into, about: 16 waves a CU, and few enough lists for the second kernel (us at 512, 1024 and 2048, 8
+// beams: 24 groups 46.3, 39.5, 39.0; 64 groups 71.8, 66.2, 65.8; one group alike).
+constexpr int kBlocks = 1024;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));

@@ -11,8 +11,9 @@
 //   n - r          of the requests r that held it: the lowest gives it back, unless
 //   kStays         a request holds it now
 // Nothing is kept from one call for the next.  Latency bounds it: launch, the
-// requests' numbers, the tables.  (The pages' numbers in memory instead of LDS:
-// 64 requests 11.9 us, 1024 30.)
+// requests' numbers, the tables: 64 requests of 160 pages 9.2 us, 1024 of 512
+// (whose tables are 2 MB each way) 18.  (The pages' numbers in memory instead of
+// LDS: 11.9 and 30.)
 #include <initializer_list>
 
 #include "moe_device.h"
@@ -283,7 +284,7 @@ __device__ __forceinline__ void fork_finish(const ForkArgs& a, ForkHead top, int
   }
 }
 
-// Few entries: all of it in one block.
+// Few entries: all of it in one block, one launch (4 requests of 40 pages 5.7 us, 16 of 128 7.5; in columns 7.7, 9.0).
 constexpr int kOnePer = 2, kFewRequests = 1024;
 __global__ __launch_bounds__(kN) void fork_one_kernel(ForkArgs a) {
   __shared__ ForkShared<kFewRequests> sh;
@@ -334,7 +335,8 @@ struct CopyArgs {
   char* side[2 * kLayers];
 };
 
-// A block a (copy, pool): the first n positions of every head of a page.  All bytes are read once and written once.
+// A block a (copy, pool, head): the first n positions of a head of a page.  All bytes are read once and written once, which
+// bounds many copies (40 copies of 9 positions or so in 48 layers of 8 heads of 128, bf16: 12 us); of one the launch does, 4.4.
 __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const int32_t* c = a.copies + 3 * (size_t)blockIdx.x;
   const int src = c[0], dst = c[1], n = min(c[2], a.map.page_size);
@@ -410,7 +412,10 @@ moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
   a.f = *f;
   a.per = make_divider((uint32_t)f->page_size);
   const bool one = f->n_req <= kFewRequests && (long long)f->n_req * f->max_pages <= kOnePer * kN;
-  const int per = f->n_req <= 256 ? 1 : f->n_req <= 1024 ? 2 : 4;   // entries of a thread
+  // Entries of a thread: every block goes through all requests first, so with many of them fewer blocks are better (us with
+  // one and two: 64 requests of 160 pages 9.3, 10.4; 256 of 512 10.0, 11.9; 512 of 512 12.4, 12.4; 1024 of 512 23.5, 18.0).
+  // Past 1024 requests a column has to fit a block: four.
+  const int per = f->n_req <= 256 ? 1 : f->n_req <= 1024 ? 2 : 4;
   a.columns = one ? f->max_pages : per * kN / f->n_req;
   if (a.columns > f->max_pages) a.columns = f->max_pages;
   a.blocks = (f->max_pages + a.columns - 1) / a.columns;

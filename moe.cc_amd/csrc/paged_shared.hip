@@ -189,7 +189,8 @@ __device__ __forceinline__ int units_in_all(int positions) { return (positions +
 // One block: the groups' prefixes, and the items.  Prefix tiles' units (128 positions) and rows' own are each cut so that
 // their items are about as many as are resident at once: pieces of ceil(all units / slots), at least one an item, so no
 // more items than `slots` and one for each tile or row.  ONE: a thread a group and a row (at most N of each), whose numbers
-// stay in its registers and LDS; else they go around through the plan, N at a time.  Latency bounds it.
+// stay in its registers and LDS; else they go around through the plan, N at a time.  Latency bounds it (us with both kernels:
+// 8 groups of 8 rows 10.3 with 256 threads, 11.6 with 1024, 12.8 around through the plan; 120 groups of 8 16.7 and 28.0).
 template <int N>
 struct PlanShared {
   int wave[N / kWave];
@@ -503,7 +504,8 @@ __device__ __forceinline__ Column column_of(const SharedLaunch& L, const Item& x
 //   values   lane l holds the keys 4 (l / 16) + i of both tiles at its 1 / 16 of the dimensions; pairs of keys are put side by
 //            side by byte permutes
 // 16-bit operands: bf16 pages with queries and weights in three parts; f16 and 8-bit pages (exact in f16) in two f16 parts.
-// fp32 pages use the fp32 instruction.
+// fp32 pages use the fp32 instruction.  A block's own chain of latencies bounds few rows: one group of 4 rows of 550 positions,
+// 32 heads over 4 of 128, fp32, takes 14 us with the join, of 1000 shared by 8 groups of 4, bf16, 19 (15 in tiles, below).
 template <int HDP>
 struct ColumnsShared {   // 128 dimensions at a time
   float o[kWaves][HDP > 128 ? HDP / 2 : HDP][17], m[kWaves][16], l[kWaves][16], div[16];
@@ -790,14 +792,22 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 
 // ---------------------------------------------------------------- many columns
 
-// A block takes an item of up to 64 columns: WC waves lie beside each other over the columns, 32 each (16 where head_dim is
-// past 128), the others over the positions, 32 each of a step (fp32 pages: 16).  K and V of a step go through LDS, a
+// A block takes an item of up to 32 or 64 columns: WC waves lie beside each other over the columns, CPW sixteens each, the
+// others over the positions, 32 each of a step (fp32 pages: 16).  K and V of a step go through LDS, a
 // step ahead, where the waves over the columns share them: rows of 16-bit values in 16-byte pieces, piece p of row r at
 // p ^ swizzle(r), so that the reads of both lie evenly over the banks.  Keys are read as rows; a value operand, 8 keys of one
 // dimension, is two reads that turn 4 rows x 16 dimensions around on their way.  16-bit pages go straight from memory into
 // LDS, 8-bit pages become f16 in registers.  A wave stages the 8 rows of one (32 positions, quad of lanes that reads them),
 // whose addresses lie in its lanes, found once for K and V.  One barrier a step.  A column's largest score is raised only
-// when one is more than 2^kSlack above it, so that most steps need no sums across lanes.
+// when one is more than 2^kSlack above it, so that most steps need no sums across lanes.  fp32 pages lie in LDS as they are and
+// use the fp32 instruction: a lane's 16 bytes of a key or a value are four operands.
+//
+// 32 heads over 4 of 128, us, and of sixteens: bf16, 8 groups of 4 rows of 4000 positions 26, 34; of 8 rows 33, 52; 64 rows of
+// 8000 41, 85.  Matrix instructions bound many rows: 64 of 16000 are 16.8 GFLOP, which fp32 does in 161 us (104 TFLOP/s of the
+// 153 that a large product reaches here), bf16 in 58, its three parts at 0.87 PFLOP/s of 1.23, 8-bit pages in 54.  What the
+// parts' instructions leave is the weights' arithmetic (two waves of a SIMD hardly overlap it with matrix instructions) and
+// about 10 us of a block's start and end.  Items of 128 columns gain 4 % where all is large and lose 10 % elsewhere (16 rows
+// of 3800 20.6, with 128 22.6).
 constexpr int type_size(int type) { return type == F32 ? 4 : type == E4M3 ? 1 : 2; }
 
 template <int CT, int HDP, int WC, int CPW>
@@ -1160,20 +1170,28 @@ __global__ __launch_bounds__(kThreads, WC || HDP <= 128 ? 2 : 1) void shared_att
 
 // ---------------------------------------------------------------- the join
 
-// A wave a (row, query head): its parts joined, four dimensions a lane, so that 64 / (head_dim / 4) parts are read side by
+// Up to this many (row, query head) a block each, whose waves take its parts in turn: few rows of long prefixes have the most
+// parts (us with that and a wave each, one group, 32 heads: 4 rows of 16000 positions 23.7, 35.1; 8 of 8000 19.9, 23.4; 32 of
+// 3800 28.3, 28.9; 8 groups of 8 rows of 1000 21.7, 20.5).
+constexpr int kFewHeads = 1024;
+
+// W waves a (row, query head): its parts joined, four dimensions a lane, so that 64 / (head_dim / 4) parts are read side by
 // side.  Latency: the parts' first rows are requested with their maxima.
+template <int W>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
   constexpr int U = 4;
+  __shared__ f32x4 acc_s[W][W > 1 ? kWave : 1];
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
-  const int t = (int)blockIdx.x, head = __builtin_amdgcn_readfirstlane((int)blockIdx.y * kWaves + (int)threadIdx.x / kWave);
+  const int t = (int)blockIdx.x, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int head = (int)blockIdx.y * (kWaves / W) + wave / W, w = wave % W;   // (W = 1, 4: a block's waves end together)
   const int hd = g.map.head_dim, lane = threadIdx.x % kWave;
   if (head >= a.n_q) return;
   const RowPlan r = L.p.rows[t];
   if (r.state == kLeave || r.state == kDone) return;
   float* out = a.out + (size_t)t * a.ldo + (size_t)head * hd;
   if (r.state != kJoin) {
-    for (int d = lane; d < hd; d += kWave) out[d] = r.state == kZero ? 0.0f : NAN;
+    for (int d = w * kWave + lane; d < hd; d += W * kWave) out[d] = r.state == kZero ? 0.0f : NAN;
     return;
   }
   const int G = L.cut.group, kv = (int)divide((uint32_t)head, L.by_group), h = head - kv * G;
@@ -1196,7 +1214,7 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
   const int width = hd / 4, rows = kWave / width, row = lane / width, d = lane % width * 4;
   f32x4 y[U];
 #pragma unroll
-  for (int x = 0; x < U; ++x) y[x] = o_of(min(row + x * rows, n - 1), d);
+  for (int x = 0; x < U; ++x) y[x] = o_of(min(w * U * rows + row + x * rows, n - 1), d);
   const float2 first = ml_of(min(lane, n - 1));
   float top = first.x;
   if (n > kWave)
@@ -1213,8 +1231,8 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
     }
   sum = wave_total(sum);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i0 = 0; i0 < n; i0 += U * rows) {
-    if (i0) {
+  for (int i0 = w * U * rows; i0 < n; i0 += W * U * rows) {
+    if (i0 >= W * U * rows) {
 #pragma unroll
       for (int x = 0; x < U; ++x) y[x] = o_of(min(i0 + row + x * rows, n - 1), d);
     }
@@ -1232,6 +1250,13 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedLaunch L) {
         if (row < rows && i < n) acc += y[x] * exp2_hw(ml_of(i).x - top);
       }
     }
+  }
+  if constexpr (W > 1) {
+    acc_s[w][lane] = acc;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) acc += acc_s[i][lane];
   }
   // the lanes of a dimension: row by row
   f32x4 all = acc;
@@ -1292,7 +1317,10 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
                        : dtype == BF16 ? launch<BF16>(L, s)
                                        : launch<E4M3>(L, s);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(shared_join_kernel, dim3((unsigned)g.a.T, (unsigned)(g.a.n_q + kWaves - 1) / kWaves), dim3(kThreads), 0, s, L);
+  if ((long long)g.a.T * g.a.n_q <= kFewHeads)
+    hipLaunchKernelGGL(shared_join_kernel<kWaves>, dim3((unsigned)g.a.T, (unsigned)g.a.n_q), dim3(kThreads), 0, s, L);
+  else
+    hipLaunchKernelGGL(shared_join_kernel<1>, dim3((unsigned)g.a.T, (unsigned)(g.a.n_q + kWaves - 1) / kWaves), dim3(kThreads), 0, s, L);
   return hipGetLastError();
 }
 
@@ -1350,6 +1378,9 @@ moe_status moe_paged_attn_shared_dev(const moe_paged_attn* a, const moe_pages* g
   const size_t need = moe_paged_attn_shared_work_bytes(a->T, s->n_groups, a->n_q, map.n_kv, map.head_dim);
   if (a->work_bytes < need || (uintptr_t)a->work % 16)
     return set_error(MOE_ERR_ARG, "paged_attn_shared: %zu bytes of work at %p, %zu needed, 16-byte aligned", a->work_bytes, a->work, need);
+  const ShareCut cut = share_cut(a->T, s->n_groups, a->n_q, map.n_kv, map.head_dim);
+  if (((long long)cut.prefix_items * (cut.columns / 16) + cut.own_items) * map.n_kv >= 1 << 24)   // (a launch holds fewer than 2^32 threads)
+    return set_error(MOE_ERR_UNSUPPORTED, "paged_attn_shared: %d rows in %d groups for %d heads over %d", a->T, s->n_groups, a->n_q, map.n_kv);
   if ((st = ensure_init())) return st;
   OnDevice on;
   if ((st = on.enter())) return st;

@@ -103,6 +103,17 @@ def test_shared_attention_refused(bad):
 
 
 @needs_lib
+def test_shared_attention_of_too_many_blocks_refused():
+    """2^24 rows' heads: more threads than a launch holds."""
+    import moehip as M
+    rows = dict(T=16384, n_req=16384, n_q=1024)
+    a = _attn(**rows, ldq=1 << 16, ldo=1 << 16, work_bytes=1 << 60)
+    g = _pages(n_kv=1024, head_stride=64, slot_stride=1 << 16, page_stride=1 << 20)
+    s = _share(**rows, n_kv=1024, plan_bytes=1 << 60)
+    _refused(M.lib().moe_paged_attn_shared_dev(ctypes.byref(a), ctypes.byref(g), ctypes.byref(s)), UNSUPPORTED)
+
+
+@needs_lib
 def test_work_of_refused_sizes():
     import moehip as M
     L = M.lib()
