@@ -9,8 +9,8 @@
 // a wave takes 1024 logits a step, sums their exponentials and keeps the
 // n_beam best as a list sorted over its lanes.  The second, a block a group,
 // joins the rows' sums and lists and ranks the candidates of all rows.  One
-// group of 4 beams over 151936 tokens takes 13.3 us, of which the launches and
-// the chain of a block's own work are most; 24 groups of 8 (117 MB) 40 us, the
+// group of 4 beams over 151936 tokens takes 13.0 us, of which the launches and
+// the chain of a block's own work are most; 24 groups of 8 (117 MB) 38.5 us, the
 // first kernel's 31 of them at 3.5 TB/s, where its exponentials, 64-bit sums
 // and bounds keep the vector units as busy as the memory.
 //
@@ -37,9 +37,11 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostBeams = kWave;          // a list is a lane a beam
 constexpr int kStep = 16 * kWave;          // logits of a wave's step
-// From here on the blocks' lists are merged by a kernel of their own (one group, 151936 columns, us with it and without: 16
-// beams 29.8, 27.6; 32 beams 42, 58; 64 beams 69, 147).
-constexpr int kMergedBeams = 32;
+// From here on a wave collects its candidates, sorts 64 at a time and merges them into its list, and blocks' lists are merged by
+// a kernel of their own; below, candidates are inserted one by one (one group over 151936 tokens, us with the first and the
+// second: 8 beams 25.0, 18.2; 16 27.1, 27.4; 24 28.9, 44.1; 32 30.5, 57.5; 24 groups of 8 52, 39; 200 groups of 64 over 1000
+// tokens 158, 707).
+constexpr int kMergedBeams = 17;
 // Blocks that rows are cut into, about: 16 waves a CU, and few enough lists for the second kernel (us at 512, 1024 and 2048, 8
 // beams: 24 groups 46.3, 39.5, 39.0; 64 groups 71.8, 66.2, 65.8; one group alike).
 constexpr int kBlocks = 1024;
@@ -78,6 +80,81 @@ __device__ __forceinline__ float before(uint32_t u) { return unordered(u - (u ==
 __device__ __forceinline__ uint64_t read_lane(uint64_t x, int l) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
          (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+}
+
+// The value of lane ^ C, C a power of two.
+template <int C>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+  if constexpr (C == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, false);   // quad_perm [1,0,3,2]
+  if constexpr (C == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, false);   // quad_perm [2,3,0,1]
+  if constexpr (C == 4) {   // row_half_mirror (^ 7), quad_perm [3,2,1,0]
+    x = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, false);
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x1B, 0xf, 0xf, false);
+  }
+  if constexpr (C == 8) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false);  // row_ror 8
+  if constexpr (C == 16) {
+    auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? p[0] : p[1];
+  }
+  if constexpr (C == 32) {
+    auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? p[0] : p[1];
+  }
+}
+// Of lane 63 - i.
+__device__ __forceinline__ uint32_t lane_mirror(uint32_t x) {
+  x = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, false);   // row_mirror
+  return lane_xor<32>(lane_xor<16>(x));
+}
+template <int C>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t x) {
+  return (uint64_t)lane_xor<C>((uint32_t)(x >> 32)) << 32 | lane_xor<C>((uint32_t)x);
+}
+__device__ __forceinline__ uint64_t lane_mirror(uint64_t x) {
+  return (uint64_t)lane_mirror((uint32_t)(x >> 32)) << 32 | lane_mirror((uint32_t)x);
+}
+
+// A candidate of a group: its place in the order of all (larger first; 0: none), then row * 64 + its place in the row's list
+// (the lower goes first where ranks are equal).
+struct Best {
+  uint64_t rank;
+  uint32_t from;
+};
+template <int C>
+__device__ __forceinline__ Best lane_xor(Best x) { return {lane_xor<C>(x.rank), lane_xor<C>(x.from)}; }
+__device__ __forceinline__ Best lane_mirror(Best x) { return {lane_mirror(x.rank), lane_mirror(x.from)}; }
+
+__device__ __forceinline__ bool precedes(uint64_t x, uint64_t y) { return x > y; }
+__device__ __forceinline__ bool precedes(Best x, Best y) { return x.rank > y.rank || (x.rank == y.rank && x.from < y.from); }
+
+// Runs of 2 C lanes that rise and fall once, sorted: the first to the lowest lane where `down`, else to the highest.
+template <int C, class T>
+__device__ __forceinline__ T sort_runs(T x, bool down) {
+  const T y = lane_xor<C>(x);
+  if (precedes(x, y) != (((threadIdx.x & C) == 0) == down)) x = y;
+  if constexpr (C > 1) x = sort_runs<C / 2>(x, down);
+  return x;
+}
+
+// The lanes', sorted, the first to lane 0 (bitonic); of which only the first n hold any.
+template <class T>
+__device__ __forceinline__ T sort_lanes(T x, int n = kWave) {
+  const int lane = threadIdx.x % kWave;
+  if (n > 1) x = sort_runs<1>(x, !(lane & 2));
+  if (n > 2) x = sort_runs<2>(x, !(lane & 4));
+  if (n > 4) x = sort_runs<4>(x, !(lane & 8));
+  if (n > 8) x = sort_runs<8>(x, !(lane & 16));
+  if (n > 16) x = sort_runs<16>(x, !(lane & 32));
+  if (n > 32) x = sort_runs<32>(x, true);
+  return x;
+}
+
+// The first 64 of two lists sorted over the lanes, sorted: of lane i's and the other's 63 - i'th the first, which fall and rise
+// once.
+template <class T>
+__device__ __forceinline__ T merge_lists(T a, T b) {
+  const T other = lane_mirror(b);
+  return sort_runs<32>(precedes(other, a) ? other : a, true);
 }
 
 // A list sorted over the lanes, the largest first; 0: nothing there.
@@ -184,6 +261,7 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   // what the block's n_beam-th has to reach at least, as an ordered number: after the first step the least of the waves'
   // share-th (share = n_beam / 4, rounded up), then any wave's n_beam-th
   __shared__ uint32_t share_s[kWaves], least_s;
+  __shared__ uint64_t pending_s[kWaves][2 * kWave];
   f32x4 next[4];
   auto load = [&](int step) {
     const int v0 = step * kStep + 4 * lane;
@@ -257,9 +335,37 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
     // of the lanes' largest the K-th bounds the K-th of all from below
     uint32_t bound = kOrderedNone + 1;
     if (__popcll(better) > K) bound = max(bound, nth_largest(top > least ? ordered(top) : 0u, K));
-    const float pass = fmaxf(before(bound), least);
+    float pass = fmaxf(before(bound), least);
+    if (K >= kMergedBeams) {   // many: 64 at a time, sorted and merged
+      auto take = [&](int n) {
+        list.key = merge_lists(list.key, sort_lanes(lane < n ? pending_s[wave][lane] : 0));
+        list.last = read_lane(list.key, K - 1);
+        if (list.last) pass = fmaxf(pass, before((uint32_t)(list.last >> 32)));
+      };
+      int n = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 16; ++j) {
+        const uint64_t who = __ballot(x[j] > pass);
+        if (!who) continue;
+        const uint32_t token = (uint32_t)(step * kStep + j / 4 * 4 * kWave + 4 * lane + j % 4);
+        if (x[j] > pass)
+          pending_s[wave][n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
+              (uint64_t)ordered(x[j]) << 32 | (0xffffffffu - token);
+        n += __popcll(who);
+        if (n < kWave) continue;
+        __builtin_amdgcn_wave_barrier();
+        take(kWave);
+        n -= kWave;
+        const uint64_t rest = pending_s[wave][kWave + lane];
+        __builtin_amdgcn_wave_barrier();
+        pending_s[wave][lane] = rest;
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (n) take(n);
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int j = 0; j < 16 && K < kMergedBeams; ++j) {
       uint64_t who = __ballot(x[j] > pass);
       while (who) {
         const int l = __builtin_ctzll(who);
@@ -285,10 +391,13 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   const int mine = threadIdx.x % kWave;
   if (mine < K && key_s[wave][mine]) {
     const uint64_t k = key_s[wave][mine];
-    int rank = 0;
+    int before[kWaves] = {}, rank = 0;   // of each wave's list, by bisection
+    for (int half = 1 << (31 - __builtin_clz(K)); half; half /= 2)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      for (int i = 0; i < K; ++i) rank += key_s[w][i] > k;
+      for (int w = 0; w < kWaves; ++w)
+        if (before[w] + half <= K && key_s[w][before[w] + half - 1] > k) before[w] += half;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) rank += before[w];
     if (rank < K) best_s[rank] = k;
   }
   __syncthreads();
@@ -303,22 +412,42 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   }
 }
 
-// The 64 largest of two lists sorted over the lanes, sorted: of lane i's and the other's 63 - i'th the larger, which rise and
-// fall once, then six exchanges.
-__device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b) {
+// exp's sum of a row from its parts, as what a logit is added to: score - lse; NaN where there is none.
+__device__ __forceinline__ double base_of(const SelectArgs& s, int row, float score) {
   const int lane = threadIdx.x % kWave;
-  const uint64_t other = __shfl(b, kWave - 1 - lane);
-  uint64_t x = a > other ? a : other;
-#pragma unroll
-  for (int c = kWave / 2; c; c /= 2) {
-    const uint64_t y = __shfl_xor(x, c);
-    x = (lane & c) == 0 ? (x > y ? x : y) : (x > y ? y : x);
-  }
-  return x;
+  const Part* p = s.parts + (size_t)row * s.blocks;
+  double most = -(double)INFINITY;
+  for (int c = lane; c < s.blocks; c += kWave) most = fmax(most, p[c].at);
+  most = wave_max_f64(most);
+  double sum = 0.0;
+  for (int c = lane; c < s.blocks; c += kWave) sum += part_at(p[c], most);
+  sum = wave_sum(sum);
+  if (!(sum > 0.0 && sum < (double)INFINITY)) return NAN;   // (a NaN or +inf among the logits makes it NaN)
+  return (double)score - (most + log(sum));
 }
 
-// Many beams: a block a row merges its blocks' lists, into the first one's place.  (Inserted one by one by the next kernel, a
-// wave a row: 64 beams 147 us.)
+// A candidate's place in the order of all, larger first: value * weight as an ordered whole number, above 0.
+__device__ __forceinline__ uint64_t rank_of(double value, double weight) {
+  const uint64_t bits = (uint64_t)__double_as_longlong(value * weight + 0.0);
+  return bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+
+__device__ __forceinline__ double value_of(double base, uint64_t key) { return base + (double)unordered((uint32_t)(key >> 32)); }
+
+__device__ __forceinline__ void write_choice(const moe_beam_select& a, int to, int parent, bool done, double value, uint64_t key) {
+  const int token = done ? a.pad : (int)(0xffffffffu - (uint32_t)key), ends = done || token == a.eos;
+  a.parent[to] = parent;
+  a.token[to] = token;
+  a.score_out[to] = (float)value;
+  a.done_out[to] = ends;
+  a.fresh[to] = !ends;
+}
+
+__device__ __forceinline__ void write_none(const moe_beam_select& a, int to) {
+  a.parent[to] = a.token[to] = -1, a.score_out[to] = -INFINITY, a.done_out[to] = a.fresh[to] = 0;
+}
+
+// Many beams: a block a row merges its blocks' lists, into the first one's place, and its sums.
 __global__ __launch_bounds__(kThreads) void select_merge_kernel(SelectArgs s) {
   const moe_beam_select& a = s.a;
   const int row = (int)blockIdx.x, K = a.n_beam, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -334,20 +463,68 @@ __global__ __launch_bounds__(kThreads) void select_merge_kernel(SelectArgs s) {
   __shared__ uint64_t list_s[kWaves][kWave];
   list_s[wave][lane] = best;
   __syncthreads();
+  if (wave == 1) {
+    const double base = base_of(s, row, a.score[row]);
+    if (lane == 0) s.parts[(size_t)row * s.blocks].sum = base;
+  }
   if (wave) return;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) best = merge_lists(best, list_s[w][lane]);
   if (lane < K) keys[lane] = best;
 }
 
-// A block a group; a wave a row, then one wave merges the rows' lists, a lane each.
+// Then a block a group: a wave merges every sixteenth row's candidates, four of the waves theirs, the first these.
+__global__ __launch_bounds__(1024) void select_many_kernel(SelectArgs s) {
+  const moe_beam_select& a = s.a;
+  constexpr int W = 1024 / kWave, R = kMostBeams / W;
+  const int K = a.n_beam, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, row0 = (int)blockIdx.x * K;
+  __shared__ uint64_t key_s[kMostBeams][kMostBeams], rank_s[W][kWave];
+  __shared__ uint32_t from_s[W][kWave];
+  __shared__ int done_s[kMostBeams];
+  __shared__ double base_s[kMostBeams];
+  Best best[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int mine = wave + i * W, row = row0 + min(mine, K - 1);
+    const bool use = mine < K && usable(a, row), done = a.done && a.done[row];
+    const float score = a.score[row];
+    const double weight = a.weight ? (double)a.weight[row] : 1.0, base = done ? (double)score : use ? s.parts[(size_t)row * s.blocks].sum : NAN;
+    const uint64_t key = !use || base != base ? 0 : done ? lane == 0 : lane < K ? s.keys[(size_t)row * K * s.blocks + lane] : 0;
+    best[i].rank = key ? rank_of(done ? base : value_of(base, key), weight) : 0;
+    best[i].from = mine * kWave + lane;
+    key_s[mine][lane] = key;
+    if (lane == 0) base_s[mine] = base, done_s[mine] = done;
+  }
+#pragma unroll
+  for (int i = 1; i < R; ++i) best[0] = merge_lists(best[0], best[i]);
+  for (int n = W; n > 1; n /= 4) {
+    if (wave < n) rank_s[wave][lane] = best[0].rank, from_s[wave][lane] = best[0].from;
+    __syncthreads();
+    if (wave < n / 4)
+      for (int i = 1; i < 4; ++i) best[0] = merge_lists(best[0], Best{rank_s[wave + i * (n / 4)][lane], from_s[wave + i * (n / 4)][lane]});
+    __syncthreads();
+  }
+  if (wave || lane >= K) return;
+  const int mine = best[0].from / kWave;
+  if (!best[0].rank) return write_none(a, row0 + lane);
+  const uint64_t key = key_s[mine][best[0].from % kWave];
+  const bool done = done_s[mine];
+  write_choice(a, row0 + lane, row0 + mine, done, done ? base_s[mine] : value_of(base_s[mine], key), key);
+}
+
+// A block a group: a wave a row, then all rows' candidates sorted at once (taken one by one, the best of a lane a row each time,
+// 8 beams take 0.9 us more, 16 2.5).  One beam has nothing to sort: the code of it, jumped over, costs 1 us of 10 in fetches.
+constexpr int kSorted = 4;   // waves that sort: 16 beams of up to 16 candidates
+static_assert(kMergedBeams <= 17);
 __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
   const moe_beam_select& a = s.a;
   constexpr int W = 1024 / kWave;
   const int K = a.n_beam, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, row0 = (int)blockIdx.x * K;
-  __shared__ uint64_t key_s[kMostBeams][kMostBeams];
-  __shared__ double base_s[kMostBeams], weight_s[kMostBeams];
-  __shared__ int count_s[kMostBeams], done_s[kMostBeams];
+  __shared__ uint64_t key_s[kMergedBeams][kMergedBeams];
+  __shared__ double base_s[kMergedBeams], weight_s[kMergedBeams];
+  __shared__ int count_s[kMergedBeams], done_s[kMergedBeams];
+  __shared__ uint64_t rank_s[kSorted][kWave];
+  __shared__ uint32_t from_s[kSorted][kWave];
   for (int i = wave; i < K; i += W) {
     const int row = row0 + i;
     const bool use = usable(a, row), done = a.done && a.done[row];
@@ -360,18 +537,10 @@ __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
       count = 1;
       list.key = lane == 0 ? 1 : 0;
     } else if (use) {
-      const Part* p = s.parts + (size_t)row * s.blocks;
-      double most = -(double)INFINITY;
-      for (int c = lane; c < s.blocks; c += kWave) most = fmax(most, p[c].at);
-      most = wave_max_f64(most);
-      double sum = 0.0;
-      for (int c = lane; c < s.blocks; c += kWave) sum += part_at(p[c], most);
-      sum = wave_sum(sum);
-      if (sum > 0.0 && sum < (double)INFINITY) {   // (a NaN or +inf among the logits makes it NaN)
-        base = (double)score - (most + log(sum));
+      base = base_of(s, row, score);
+      if (base == base) {
         const uint64_t* keys = s.keys + (size_t)row * K * s.blocks;
-        if (s.merged) list.key = lane < K ? keys[lane] : 0;
-        for (int c0 = s.merged ? K * s.blocks : 0; c0 < K * s.blocks; c0 += kWave) {
+        for (int c0 = 0; c0 < K * s.blocks; c0 += kWave) {
           const uint64_t k = c0 + lane < K * s.blocks ? keys[c0 + lane] : 0;
           if (!__any(k > list.last)) continue;
           const uint32_t bound = nth_largest(k > list.last ? (uint32_t)(k >> 32) : 0u, K);
@@ -390,35 +559,28 @@ __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
     if (lane == 0) count_s[i] = count, base_s[i] = base, done_s[i] = done, weight_s[i] = weight;
   }
   __syncthreads();
-  if (wave) return;
-  // ---- lane i: row i's best candidate that is left; the best of all goes first, of equal ones the lowest row's
-  const int mine = min(lane, K - 1), count = lane < K ? count_s[mine] : 0;
-  const bool done = done_s[mine];
-  const double base = base_s[mine], weight = weight_s[mine];
-  int at = 0;
-  uint64_t key = key_s[mine][0];
-  auto value = [&]() { return done ? base : base + (double)unordered((uint32_t)(key >> 32)); };
-  for (int i = 0; i < K; ++i) {
-    const uint64_t bits = (uint64_t)__double_as_longlong(value() * weight + 0.0);
-    const uint64_t rank = at < count ? (bits >> 63 ? ~bits : bits | 1ull << 63) : 0;
-    const uint32_t hi = wave_max((uint32_t)(rank >> 32));
-    const uint32_t lo = wave_max((uint32_t)(rank >> 32) == hi ? (uint32_t)rank : 0u);
-    const uint64_t best = __ballot(at < count && rank == ((uint64_t)hi << 32 | lo));
-    const int to = row0 + i;
-    if (!best) {
-      if (lane == 0) a.parent[to] = a.token[to] = -1, a.score_out[to] = -INFINITY, a.done_out[to] = a.fresh[to] = 0;
-      continue;
-    }
-    if (lane == __builtin_ctzll(best)) {
-      const int token = done ? a.pad : (int)(0xffffffffu - (uint32_t)key), ends = done || token == a.eos;
-      a.parent[to] = row0 + lane;
-      a.token[to] = token;
-      a.score_out[to] = (float)value();
-      a.done_out[to] = ends;
-      a.fresh[to] = !ends;
-      if (++at < count) key = key_s[mine][at];
-    }
+  // ---- all candidates a lane each, 1 << side lanes a row, sorted; past 64 of them by as many waves, whose lists the first one
+  // merges
+  const int side = K <= 1 ? 0 : 32 - __builtin_clz(K - 1), waves = ((K << side) + kWave - 1) / kWave;
+  Best best = {0, (uint32_t)tid};
+  if (wave < waves) {
+    const int mine = min(tid >> side, K - 1), at = tid & ((1 << side) - 1);
+    best.from = (uint32_t)(mine * kWave + at);
+    if (tid >> side < K && at < count_s[mine]) best.rank = rank_of(done_s[mine] ? base_s[mine] : value_of(base_s[mine], key_s[mine][at]), weight_s[mine]);
+    if (K > 1) best = sort_lanes(best, K << side);
   }
+  if (waves > 1) {
+    if (wave < waves) rank_s[wave][lane] = best.rank, from_s[wave][lane] = best.from;
+    __syncthreads();
+  }
+  if (wave) return;
+  for (int w = 1; w < waves; ++w) best = merge_lists(best, Best{rank_s[w][lane], from_s[w][lane]});
+  if (lane >= K) return;
+  if (!best.rank) return write_none(a, row0 + lane);
+  const int mine = (int)best.from / kWave;
+  const uint64_t key = key_s[mine][best.from % kWave];
+  const bool done = done_s[mine];
+  write_choice(a, row0 + lane, row0 + mine, done, done ? base_s[mine] : value_of(base_s[mine], key), key);
 }
 
 // Blocks that a row is cut into: as many steps a wave as leave about kBlocks in all.
@@ -470,7 +632,7 @@ moe_status moe_beam_select_dev(const moe_beam_select* a) {
   SelectArgs s;
   s.a = *a;
   s.blocks = blocks_for(rows, a->vocab);
-  s.merged = a->n_beam >= kMergedBeams && s.blocks > 1;
+  s.merged = a->n_beam >= kMergedBeams;
   s.parts = (Part*)a->work;
   s.keys = (uint64_t*)(s.parts + (size_t)rows * s.blocks);
   hipLaunchKernelGGL(select_rows_kernel, dim3((unsigned)s.blocks, (unsigned)rows), dim3(kThreads), 0, stream(), s);
@@ -479,7 +641,7 @@ moe_status moe_beam_select_dev(const moe_beam_select* a) {
     hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream(), s);
     if ((st = check_hip(hipGetLastError(), "beam_select launch"))) return st;
   }
-  hipLaunchKernelGGL(select_groups_kernel, dim3((unsigned)a->n_groups), dim3(1024), 0, stream(), s);
+  hipLaunchKernelGGL(s.merged ? select_many_kernel : select_groups_kernel, dim3((unsigned)a->n_groups), dim3(1024), 0, stream(), s);
   return check_hip(hipGetLastError(), "beam_select launch");
 }
 
