@@ -74,7 +74,11 @@ ShareCut share_cut(int T, int n_groups, int n_q, int n_kv, int head_dim) {
   c.columns = 1 << c.shift;
   c.own_columns = c.group < 16 ? c.group : 16;
   c.own_tiles = (c.group + 15) / 16;
-  const int resident = kCUs * (head_dim <= 128 ? 2 : 1);
+  // Two blocks a CU are resident; as many pieces pay where the products do (bf16, us with two and with one: 64 rows of 8000 41.0,
+  // 45.2; 8 groups of 8 rows of 4000 33.6, 32.6), else the parts that a piece more writes and the join reads cost more than
+  // they gain (32 groups of 4 rows of 1000 27.7, 23.8; 4 of 4 of 4000 21.9, 17.2; 4 rows of 16000 24.2, 17.6; twice the
+  // pieces: 8 of 8 of 4000 43.3, 64 of 8000 48.2).
+  const int resident = kCUs * (head_dim <= 128 && c.columns == kTile ? 2 : 1);
   c.slots = resident > n_kv ? resident / n_kv : 1;
   c.prefix_items = c.slots + (int)((long long)T * c.group / c.columns) + n_groups;
   c.own_slots = 2 * kCUs > n_kv ? 2 * kCUs / n_kv : 1;
