@@ -353,16 +353,16 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
               (uint64_t)ordered(x[j]) << 32 | (0xffffffffu - token);
         n += __popcll(who);
         if (n < kWave) continue;
-        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         take(kWave);
         n -= kWave;
         const uint64_t rest = pending_s[wave][kWave + lane];
-        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         pending_s[wave][lane] = rest;
       }
-      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       if (n) take(n);
-      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
     for (int j = 0; j < 16 && K < kMergedBeams; ++j) {

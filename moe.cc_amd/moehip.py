@@ -646,7 +646,8 @@ class Model:
             raise MoeError(f"a search of {n_beam} beams over {len(prompts)} prompts, {n_new} new tokens")
         width = -(-(max(p.size for p in prompts) + n_new) // page_size)
         cfg = self.cfg
-        cache = PagedCache(cfg.n_layers, cfg.n_kv, cfg.head_dim, R * width if n_pages is None else n_pages, page_size,
+        # (a fork takes the pages of its copies before it gives any back: one a beam more than they hold)
+        cache = PagedCache(cfg.n_layers, cfg.n_kv, cfg.head_dim, R * (width + 1) if n_pages is None else n_pages, page_size,
                            R, width, max(R, sum(p.size for p in prompts)), dtype)
         # the prompts, each its group's first request
         fresh = np.zeros(R, np.int32)
@@ -661,6 +662,7 @@ class Model:
         score = np.where(np.arange(R) % n_beam == 0, 0, -np.inf).astype(np.float32)
         state = {"score": DeviceBuffer.from_array(score), "done": DeviceBuffer.from_array(np.zeros(R, np.int32))}
         told = DeviceBuffer(n_new * 2 * R * 4)   # parents and tokens of every step
+        status = DeviceBuffer.from_array(np.zeros((n_new, 2), np.int32))
         need = lib().moe_beam_select_work_bytes(G, n_beam, V)
         work = DeviceBuffer(need)
         for i in range(n_new):
@@ -671,15 +673,18 @@ class Model:
                 check(lib().moe_beam_select_dev(ctypes.byref(sel)), "moe_beam_select_dev")
                 break
             fork = cache.fork_args(parent)
+            fork.status, cache.plan.status = status.ptr + 8 * i, status.ptr + 8 * i + 4
             check(lib().moe_model_step_beams(self.h, ctypes.byref(sel), ctypes.byref(fork), ctypes.byref(cache.plan),
                                              cache.layers, logits.ptr), "moe_model_step_beams")
-            if cache.fork_status or cache.status:
-                raise MoeError(f"step {i}: fork status {cache.fork_status}, plan status {cache.status}")
+        failed = status.download((n_new, 2), np.int32)
+        if failed.any():
+            i = int(np.argmax(failed.any(1)))
+            raise MoeError(f"step {i}: fork status {failed[i, 0]}, plan status {failed[i, 1]}")
         told = told.download((n_new, 2, R), np.int32)
         out, at = [[] for _ in range(R)], np.arange(R)
         for parent, token in told[::-1]:
             for r in range(R):
-                if at[r] >= 0:
+                if at[r] >= 0 and parent[at[r]] >= 0:   # (a group with too few candidates leaves beams without one)
                     out[r].append(int(token[at[r]]))
             at = np.where(at >= 0, parent[at], -1)
         for r in range(R):

@@ -154,6 +154,38 @@ def test_search(moehip, kind, experts, nq):
     m.close()
 
 
+@pytest.mark.parametrize("n_prompt,n_beam,n_new,ps", [(5, 4, 10, 16), (1, 8, 15, 16), (3, 6, 20, 4), (2, 3, 1, 1)])
+def test_search_with_no_page_to_spare(moehip, n_prompt, n_beam, n_new, ps):
+    """Beams that fill their last pages at once: what a search takes by itself is enough, and what it finds does not depend on it;
+    too few pages raise."""
+    M = moehip
+    tm = model64.plain_model(O, 50, 1, False, nq=4, nkv=2)
+    m = M.model_from_tiny(tm, 256)
+    prompt = [np.random.default_rng(n_new).integers(0, tm.V, n_prompt)]
+    ids, score = m.beam_search(prompt, n_beam, n_new, page_size=ps)
+    assert [len(x) for x in ids[0]] == [n_new] * n_beam
+    more, other = m.beam_search(prompt, n_beam, n_new, page_size=ps, n_pages=300)
+    assert ids == more
+    np.testing.assert_array_equal(score, other)
+    if n_new > 1:
+        with pytest.raises(M.MoeError):
+            m.beam_search(prompt, n_beam, n_new, page_size=ps, n_pages=-(-n_prompt // ps))
+    m.close()
+
+
+def test_search_of_fewer_tokens_than_beams(moehip):
+    """One step of more beams than tokens: a beam a token, the others without one."""
+    M = moehip
+    tm = O.TinyModel(D=64, L=1, hd=16, nq=4, nkv=2, dff=32, E=8, top_k=8, V=7, seed=6, std=0.3, theta=1e4)
+    m = M.model_from_tiny(tm, 64)
+    ids, score = m.beam_search([[1, 2]], 10, 1)
+    assert sorted(x[0] for x in ids[0][:7]) == list(range(7)) and ids[0][7:] == [[]] * 3
+    assert np.isfinite(score[0, :7]).all() and (score[0, 7:] == -np.inf).all()
+    ids, score = m.beam_search([[1, 2]], 10, 3)
+    assert [len(x) for x in ids[0]] == [3] * 10 and np.isfinite(score).all()
+    m.close()
+
+
 def test_fork_of_a_cache(moehip):
     """PagedCache.fork between steps of any kind: answers that part ways after a common prompt are those of separate requests."""
     M = moehip
