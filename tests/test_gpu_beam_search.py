@@ -215,6 +215,83 @@ def test_fork_of_a_cache(moehip):
     m.close()
 
 
+class Step:
+    """The operators of a search's step over a cache of two layers, without a model."""
+
+    def __init__(self, M, G, K, V, ps, kind, n_prompt):
+        self.M, self.G, self.K, self.V, self.R = M, G, K, V, G * K
+        rng, R, nq, nkv, hd = np.random.default_rng(G * K), G * K, 8, 2, 64
+        width = -(-(n_prompt + 40) // ps)
+        self.c = c = M.PagedCache(2, nkv, hd, R * (width + 1), ps, R, width, max(R, G * n_prompt), C.TYPES[kind])
+        for pool in c._pools:
+            x = rng.standard_normal(pool.nbytes // 2).astype(np.float16)
+            pool.upload(x if kind == "f16" else x.view(np.float32) if kind == "f32" else x)
+        fresh = np.zeros(R, np.int32)
+        fresh[::K] = n_prompt
+        c.set_step(fresh, np.zeros(G * n_prompt, np.int32))
+        M.check(M.lib().moe_paged_plan_dev(ctypes.byref(c.plan)))
+        assert c.status == 0
+        c.plan.max_tokens = R
+        buf, zero = M.DeviceBuffer.from_array, np.zeros(R, np.int32)
+        L = M.lib()
+        sizes = (R, G, nq, nkv, hd)
+        need = [L.moe_beam_select_work_bytes(G, K, V), L.moe_paged_share_plan_bytes(*sizes), L.moe_paged_attn_shared_work_bytes(*sizes)]
+        self.b = b = {"logits": M.DeviceBuffer(4 * R * V), "score": buf(np.where(np.arange(R) % K == 0, 0, -np.inf).astype(np.float32)), "done": buf(zero), "parent": buf(zero),
+                      "token": buf(zero), "q": M.DeviceBuffer(4 * R * nq * hd), "out": buf(np.zeros(R * nq * hd, np.float32)), "first": buf(np.arange(0, R + 1, K).astype(np.int32)),
+                      "prefix": buf(np.zeros(G, np.int32)), "work": M.DeviceBuffer(need[0]), "plan": M.DeviceBuffer(need[1]), "attn": M.DeviceBuffer(need[2])}
+        p, d = {n: x.ptr for n, x in b.items()}, {n: x.ptr for n, x in c._b.items()}
+        self.select = M.BeamSelect(G, K, V, p["logits"], V, p["score"], p["done"], None, -1, 0, p["parent"], p["token"], p["score"], p["done"], d["fresh"], p["work"], need[0])
+        self.fork = c.fork_args(p["parent"])
+        self.share = M.PagedShare(R, R, width, ps, nq, nkv, hd, d["req"], d["pos"], d["tables"], G, p["first"], p["prefix"], p["plan"], need[1])
+        self.attn = M.PagedAttn(p["q"], nq * hd, R, nq, d["req"], d["pos"], d["tables"], R, width, 0.125, p["out"], nq * hd, p["attn"], need[2])
+
+    def calls(self):
+        M, L, c, ref = self.M, self.M.lib(), self.c, ctypes.byref
+        M.check(L.moe_beam_select_dev(ref(self.select)))
+        M.check(L.moe_paged_fork_dev(ref(self.fork)))
+        M.check(L.moe_paged_copy_dev(self.fork.copies, self.fork.max_copies, c.layers, 2))
+        M.check(L.moe_paged_plan_dev(ref(c.plan)))
+        M.check(L.moe_paged_share_dev(ref(self.share)))
+        for l in range(2):
+            M.check(L.moe_paged_attn_shared_dev(ref(self.attn), ref(c.layers[l]), ref(self.share)))
+
+    def state(self):
+        R, p = self.R, self.c.plan
+        got = {n: self.c.array(n, *s) for n, s in (("held", (R,)), ("tables", (R, p.max_pages)), ("ring", (p.n_pages,)), ("ring_at", (2,)), ("req", (R,)), ("pos", (R,)))}
+        got.update({n: self.b[n].download((R,), np.int32) for n in ("parent", "token")}, prefix=self.b["prefix"].download((self.G,), np.int32),
+                   score=self.b["score"].download((R,), np.float32), out=self.b["out"].download((R * 512,), np.float32),
+                   **{f"pool {i}": x.download((x.nbytes,), np.uint8) for i, x in enumerate(self.c._pools)})
+        return got
+
+
+@pytest.mark.parametrize("G,K,kind,n_prompt", [(2, 4, "f16", 45), (1, 20, "f32", 130), (3, 16, "bf16", 70)])
+def test_operators_in_a_graph(moehip, G, K, kind, n_prompt):
+    """The operators of a step, captured together and replayed over a state that moves on, between eager steps of another cache:
+    every replay leaves what the eager step leaves."""
+    import test_gpu_paged_serving as S2
+    hip, V, ps = S2.Hip(moehip), 600, 16
+    a, e = (Step(moehip, G, K, V, ps, kind, n_prompt) for _ in "ab")
+    rng = np.random.default_rng(7)
+    graph = hip.capture(a.calls)
+    shared = 0
+    for step in range(20):
+        logits, q = (3 * rng.standard_normal((G * K, V))).astype(np.float32), rng.standard_normal((G * K, 512)).astype(np.float32)
+        for x in (a, e):
+            x.b["logits"].upload(logits)
+            x.b["q"].upload(q)
+        hip.launch(graph)
+        moehip.synchronize()
+        e.calls()
+        assert a.c.status == e.c.status == a.c.fork_status == e.c.fork_status == 0
+        got, want = a.state(), e.state()
+        for n in want:
+            np.testing.assert_array_equal(got[n], want[n], err_msg=f"step {step}, {n}")
+        shared += int((want["prefix"] > 0).all())
+        assert (want["held"] == n_prompt + step + 1).all()
+    assert shared == 20
+    hip.destroy(graph)
+
+
 def test_step_beams_refused(moehip):
     """What the three descriptions hand on to each other has to be the same; a capture is refused."""
     import test_gpu_paged_serving as G
