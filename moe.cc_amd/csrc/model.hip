@@ -20,7 +20,6 @@
 #include <unistd.h>
 
 #include <initializer_list>
-#include <functional>
 #include <mutex>
 #include <new>
 #include <string>
@@ -628,6 +627,27 @@ moe_status validate_file(const BinIndex& b, const char* path, QwenConfig* out, i
 
 }  // namespace
 
+// What a step of any kind asks of the plan and the layers, and of the library: `take` is run with the model held.
+template <class Take>
+static moe_status checked_step(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers, const char* who, Take take) {
+  if (plan->n_req < 1 || plan->max_tokens < 1)
+    return set_error(MOE_ERR_ARG, "%s: %d requests, %d tokens", who, plan->n_req, plan->max_tokens);
+  for (int l = 0; l < m->cfg.n_layers; ++l)
+    if (layers[l].n_kv != m->cfg.n_kv || layers[l].head_dim != m->cfg.head_dim || layers[l].n_pages != plan->n_pages ||
+        layers[l].page_size != plan->page_size)
+      return set_error(MOE_ERR_ARG, "%s: layer %d has %d pages of %d positions, %d heads of %d", who, l, layers[l].n_pages,
+                       layers[l].page_size, layers[l].n_kv, layers[l].head_dim);
+  moe_status st = check_paged_step(plan, layers, m->cfg.n_layers, m->cfg.n_q, m->cfg.n_kv);
+  if (st || (st = ensure_init())) return st;
+  OnDevice on;
+  if ((st = on.enter())) return st;
+  std::lock_guard<std::mutex> lk(m->mu);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if ((st = check_hip(hipStreamIsCapturing(stream(), &capture), "step capture"))) return st;
+  if (capture != hipStreamCaptureStatusNone) return set_error(MOE_ERR_ARG, "%s: the stream is being captured", who);
+  return take();
+}
+
 extern "C" {
 
 moe_status moe_model_create(const QwenConfig* cfg, const QwenWeights* w, int max_seq,
@@ -889,27 +909,6 @@ moe_status moe_model_forward(moe_model* m, const int32_t* ids, int T, int ids_on
   if (!m || !ids) return set_error(MOE_ERR_ARG, "model_forward: null argument");
   std::lock_guard<std::mutex> lk(m->mu);
   return forward_checked(m, ids, T, ids_on_device, logits_dev, next_dev);
-}
-
-// What a step of any kind asks of the plan and the layers, and of the library: `take` is run with the model held.
-static moe_status checked_step(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers, const char* who,
-                               const std::function<moe_status()>& take) {
-  if (plan->n_req < 1 || plan->max_tokens < 1)
-    return set_error(MOE_ERR_ARG, "%s: %d requests, %d tokens", who, plan->n_req, plan->max_tokens);
-  for (int l = 0; l < m->cfg.n_layers; ++l)
-    if (layers[l].n_kv != m->cfg.n_kv || layers[l].head_dim != m->cfg.head_dim || layers[l].n_pages != plan->n_pages ||
-        layers[l].page_size != plan->page_size)
-      return set_error(MOE_ERR_ARG, "%s: layer %d has %d pages of %d positions, %d heads of %d", who, l, layers[l].n_pages,
-                       layers[l].page_size, layers[l].n_kv, layers[l].head_dim);
-  moe_status st = check_paged_step(plan, layers, m->cfg.n_layers, m->cfg.n_q, m->cfg.n_kv);
-  if (st || (st = ensure_init())) return st;
-  OnDevice on;
-  if ((st = on.enter())) return st;
-  std::lock_guard<std::mutex> lk(m->mu);
-  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  if ((st = check_hip(hipStreamIsCapturing(stream(), &capture), "step capture"))) return st;
-  if (capture != hipStreamCaptureStatusNone) return set_error(MOE_ERR_ARG, "%s: the stream is being captured", who);
-  return take();
 }
 
 moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const moe_pages* layers,
