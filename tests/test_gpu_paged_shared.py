@@ -126,6 +126,7 @@ GROUPS = [
     [(1, 200, (1, 50)), (5, 64, (1, 100)), (3, 0, (1, 30))],
     [(8, 700, (1, 60)), (8, 300, (1, 60)), (2, 1000, (1, 1))],
     [(33, 260, (0, 33))],
+    [(6, 144, (0, 20)), (40, 128, (0, 40)), (1, 300, (1, 9)), (7, 145, (100, 150))],
 ]
 
 
@@ -151,11 +152,11 @@ def test_many_parts(moehip, kind, nq, nkv, hd, groups, wide):
 
 def test_rows_of_no_request_and_empty_ones(moehip):
     """In a group, at its start, and a whole group of them; rows outside every group."""
-    b = Batch(moehip, "bf16", [(6, 96, (1, 40)), (3, 64, (1, 20)), (4, 48, (2, 9))], 8, 2, 64, 16, seed=2, first=[1, 6, 9, 12])
+    b = Batch(moehip, "bf16", [(6, 192, (1, 40)), (3, 160, (1, 20)), (4, 48, (2, 9))], 8, 2, 64, 16, seed=2, first=[1, 6, 9, 12])
     b.req[[1, 4, 6, 7, 8]] = -1
     b.pos[[2, 10]] = -1
     want, _ = b.run()
-    assert want[0] == 96 and want[1] == 0 and want[2] >= 48
+    assert want[0] == 192 and want[1] == 0 and want[2] >= 48
     b.pos[:] = -1
     b.run()
     b.req[:] = -5
@@ -183,17 +184,18 @@ def test_outside_and_bad_pages(moehip, wide):
 @pytest.mark.parametrize("wide", [False, True])
 def test_firsts(moehip, first, wide):
     """Empty groups, groups that are none: every row has its attention all the same."""
-    Batch(moehip, "bf16", [(9, 128, (1, 20))], 4, 2, 64, 16, seed=5, first=first).run()
-    Batch(moehip, "bf16", [(9, 128, (1, 20))], 48, 2, 64, 16, seed=5, first=first, wide=wide).run()
+    Batch(moehip, "bf16", [(9, 192, (1, 20))], 4, 2, 64, 16, seed=5, first=first).run()
+    Batch(moehip, "bf16", [(9, 192, (1, 20))], 48, 2, 64, 16, seed=5, first=first, wide=wide).run()
 
 
 def test_rows_of_one_request(moehip):
     """Several tokens of one request in a group (a prompt's end, tokens to be checked)."""
-    b = Batch(moehip, "bf16", [(5, 0, (150, 150)), (4, 64, (30, 60))], 16, 2, 128, 16, seed=6, spare_rows=1)
+    b = Batch(moehip, "bf16", [(5, 0, (250, 250)), (4, 64, (30, 60))], 16, 2, 128, 16, seed=6, spare_rows=1)
     b.req[:5] = b.req[0]
-    b.pos[:5] = [140, 141, 142, 143, 149]
-    want, _ = b.run()
-    assert want[0] == 128
+    for pos, common in (([240, 241, 242, 243, 249], 240), ([140, 141, 142, 143, 149], 128)):
+        b.pos[:5] = pos
+        want, _ = b.run()
+        assert want[0] == common
 
 
 def test_as_the_unshared_call(moehip):
