@@ -1007,42 +1007,52 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       for (int ct = 0; ct < CPW; ++ct)
 #pragma unroll
         for (int t = 0; t < KT; ++t) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      u32x4 k[NK][KT];
+      // operands at a time: with all of them in registers 256 dimensions do not fit (8 groups of 8 rows of 2000 positions, bf16
+      // 79 us, in halves 53, in quarters 40; 128 dimensions, 64 rows of 16000 64, in halves 60)
+      constexpr int CUT = HDP > 128 ? 4 : HDP > 64 ? 2 : 1, KC = NK / CUT, VN = CT == F32 ? KT * VE : VE / CUT;
 #pragma unroll
-      for (int j = 0; j < NK; ++j)
+      for (int j0 = 0; j0 < NK; j0 += KC) {
+        u32x4 k[KC][KT];
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const int row = 8 * (col / 4) + 4 * t + col % 4;
-          k[j][t] = *(const u32x4*)(ks + row * RB + ((4 * j + quad) ^ swizzle(row)) * 16);
-        }
-      if constexpr (CT != F32) __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < KC; ++j)
 #pragma unroll
-      for (int j = 0; j < NK; ++j)
+          for (int t = 0; t < KT; ++t) {
+            const int row = 8 * (col / 4) + 4 * t + col % 4;
+            k[j][t] = *(const u32x4*)(ks + row * RB + ((4 * (j0 + j) + quad) ^ swizzle(row)) * 16);
+          }
+        if constexpr (CT != F32) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < (CT == F32 ? 4 : NP); ++n)
+        for (int j = 0; j < KC; ++j)
 #pragma unroll
-          for (int t = 0; t < KT; ++t)
+          for (int n = 0; n < (CT == F32 ? 4 : NP); ++n)
 #pragma unroll
-            for (int ct = 0; ct < CPW; ++ct) {
-              if constexpr (CT == F32)
-                s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[j][t][n]), __uint_as_float(qp[ct][0][j][n]), s[ct][t], 0, 0, 0);
-              else
-                s[ct][t] = mfma32<HALF>(k[j][t], qp[ct][n][j], s[ct][t]);
-            }
-      // the values' operands are requested before the weights are worked on: of fp32 pages four dimensions of keys
-      // 16 t + 4 quad + i in v[(4 t + i) HDP / 64 + h]
-      u32x4 v[CT == F32 ? KT * VE : VE];
+            for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int e = 0; e < (CT == F32 ? KT * VE : VE); ++e) {
-        if constexpr (CT == F32) {
-          const int row = 8 * quad + e / (VE / 4), piece = 16 * (e % (VE / 4)) + col;
-          v[e] = *(const u32x4*)(ks + T::ROWS * RB + row * RB + (piece ^ swizzle(row)) * 16);
-        } else {
-          const u32x2 x = read_turned(vs + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + col / 4)) * 16);
-          const u32x2 y = read_turned(vs + 4 * RB + ((2 * e + col % 4 / 2) ^ swizzle(quad * 8 + 4 + col / 4)) * 16);
-          v[e] = u32x4{x[0], x[1], y[0], y[1]};
-        }
+              for (int ct = 0; ct < CPW; ++ct) {
+                if constexpr (CT == F32)
+                  s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[j][t][n]), __uint_as_float(qp[ct][0][j0 + j][n]), s[ct][t], 0, 0, 0);
+                else
+                  s[ct][t] = mfma32<HALF>(k[j][t], qp[ct][n][j0 + j], s[ct][t]);
+              }
       }
+      // the values' first operands are requested before the weights are worked on: of fp32 pages four dimensions of keys
+      // 16 t + 4 quad + i in v[(4 t + i) HDP / 64 + h]
+      u32x4 v[VN];
+      auto load_v = [&](int e0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          if constexpr (CT == F32) {
+            const int row = 8 * quad + e / (VE / 4), piece = 16 * (e % (VE / 4)) + col;
+            v[e] = *(const u32x4*)(ks + T::ROWS * RB + row * RB + (piece ^ swizzle(row)) * 16);
+          } else {
+            const int piece = 2 * (e0 + e) + col % 4 / 2;
+            const u32x2 x = read_turned(vs + (piece ^ swizzle(quad * 8 + col / 4)) * 16);
+            const u32x2 y = read_turned(vs + 4 * RB + (piece ^ swizzle(quad * 8 + 4 + col / 4)) * 16);
+            v[e] = u32x4{x[0], x[1], y[0], y[1]};
+          }
+        }
+      };
+      load_v(0);
       __builtin_amdgcn_sched_barrier(0);
       // ---- weights
       u32x4 pp[CPW][NP];
@@ -1093,11 +1103,15 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
               o[ct][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[i * (VE / 4) + e / 4][e % 4]), p[ct][i], o[ct][e], 0, 0, 0);
       } else {
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
+        for (int e0 = 0; e0 < VE; e0 += VN) {
+          if (e0) load_v(e0);
 #pragma unroll
-          for (int n = 0; n < NP; ++n)
+          for (int e = 0; e < VN; ++e)
 #pragma unroll
-            for (int ct = 0; ct < CPW; ++ct) o[ct][e] = mfma32<HALF>(v[e], pp[ct][n], o[ct][e]);
+            for (int n = 0; n < NP; ++n)
+#pragma unroll
+              for (int ct = 0; ct < CPW; ++ct) o[ct][e0 + e] = mfma32<HALF>(v[e], pp[ct][n], o[ct][e0 + e]);
+        }
       }
     }
     if (step + 1 < steps) store(step + 1);
