@@ -36,7 +36,6 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostBeams = kWave;          // a list is a lane a beam
-constexpr int kStep = 16 * kWave;          // logits of a wave's step
 // From here on a wave collects its candidates, sorts 64 at a time and merges them into its list, and blocks' lists are merged by
 // a kernel of their own; below, candidates are inserted one by one (one group over 151936 tokens, us with the first and the
 // second: 8 beams 25.0, 18.2; 16 27.1, 27.4; 24 28.9, 44.1; 32 30.5, 57.5; 24 groups of 8 52, 39; 200 groups of 64 over 1000
@@ -45,6 +44,9 @@ constexpr int kMergedBeams = 17;
 // Blocks that rows are cut into, about: 16 waves a CU, and few enough lists for the second kernel (us at 512, 1024 and 2048, 8
 // beams: 24 groups 46.3, 39.5, 39.0; 64 groups 71.8, 66.2, 65.8; one group alike).
 constexpr int kBlocks = 1024;
+// Rows of up to this many tokens, one step of a wave, go in quarters to all four (us with whole steps and quarters: 200 groups of
+// 64 beams over 1000 tokens 144, 96, over 300 123, 113; of 4 beams 12.6, 13.5, 12.5, 12.4; over 3000 tokens 121, 145).
+constexpr int kShort = 1024;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -244,14 +246,18 @@ __device__ __forceinline__ bool usable(const moe_beam_select& a, int r) {
   return fabsf(a.score[r]) < INFINITY && w > 0.0f && w < INFINITY;
 }
 
+// A wave's step: 16 bytes of a lane, J times.
+template <int J>
 __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
+  constexpr int N = 4 * J, STEP = N * kWave;
   const moe_beam_select& a = s.a;
   const int row = (int)blockIdx.y, b = (int)blockIdx.x, K = a.n_beam;
   if (!usable(a, row) || (a.done && a.done[row])) return;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int steps = (a.vocab + kStep - 1) / kStep;
+  const int steps = (a.vocab + STEP - 1) / STEP;
   const int first = (int)((long long)b * steps / s.blocks), end = (int)((long long)(b + 1) * steps / s.blocks);
   const float* x0 = a.logits + (size_t)row * a.ld;
+  const int active = min(kWaves, end - first);
   List list;
   float from = -INFINITY, power = 0.0f, floor = 0.0f;   // the logit that sums are taken from, its power of two
   double at = -(double)INFINITY;                        // as Part's
@@ -259,18 +265,18 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   float least = -INFINITY;                              // what a logit has to pass
   double sum = 0.0;
   // what the block's n_beam-th has to reach at least, as an ordered number: after the first step the least of the waves'
-  // share-th (share = n_beam / 4, rounded up), then any wave's n_beam-th
+  // share-th (share: n_beam by the waves that have a step, rounded up), then any wave's n_beam-th
   __shared__ uint32_t share_s[kWaves], least_s;
   __shared__ uint64_t pending_s[kWaves][2 * kWave];
-  f32x4 next[4];
+  f32x4 next[J];
   auto load = [&](int step) {
-    const int v0 = step * kStep + 4 * lane;
-    if ((step + 1) * kStep <= a.vocab) {
+    const int v0 = step * STEP + 4 * lane;
+    if ((step + 1) * STEP <= a.vocab) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) next[j] = *(const f32x4u*)(x0 + v0 + j * 4 * kWave);
+      for (int j = 0; j < J; ++j) next[j] = *(const f32x4u*)(x0 + v0 + j * 4 * kWave);
     } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < N; ++j) {
         const int v = v0 + j / 4 * 4 * kWave + j % 4;
         next[j / 4][j % 4] = v < a.vocab ? x0[v] : -INFINITY;
       }
@@ -280,17 +286,17 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   if (first + wave < end) {
     load(first + wave);
   } else {   // a wave without a step comes to the first one's barrier all the same
-    if (lane == 0) share_s[wave] = 0;
+    if (lane == 0) share_s[wave] = 0xffffffffu;
     __syncthreads();
   }
   for (int step = first + wave; step < end; step += kWaves) {
-    float x[16];
+    float x[N];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = next[j / 4][j % 4];
+    for (int j = 0; j < N; ++j) x[j] = next[j / 4][j % 4];
     if (step + kWaves < end) load(step + kWaves);
     float top = x[0];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
+    for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
     // ---- the sum.  Its power of two moves only when a term would leave fp32; terms below 2^-100 of that count as 2^-100
     const float most = wave_max(top);
     if (!(most < INFINITY)) sum = NAN;
@@ -303,22 +309,22 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
     }
     if (far) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum += (double)exp_from(x[j], from);
+      for (int j = 0; j < N; ++j) sum += (double)exp_from(x[j], from);
     } else if (from > -INFINITY) {
       float check = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
+      for (int j = 0; j < N; j += 4) {
         check += (x[j] + x[j + 1]) + (x[j + 2] + x[j + 3]);
         sum += (double)((exp_at(x[j], floor, power) + exp_at(x[j + 1], floor, power)) + (exp_at(x[j + 2], floor, power) + exp_at(x[j + 3], floor, power)));
       }
       if (check != check) sum = NAN;   // one of them is (no infinity but -inf is left)
     } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum += x[j] == -INFINITY ? 0.0 : (double)NAN;
+      for (int j = 0; j < N; ++j) sum += x[j] == -INFINITY ? 0.0 : (double)NAN;
     }
     // ---- the best
     if (step == first + wave) {
-      const uint32_t mine = nth_largest(top > -INFINITY ? ordered(top) : 0u, (K + kWaves - 1) / kWaves);
+      const uint32_t mine = nth_largest(top > -INFINITY ? ordered(top) : 0u, active >= kWaves ? (K + kWaves - 1) / kWaves : active == 3 ? (K + 2) / 3 : active == 2 ? (K + 1) / 2 : K);
       if (lane == 0) share_s[wave] = mine;
       __syncthreads();
       uint32_t all = share_s[0];
@@ -344,10 +350,10 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
       };
       int n = 0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < N; ++j) {
         const uint64_t who = __ballot(x[j] > pass);
         if (!who) continue;
-        const uint32_t token = (uint32_t)(step * kStep + j / 4 * 4 * kWave + 4 * lane + j % 4);
+        const uint32_t token = (uint32_t)(step * STEP + j / 4 * 4 * kWave + 4 * lane + j % 4);
         if (x[j] > pass)
           pending_s[wave][n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
               (uint64_t)ordered(x[j]) << 32 | (0xffffffffu - token);
@@ -365,12 +371,12 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
-    for (int j = 0; j < 16 && K < kMergedBeams; ++j) {
+    for (int j = 0; j < N && K < kMergedBeams; ++j) {
       uint64_t who = __ballot(x[j] > pass);
       while (who) {
         const int l = __builtin_ctzll(who);
         who &= who - 1;
-        const uint32_t token = (uint32_t)(step * kStep + j / 4 * 4 * kWave + 4 * l + j % 4);
+        const uint32_t token = (uint32_t)(step * STEP + j / 4 * 4 * kWave + 4 * l + j % 4);
         const uint64_t k = (uint64_t)ordered(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[j]), l))) << 32 | (0xffffffffu - token);
         if (k > list.last) list.insert(k, K);
       }
@@ -583,9 +589,12 @@ __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
   write_choice(a, row0 + lane, row0 + mine, done, done ? base_s[mine] : value_of(base_s[mine], key), key);
 }
 
+// Logits of a wave's step.
+int step_for(int vocab) { return vocab <= kShort ? 4 * kWave : 16 * kWave; }
+
 // Blocks that a row is cut into: as many steps a wave as leave about kBlocks in all.
 int blocks_for(long long rows, int vocab) {
-  const long long steps = (vocab + kStep - 1) / kStep, most = (steps + kWaves - 1) / kWaves;
+  const long long step = step_for(vocab), steps = (vocab + step - 1) / step, most = (steps + kWaves - 1) / kWaves;
   const long long want = kBlocks / rows;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
@@ -635,7 +644,7 @@ moe_status moe_beam_select_dev(const moe_beam_select* a) {
   s.merged = a->n_beam >= kMergedBeams;
   s.parts = (Part*)a->work;
   s.keys = (uint64_t*)(s.parts + (size_t)rows * s.blocks);
-  hipLaunchKernelGGL(select_rows_kernel, dim3((unsigned)s.blocks, (unsigned)rows), dim3(kThreads), 0, stream(), s);
+  hipLaunchKernelGGL(a->vocab <= kShort ? select_rows_kernel<1> : select_rows_kernel<4>, dim3((unsigned)s.blocks, (unsigned)rows), dim3(kThreads), 0, stream(), s);
   if ((st = check_hip(hipGetLastError(), "beam_select launch"))) return st;
   if (s.merged) {
     hipLaunchKernelGGL(select_merge_kernel, dim3((unsigned)rows), dim3(kThreads), 0, stream(), s);

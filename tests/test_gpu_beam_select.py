@@ -72,7 +72,7 @@ def check(got, logits, score, done, weight, n_beam, eos, pad):
 
 
 @pytest.mark.parametrize("n_groups,n_beam,vocab", [(1, 1, 1), (1, 4, 3), (2, 3, 7), (3, 2, 1023), (1, 5, 1024), (2, 8, 1025), (1, 64, 64), (2, 64, 5000), (7, 5, 50257),
-                                                   (1, 4, 151936), (70, 2, 4097), (5, 33, 9000), (300, 1, 300), (1, 64, 151936), (3, 31, 50257), (2, 32, 50257)])
+                                                   (1, 4, 151936), (70, 2, 4097), (5, 33, 9000), (300, 1, 300), (1, 64, 151936), (3, 31, 50257), (2, 32, 50257), (3, 20, 1000), (2, 64, 257), (5, 7, 256), (2, 17, 40)])
 @pytest.mark.parametrize("style", ["plain", "masked", "ended"])
 def test_select(moehip, n_groups, n_beam, vocab, style):
     print("beam select", n_groups, n_beam, vocab, style, flush=True)
