@@ -63,6 +63,7 @@ __device__ __forceinline__ double part_at(const Part& p, double at) {
 struct SelectArgs {
   moe_beam_select a;
   int blocks;       // of a row
+  int each, rest;   // steps of a block, one more for the first `rest`
   Part* parts;      // work [rows][blocks]
   int merged;       // the blocks' lists are merged by a kernel of their own
   uint64_t* keys;   // work [rows][n_beam][blocks], or merged [rows][blocks][n_beam]: each block's best, in order; 0: none
@@ -254,8 +255,7 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   const int row = (int)blockIdx.y, b = (int)blockIdx.x, K = a.n_beam;
   if (!usable(a, row) || (a.done && a.done[row])) return;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int steps = (a.vocab + STEP - 1) / STEP;
-  const int first = (int)((long long)b * steps / s.blocks), end = (int)((long long)(b + 1) * steps / s.blocks);
+  const int first = s.each * b + min(b, s.rest), end = first + s.each + (b < s.rest);
   const float* x0 = a.logits + (size_t)row * a.ld;
   const int active = min(kWaves, end - first);
   List list;
@@ -641,6 +641,8 @@ moe_status moe_beam_select_dev(const moe_beam_select* a) {
   SelectArgs s;
   s.a = *a;
   s.blocks = blocks_for(rows, a->vocab);
+  const int steps = (a->vocab + step_for(a->vocab) - 1) / step_for(a->vocab);
+  s.each = steps / s.blocks, s.rest = steps % s.blocks;
   s.merged = a->n_beam >= kMergedBeams;
   s.parts = (Part*)a->work;
   s.keys = (uint64_t*)(s.parts + (size_t)rows * s.blocks);
