@@ -324,7 +324,8 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
     }
     // ---- the best
     if (step == first + wave) {
-      const uint32_t mine = nth_largest(top > -INFINITY ? ordered(top) : 0u, active >= kWaves ? (K + kWaves - 1) / kWaves : active == 3 ? (K + 2) / 3 : active == 2 ? (K + 1) / 2 : K);
+      const int share = active >= kWaves ? (K + kWaves - 1) / kWaves : active == 3 ? (K + 2) / 3 : active == 2 ? (K + 1) / 2 : K;
+      const uint32_t mine = share > 1 ? nth_largest(top > -INFINITY ? ordered(top) : 0u, share) : most > -INFINITY ? ordered(most) : 0u;
       if (lane == 0) share_s[wave] = mine;
       __syncthreads();
       uint32_t all = share_s[0];
