@@ -544,11 +544,15 @@ __global__ __launch_bounds__(1024) void select_groups_kernel(SelectArgs s) {
       count = 1;
       list.key = lane == 0 ? 1 : 0;
     } else if (use) {
+      const uint64_t* keys = s.keys + (size_t)row * K * s.blocks;
+      auto load = [&](int c0) { return c0 + lane < K * s.blocks ? keys[c0 + lane] : 0; };
+      uint64_t next = load(0), after = load(kWave);   // (two ahead)
       base = base_of(s, row, score);
       if (base == base) {
-        const uint64_t* keys = s.keys + (size_t)row * K * s.blocks;
         for (int c0 = 0; c0 < K * s.blocks; c0 += kWave) {
-          const uint64_t k = c0 + lane < K * s.blocks ? keys[c0 + lane] : 0;
+          const uint64_t k = next;
+          next = after;
+          after = load(c0 + 2 * kWave);
           if (!__any(k > list.last)) continue;
           const uint32_t bound = nth_largest(k > list.last ? (uint32_t)(k >> 32) : 0u, K);
           uint64_t who = __ballot(k > list.last && (uint32_t)(k >> 32) >= bound);
