@@ -113,6 +113,8 @@ template <int C>
 __device__ __forceinline__ uint64_t lane_xor(uint64_t x) {
   return (uint64_t)lane_xor<C>((uint32_t)(x >> 32)) << 32 | lane_xor<C>((uint32_t)x);
 }
+template <int C>
+__device__ __forceinline__ double lane_xor(double x) { return __longlong_as_double((long long)lane_xor<C>((uint64_t)__double_as_longlong(x))); }
 __device__ __forceinline__ uint64_t lane_mirror(uint64_t x) {
   return (uint64_t)lane_mirror((uint32_t)(x >> 32)) << 32 | lane_mirror((uint32_t)x);
 }
@@ -205,15 +207,14 @@ __device__ __forceinline__ T wave_max(T x) {
 }
 
 __device__ __forceinline__ double wave_max_f64(double x) {
-#pragma unroll
-  for (int c = 32; c; c /= 2) x = fmax(x, __shfl_xor(x, c));
-  return x;
+  x = fmax(x, lane_xor<1>(x)), x = fmax(x, lane_xor<2>(x)), x = fmax(x, lane_xor<4>(x));
+  x = fmax(x, lane_xor<8>(x)), x = fmax(x, lane_xor<16>(x));
+  return fmax(x, lane_xor<32>(x));
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int c = 32; c; c /= 2) x += __shfl_xor(x, c);
-  return x;
+  x += lane_xor<1>(x), x += lane_xor<2>(x), x += lane_xor<4>(x), x += lane_xor<8>(x), x += lane_xor<16>(x);
+  return x + lane_xor<32>(x);
 }
 
 constexpr float kLog2eHi = 1.44269504088896340736f;
@@ -423,11 +424,12 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
 __device__ __forceinline__ double base_of(const SelectArgs& s, int row, float score) {
   const int lane = threadIdx.x % kWave;
   const Part* p = s.parts + (size_t)row * s.blocks;
-  double most = -(double)INFINITY;
-  for (int c = lane; c < s.blocks; c += kWave) most = fmax(most, p[c].at);
+  const Part first = lane < s.blocks ? p[lane] : Part{0.0, -(double)INFINITY};
+  double most = first.at;
+  for (int c = lane + kWave; c < s.blocks; c += kWave) most = fmax(most, p[c].at);
   most = wave_max_f64(most);
-  double sum = 0.0;
-  for (int c = lane; c < s.blocks; c += kWave) sum += part_at(p[c], most);
+  double sum = part_at(first, most);
+  for (int c = lane + kWave; c < s.blocks; c += kWave) sum += part_at(p[c], most);
   sum = wave_sum(sum);
   if (!(sum > 0.0 && sum < (double)INFINITY)) return NAN;   // (a NaN or +inf among the logits makes it NaN)
   return (double)score - (most + log(sum));
