@@ -411,12 +411,15 @@ __global__ __launch_bounds__(kThreads) void select_rows_kernel(SelectArgs s) {
   __syncthreads();
   if ((int)threadIdx.x < K)
     s.keys[(size_t)row * K * s.blocks + (s.merged ? (size_t)b * K + threadIdx.x : (size_t)threadIdx.x * s.blocks + b)] = best_s[threadIdx.x];
-  if (threadIdx.x == 0) {
-    double most = part_s[0].at;
-    for (int w = 1; w < kWaves; ++w) most = fmax(most, part_s[w].at);
-    double total = 0.0;
-    for (int w = 0; w < kWaves; ++w) total += part_at(part_s[w], most);
-    s.parts[(size_t)row * s.blocks + b] = Part{total, most};
+  if (wave == 1) {   // (the first stores the list) a lane of four a wave's
+    static_assert(kWaves == 4);
+    const Part p = part_s[lane % kWaves];
+    double most = fmax(p.at, lane_xor<1>(p.at));
+    most = fmax(most, lane_xor<2>(most));
+    double total = part_at(p, most);
+    total += lane_xor<1>(total);
+    total += lane_xor<2>(total);
+    if (lane == 0) s.parts[(size_t)row * s.blocks + b] = Part{total, most};
   }
 }
 

@@ -16,6 +16,7 @@
 // LDS: 11.9 and 30.)
 #include <initializer_list>
 
+#include "block_scan.h"
 #include "moe_device.h"
 #include "moe_lib.h"
 #include "paged_attn.h"
@@ -49,29 +50,6 @@ struct ForkArgs {
   int* counts;      // work [blocks] pages that come back
   int* list;        // work [n_req * max_pages] these, a block's from n_req * its first column on
 };
-
-// Sum over the block's threads up to and without this one, and of all.
-__device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  int x = v;
-#pragma unroll
-  for (int c = 1; c < kWave; c *= 2) {
-    const int y = __shfl_up(x, c);
-    if (lane >= c) x += y;
-  }
-  if (lane == kWave - 1) wave_s[wave] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kN / kWave; ++w) {
-    const int y = wave_s[w];
-    if (w < wave) before += y;
-    all += y;
-  }
-  __syncthreads();
-  *total = all;
-  return before + x - v;
-}
 
 template <int MOST>
 struct ForkShared {
@@ -113,7 +91,7 @@ __device__ __forceinline__ ForkHead fork_requests(const ForkArgs& a, ForkShared<
       }
     }
     int all;
-    const int at = done + block_scan(copied, sh.wave, &all);
+    const int at = done + block_scan<kN>(copied, sh.wave, &all);
     // (the keepers of the requests behind these are still to be read)
     if (r < n) sh.parent[r] = bad ? -1 : copied ? sh.parent[r] | at << 12 | 1 << 30 : sh.parent[r];
     done += all;
@@ -226,7 +204,7 @@ __device__ __forceinline__ int fork_columns(const ForkArgs& a, ForkShared<MOST>&
   // a thread a word: places within the block
   static_assert(WORDS <= kN);
   int all;
-  const int before = block_scan(tid < WORDS ? __popc(bits_s[tid]) : 0, sh.wave, &all);
+  const int before = block_scan<kN>(tid < WORDS ? __popc(bits_s[tid]) : 0, sh.wave, &all);
   if (tid < WORDS) first_s[tid] = before;
   __syncthreads();
 #pragma unroll
@@ -314,7 +292,7 @@ __global__ __launch_bounds__(kN) void fork_finish_kernel(ForkArgs a) {
   for (int b0 = 0; b0 < a.blocks; b0 += kN) {
     const int b = b0 + (int)threadIdx.x, c = b < a.blocks ? a.counts[b] : 0;
     int all;
-    const int at = block_scan(c, wave_s, &all);
+    const int at = block_scan<kN>(c, wave_s, &all);
     if (b == (int)blockIdx.x) before_s = back + at, mine_s = c;
     back += all;
   }

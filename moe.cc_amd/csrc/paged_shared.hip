@@ -15,6 +15,7 @@
 
 #include <type_traits>
 
+#include "block_scan.h"
 #include "moe_device.h"
 #include "paged_attn.h"
 #include "paged_tile.h"
@@ -162,30 +163,6 @@ __global__ __launch_bounds__(256) void share_rows_kernel(ShareArgs a) {
       }
     }
   if (lane == 0) a.p.common[t] = same;
-}
-
-// Sum over the block's threads up to and without this one, and of all.
-template <int N>
-__device__ __forceinline__ int block_scan(int v, int* wave_s, int* total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  int x = v;
-#pragma unroll
-  for (int c = 1; c < kWave; c *= 2) {
-    const int y = __shfl_up(x, c);
-    if (lane >= c) x += y;
-  }
-  if (lane == kWave - 1) wave_s[wave] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < N / kWave; ++w) {
-    const int y = wave_s[w];
-    if (w < wave) before += y;
-    all += y;
-  }
-  __syncthreads();
-  *total = all;
-  return before + x - v;
 }
 
 __device__ __forceinline__ int units_in_all(int positions) { return (positions + kUnit - 1) / kUnit; }
