@@ -9,8 +9,8 @@
 // a wave takes 1024 logits a step, sums their exponentials and keeps the
 // n_beam best as a list sorted over its lanes.  The second, a block a group,
 // joins the rows' sums and lists and ranks the candidates of all rows.  One
-// group of 4 beams over 151936 tokens takes 13.0 us, of which the launches and
-// the chain of a block's own work are most; 24 groups of 8 (117 MB) 38.5 us, the
+// group of 4 beams over 151936 tokens takes 11.5 us, of which the launches and
+// the chain of a block's own work are most; 24 groups of 8 (117 MB) 37.9 us, the
 // first kernel's 31 of them at 3.5 TB/s, where its exponentials, 64-bit sums
 // and bounds keep the vector units as busy as the memory.
 //
@@ -38,14 +38,14 @@ constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostBeams = kWave;          // a list is a lane a beam
 // From here on a wave collects its candidates, sorts 64 at a time and merges them into its list, and blocks' lists are merged by
 // a kernel of their own; below, candidates are inserted one by one (one group over 151936 tokens, us with the first and the
-// second: 8 beams 25.0, 18.2; 16 27.1, 27.4; 24 28.9, 44.1; 32 30.5, 57.5; 24 groups of 8 52, 39; 200 groups of 64 over 1000
-// tokens 158, 707).
+// second: 8 beams 23.7, 14.8; 16 25.9, 23.2; 24 27.7, about 43; 32 29.3, about 57; 24 groups of 8 51.6, 38.0; 200 groups of 64
+// over 1000 tokens, whole steps, 158, 707).
 constexpr int kMergedBeams = 17;
 // Blocks that rows are cut into, about: 16 waves a CU, and few enough lists for the second kernel (us at 512, 1024 and 2048, 8
-// beams: 24 groups 46.3, 39.5, 39.0; 64 groups 71.8, 66.2, 65.8; one group alike).
+// beams: 24 groups 44.7, 38.1, 38.6; 64 groups 70.5, 63.8, 65.5; one group alike; one of 64 37.6, 36.3, 41.7).
 constexpr int kBlocks = 1024;
 // Rows of up to this many tokens, one step of a wave, go in quarters to all four (us with whole steps and quarters: 200 groups of
-// 64 beams over 1000 tokens 144, 96, over 300 123, 113; of 4 beams 12.6, 13.5, 12.5, 12.4; over 3000 tokens 121, 145).
+// 64 beams over 1000 tokens 136, 86, over 300 116, 105; of 4 beams 11.6, 11.1, 11.2, 10.9; over 3000 tokens 112, 133).
 constexpr int kShort = 1024;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));

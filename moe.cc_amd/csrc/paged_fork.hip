@@ -11,9 +11,9 @@
 //   n - r          of the requests r that held it: the lowest gives it back, unless
 //   kStays         a request holds it now
 // Nothing is kept from one call for the next.  Latency bounds it: launch, the
-// requests' numbers, the tables: 64 requests of 160 pages 9.2 us, 1024 of 512
-// (whose tables are 2 MB each way) 18.  (The pages' numbers in memory instead of
-// LDS: 11.9 and 30.)
+// requests' numbers, the tables: 64 requests of 160 pages 8.4 us, 1024 of 512
+// (whose tables are 2 MB each way) 16.9.  (The pages' numbers in memory instead of
+// LDS: 2.6 and 12 more.)
 #include <initializer_list>
 
 #include "block_scan.h"
@@ -262,7 +262,7 @@ __device__ __forceinline__ void fork_finish(const ForkArgs& a, ForkHead top, int
   }
 }
 
-// Few entries: all of it in one block, one launch (4 requests of 40 pages 5.7 us, 16 of 128 7.5; in columns 7.7, 9.0).
+// Few entries: all of it in one block, one launch (4 requests of 40 pages 5.0 us, 16 of 128 6.7; in columns 6.6, 7.8).
 constexpr int kOnePer = 2, kFewRequests = 1024;
 __global__ __launch_bounds__(kN) void fork_one_kernel(ForkArgs a) {
   __shared__ ForkShared<kFewRequests> sh;
@@ -391,7 +391,7 @@ moe_status moe_paged_fork_dev(const moe_paged_fork* f) {
   a.per = make_divider((uint32_t)f->page_size);
   const bool one = f->n_req <= kFewRequests && (long long)f->n_req * f->max_pages <= kOnePer * kN;
   // Entries of a thread: every block goes through all requests first, so with many of them fewer blocks are better (us with
-  // one and two: 64 requests of 160 pages 9.3, 10.4; 256 of 512 10.0, 11.9; 512 of 512 12.4, 12.4; 1024 of 512 23.5, 18.0).
+  // one and two: 64 requests of 160 pages 8.2, 9.6; 256 of 512 9.1, 11.5; 512 of 512 11.4, 11.6; 1024 of 512 21.4, 16.8).
   // Past 1024 requests a column has to fit a block: four.
   const int per = f->n_req <= 256 ? 1 : f->n_req <= 1024 ? 2 : 4;
   a.columns = one ? f->max_pages : per * kN / f->n_req;

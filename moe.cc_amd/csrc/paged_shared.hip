@@ -171,7 +171,7 @@ __device__ __forceinline__ int units_in_all(int positions) { return (positions +
 // their items are about as many as are resident at once: pieces of ceil(all units / slots), at least one an item, so no
 // more items than `slots` and one for each tile or row.  ONE: a thread a group and a row (at most N of each), whose numbers
 // stay in its registers and LDS; else they go around through the plan, N at a time.  Latency bounds it (us with both kernels:
-// 8 groups of 8 rows 10.3 with 256 threads, 11.6 with 1024, 12.8 around through the plan; 120 groups of 8 16.7 and 28.0).
+// 8 groups of 8 rows 9.9 with 256 threads, 11.3 with 1024, 12.1 around through the plan; 120 groups of 8 16.1 and 27.7).
 template <int N>
 struct PlanShared {
   int wave[N / kWave];
