@@ -1150,7 +1150,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
 // WC: waves over a prefix item's columns, CPW: their sixteens; 0: the item in sixteens.  Prefix items first, of all heads, then the rows' own:
 // the long ones start together.
 template <int CT, int HDP, int WC, int CPW>
-__global__ __launch_bounds__(kThreads, WC || HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
+__global__ __launch_bounds__(kThreads, HDP <= 128 || (WC == 4 && CT != F32) ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
   constexpr int TILE = TileShape<CT, HDP, WC ? WC : 4, 1>::BYTES, COLUMNS = (int)sizeof(ColumnsShared<HDP>);
   constexpr int BYTES = WC && TILE > COLUMNS ? TILE : COLUMNS;
   __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
@@ -1289,11 +1289,9 @@ hipError_t launch(const SharedLaunch& L, hipStream_t s) {
   const unsigned prefix = (unsigned)L.cut.prefix_items, own = (unsigned)L.cut.own_items;
   if constexpr (HDP <= 128) {
     if (L.tiles) return L.cut.columns == kTile ? launch<CT, HDP, 2, 2>(L, prefix, own, s) : launch<CT, HDP, 2, 1>(L, prefix, own, s);
-  } else if constexpr (CT != F32) {
-    if (L.tiles) {
-      const hipError_t e = launch<CT, HDP, 4, 1>(L, prefix, 0, s);
-      return e == hipSuccess ? launch<CT, HDP, 0, 0>(L, 0, own, s) : e;
-    }
+  } else if (L.tiles) {
+    const hipError_t e = L.cut.columns == kTile ? launch<CT, HDP, 4, 1>(L, prefix, 0, s) : launch<CT, HDP, 2, 1>(L, prefix, 0, s);
+    return e == hipSuccess ? launch<CT, HDP, 0, 0>(L, 0, own, s) : e;
   }
   return launch<CT, HDP, 0, 0>(L, prefix * (unsigned)(L.cut.columns / 16), own, s);
 }
@@ -1314,10 +1312,11 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
   L.by_kv = make_divider((uint32_t)g.map.n_kv);
   // Items of 32 and 64 columns are taken whole, but where all of them in sixteens, at their longest, would be resident at once:
   // then only a block's latency counts (us of bf16 pages, 32 heads over 4 of 128, whole and in sixteens: 8 rows of 600
-  // positions 14.9, 12.0; 8 groups of 8 rows of 250 16.8, 14.6, of 600 18.6, 21.1).
+  // positions 14.9, 12.0; 8 groups of 8 rows of 250 16.8, 14.6, of 600 18.6, 21.1; heads of 256, one block a CU, 4 rows of 8000
+  // 29.2, 34.8, 8 of 2200 27.1, 26.6, fp32 45.6, 36.0).
   const long long all = ((long long)g.a.T * L.cut.group + L.cut.columns - 1) / L.cut.columns, units = ((long long)g.a.max_pages * g.map.page_size + kUnit - 1) / kUnit;
-  L.tiles = (L.cut.columns == kTile || (L.cut.columns == kTile / 2 && g.map.head_dim <= 128)) &&
-            (all > sh.n_groups ? all : sh.n_groups) * units * (L.cut.columns / 16) * g.map.n_kv > 2 * kCUs;
+  L.tiles = L.cut.columns >= kTile / 2 &&
+            (all > sh.n_groups ? all : sh.n_groups) * units * (L.cut.columns / 16) * g.map.n_kv > (g.map.head_dim <= 128 ? 2 * kCUs : 3 * kCUs / 2);
   const hipError_t e = dtype == F32    ? launch<F32>(L, s)
                        : dtype == F16  ? launch<F16>(L, s)
                        : dtype == BF16 ? launch<BF16>(L, s)
