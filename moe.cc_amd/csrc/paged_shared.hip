@@ -1150,7 +1150,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
 // WC: waves over a prefix item's columns, CPW: their sixteens; 0: the item in sixteens.  Prefix items first, of all heads, then the rows' own:
 // the long ones start together.
 template <int CT, int HDP, int WC, int CPW>
-__global__ __launch_bounds__(kThreads, HDP <= 128 || (WC == 4 && CT != F32) ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
+__global__ __launch_bounds__(kThreads, HDP <= 128 ? 2 : 1) void shared_attn_kernel(SharedLaunch L) {
   constexpr int TILE = TileShape<CT, HDP, WC ? WC : 4, 1>::BYTES, COLUMNS = (int)sizeof(ColumnsShared<HDP>);
   constexpr int BYTES = WC && TILE > COLUMNS ? TILE : COLUMNS;
   __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
@@ -1170,7 +1170,6 @@ __global__ __launch_bounds__(kThreads, HDP <= 128 || (WC == 4 && CT != F32) ? 2 
       return;
     }
   }
-  if constexpr (WC && HDP > 128) return;   // (its registers would not do: launched by themselves)
   columns_block<CT, HDP>(L, it, kv, sub, own, *(ColumnsShared<HDP>*)lds);
 }
 
@@ -1290,8 +1289,7 @@ hipError_t launch(const SharedLaunch& L, hipStream_t s) {
   if constexpr (HDP <= 128) {
     if (L.tiles) return L.cut.columns == kTile ? launch<CT, HDP, 2, 2>(L, prefix, own, s) : launch<CT, HDP, 2, 1>(L, prefix, own, s);
   } else if (L.tiles) {
-    const hipError_t e = L.cut.columns == kTile ? launch<CT, HDP, 4, 1>(L, prefix, 0, s) : launch<CT, HDP, 2, 1>(L, prefix, 0, s);
-    return e == hipSuccess ? launch<CT, HDP, 0, 0>(L, 0, own, s) : e;
+    return L.cut.columns == kTile ? launch<CT, HDP, 4, 1>(L, prefix, own, s) : launch<CT, HDP, 2, 1>(L, prefix, own, s);
   }
   return launch<CT, HDP, 0, 0>(L, prefix * (unsigned)(L.cut.columns / 16), own, s);
 }
@@ -1310,13 +1308,15 @@ hipError_t launch_shared(const AttnPages& g, const moe_paged_share& sh, int dtyp
   shared_work(L.cut, g.map.n_kv, g.map.head_dim, g.a.work, &L);
   L.by_group = make_divider((uint32_t)L.cut.group);
   L.by_kv = make_divider((uint32_t)g.map.n_kv);
-  // Items of 32 and 64 columns are taken whole, but where all of them in sixteens, at their longest, would be resident at once:
-  // then only a block's latency counts (us of bf16 pages, 32 heads over 4 of 128, whole and in sixteens: 8 rows of 600
-  // positions 14.9, 12.0; 8 groups of 8 rows of 250 16.8, 14.6, of 600 18.6, 21.1; heads of 256, one block a CU, 4 rows of 8000
-  // 29.2, 34.8, 8 of 2200 27.1, 26.6, fp32 45.6, 36.0).
-  const long long all = ((long long)g.a.T * L.cut.group + L.cut.columns - 1) / L.cut.columns, units = ((long long)g.a.max_pages * g.map.page_size + kUnit - 1) / kUnit;
-  L.tiles = L.cut.columns >= kTile / 2 &&
-            (all > sh.n_groups ? all : sh.n_groups) * units * (L.cut.columns / 16) * g.map.n_kv > (g.map.head_dim <= 128 ? 2 * kCUs : 3 * kCUs / 2);
+  // Items of 32 and 64 columns are taken whole, but where all of them in sixteens, at their longest, would be resident at once
+  // (heads past 128, one block a CU: with the rows' own): then only a block's latency counts (us of bf16 pages, 32 heads over 4,
+  // whole and in sixteens; of 128: 8 rows of 600 positions 14.9, 12.0; 8 groups of 8 rows of 250 16.8, 14.6, of 600 18.6, 21.1;
+  // of 256: 8 rows of 600 18.4, 15.5, of 2200 20.8, 26.7; 8 groups of 4 of 400 18.5, 24.3).
+  const long long tiles = ((long long)g.a.T * L.cut.group + L.cut.columns - 1) / L.cut.columns;
+  const long long units = ((long long)g.a.max_pages * g.map.page_size + kUnit - 1) / kUnit;
+  const long long blocks = (tiles > sh.n_groups ? tiles : sh.n_groups) * units * (L.cut.columns / 16) * g.map.n_kv;
+  const long long own = (long long)g.a.T * L.cut.own_tiles * g.map.n_kv;
+  L.tiles = L.cut.columns >= kTile / 2 && (g.map.head_dim <= 128 ? blocks > 2 * kCUs : blocks + own > kCUs);
   const hipError_t e = dtype == F32    ? launch<F32>(L, s)
                        : dtype == F16  ? launch<F16>(L, s)
                        : dtype == BF16 ? launch<BF16>(L, s)
