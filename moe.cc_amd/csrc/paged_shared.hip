@@ -794,9 +794,10 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 // when one is more than 2^kSlack above it, so that most steps need no sums across lanes.  fp32 pages lie in LDS as they are and
 // use the fp32 instruction: a lane's 16 bytes of a key or a value are four operands.
 //
-// 32 heads over 4 of 128, us, and of sixteens: bf16, 8 groups of 4 rows of 4000 positions 26, 34; of 8 rows 33, 52; 64 rows of
-// 8000 41, 85.  Matrix instructions bound many rows: 64 of 16000 are 16.8 GFLOP, which fp32 does in 161 us (104 TFLOP/s of the
-// 153 that a large product reaches here), bf16 in 58, its three parts at 0.87 PFLOP/s of 1.23, 8-bit pages in 54.  What the
+// 32 heads over 4 of 128, us, and of sixteens: bf16, 8 groups of 4 rows of 4000 positions 23, 34; of 8 rows 33, 52; 64 rows of
+// 8000 41, 85; 32 heads over 4 of 256, 8 groups of 4 rows of 2000 32, 44, of 8 rows 39, 66.  Matrix instructions bound many
+// rows: 64 of 16000 are 16.8 GFLOP, which fp32 does in 158 us (106 TFLOP/s of the 153 that a large product reaches here), bf16
+// in 60, its three parts at 0.84 PFLOP/s of 1.23, 16- and 8-bit pages of two parts in 52.  What the
 // parts' instructions leave is the weights' arithmetic (two waves of a SIMD hardly overlap it with matrix instructions) and
 // about 10 us of a block's start and end.  Items of 128 columns gain 4 % where all is large and lose 10 % elsewhere (16 rows
 // of 3800 20.6, with 128 22.6).
@@ -984,8 +985,8 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
       for (int ct = 0; ct < CPW; ++ct)
 #pragma unroll
         for (int t = 0; t < KT; ++t) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      // operands at a time: with all of them in registers 256 dimensions do not fit (8 groups of 8 rows of 2000 positions, bf16
-      // 79 us, in halves 53, in quarters 40; 128 dimensions, 64 rows of 16000 64, in halves 60)
+      // operands in pieces, which leave registers for the rest (bf16, 128 dimensions, 64 rows of 16000 positions 64 us, in halves
+      // 60; 256 dimensions, 8 groups of 8 rows of 700 in halves 30.0, in quarters 28.9)
       constexpr int CUT = HDP > 128 ? 4 : HDP > 64 ? 2 : 1, KC = NK / CUT, VN = CT == F32 ? KT * VE : VE / CUT;
 #pragma unroll
       for (int j0 = 0; j0 < NK; j0 += KC) {
