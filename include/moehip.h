@@ -327,6 +327,9 @@ moe_status moe_model_config(const moe_model* m, QwenConfig* cfg);
 moe_status moe_model_reset(moe_model* m);
 /* Number of positions in the KV cache. */
 int moe_model_position(const moe_model* m);
+
+/* Positions that the model has: max_seq of its creation; -1: no model. */
+int moe_model_max_seq(const moe_model* m);
 /* T new tokens at the current position (ids on the device if ids_on_device,
  * else host ids checked against [0, vocab)); K/V appended to the cache.
  * The last row's logits go to logits_dev [vocab] and the next token the
@@ -665,7 +668,9 @@ moe_status moe_model_step_paged(moe_model* m, const moe_paged_plan* plan, const 
  * moe_model_step_paged on its prompts, each as its group's first request, and
  * scores of 0 for those, -inf for the others; it ends with a last
  * moe_beam_select_dev.  fork->status or plan->status other than 0: the step's
- * logits are worthless, the search has lost its place.  Checks, scratch and
+ * logits are worthless, the search has lost its place.  A beam's logits at or
+ * past the model's max_seq are NaN and leave it without candidates: a search
+ * takes at most moe_model_max_seq positions.  Checks, scratch and
  * captures as moe_model_step_paged's. */
 moe_status moe_model_step_beams(moe_model* m, const moe_beam_select* select, const moe_paged_fork* fork,
                                 const moe_paged_plan* plan, const moe_pages* layers, float* logits);

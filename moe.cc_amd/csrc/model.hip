@@ -902,6 +902,8 @@ moe_status moe_model_reset(moe_model* m) {
 
 int moe_model_position(const moe_model* m) { return m ? m->pos : -1; }
 
+int moe_model_max_seq(const moe_model* m) { return m ? m->max_seq : -1; }
+
 moe_status moe_model_forward(moe_model* m, const int32_t* ids, int T, int ids_on_device,
                              float* logits_dev, int32_t* next_dev) {
   moe_status st = ensure_init();

@@ -187,6 +187,7 @@ _SIGS = {
     "moe_model_config": (_I, [_P, _P]),
     "moe_model_reset": (_I, [_P]),
     "moe_model_position": (_I, [_P]),
+    "moe_model_max_seq": (_I, [_P]),
     "moe_model_forward": (_I, [_P, _P, _I, _I, _P, _P]),
     "moe_model_forward_full": (_I, [_P, _P, _I, _I, _P]),
     "moe_model_step_paged": (_I, [_P] * 6),
@@ -544,6 +545,7 @@ class Model:
         check(lib().moe_model_config(self.h, ctypes.byref(cfg)), "moe_model_config")
         self.cfg = cfg
         self.V = cfg.vocab_size
+        self.max_seq = lib().moe_model_max_seq(self.h)
 
     @classmethod
     def synthetic(cls, cfg: QwenConfig, expert_dtype=3, untied_head=True, seed=1, std=0.02,
@@ -639,12 +641,15 @@ class Model:
         """Beam searches over `prompts` (lists of ids), all steps on the device.
 
         -> (ids [len(prompts)][n_beam]: lists of up to n_new new ids, the best beam first, a list ending with `eos` where
-        it came; their log probabilities [len(prompts), n_beam])"""
+        it came; their log probabilities [len(prompts), n_beam]).  A prompt and its new tokens but the last fit max_seq."""
         prompts = [np.ascontiguousarray(p, np.int32) for p in prompts]
         G, R, V = len(prompts), len(prompts) * n_beam, self.V
         if not prompts or min(p.size for p in prompts) < 1 or n_beam < 1 or n_new < 1:
             raise MoeError(f"a search of {n_beam} beams over {len(prompts)} prompts, {n_new} new tokens")
-        width = -(-(max(p.size for p in prompts) + n_new) // page_size)
+        longest = max(p.size for p in prompts)
+        if longest + n_new - 1 > self.max_seq:   # (logits are NaN from there on, and a row of those has no candidates)
+            raise MoeError(f"a search of {longest} + {n_new} tokens exceeds max_seq {self.max_seq}")
+        width = -(-(longest + n_new) // page_size)
         cfg = self.cfg
         # (a fork takes the pages of its copies before it gives any back: one a beam more than they hold)
         cache = PagedCache(cfg.n_layers, cfg.n_kv, cfg.head_dim, R * (width + 1) if n_pages is None else n_pages, page_size,
