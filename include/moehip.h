@@ -429,7 +429,9 @@ typedef struct {
 } moe_paged_plan;
 /* Takes free pages, oldest first, for the requests in order, extends their
  * tables, gives an ended request's pages back behind the free ones (for the
- * next step; its held becomes 0), and places the tokens: request r's are rows
+ * next step; its held becomes 0; one that shares pages with others, by
+ * moe_paged_fork_dev, is ended there, since what others hold is given back here
+ * too), and places the tokens: request r's are rows
  * starts[r] .. starts[r + 1] - 1.  Rows behind the last token get req = pos =
  * slot = -1.  *status: 0 done; 1 too few free pages, 2 more than max_tokens
  * tokens, 3 a request outgrows its table row, 4 the state is broken (a

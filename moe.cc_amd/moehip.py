@@ -429,7 +429,11 @@ class PagedCache:
     ``layers`` is an array of Pages (head-major, which the attention reads a
     twentieth faster than slot-major pages; one K and one V pool a layer),
     ``plan`` the PagedPlan whose state is updated in place; the free
-    pages are 0 .. n_pages - 1 in order at the start."""
+    pages are 0 .. n_pages - 1 in order at the start.  Requests may share pages
+    after a fork; moe_paged_plan_dev would give those back whoever else holds
+    them, so from then on set_step ends requests by a fork."""
+
+    forked = False   # requests may share pages
 
     def __init__(self, n_layers, n_kv, head_dim, n_pages, page_size, n_req, max_pages, max_tokens,
                  dtype=PAGE_F32, k_scale=None, v_scale=None):
@@ -459,11 +463,14 @@ class PagedCache:
                               p["starts"], p["req"], p["pos"], p["slot"], p["status"])
 
     def set_step(self, fresh, ids):
-        """New tokens of each request (-1: it ended) and their ids, request after request."""
+        """New tokens of each request (-1: it ended) and their ids, request after request.  In a cache that was forked the
+        ended ones end here, not with the step's plan."""
         fresh, ids = np.asarray(fresh, np.int32), np.asarray(ids, np.int32)
         fits = fresh.shape == (self.n_req,) and ids.size <= self.max_tokens
         if not fits or ids.size < min(int(np.maximum(fresh, 0).sum()), self.max_tokens):
             raise MoeError(f"a step of {fresh.size} requests and {ids.size} tokens")
+        if self.forked and (fresh == -1).any():   # (pages that others hold stay with them)
+            self.fork(np.where(fresh == -1, -1, np.arange(self.n_req)))
         self._b["fresh"].upload(fresh)
         self._b["ids"].upload(ids)
 
@@ -476,6 +483,7 @@ class PagedCache:
             self._b["copies"] = DeviceBuffer(12 * self.n_req)
             self._b["fork_status"] = DeviceBuffer.from_array(np.zeros(1, np.int32))
             self._b["fork_work"] = DeviceBuffer(need)
+        self.forked = True
         b = {n: x.ptr for n, x in self._b.items()}
         return PagedFork(self.n_req, self.plan.max_pages, self.plan.n_pages, self.plan.page_size, self.n_req,
                          parent_ptr, b["held"], b["ring_at"], b["ring"], b["tables"], b["held"], b["ring_at"],
