@@ -627,7 +627,10 @@ size_t moe_paged_share_plan_bytes(int T, int n_groups, int n_q, int n_kv, int he
 moe_status moe_paged_share_dev(const moe_paged_share* s);
 
 /* moe_paged_attn_dev's results (a, pages: its arguments), with each group's
- * prefix read once for all its rows instead of once a row.  s: as
+ * prefix read once for all its rows instead of once a row: as close to the
+ * formula, queries and weights in all their bits (in both calls over fp16
+ * pages to 2^-38 of a head's largest).  Rows' own positions are read once a
+ * row, also where several rows are of one request.  s: as
  * moe_paged_share_dev was given it for the same rows, tables and heads.
  * work: moe_paged_attn_shared_work_bytes, else as moe_paged_attn's.  Few rows of
  * short prefixes (bf16: 8 of 600 positions) are as fast by moe_paged_attn_dev. */

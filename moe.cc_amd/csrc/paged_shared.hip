@@ -447,31 +447,28 @@ __device__ __forceinline__ bool item_ok(const SharedLaunch& L, const Item& x, in
          x.begin >= 0 && x.begin < x.end && x.end <= a.max_pages * L.g.map.page_size && (uint32_t)x.part < (uint32_t)parts;
 }
 
-__device__ __forceinline__ u32x2 widen16(uint32_t x) {   // four 8-bit values -> two dwords of f16 pairs (exact)
-  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true))};
-}
-
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// 1, which the compiler does not know: a product with it makes x - (float)h, rounded, one instruction that takes and gives fp16
-// instead of three (8 groups of 64 rows of 4000 positions, fp16 107 -> 102 us).
+// 1, which the compiler does not know: a product with it makes x - (float)h one instruction that takes fp16 instead of two.
 __device__ __forceinline__ float opaque_one() {
   float one = 1.0f;
   asm("" : "+s"(one));
   return one;
 }
 
-// Two fp32 values into the same place of NP operands: three bf16 parts, whose sum they are, or two f16 parts, each rounded
-// to nearest even, whose sum is off by at most 2^-23 of the value (twice an fp32 rounding, at the worst bits) and by 2^-25.
-template <bool HALF, int NP>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&p)[NP]) {
+// Two fp32 values into the same place of three operands whose sum they are: bf16 parts by truncation, f16 parts each rounded
+// to nearest even, which hold all bits but those below 2^-24.
+template <bool HALF>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&p)[3]) {
   if constexpr (HALF) {
-    const f16x2 h = __builtin_convertvector(f32x2{x, y}, f16x2);
     const float one = opaque_one();
-    const f16x2 l = {(_Float16)__builtin_fmaf(-(float)h[0], one, x), (_Float16)__builtin_fmaf(-(float)h[1], one, y)};
+    const f16x2 h = __builtin_convertvector(f32x2{x, y}, f16x2);
+    const float x1 = __builtin_fmaf(-(float)h[0], one, x), y1 = __builtin_fmaf(-(float)h[1], one, y);
+    const f16x2 m = __builtin_convertvector(f32x2{x1, y1}, f16x2);
+    const f16x2 l = {(_Float16)__builtin_fmaf(-(float)m[0], one, x1), (_Float16)__builtin_fmaf(-(float)m[1], one, y1)};
     p[0] = __builtin_bit_cast(uint32_t, h);
-    p[1] = __builtin_bit_cast(uint32_t, l);
+    p[1] = __builtin_bit_cast(uint32_t, m);
+    p[2] = __builtin_bit_cast(uint32_t, l);
   } else {
     split2<false>(x, y, &p[0], &p[1], &p[2]);
   }
@@ -495,8 +492,8 @@ __device__ __forceinline__ Column column_of(const SharedLaunch& L, const Item& x
 //   weights  come out as keys 4 (l / 16) + i of column l % 16 and go back in as the second operand from the same lane
 //   values   lane l holds the keys 4 (l / 16) + i of both tiles at its 1 / 16 of the dimensions; pairs of keys are put side by
 //            side by byte permutes
-// 16-bit operands: bf16 pages with queries and weights in three parts; f16 and 8-bit pages (exact in f16) in two f16 parts.
-// fp32 pages use the fp32 instruction.  A block's own chain of latencies bounds few rows: one group of 4 rows of 550 positions,
+// 16-bit operands, queries and weights in three parts: f16 for f16 pages, bf16 for bf16 and 8-bit ones (exact in bf16).  fp32
+// pages use the fp32 instruction.  A block's own chain of latencies bounds few rows: one group of 4 rows of 550 positions,
 // 32 heads over 4 of 128, fp32, takes 14 us with the join, of 1000 shared by 8 groups of 4, bf16, 19 (15 in tiles, below).
 template <int HDP>
 struct ColumnsShared {   // 128 dimensions at a time
@@ -505,8 +502,8 @@ struct ColumnsShared {   // 128 dimensions at a time
 
 template <int CT, int HDP>
 __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item& it, int kv, int sub, bool own, ColumnsShared<HDP>& sh) {
-  constexpr bool HALF = CT == F16 || CT == E4M3;
-  constexpr int NP = HALF ? 2 : 3;                 // parts of an fp32 value
+  constexpr bool HALF = CT == F16;
+  constexpr int NP = 3;                            // parts of an fp32 value
   constexpr int S = CT == F32 ? 4 : CT == E4M3 ? 1 : 2;
   constexpr int E = 16 / S;                        // elements of a 16-byte piece
   constexpr int NK = HDP / E / 4;                  // a lane's pieces of a key
@@ -600,7 +597,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
         } else if constexpr (CT == E4M3) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const u32x2 y = widen16(kr[t][j][2 * u]), z = widen16(kr[t][j][2 * u + 1]);
+            const u32x2 y = widen(kr[t][j][2 * u]), z = widen(kr[t][j][2 * u + 1]);
             const u32x4 k = {y[0], y[1], z[0], z[1]};
 #pragma unroll
             for (int n = 0; n < NP; ++n) s[t] = mfma32<HALF>(k, qp[n][2 * j + u], s[t]);
@@ -652,7 +649,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t u[NP];
-        split_pair<HALF, NP>(p[c / 2][2 * (c % 2)], p[c / 2][2 * (c % 2) + 1], u);
+        split_pair<HALF>(p[c / 2][2 * (c % 2)], p[c / 2][2 * (c % 2) + 1], u);
 #pragma unroll
         for (int n = 0; n < NP; ++n) pp[n][c] = u[n];
       }
@@ -664,7 +661,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 #pragma unroll
           for (int d = 0; d < VW; ++d) {
             if constexpr (CT == E4M3) {
-              const u32x2 y = widen16(vr[k][h][d]);
+              const u32x2 y = widen(vr[k][h][d]);
               w16[k][2 * d] = y[0], w16[k][2 * d + 1] = y[1];
             } else {
               w16[k][d] = vr[k][h][d];
@@ -712,7 +709,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
         for (int c = 0; c < 4; ++c) {
           const f32x4 y = x[2 * s + c / 2];
           uint32_t u[NP];
-          split_pair<HALF, NP>(y[2 * (c % 2)] * lift, y[2 * (c % 2) + 1] * lift, u);
+          split_pair<HALF>(y[2 * (c % 2)] * lift, y[2 * (c % 2) + 1] * lift, u);
 #pragma unroll
           for (int n = 0; n < NP; ++n) qp[n][s][c] = u[n];
         }
@@ -789,7 +786,7 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 // step ahead, where the waves over the columns share them: rows of 16-bit values in 16-byte pieces, piece p of row r at
 // p ^ swizzle(r), so that the reads of both lie evenly over the banks.  Keys are read as rows; a value operand, 8 keys of one
 // dimension, is two reads that turn 4 rows x 16 dimensions around on their way.  16-bit pages go straight from memory into
-// LDS, 8-bit pages become f16 in registers.  A wave stages the 8 rows of one (32 positions, quad of lanes that reads them),
+// LDS, 8-bit pages become bf16 in registers.  A wave stages the 8 rows of one (32 positions, quad of lanes that reads them),
 // whose addresses lie in its lanes, found once for K and V.  One barrier a step.  A column's largest score is raised only
 // when one is more than 2^kSlack above it, so that most steps need no sums across lanes.  fp32 pages lie in LDS as they are and
 // use the fp32 instruction: a lane's 16 bytes of a key or a value are four operands.
@@ -797,7 +794,8 @@ __device__ __forceinline__ void columns_block(const SharedLaunch& L, const Item&
 // 32 heads over 4 of 128, us, and of sixteens: bf16, 8 groups of 4 rows of 4000 positions 23, 34; of 8 rows 33, 52; 64 rows of
 // 8000 41, 85; 32 heads over 4 of 256, 8 groups of 4 rows of 2000 32, 44, of 8 rows 39, 66.  Matrix instructions bound many
 // rows: 64 of 16000 are 16.8 GFLOP, which fp32 does in 158 us (106 TFLOP/s of the 153 that a large product reaches here), bf16
-// in 60, its three parts at 0.84 PFLOP/s of 1.23, 16- and 8-bit pages of two parts in 52.  What the
+// and 8-bit pages in 60, their three parts at 0.84 PFLOP/s of 1.23, fp16 in 63.  (Two fp16 parts, 22 bits, took 52 to 55: a
+// score of 2^17 was then off by up to 2^-6, and weights below 2^-35 of a row's largest were lost.)  What the
 // parts' instructions leave is the weights' arithmetic (two waves of a SIMD hardly overlap it with matrix instructions) and
 // about 10 us of a block's start and end.  Items of 128 columns gain 4 % where all is large and lose 10 % elsewhere (16 rows
 // of 3800 20.6, with 128 22.6).
@@ -824,13 +822,13 @@ __device__ __forceinline__ u32x2 read_turned(const uint8_t* p) {
 template <int CT, int HDP, int WC, int CPW>
 __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it, int kv, uint8_t* lds) {
   using T = TileShape<CT, HDP, WC, CPW>;
-  constexpr bool HALF = CT == F16 || CT == E4M3;
-  constexpr int NP = HALF ? 2 : CT == BF16 ? 3 : 1, S = T::S, RB = T::RB;
+  constexpr bool HALF = CT == F16;
+  constexpr int NP = CT == F32 ? 1 : 3, S = T::S, RB = T::RB;
   constexpr int NK = CT == F32 ? HDP / 16 : HDP / 32, VE = HDP / 16, KT = T::PW / 16;
   constexpr int SETS = T::ROWS / 32;                              // (32 positions, q) that a wave stages
   constexpr int NL = (8 * HDP * S + 1023) / 1024;              // 16-byte loads of a lane for their keys
   constexpr int KP = HDP * S / 16;                             // such pieces of a row
-  constexpr float kSlack = 4.0f, kLift = HALF ? 10.0f : 0.0f;  // weights reach 2^(kSlack + kLift)
+  constexpr float kSlack = HALF ? 2.0f : 4.0f, kLift = HALF ? 13.0f : 0.0f;  // weights reach 2^(kSlack + kLift)
   const AttnPages& g = L.g;
   const moe_paged_attn& a = g.a;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -899,7 +897,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
           for (int side = 0; side < 2; ++side)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const u32x2 y = widen16(raw[n][i][side][2 * u]), z = widen16(raw[n][i][side][2 * u + 1]);
+              const u32x2 y = widen(raw[n][i][side][2 * u]), z = widen(raw[n][i][side][2 * u + 1]);
               *(u32x4*)(to + side * T::ROWS * RB + (set * 8 + k) * RB + ((piece + u) ^ sw) * 16) = u32x4{y[0], y[1], z[0], z[1]};
             }
         }
@@ -951,7 +949,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
         for (int i = 0; i < 4; ++i) {
           const f32x4 y = x[2 * s + i / 2];
           uint32_t u[NP];
-          split_pair<HALF, NP>(y[2 * (i % 2)] * lift, y[2 * (i % 2) + 1] * lift, u);
+          split_pair<HALF>(y[2 * (i % 2)] * lift, y[2 * (i % 2) + 1] * lift, u);
 #pragma unroll
           for (int n = 0; n < NP; ++n) qp[ct][n][s][i] = u[n];
         }
@@ -986,8 +984,9 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
 #pragma unroll
         for (int t = 0; t < KT; ++t) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       // operands in pieces, which leave registers for the rest (bf16, 128 dimensions, 64 rows of 16000 positions 64 us, in halves
-      // 60; 256 dimensions, 8 groups of 8 rows of 700 in halves 30.0, in quarters 28.9)
-      constexpr int CUT = HDP > 128 ? 4 : HDP > 64 ? 2 : 1, KC = NK / CUT, VN = CT == F32 ? KT * VE : VE / CUT;
+      // 60; 256 dimensions, 8 groups of 8 rows of 700 in halves 30.0, in quarters 28.9; 8-bit pages, whose next rows lie in
+      // registers, 64 columns, 8 groups of 64 rows of 4000 in halves 126, in quarters 113)
+      constexpr int CUT = HDP > 128 || (CT == E4M3 && CPW == 2 && HDP > 64) ? 4 : HDP > 64 ? 2 : 1, KC = NK / CUT, VN = CT == F32 ? KT * VE : VE / CUT;
 #pragma unroll
       for (int j0 = 0; j0 < NK; j0 += KC) {
         u32x4 k[KC][KT];
@@ -1065,7 +1064,7 @@ __device__ __forceinline__ void tile_block(const SharedLaunch& L, const Item& it
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t u[NP];
-            split_pair<HALF, NP>(p[ct][2 * c], p[ct][2 * c + 1], u);
+            split_pair<HALF>(p[ct][2 * c], p[ct][2 * c + 1], u);
 #pragma unroll
             for (int n = 0; n < NP; ++n) pp[ct][n][c] = u[n];
           }
