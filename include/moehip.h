@@ -522,7 +522,10 @@ moe_status moe_paged_attn_dev(const moe_paged_attn* a, const moe_pages* pages);
  * value score.  The n_beam candidates of a group with the largest value *
  * weight[r] (NULL: 1; a length penalty is the caller's), largest first, become
  * its rows.  Candidates of one row are ordered by logit, then the lower token;
- * of several by value * weight in 64 bits, then the lower row.  A -inf logit is
+ * of several by value * weight in 64 bits, then the lower row.  The logarithm is
+ * within 2^-21 of the formula's: several rows' candidates whose values differ by
+ * less than twice that may change places, and a value may pass its row's score
+ * by as much.  A -inf logit is
  * no candidate; a row with a NaN or +inf logit, a score that is not finite or a
  * weight that is not finite and above 0 has none.
  * New row r continues row parent[r] with token[r] (`pad` if that had ended);

@@ -17,12 +17,13 @@
 // Order.  Inside a row candidates are ordered by (logit, token), which a
 // 64-bit whole number holds exactly: the logit's bits as an ordered whole
 // number above, the token's complement below.  Between rows by value * weight
-// in 64 bits, so that two candidates are told apart unless they are 1e-8 close
-// to each other; that is also how exact the sums are.  Sums: exp(x) = 2^(x
-// log2(e)), the product carried in two floats and split into a whole number and
-// what is left, so that a term's error is that of the hardware's exp2 on
-// [-1/2, 1/2] (2^-23 of it, either way) and 2^-25; four terms are added in fp32,
-// the rest in 64 bits.
+// in 64 bits, of values that are as exact as the sums: exp(x) = 2^(x log2(e)),
+// the product carried in two floats and split into a whole number and what is
+// left, so that a term's error is that of the hardware's exp2 on [-1/2, 1/2]
+// (2^-23 of it, either way) and 2^-25; four terms are added in fp32 (2^-23), the
+// rest in 64 bits.  Errors of many terms average out; of a token that holds
+// nearly all of its row's probability they do not: lse is within 2^-21 (5e-7),
+// and rows whose values differ by less than twice that may change places.
 #include <math.h>
 
 #include <type_traits>
