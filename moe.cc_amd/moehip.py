@@ -654,6 +654,8 @@ class Model:
         G, R, V = len(prompts), len(prompts) * n_beam, self.V
         if not prompts or min(p.size for p in prompts) < 1 or n_beam < 1 or n_new < 1:
             raise MoeError(f"a search of {n_beam} beams over {len(prompts)} prompts, {n_new} new tokens")
+        if any(((p < 0) | (p >= V)).any() for p in prompts):
+            raise MoeError(f"a prompt has an id outside 0 .. {V - 1}")
         longest = max(p.size for p in prompts)
         if longest + n_new - 1 > self.max_seq:   # (logits are NaN from there on, and a row of those has no candidates)
             raise MoeError(f"a search of {longest} + {n_new} tokens exceeds max_seq {self.max_seq}")

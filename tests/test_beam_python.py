@@ -32,6 +32,15 @@ def test_search_past_the_model(lengths, n_new, fits, no_memory):
         _model(20).beam_search([np.zeros(n, np.int32) for n in lengths], 3, n_new)
 
 
+@pytest.mark.parametrize("bad", [-1, 90, 1 << 30])
+def test_search_of_no_token(bad, no_memory):
+    """An id that is none is refused, as moe_model_generate does, not clamped."""
+    with pytest.raises(M.MoeError, match="id outside 0 .. 89"):
+        _model(20).beam_search([[1, 2], [0, 89, bad, 3]], 2, 3)
+    with pytest.raises(Made):
+        _model(20).beam_search([[1, 2], [0, 89, 3]], 2, 3)
+
+
 class Buffer:
     def __init__(self):
         self.ptr, self.nbytes, self.got = 1, 1 << 20, []
